@@ -103,6 +103,7 @@ class Context:
         self.h = h
         self.device = device
         s = stream if stream is not None else torch.cuda.current_stream(device)
+        self.stream = s
         self.check(self.L.kdec_set_stream(self.h, ctypes.c_void_p(s.cuda_stream)))
 
     def close(self):

@@ -1,0 +1,161 @@
+"""Token operators on torch tensors: attention over packed documents, the
+projection with low-rank adapters chosen per row, and dropout (the last
+section of kdec.h). Each call checks its tensors, allocates what it returns
+and makes one C ABI call on the context's stream; nothing synchronises. A
+tensor made on another stream has to be ordered before the context's by the
+caller, as for every call of the library.
+
+Tensors are float32 or bfloat16 (one type per call), on the context's device;
+offsets and adapter choices are int32 tensors there. Errors are
+``native.KdecError`` (what the library refuses) and ``ValueError`` (tensors
+that do not fit each other)."""
+from __future__ import annotations
+
+import torch
+
+from .native import Context
+
+_TYPES = {torch.float32: 0, torch.bfloat16: 1}
+
+
+def _need(cond, what):
+    if not cond:
+        raise ValueError("brosoundml: " + what)
+
+
+def _dtype(x, *others):
+    """The C ABI's type of x, which the others must share, all on one HIP device."""
+    _need(x.dtype in _TYPES, "tensors must be float32 or bfloat16")
+    _need(x.is_cuda, "tensors must be on the HIP device")
+    for t in others:
+        _need(t.dtype == x.dtype and t.device == x.device, "tensors must share one type and device")
+    return _TYPES[x.dtype]
+
+
+def _ints(x, n, what):
+    """Address of an int32 tensor of n values on the device (None passes)."""
+    if x is None:
+        return None
+    _need(x.dtype == torch.int32 and x.is_cuda and x.is_contiguous() and x.numel() == n,
+          f"{what} must hold {n} contiguous int32 values on the device")
+    return x.data_ptr()
+
+
+def _floats(x, shape, what):
+    if x is None:
+        return None
+    _need(x.dtype == torch.float32 and x.is_cuda and x.is_contiguous() and tuple(x.shape) == tuple(shape),
+          f"{what} must be a contiguous float32 tensor of shape {tuple(shape)}")
+    return x.data_ptr()
+
+
+def _heads(x, what):
+    """Address, row stride and head stride of a (rows, heads, width) tensor with contiguous width."""
+    _need(x.dim() == 3, f"{what} must be (rows, heads, width)")
+    _need(x.stride(2) == 1 or x.shape[2] <= 1, f"{what}: the width must be contiguous")
+    return x.data_ptr(), x.stride(0), x.stride(1)
+
+
+def _rows(x, what):
+    """Address and row stride of a (rows, columns) tensor with contiguous columns."""
+    _need(x.dim() == 2, f"{what} must be (rows, columns)")
+    _need(x.stride(1) == 1 or x.shape[1] <= 1, f"{what}: the columns must be contiguous")
+    return x.data_ptr(), x.stride(0)
+
+
+def _whole(x, shape, what):
+    _need(tuple(x.shape) == tuple(shape) and x.is_contiguous(), f"{what} must be contiguous, of shape {tuple(shape)}")
+    return x.data_ptr()
+
+
+class _on:
+    """Allocations inside belong to the context's stream."""
+
+    def __init__(self, ctx: Context):
+        self.cm = None if torch.cuda.current_stream(ctx.device) == ctx.stream else torch.cuda.stream(ctx.stream)
+
+    def __enter__(self):
+        if self.cm is not None:
+            self.cm.__enter__()
+
+    def __exit__(self, *a):
+        if self.cm is not None:
+            self.cm.__exit__(*a)
+
+
+def _attn_args(q, k, v, q_off, k_off, k_len, causal, prefix, scale, cap, slopes):
+    dt = _dtype(q, k, v)
+    Q, K, V = _heads(q, "q"), _heads(k, "k"), _heads(v, "v")
+    tq, hq, d = q.shape
+    tk, hkv, _ = k.shape
+    _need(v.shape == k.shape and k.shape[2] == d, "k and v must share their shape, and q their width")
+    docs = q_off.numel() - 1
+    _need(docs >= 0, "q_off must hold one offset more than there are documents")
+    if k_off is None:
+        _need(tq == tk, "without k_off the keys are the query rows' own")
+        k_off = q_off
+    # where / length / mask arguments, in the C ABI's order
+    mask = (_ints(q_off, docs + 1, "q_off"), _ints(k_off, docs + 1, "k_off"), _ints(k_len, docs, "k_len"),
+            _ints(prefix, docs, "prefix"), docs, int(causal), _floats(slopes, (hq,), "slopes"),
+            float(d ** -0.5 if scale is None else scale), float(cap), tq, tk, hq, hkv, d)
+    return dt, Q, K, V, mask
+
+
+def attention(ctx: Context, q, k, v, q_off, k_off=None, k_len=None, *, causal=False, prefix=None, scale=None,
+              cap=0.0, slopes=None, out=None):
+    """Attention of packed documents (kdec_attn_fwd): q (Tq, Hq, D), k and v
+    (Tk, Hkv, D) with any row and head strides; document d holds the query
+    rows q_off[d]:q_off[d+1] and the keys k_off[d]:k_off[d+1] (the query rows'
+    own without k_off), of which the first k_len[d] are filled. ``causal``
+    rows see the keys up to their own position, counted from the document's
+    end, and its first prefix[d]. ``cap`` caps the scores by cap * tanh(s /
+    cap), ``slopes`` (Hq floats) lowers them by slope * distance; ``scale``
+    is 1 / sqrt(D) by default. Returns (o, lse): o as q, lse (Hq, Tq) float.
+    Single tokens over long caches take a kernel of their own in this call."""
+    dt, Q, K, V, mask = _attn_args(q, k, v, q_off, k_off, k_len, causal, prefix, scale, cap, slopes)
+    tq, hq, _ = q.shape
+    with _on(ctx):
+        o = torch.empty(q.shape, dtype=q.dtype, device=q.device) if out is None else out
+        lse = torch.empty((hq, tq), dtype=torch.float32, device=q.device)
+    _need(o.shape == q.shape and o.dtype == q.dtype, "out must be as q")
+    ctx.call("kdec_attn_fwd", dt, *Q, *K, *V, *mask, *_heads(o, "out"), lse.data_ptr())
+    return o, lse
+
+
+def attention_bwd(ctx: Context, q, k, v, o, lse, do, q_off, k_off=None, k_len=None, *, causal=False, prefix=None,
+                  scale=None, cap=0.0, slopes=None, dq=None, dk=None, dv=None):
+    """The gradients (dq, dk, dv) of ``attention`` from ``do``, with its o and
+    lse and the same mask arguments (kdec_attn_bwd). dq, dk and dv may be
+    given, for example as the parts of a fused projection's gradient."""
+    dt, Q, K, V, mask = _attn_args(q, k, v, q_off, k_off, k_len, causal, prefix, scale, cap, slopes)
+    _dtype(q, o, do)
+    _need(o.shape == q.shape and do.shape == q.shape, "o and do must be as q")
+    with _on(ctx):
+        dq = torch.empty(q.shape, dtype=q.dtype, device=q.device) if dq is None else dq
+        dk = torch.empty(k.shape, dtype=k.dtype, device=k.device) if dk is None else dk
+        dv = torch.empty(v.shape, dtype=v.dtype, device=v.device) if dv is None else dv
+    _dtype(q, dq, dk, dv)
+    _need(dq.shape == q.shape and dk.shape == k.shape and dv.shape == v.shape, "dq, dk and dv must be as q, k and v")
+    ctx.call("kdec_attn_bwd", dt, *Q, *K, *V, *_heads(o, "o"), _floats(lse, (q.shape[1], q.shape[0]), "lse"),
+             *_heads(do, "do"), *mask, *_heads(dq, "dq"), *_heads(dk, "dk"), *_heads(dv, "dv"))
+    return dq, dk, dv
+
+
+def dropout(ctx: Context, x, p, seed, offset=0, *, residual=None, out=None):
+    """residual + x with values dropped with probability p and the kept ones
+    scaled by 1 / (1 - p) (kdec_dropout; p in steps of 1 / 65536). The mask is
+    the seed's and offset's alone: the backward is this call on the gradient
+    with the same seed and offset and no residual. ``out`` may be x."""
+    dt = _dtype(x)
+    X = _rows(x, "x")
+    with _on(ctx):
+        y = torch.empty(x.shape, dtype=x.dtype, device=x.device) if out is None else out
+    _dtype(x, y)
+    _need(y.shape == x.shape, "out must be as x")
+    R = (None, 0)
+    if residual is not None:
+        _dtype(x, residual)
+        _need(residual.shape == x.shape, "residual must be as x")
+        R = _rows(residual, "residual")
+    ctx.call("kdec_dropout", dt, *X, *R, *_rows(y, "out"), x.shape[0], x.shape[1], p, seed, offset)
+    return y

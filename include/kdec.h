@@ -426,6 +426,71 @@ int kdec_length_regulate(kdec_ctx* ctx, const float* t_en, long te_bs,
                          const int* dur, long dur_bs, int N, int C, int L,
                          float* asr, long asr_bs, int T, int* totals);
 
+/* ─── token operators ─────────────────────────────────────────────────── */
+/*
+ * For the text networks beside the decoder and for batches whose requests
+ * each have adapters of their own. They have no counterpart on the
+ * reference's path. Tensors are FP32 or bf16 (`dtype`, one type for all of a
+ * call's tensors unless noted), sums and softmax statistics are float, and
+ * each output is rounded once. Rows are tokens; a row stride (`_rs`, in
+ * elements) is the distance of two tokens, a head stride (`_hs`) that of two
+ * heads; the innermost axis is contiguous. Any alignment and any stride is
+ * taken; tensors whose base, strides and widths are multiples of 16 bytes
+ * take the wide loads. Offsets and adapter choices are int32 on the device.
+ * Outputs must not overlap inputs unless noted.
+ */
+#define KDEC_F32 0
+#define KDEC_BF16 1
+
+/* Y = R + drop(X) over `rows` rows of `cols` (R may be NULL): an element is
+ * dropped where its 16 random bits are below thr = round(p * 65536), a kept
+ * one is multiplied by 65536 / (65536 - thr). The bits are those of
+ * Philox4x32-10 under key `seed` and counter (col / 8, row, offset's low and
+ * high word): the same seed, offset, row and column give the same mask, so
+ * the backward is this call on dY with R = NULL. Y may be X or R.
+ * 0 <= p, and p and its rounding below 1. r_rs = 0 broadcasts one row. */
+int kdec_dropout(kdec_ctx* ctx, int dtype, const void* X, long x_rs,
+                 const void* R, long r_rs, void* Y, long y_rs, long rows,
+                 int cols, float p, long seed, long offset);
+
+/* Attention of packed documents. Document d has the query rows
+ * [q_off[d], q_off[d+1]) and, within its slot [k_off[d], k_off[d+1]) of the
+ * key rows, the first k_len[d] (all where k_len is NULL). A document's last
+ * query row stands at its last key. Where `causal`, a row sees the keys up to
+ * its own position and the first prefix[d] (none where prefix is NULL);
+ * otherwise all of its document's. The score of a row at position i and a
+ * key at j is
+ *   s = scale q.k;  s = cap tanh(s / cap) if cap > 0;
+ *   s -= slopes[h] |i - j| if slopes (Hq floats),
+ * O = softmax(s) V over the keys that the row sees, lse (Hq, Tq) = log sum
+ * exp s. A row that sees nothing, or that no document holds, gets O = 0 and
+ * lse = -inf. Query head h reads key head h / (Hq / Hkv). Offsets must not
+ * decrease; they are clamped to the Tq and Tk rows. Key and value rows that
+ * a row does not see do not reach it, whatever they hold; one that it sees
+ * and that is not finite makes it NaN.
+ * D <= 128, Hq a multiple of Hkv, scale > 0. */
+int kdec_attn_fwd(kdec_ctx* ctx, int dtype, const void* Q, long q_rs,
+                  long q_hs, const void* K, long k_rs, long k_hs,
+                  const void* V, long v_rs, long v_hs, const int* q_off,
+                  const int* k_off, const int* k_len, const int* prefix,
+                  int docs, int causal, const float* slopes, float scale,
+                  float cap, int Tq, int Tk, int Hq, int Hkv, int D, void* O,
+                  long o_rs, long o_hs, float* lse);
+/* Its backward from dO, with the forward's O and lse: dQ, dK and dV are
+ * overwritten (zeros in rows that nothing sees), dK and dV summed over the
+ * query heads of a key head in a fixed order. Scores are formed again; the
+ * slopes are constants. */
+int kdec_attn_bwd(kdec_ctx* ctx, int dtype, const void* Q, long q_rs,
+                  long q_hs, const void* K, long k_rs, long k_hs,
+                  const void* V, long v_rs, long v_hs, const void* O,
+                  long o_rs, long o_hs, const float* lse, const void* dO,
+                  long do_rs, long do_hs, const int* q_off, const int* k_off,
+                  const int* k_len, const int* prefix, int docs, int causal,
+                  const float* slopes, float scale, float cap, int Tq, int Tk,
+                  int Hq, int Hkv, int D, void* dQ, long dq_rs, long dq_hs,
+                  void* dK, long dk_rs, long dk_hs, void* dV, long dv_rs,
+                  long dv_hs);
+
 #ifdef __cplusplus
 }
 #endif
