@@ -161,20 +161,6 @@ struct Stage {
     Frag<T> f[N];
 };
 
-template <class T>
-__device__ inline void store4(T* p, int n, bool vec, float a, float b, float c, float d) {
-    const T v[4] = {static_cast<T>(a), static_cast<T>(b), static_cast<T>(c), static_cast<T>(d)};
-    if (n <= 0) return;
-    if (vec) {
-        typedef T V4 __attribute__((ext_vector_type(4)));
-        *reinterpret_cast<V4*>(p) = V4{v[0], v[1], v[2], v[3]};
-        return;
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-        if (i < n) p[i] = v[i];
-}
-
 // Rows j0 .. of a key-side tensor (base of the key head) into a stage; rows
 // at or past `end` are zeros.
 template <class T, int DP, int ROWS, int NT>

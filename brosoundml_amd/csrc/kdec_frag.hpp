@@ -52,21 +52,27 @@ __device__ inline Frag<T> acc_frag(const f32x16& s, int c) {
 }
 
 // 8 elements at p, of which the first n are the tensor's (zeros beyond).
-// vec: p is aligned to 16 bytes and n is 0 or 8.
-template <class T>
-__device__ inline Frag<T> load8(const T* p, int n, bool vec) {
-    Frag<T> f;
+// vec: p is aligned to 16 bytes and n is a multiple of 16 bytes' elements.
+__device__ inline bf16x8 load8(const bf16* p, int n, bool vec) {
+    bf16x8 f = bf16x8{};
     if (vec) {
-        if (n > 0) {
-            f = *reinterpret_cast<const Frag<T>*>(p);
-        } else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) f[i] = static_cast<T>(0.0f);
-        }
+        if (n > 0) f = *reinterpret_cast<const bf16x8*>(p);
         return f;
     }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = i < n ? p[i] : static_cast<T>(0.0f);
+    for (int i = 0; i < 8; ++i) f[i] = i < n ? p[i] : static_cast<bf16>(0.0f);
+    return f;
+}
+__device__ inline f32x8 load8(const float* p, int n, bool vec) {
+    f32x8 f = f32x8{};
+    if (vec) {
+        f32x4 a = f32x4{}, b = f32x4{};
+        if (n > 0) a = *reinterpret_cast<const f32x4*>(p);
+        if (n > 4) b = *reinterpret_cast<const f32x4*>(p + 4);
+        return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = i < n ? p[i] : 0.0f;
     return f;
 }
 
@@ -99,6 +105,59 @@ __device__ inline f32x8 lds_cols(const float* tile, int ls, int row0, int col0, 
 #pragma unroll
     for (int i = 0; i < 8; ++i) f[i] = p[(8 * (i >> 2) + (i & 3)) * ls];
     return f;
+}
+
+// lds_rows with the depth slots of acc_frag, the other operand of lds_cols.
+__device__ inline bf16x8 lds_rows_acc(const bf16* tile, int ls, int row0, int c) {
+    const int l = threadIdx.x & 63;
+    const bf16* p = tile + (row0 + (l & 31)) * ls + 16 * c + 4 * (l >> 5);
+    const bf16x4 a = *reinterpret_cast<const bf16x4*>(p), b = *reinterpret_cast<const bf16x4*>(p + 8);
+    return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+}
+__device__ inline f32x8 lds_rows_acc(const float* tile, int ls, int row0, int c) {
+    const int l = threadIdx.x & 63;
+    const float* p = tile + (row0 + (l & 31)) * ls + 16 * c + 4 * (l >> 5);
+    const f32x4 a = *reinterpret_cast<const f32x4*>(p), b = *reinterpret_cast<const f32x4*>(p + 8);
+    return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+}
+
+// A float fragment as bf16 terms whose sum holds it to 16 (two terms) or 24
+// bits (three): products with a bf16 operand then lose nothing that float
+// sums would keep. Float operands are one term.
+template <class T, int N> struct Terms;
+template <int N> struct Terms<bf16, N> {
+    static constexpr int n = N;
+    bf16x8 t[N];
+    __device__ explicit Terms(f32x8 f) {
+#pragma unroll
+        for (int k = 0; k < N; ++k)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                t[k][i] = static_cast<bf16>(f[i]);
+                f[i] -= static_cast<float>(t[k][i]);
+            }
+    }
+};
+template <int N> struct Terms<float, N> {
+    static constexpr int n = 1;
+    f32x8 t[1];
+    __device__ explicit Terms(f32x8 f) { t[0] = f; }
+};
+
+// Four values rounded to T at p, of which the first n are the tensor's.
+// vec: p is aligned to the four and n is 0 or 4 (or less).
+template <class T>
+__device__ inline void store4(T* p, int n, bool vec, float a, float b, float c, float d) {
+    const T v[4] = {static_cast<T>(a), static_cast<T>(b), static_cast<T>(c), static_cast<T>(d)};
+    if (n <= 0) return;
+    if (vec) {
+        typedef T V4 __attribute__((ext_vector_type(4)));
+        *reinterpret_cast<V4*>(p) = V4{v[0], v[1], v[2], v[3]};
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        if (i < n) p[i] = v[i];
 }
 
 // Whether any of the fragment's values is not finite.

@@ -141,6 +141,64 @@ def attention_bwd(ctx: Context, q, k, v, o, lse, do, q_off, k_off=None, k_len=No
     return dq, dk, dv
 
 
+def _adapter_args(x, w, a, b, scale, idx, unit_off):
+    t, cin = x.shape
+    out = w.shape[0]
+    n, units = a.shape[0], unit_off.numel() - 1
+    _need(b.dim() == 3 and units >= 1, "b must be (adapters, out, rank), unit_off units + 1 offsets")
+    rank = b.shape[2]
+    return (_whole(w, (out, cin), "w"), _whole(a, (n, units * rank, cin), "a"), _whole(b, (n, out, rank), "b"),
+            _floats(scale, (n,), "scale"), _ints(idx, t, "idx"), _ints(unit_off, units + 1, "unit_off"), t, cin, out,
+            n, units, rank)
+
+
+def adapter_proj(ctx: Context, x, w, a, b, scale, idx, unit_off, *, bias=None, drop=None, keep_h=False, out=None):
+    """x W^T + bias with row t's own low-rank adapter idx[t] beside it
+    (kdec_adapter_fwd): x (T, in), w (out, in), a (adapters, units * rank,
+    in), b (adapters, out, rank), scale (adapters floats); rows whose idx is
+    outside [0, adapters) take none. unit_off (units + 1) cuts the output rows
+    into units with adapters of their own. ``drop`` = (p, seed, offset) drops
+    inputs of the adapters. Returns y (T, out), and with ``keep_h`` the pair
+    (y, h) whose h the backward takes."""
+    dt = _dtype(x, w, a, b)
+    X = _rows(x, "x")
+    W, A, B, S, I, U, t, cin, cout, n, units, rank = _adapter_args(x, w, a, b, scale, idx, unit_off)
+    p, seed, offset = drop if drop is not None else (0.0, 0, 0)
+    with _on(ctx):
+        y = torch.empty((t, cout), dtype=x.dtype, device=x.device) if out is None else out
+        h = torch.empty((t, units * rank), dtype=torch.float32, device=x.device) if keep_h else None
+    _need(y.shape == (t, cout), "out must be (T, out)")
+    _dtype(x, y)
+    if bias is not None:
+        _dtype(x, bias)
+        _whole(bias, (cout,), "bias")
+    ctx.call("kdec_adapter_fwd", dt, *X, W, None if bias is None else bias.data_ptr(), A, B, S, I, U, t, cin, cout,
+             n, units, rank, p, seed, offset, None if h is None else h.data_ptr(), *_rows(y, "out"))
+    return (y, h) if keep_h else y
+
+
+def adapter_proj_bwd(ctx: Context, x, w, a, b, scale, idx, unit_off, h, dy, *, drop=None, need_dx=True, da=None,
+                     db=None, beta=0.0):
+    """The gradients (dx, da, db) of ``adapter_proj`` from ``dy`` and its h,
+    w and bias frozen (kdec_adapter_bwd). dx is of x's type (None without
+    ``need_dx``); da and db are float and, where given, become beta times
+    what they held plus the gradient."""
+    dt = _dtype(x, w, a, b, dy)
+    X = _rows(x, "x")
+    W, A, B, S, I, U, t, cin, cout, n, units, rank = _adapter_args(x, w, a, b, scale, idx, unit_off)
+    p, seed, offset = drop if drop is not None else (0.0, 0, 0)
+    _need(dy.shape == (t, cout), "dy must be (T, out)")
+    _need(beta == 0.0 or (da is not None and db is not None), "beta without da and db to add to")
+    with _on(ctx):
+        dx = torch.empty((t, cin), dtype=x.dtype, device=x.device) if need_dx else None
+        da = torch.empty(a.shape, dtype=torch.float32, device=x.device) if da is None else da
+        db = torch.empty(b.shape, dtype=torch.float32, device=x.device) if db is None else db
+    ctx.call("kdec_adapter_bwd", dt, *X, W, A, B, S, I, U, t, cin, cout, n, units, rank, p, seed, offset,
+             _floats(h, (t, units * rank), "h"), *_rows(dy, "dy"), None if dx is None else dx.data_ptr(), cin,
+             _floats(da, a.shape, "da"), _floats(db, b.shape, "db"), beta)
+    return dx, da, db
+
+
 def dropout(ctx: Context, x, p, seed, offset=0, *, residual=None, out=None):
     """residual + x with values dropped with probability p and the kept ones
     scaled by 1 / (1 - p) (kdec_dropout; p in steps of 1 / 65536). The mask is

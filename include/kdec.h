@@ -491,6 +491,45 @@ int kdec_attn_bwd(kdec_ctx* ctx, int dtype, const void* Q, long q_rs,
                   void* dK, long dk_rs, long dk_hs, void* dV, long dv_rs,
                   long dv_hs);
 
+/* A projection shared by all rows and the low-rank adapters that each row
+ * chooses beside it: row t takes adapter a = idx[t], none where idx[t] is
+ * outside [0, adapters);
+ *   H[t, u*rank + j] = sum_i A[a][u*rank + j, i] drop(X)[t, i]
+ *   Y[t, r] = W[r, :] . X[t, :] + bias[r]
+ *             + scale[a] sum_j B[a][r, j] H[t, u(r)*rank + j]
+ * with the output rows cut into `units` units, unit u owning
+ * [unit_off[u], unit_off[u+1]) (units+1 ints on the device, from 0 to out:
+ * one unit for a plain projection, three for a fused query / key / value,
+ * one per AdaIN unit for the stacked style projection). X (T, in) at row
+ * stride x_rs, W (out, in), bias (out) or NULL, A (adapters, units*rank, in),
+ * B (adapters, out, rank), scale (adapters floats), Y (T, out) at y_rs.
+ * p > 0 drops inputs of the adapters (not of W) as kdec_dropout does with
+ * this seed and offset. H (T, units*rank floats; zero rows where no adapter
+ * is chosen) is written when not NULL, for the backward.
+ * rank <= 128, units <= 4096. */
+int kdec_adapter_fwd(kdec_ctx* ctx, int dtype, const void* X, long x_rs,
+                     const void* W, const void* bias, const void* A,
+                     const void* B, const float* scale, const int* idx,
+                     const int* unit_off, int T, int in, int out,
+                     int adapters, int units, int rank, float p, long seed,
+                     long offset, float* H, void* Y, long y_rs);
+/* Its backward from dY (T, out) and the forward's H, W and bias frozen:
+ *   dH[t, u*rank+j] = scale[a] sum_{r in u} B[a][r, j] dY[t, r]
+ *   dX = dY W + drop(A[a]^T dH)
+ *   dA[a] = beta dA[a] + sum_{t of a} dH[t]^T drop(X)[t]
+ *   dB[a][r, j] = beta dB[a][r, j]
+ *                 + scale[a] sum_{t of a} dY[t, r] H[t, u(r)*rank + j]
+ * dA and dB are floats of A's and B's shapes; adapters that no row chooses
+ * get zeros (beta = 0: overwritten, what they held is not read). dX (T, in)
+ * at dx_rs. dX, or dA and dB together, may be NULL. */
+int kdec_adapter_bwd(kdec_ctx* ctx, int dtype, const void* X, long x_rs,
+                     const void* W, const void* A, const void* B,
+                     const float* scale, const int* idx, const int* unit_off,
+                     int T, int in, int out, int adapters, int units,
+                     int rank, float p, long seed, long offset,
+                     const float* H, const void* dY, long dy_rs, void* dX,
+                     long dx_rs, float* dA, float* dB, float beta);
+
 #ifdef __cplusplus
 }
 #endif
