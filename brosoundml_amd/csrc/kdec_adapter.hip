@@ -203,11 +203,12 @@ template <class T> constexpr int depth_of() { return sizeof(T) == 2 ? 64 : 32; }
 // LDS read turns them.
 template <class T, bool BWD>
 __global__ __launch_bounds__(NT, 1) void adapter_gemm_k(Adapter p, Product g) {
-    constexpr int BK = depth_of<T>(), PAD = 16 / sizeof(T);
-    constexpr int LZ = BK + PAD, LW = BWD ? GM + PAD : BK + PAD, WR = BWD ? BK : GM, WC = (BWD ? GM : BK) / 8;
+    constexpr int BK = depth_of<T>(), WC = (BWD ? GM : BK) / 8;
+    typedef Tile<T, BWD ? GM : BK> Tw;
+    typedef Tile<T, BK> Tz;
     constexpr int NZ = GN * BK / 8 / NT, NW = GM * BK / 8 / NT;
-    __shared__ __align__(16) T sw[WR * LW];
-    __shared__ __align__(16) T sz[GN * LZ];
+    __shared__ __align__(16) T sw[GM * BK];
+    __shared__ __align__(16) T sz[GN * BK];
     __shared__ int srow[GN], sid[GN];
     const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, half = lane >> 5, col = lane & 31;
     const int mt = (g.M + GM - 1) / GM;
@@ -337,12 +338,12 @@ __global__ __launch_bounds__(NT, 1) void adapter_gemm_k(Adapter p, Product g) {
 #pragma unroll
         for (int i = 0; i < NZ; ++i) {
             const int e = tid + i * NT;
-            *reinterpret_cast<Frag<T>*>(sz + (e / (BK / 8)) * LZ + 8 * (e % (BK / 8))) = fz[i];
+            Tz::put8(sz, e / (BK / 8), e % (BK / 8), fz[i]);
         }
 #pragma unroll
         for (int i = 0; i < NW; ++i) {
             const int e = tid + i * NT;
-            *reinterpret_cast<Frag<T>*>(sw + (e / WC) * LW + 8 * (e % WC)) = fw[i];
+            Tw::put8(sw, e / WC, e % WC, fw[i]);
         }
         __syncthreads();
         if (c + 1 < c1) load(c + 1);
@@ -352,13 +353,9 @@ __global__ __launch_bounds__(NT, 1) void adapter_gemm_k(Adapter p, Product g) {
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
                 const int m = 64 * (wave & 1) + 32 * i;
-                if (BWD) {
-                    w[i] = lds_cols(sw, LW, 32 * (k >> 1), m, k & 1);
-                    z[i] = lds_rows_acc(sz, LZ, wn + 32 * i, k);
-                } else {
-                    w[i] = lds_rows(sw, LW, m, k);
-                    z[i] = lds_rows(sz, LZ, wn + 32 * i, k);
-                }
+                if constexpr (BWD) w[i] = lds_cols<GM, false>(sw, 16 * k, m);
+                else w[i] = lds_rows<T, BK>(sw, m, k);
+                z[i] = lds_rows<T, BK>(sz, wn + 32 * i, k);
             }
 #pragma unroll
             for (int i = 0; i < 2; ++i)
@@ -409,10 +406,9 @@ __global__ __launch_bounds__(NT) void adapter_join_k(const float* part, int spli
 template <class T, bool DB>
 __global__ __launch_bounds__(NT) void adapter_outer_k(Adapter p, const float* P, const T* Z, long z_rs, int C, bool vec_z,
                                                       float* out, float beta, int mt) {
-    constexpr int LC = 128 + 16 / sizeof(T), LP = 32 + 16 / sizeof(T);
     constexpr int NTERM = Terms<T, 3>::n;
-    __shared__ __align__(16) T sz[32 * LC];
-    __shared__ __align__(16) T sp[NTERM][32 * LP];
+    __shared__ __align__(16) T sz[32 * 128];
+    __shared__ __align__(16) T sp[NTERM][32 * 64];
     const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, half = lane >> 5, col = lane & 31;
     const int ct = (C + 127) / 128;
     int b = blockIdx.x;
@@ -436,21 +432,21 @@ __global__ __launch_bounds__(NT) void adapter_outer_k(Adapter p, const float* P,
                 const int t = e >> 4, d = c0 + 8 * (e & 15), row = s + t < s1 ? p.perm[s + t] : 0;
                 Frag<T> z = load8(Z + row * z_rs + d, s + t < s1 ? min(8, C - d) : 0, vec_z);
                 if (!DB && p.dropping) z = dropped<T>(p.drop, row, d, z);
-                *reinterpret_cast<Frag<T>*>(sz + t * LC + 8 * (e & 15)) = z;
+                Tile<T, 128>::put8(sz, t, e & 15, z);
             }
             if (tid < 32 * 4) {
                 const int t = tid >> 2, d = m0 + 8 * (tid & 3), row = s + t < s1 ? p.perm[s + t] : 0;
                 const float* q = base + static_cast<long>(row) * p.R + (d < cols ? d : 0);
                 const Terms<T, 3> v(load8(q, s + t < s1 ? min(8, cols - d) : 0, false));
 #pragma unroll
-                for (int x = 0; x < NTERM; ++x) *reinterpret_cast<Frag<T>*>(sp[x] + t * LP + 8 * (tid & 3)) = v.t[x];
+                for (int x = 0; x < NTERM; ++x) Tile<T, 64>::put8(sp[x], t, tid & 3, v.t[x]);
             }
             __syncthreads();
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
-                const Frag<T> z = lds_cols(sz, LC, 0, 32 * wave, k);
+                const Frag<T> z = lds_cols<128, false>(sz, 16 * k, 32 * wave);
 #pragma unroll
-                for (int x = 0; x < NTERM; ++x) acc = mma32(lds_cols(sp[x], LP, 0, 0, k), z, acc);
+                for (int x = 0; x < NTERM; ++x) acc = mma32(lds_cols<64, false>(sp[x], 16 * k, 0), z, acc);
             }
             __syncthreads();
         }

@@ -1,0 +1,212 @@
+// What the attention kernels of both directions share: the documents, the
+// score's formula, and the checks and layouts of their arguments.
+#pragma once
+
+#include <climits>
+#include <cmath>
+#include <memory>
+#include <type_traits>
+
+#include "kdec_frag.hpp"
+#include "kdec_internal.hpp"
+
+namespace kdec {
+namespace attn {
+
+constexpr int AT = 256;  // threads of a block
+constexpr int BM = 128;  // entries or keys that a block holds, 32 per wave
+constexpr int BN = 64;   // keys or rows of a tile that it walks
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr float LN2 = 0.6931471805599453f;
+constexpr float INF = __builtin_inff();
+
+// Keeps the operand reads of later products behind this one: a float product
+// takes eight matrix instructions, which cover the next read, and its operands
+// twice the registers, which more reads ahead would not leave.
+template <class T>
+__device__ inline void hold() {
+    if (sizeof(T) == 4) __builtin_amdgcn_sched_barrier(0);
+}
+
+struct Docs {
+    const int *q_off, *k_off, *k_len, *prefix;
+    int docs, causal, Tq, Tk;
+};
+
+struct Heads {  // a (rows, heads, D) tensor
+    const void* p;
+    long rs, hs;
+};
+
+struct Args {
+    Heads Q, K, V;
+    Docs m;
+    const float* slopes;
+    float scale, cap;
+    int Hq, Hkv, G, D, E;  // G = Hq / Hkv, E = Tq * G entries per key head
+};
+
+struct Row {
+    int lo, hi, pos;  // keys [lo, hi), the key row at the row's own position
+};
+
+// The last document whose offset is not past i, or -1.
+__device__ inline int doc_of(const int* off, int docs, int i) {
+    int a = 0, b = docs;
+    while (a < b) {
+        const int mid = (a + b) >> 1;
+        if (off[mid] <= i) a = mid + 1;
+        else b = mid;
+    }
+    return a - 1;
+}
+
+struct Doc {
+    int q0, lq, k0, lk, prefix;
+};
+__device__ inline Doc doc_at(const Docs& m, int d) {
+    Doc r;
+    r.q0 = min(max(m.q_off[d], 0), m.Tq);
+    r.lq = max(min(m.q_off[d + 1], m.Tq) - r.q0, 0);
+    r.k0 = min(max(m.k_off[d], 0), m.Tk);
+    const int slot = max(min(m.k_off[d + 1], m.Tk) - r.k0, 0);
+    r.lk = m.k_len ? min(max(m.k_len[d], 0), slot) : slot;
+    r.prefix = m.prefix ? min(max(m.prefix[d], 0), r.lk) : 0;
+    return r;
+}
+
+__device__ inline Row row_at(const Docs& m, int i) {
+    Row r{INT_MAX, INT_MIN, 0};
+    const int d = doc_of(m.q_off, m.docs, i);
+    if (d < 0 || i >= m.q_off[d + 1]) return r;
+    const Doc c = doc_at(m, d);
+    const int p = i - c.q0 + c.lk - c.lq;  // position of its last key
+    const int n = m.causal ? min(max(max(p + 1, c.prefix), 0), c.lk) : c.lk;
+    if (n <= 0) return r;
+    r.lo = c.k0;
+    r.hi = c.k0 + n;
+    r.pos = c.k0 + p;
+    return r;
+}
+
+// Scores in log2 units from raw products. T says how exact the cap's tanh has
+// to be: 1 - 2 / (1 + e^2x) is off by 2^-24 absolutely, which a bf16 score
+// cannot show; for float the odd series takes over near zero (its next term,
+// 62/2835 x^9, is below 2^-25 of x up to 0.15).
+template <class T, bool CAP, bool BIAS>
+struct Score {
+    float unit;   // product to log2 units
+    float k, c2;  // cap: tanh's argument is s k / (2 log2 e), the score c2 tanh
+    float slope;  // bias per step of distance, log2 units
+    __device__ inline Score(const Args& a, int head) {
+        unit = a.scale * LOG2E;
+        k = CAP ? 2.0f * LOG2E * a.scale / a.cap : 0.0f;
+        c2 = a.cap * LOG2E;
+        slope = BIAS ? a.slopes[head] * LOG2E : 0.0f;
+    }
+    __device__ inline float tanh_(float s) const {
+        const float x2 = s * k;
+        float th = __builtin_fmaf(-2.0f, __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x2)), 1.0f);
+        if (sizeof(T) == 4) {
+            const float x = x2 * (0.5f / LOG2E), q = x * x;
+            const float near = x * (1.0f + q * (-1.0f / 3 + q * (2.0f / 15 + q * (-17.0f / 315))));
+            th = __builtin_fabsf(x) < 0.15f ? near : th;
+        }
+        return th;
+    }
+    // dist = position - key, dt: the score's derivative by scale * product
+    __device__ inline float of(float s, float dist, float& dt) const {
+        float t;
+        dt = 1.0f;
+        if (CAP) {
+            const float th = tanh_(s);
+            dt = __builtin_fmaf(-th, th, 1.0f);
+            t = c2 * th;
+            if (BIAS) t = __builtin_fmaf(-slope, __builtin_fabsf(dist), t);
+        } else {
+            t = s * unit;
+            if (BIAS) t = __builtin_fmaf(s, unit, -slope * __builtin_fabsf(dist));
+        }
+        return t;
+    }
+};
+
+// A probability formed again from a raw product and the row's lse in log2
+// units; dt is the score's derivative by scale * product.
+template <class T, bool CAP, bool BIAS>
+__device__ inline float grad_p(const Score<T, CAP, BIAS>& rule, float s, float dist, float lse2, float& dt) {
+    if (!CAP && !BIAS) {
+        dt = 1.0f;
+        return __builtin_amdgcn_exp2f(__builtin_fmaf(s, rule.unit, -lse2));
+    }
+    return __builtin_amdgcn_exp2f(rule.of(s, dist, dt) - lse2);
+}
+
+// ─── host ───
+
+// Kernels of a call by its type, width and score: L::run<T, DP, CAP, BIAS>.
+template <class L, class T, int DP, class... P>
+int by_score(bool cap, bool bias, P&&... p) {
+    if (cap) return bias ? L::template run<T, DP, true, true>(p...) : L::template run<T, DP, true, false>(p...);
+    return bias ? L::template run<T, DP, false, true>(p...) : L::template run<T, DP, false, false>(p...);
+}
+template <class L, class... P>
+int dispatch(int dtype, int D, bool cap, bool bias, P&&... p) {
+    if (dtype == KDEC_F32) return D <= 64 ? by_score<L, float, 64>(cap, bias, p...) : by_score<L, float, 128>(cap, bias, p...);
+    return D <= 64 ? by_score<L, bf16, 64>(cap, bias, p...) : by_score<L, bf16, 128>(cap, bias, p...);
+}
+
+inline int check(kdec_ctx* ctx, const char* who, int dtype, const void* q_off, const void* k_off, int docs, float scale,
+                 float cap, int Tq, int Tk, int Hq, int Hkv, int D) {
+    const auto bad = [&](const char* why) { return fail(ctx, KDEC_EINVAL, std::string(who) + ": " + why); };
+    if (dtype != KDEC_F32 && dtype != KDEC_BF16) return bad("unknown type");
+    if (Tq < 0 || Tk < 0 || docs < 0) return bad("negative size");
+    if (Hq <= 0 || Hkv <= 0 || Hq % Hkv) return bad("query heads are not a multiple of the key heads");
+    if (D <= 0 || D > 128) return bad("head width outside 1..128");
+    if (static_cast<long>(Tq) * Hq >= INT_MAX - BM || static_cast<long>(Tk) >= INT_MAX - BM) return bad("too many rows");
+    if (!(scale > 0.0f) || !(scale < HUGE_VALF)) return bad("scale must be positive");
+    if (!(cap >= 0.0f) || !(cap < HUGE_VALF)) return bad("cap must be at least 0");
+    if (docs > 0 && (!q_off || !k_off)) return bad("null offsets");
+    return KDEC_OK;
+}
+
+// Whether a tensor's rows and heads start on multiples of `to` bytes.
+inline bool aligned(const Heads& h, size_t size, size_t to) {
+    return reinterpret_cast<size_t>(h.p) % to == 0 && (h.rs * size) % to == 0 && (h.hs * size) % to == 0;
+}
+// Whether the kernels' loads take a tensor as it stands: 16 bytes at a time,
+// a tile's offsets below 2^30 bytes.
+inline bool plain(const Heads& h, int D, size_t size) {
+    return D % 8 == 0 && aligned(h, size, 16) && (BM * h.rs + D) * static_cast<long>(size) < (1L << 30) && h.rs >= 0;
+}
+
+// Copies a tensor that they do not take into aligned rows, padded to a
+// multiple of 8 columns. The kernels then run on the copy with D8 columns.
+template <class T>
+__global__ __launch_bounds__(AT) void pack_k(Heads h, T* out, long n, int heads, int D, int D8) {
+    for (long e = static_cast<long>(blockIdx.x) * AT + threadIdx.x; e < n; e += static_cast<long>(gridDim.x) * AT) {
+        const long r = e / D8;
+        const int d = static_cast<int>(e - r * D8);
+        const long row = r / heads;
+        out[e] = d < D ? static_cast<const T*>(h.p)[row * h.rs + (r - row * heads) * h.hs + d] : static_cast<T>(0.0f);
+    }
+}
+inline int pack(kdec_ctx* ctx, int dtype, Heads& h, int rows, int heads, int D, std::unique_ptr<Workspace>& ws) {
+    const int D8 = (D + 7) & ~7;
+    const long n = static_cast<long>(rows) * heads * D8;
+    if (n == 0) return KDEC_OK;
+    ws = std::make_unique<Workspace>(ctx, n * (dtype == KDEC_F32 ? 4 : 2));
+    if (!ws->p) return KDEC_ENOMEM;
+    const long blocks = cdiv(n, AT) < 16L * ctx->num_cus ? cdiv(n, AT) : 16L * ctx->num_cus;
+    if (dtype == KDEC_F32)
+        hipLaunchKernelGGL(pack_k<float>, dim3(static_cast<unsigned>(blocks)), dim3(AT), 0, ctx->stream, h, ws->as<float>(), n, heads,
+                           D, D8);
+    else
+        hipLaunchKernelGGL(pack_k<bf16>, dim3(static_cast<unsigned>(blocks)), dim3(AT), 0, ctx->stream, h, ws->as<bf16>(), n, heads, D,
+                           D8);
+    h = Heads{ws->p, static_cast<long>(heads) * D8, D8};
+    return KDEC_OK;
+}
+
+}  // namespace attn
+}  // namespace kdec

@@ -1,0 +1,522 @@
+// Attention of packed documents on gfx950, backward.
+//
+// With P = exp(s - lse) formed again from the products and the forward's lse,
+// delta = dO . O and dS = P (dO V^T - delta) (times the cap's derivative):
+//   dQ = scale dS K,  dK = scale dS^T Q,  dV = P^T dO.
+// Two walks rather than one: dQ sums over a row's keys and is a walk over the
+// keys as the forward is, dK and dV sum over a key's rows and heads and are a
+// walk over those. Each then has one owner per result, which no other block
+// adds to: five products would do for seven, but the sums would be made by
+// atomics in an order that changes from call to call.
+//
+// P and dS are rounded to the tensors' type for the products they enter.
+#include "kdec_attn.hpp"
+
+namespace kdec {
+namespace attn {
+namespace {
+
+struct Bwd {
+    Args a;
+    Heads O, dO;
+    bool vec_o;  // O takes 16-byte loads
+    const float* lse;
+    int D_out;  // the gradients' width (a.D may be padded)
+    void *dQ, *dK, *dV;
+    long dq_rs, dq_hs, dk_rs, dk_hs, dv_rs, dv_hs;
+    bool vec_dq, vec_dk, vec_dv;
+    Row* rows;    // (Tq)
+    float2* stat; // (Hq, Tq): lse in log2 units, delta = dO . O
+    int parts;    // blocks that share a key tile's rows
+    float* part;  // (parts, Hkv, Tk, 2, D): their dK / scale and dV
+};
+
+// delta = dO . O and lse in log2 units of every row and head, and the rows'
+// keys. A row without keys gets lse = +inf, so that its probabilities are
+// zeros; one whose delta is not finite gets NaN, which then marks every
+// gradient that the row reaches. 16 lanes per row and head.
+template <class T>
+__global__ __launch_bounds__(AT) void attn_stat_k(Bwd b) {
+    const Args& a = b.a;
+    const int lane = threadIdx.x & 15;
+    const long w = static_cast<long>(blockIdx.x) * (AT / 16) + (threadIdx.x >> 4);
+    if (w >= static_cast<long>(a.m.Tq) * a.Hq) return;
+    const int row = static_cast<int>(w / a.Hq), head = static_cast<int>(w - static_cast<long>(row) * a.Hq);
+    const int d = 8 * lane;
+    const Frag<T> o = load8(static_cast<const T*>(b.O.p) + row * b.O.rs + head * b.O.hs + d, min(8, b.D_out - d), b.vec_o);
+    const Frag<T> g = load8(static_cast<const T*>(b.dO.p) + row * b.dO.rs + head * b.dO.hs + d, min(8, a.D - d), true);
+    float s = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) s += static_cast<float>(o[i]) * static_cast<float>(g[i]);
+    for (int x = 8; x; x >>= 1) s += __shfl_xor(s, x);
+    if (lane) return;
+    const float lse = b.lse[static_cast<long>(head) * a.m.Tq + row];
+    float l2 = lse == -INF ? INF : lse * LOG2E;
+    if (lse != -INF && !(__builtin_fabsf(s) < INF)) l2 = __builtin_nanf("");
+    b.stat[static_cast<long>(head) * a.m.Tq + row] = make_float2(l2, lse == -INF ? 0.0f : s);
+    if (head == 0) b.rows[row] = row_at(a.m, row);
+}
+
+// dQ: the forward's walk over the keys, with dQ^T = K^T dS^T in place of the
+// output.
+template <class T, int DP, bool CAP, bool BIAS>
+__global__ __launch_bounds__(AT, sizeof(T) == 2 ? 2 : 1) void attn_dq_k(Bwd b) {
+    constexpr int NC = DP / 16, ND = DP / 32;
+    __shared__ __align__(16) T sk0[BN * DP], sk1[BN * DP], sv0[BN * DP], sv1[BN * DP];
+    __shared__ int red[4][4];
+    const Args& a = b.a;
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, half = lane >> 5;
+    const int kvh = blockIdx.x % a.Hkv;
+    int tile = blockIdx.x / a.Hkv;
+    if (a.m.causal) tile = gridDim.x / a.Hkv - 1 - tile;  // the longest walks first
+    const int e = tile * BM + wave * 32 + (lane & 31);
+    const bool valid = e < a.E;
+    const int row = valid ? e / a.G : 0, head = kvh * a.G + (valid ? e - row * a.G : 0);
+    const Row me = valid ? b.rows[row] : Row{INT_MAX, INT_MIN, 0};
+    int lo = me.lo, hi = me.hi, full_lo = valid ? me.lo : INT_MIN, full_hi = valid ? me.hi : INT_MAX;
+    for (int o = 16; o; o >>= 1) {
+        lo = min(lo, __shfl_xor(lo, o));
+        hi = max(hi, __shfl_xor(hi, o));
+        full_lo = max(full_lo, __shfl_xor(full_lo, o));
+        full_hi = min(full_hi, __shfl_xor(full_hi, o));
+    }
+    if (lane == 0) {
+        red[wave][0] = lo;
+        red[wave][1] = hi;
+        red[wave][2] = full_lo;
+        red[wave][3] = full_hi;
+    }
+    const int wlo = __builtin_amdgcn_readfirstlane(lo), whi = __builtin_amdgcn_readfirstlane(hi);
+    __syncthreads();
+    const int blo = __builtin_amdgcn_readfirstlane(min(min(red[0][0], red[1][0]), min(red[2][0], red[3][0])));
+    const int bhi = __builtin_amdgcn_readfirstlane(max(max(red[0][1], red[1][1]), max(red[2][1], red[3][1])));
+    full_lo = __builtin_amdgcn_readfirstlane(max(max(red[0][2], red[1][2]), max(red[2][2], red[3][2])));
+    full_hi = __builtin_amdgcn_readfirstlane(min(min(red[0][3], red[1][3]), min(red[2][3], red[3][3])));
+    const int t1 = bhi > blo ? (bhi - blo + BN - 1) / BN : 0;
+
+    const Score<T, CAP, BIAS> rule(a, head);
+    const float2 stat = valid ? b.stat[static_cast<long>(head) * a.m.Tq + row] : make_float2(INF, 0.0f);
+    Frag<T> q[NC], g[NC];
+    const T* qp = static_cast<const T*>(a.Q.p) + row * a.Q.rs + head * a.Q.hs;
+    const T* gp = static_cast<const T*>(b.dO.p) + row * b.dO.rs + head * b.dO.hs;
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+        const int d = 16 * c + 8 * half, n = valid ? min(8, a.D - d) : 0;
+        q[c] = load8(qp + d, n, true);
+        g[c] = load8(gp + d, n, true);
+    }
+    const T* kb = static_cast<const T*>(a.K.p) + kvh * a.K.hs;
+    const T* vb = static_cast<const T*>(a.V.p) + kvh * a.V.hs;
+    Copy<T, DP, BN, AT> ks, vs;
+    ks.init(a.K.rs, a.D, tid);
+    vs.init(a.V.rs, a.D, tid);
+    const auto load = [&](int t, T* tk, T* tv) __attribute__((always_inline)) {
+        const int j = blo + t * BN;
+        ks.load(tk, kb + j * a.K.rs, a.K.rs, bhi - j, a.D, wave);
+        vs.load(tv, vb + j * a.V.rs, a.V.rs, bhi - j, a.D, wave);
+    };
+    // Tiles [0, f0) and [f1, t1) are masked, as in the forward.
+    int f0 = 0, f1 = 0;
+    if (full_hi > full_lo && full_lo <= bhi) {
+        f0 = min(max((full_lo - blo + BN - 1) / BN, 0), t1);
+        f0 = min(f0 + (f0 & 1), t1);
+        f1 = min(max((full_hi - blo) / BN, f0), t1);
+        f1 -= (f1 - f0) & 1;
+    }
+    if (f0 >= f1) f0 = f1 = 0;
+    const auto landed = [&](int t, T* tk) __attribute__((always_inline)) {
+        __builtin_amdgcn_s_waitcnt(0);
+        if (t < f0 || t >= f1) ks.clean(tk, tid, [](int) {});  // a zero of dS times such a key
+    };
+    f32x16 acc[ND];
+#pragma unroll
+    for (int d = 0; d < ND; ++d) acc[d] = f32x16{};
+    const auto step = [&](auto masked, int j0, const T* tk, const T* tv) __attribute__((always_inline)) {
+        const unsigned at = static_cast<unsigned>(j0 + 4 * half - me.lo);
+        const unsigned len = me.hi > me.lo ? static_cast<unsigned>(me.hi - me.lo) : 0u;
+        const float dist = static_cast<float>(me.pos - j0 - 4 * half);
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+            f32x16 s = f32x16{}, dp = f32x16{};
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+                s = mma32(lds_rows<T, DP>(tk, 32 * n, c), q[c], s);
+                hold<T>();
+                dp = mma32(lds_rows<T, DP>(tv, 32 * n, c), g[c], dp);
+                hold<T>();
+            }
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const int k = 32 * n + acc_row(r, 0);
+                float dt;
+                float p = grad_p(rule, s[r], dist - static_cast<float>(k), stat.x, dt);
+                p *= (dp[r] - stat.y) * dt;
+                if (decltype(masked)::value) p = at + static_cast<unsigned>(k) < len ? p : 0.0f;
+                s[r] = p;
+            }
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                const Frag<T> ds = acc_frag<T>(s, c);
+#pragma unroll
+                for (int d = 0; d < ND; ++d) {
+                    acc[d] = mma32(lds_cols<DP, true>(tk, 32 * n + 16 * c, 32 * d), ds, acc[d]);
+                    hold<T>();
+                }
+            }
+        }
+    };
+    const auto walk = [&](auto masked, int t, const T* tk, const T* tv, T* nk, T* nv) __attribute__((always_inline)) {
+        const int j0 = blo + t * BN;
+        if (t + 1 < t1) load(t + 1, nk, nv);
+        if (!decltype(masked)::value || (wlo < j0 + BN && whi > j0)) step(masked, j0, tk, tv);
+        if (t + 1 < t1) landed(t + 1, nk);
+        __syncthreads();
+    };
+    const auto walks = [&](auto masked, int from, int to) __attribute__((always_inline)) {
+        for (int t = from; t < to; t += 2) {
+            walk(masked, t, sk0, sv0, sk1, sv1);
+            if (t + 1 < to) walk(masked, t + 1, sk1, sv1, sk0, sv0);
+        }
+    };
+    if (t1 > 0) {
+        load(0, sk0, sv0);
+        landed(0, sk0);
+        __syncthreads();
+    }
+    walks(std::true_type{}, 0, f0);
+    walks(std::false_type{}, f0, f1);
+    walks(std::true_type{}, f1, t1);
+    if (!valid) return;
+    T* o = static_cast<T*>(b.dQ) + row * b.dq_rs + head * b.dq_hs;
+#pragma unroll
+    for (int dt = 0; dt < ND; ++dt)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+            const int d = 32 * dt + 8 * x + 4 * half;
+            store4(o + d, b.D_out - d, b.vec_dq, acc[dt][4 * x] * a.scale, acc[dt][4 * x + 1] * a.scale,
+                   acc[dt][4 * x + 2] * a.scale, acc[dt][4 * x + 3] * a.scale);
+        }
+}
+
+// dK and dV: a block holds 128 keys of one key head (32 per wave, keys and
+// values in registers) and walks the rows that see them, head by head of the
+// group, in tiles of 64 whose queries and output gradients are staged in
+// shared memory, two buffers deep and two tiles a turn. All heads of the group
+// belong to the same walk, so the sums over shared heads need no joining;
+// where the key tiles alone do not fill the device, `parts` blocks share a
+// walk and attn_dkv_join_k adds their sums. Scores are S = Q K^T here, a lane
+// holding one key's column.
+template <class T, int DP, bool CAP, bool BIAS>
+__global__ __launch_bounds__(AT, DP == 64 && sizeof(T) == 2 ? 2 : 1) void attn_dkv_k(Bwd b) {
+    constexpr int NC = DP / 16, ND = DP / 32, BE = 64, PAIR = 2 * BE;
+    __shared__ __align__(16) T sq0[BE * DP], sq1[BE * DP], sg0[BE * DP], sg1[BE * DP];
+    __shared__ __align__(16) float slse[2][BE], sdelta[2][BE];
+    __shared__ __align__(16) int slo[2][BE], shi[2][BE], spos[2][BE];
+    const Args& a = b.a;
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, half = lane >> 5;
+    const int kvh = blockIdx.x % a.Hkv, j0 = (blockIdx.x / a.Hkv) * BM, part = blockIdx.y;
+    const int wkey = j0 + wave * 32, key = wkey + (lane & 31);
+    const bool valid = key < a.m.Tk;
+
+    // the rows [e0, e1) that may see keys of the block, and those [f0, f1)
+    // that all see all of them
+    int e0 = 0, e1 = 0, f0 = 0, f1 = 0;
+    {
+        const int d0 = max(doc_of(a.m.k_off, a.m.docs, j0), 0);
+        const int d1 = doc_of(a.m.k_off, a.m.docs, min(j0 + BM, a.m.Tk) - 1);
+        if (d1 >= 0) {
+            const Doc c = doc_at(a.m, d0), z = doc_at(a.m, d1);
+            const int skip = c.lk - c.lq;  // position of the first row's key
+            e0 = c.q0;
+            if (a.m.causal && j0 - c.k0 >= c.prefix) e0 = min(max(c.q0 + (j0 - c.k0) - skip, c.q0), c.q0 + c.lq);
+            e1 = z.q0 + z.lq;
+            if (d0 == d1 && j0 >= c.k0 && j0 + BM <= c.k0 + c.lk) {
+                f0 = c.q0;
+                if (a.m.causal && j0 + BM - c.k0 > c.prefix)
+                    f0 = min(max(c.q0 + (j0 + BM - 1 - c.k0) - skip, c.q0), c.q0 + c.lq);
+                f1 = c.q0 + c.lq;
+            }
+        }
+        e0 = __builtin_amdgcn_readfirstlane(e0);
+        e1 = __builtin_amdgcn_readfirstlane(e1);
+        f0 = __builtin_amdgcn_readfirstlane(f0);
+        f1 = __builtin_amdgcn_readfirstlane(f1);
+    }
+    // Turns of two tiles, the group's heads one after another; of a head's
+    // `per` turns, [p0, p1) are seen whole.
+    const int per = e1 > e0 ? (e1 - e0 + PAIR - 1) / PAIR : 0;
+    int p0 = 0, p1 = 0;
+    if (f1 > f0) {
+        p0 = max((f0 - e0 + PAIR - 1) / PAIR, 0);
+        p1 = min((f1 - e0) / PAIR, per);
+        if (p0 >= p1) p0 = p1 = 0;
+    }
+    const long turns = static_cast<long>(per) * a.G;
+    const int u0 = static_cast<int>(turns * part / b.parts), u1 = static_cast<int>(turns * (part + 1) / b.parts);
+
+    Frag<T> k[NC], v[NC];
+    const T* kp = static_cast<const T*>(a.K.p) + kvh * a.K.hs + static_cast<long>(valid ? key : 0) * a.K.rs;
+    const T* vp = static_cast<const T*>(a.V.p) + kvh * a.V.hs + static_cast<long>(valid ? key : 0) * a.V.rs;
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+        const int d = 16 * c + 8 * half, n = valid ? min(8, a.D - d) : 0;
+        k[c] = load8(kp + d, n, true);
+        v[c] = load8(vp + d, n, true);
+    }
+    Copy<T, DP, BE, AT> qs, gs;
+    qs.init(a.Q.rs, a.D, tid);
+    gs.init(b.dO.rs, a.D, tid);
+    int left = 2 * (u1 - u0), lg = 0, li = 0;  // tiles to load; the next one's head and place
+    if (left) {
+        lg = u0 / per;
+        li = 2 * (u0 - lg * per);
+    }
+    float2 r_stat = make_float2(0.0f, 0.0f);
+    Row r_row{0, 0, 0};
+    bool l_masked = true;  // of the tile last asked for
+    const auto load = [&](T* tq, T* tg) __attribute__((always_inline)) {
+        const int head = kvh * a.G + lg, r = e0 + li * BE;
+        qs.load(tq, static_cast<const T*>(a.Q.p) + head * a.Q.hs + r * a.Q.rs, a.Q.rs, e1 - r, a.D, wave);
+        gs.load(tg, static_cast<const T*>(b.dO.p) + head * b.dO.hs + r * b.dO.rs, b.dO.rs, e1 - r, a.D, wave);
+        if (tid < BE) {
+            r_stat = make_float2(INF, 0.0f);
+            r_row = Row{INT_MAX, INT_MIN, 0};
+            if (r + tid < e1) {
+                r_stat = b.stat[static_cast<long>(head) * a.m.Tq + r + tid];
+                r_row = b.rows[r + tid];
+            }
+        }
+        l_masked = (li >> 1) < p0 || (li >> 1) >= p1;
+        --left;
+        if (++li == 2 * per) {
+            li = 0;
+            ++lg;
+        }
+    };
+    const auto landed = [&](T* tq, T* tg, int buf) __attribute__((always_inline)) {
+        __builtin_amdgcn_s_waitcnt(0);
+        if (tid < BE) {
+            slse[buf][tid] = r_stat.x;
+            sdelta[buf][tid] = r_stat.y;
+            slo[buf][tid] = r_row.lo;
+            shi[buf][tid] = r_row.hi;
+            spos[buf][tid] = r_row.pos;
+        }
+        if (l_masked) {
+            qs.clean(tq, tid, [](int) {});
+            gs.clean(tg, tid, [](int) {});
+        }
+    };
+    f32x16 dk[ND], dv[ND];
+#pragma unroll
+    for (int d = 0; d < ND; ++d) dk[d] = dv[d] = f32x16{};
+    const auto step = [&](auto masked, const Score<T, CAP, BIAS>& rule, const T* tq, const T* tg, int buf)
+        __attribute__((always_inline)) {
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+            if (decltype(masked)::value) {  // rows of 32 that see none of the wave's keys
+                const int i = 32 * n + (lane & 31);
+                if (!__builtin_amdgcn_ballot_w64(slo[buf][i] < wkey + 32 && shi[buf][i] > wkey)) continue;
+            }
+            f32x16 s = f32x16{}, dp = f32x16{}, p;
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+                s = mma32(lds_rows<T, DP>(tq, 32 * n, c), k[c], s);
+                hold<T>();
+                dp = mma32(lds_rows<T, DP>(tg, 32 * n, c), v[c], dp);
+                hold<T>();
+            }
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const int i0 = 32 * n + 8 * q + 4 * half;
+                const f32x4 lse = *reinterpret_cast<const f32x4*>(&slse[buf][i0]);
+                const f32x4 delta = *reinterpret_cast<const f32x4*>(&sdelta[buf][i0]);
+#pragma unroll
+                for (int x = 0; x < 4; ++x) {
+                    const int r = 4 * q + x, i = i0 + x;
+                    float dt;
+                    float pr = grad_p(rule, s[r], BIAS ? static_cast<float>(spos[buf][i] - key) : 0.0f, lse[x], dt);
+                    float ds = pr * (dp[r] - delta[x]) * dt;
+                    if (decltype(masked)::value) {
+                        const bool seen = key >= slo[buf][i] && key < shi[buf][i];
+                        pr = seen ? pr : 0.0f;
+                        ds = seen ? ds : 0.0f;
+                    }
+                    p[r] = pr;
+                    s[r] = ds;
+                }
+                hold<T>();
+            }
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                const Frag<T> pf = acc_frag<T>(p, c), ds = acc_frag<T>(s, c);
+#pragma unroll
+                for (int d = 0; d < ND; ++d) {
+                    dv[d] = mma32(lds_cols<DP, true>(tg, 32 * n + 16 * c, 32 * d), pf, dv[d]);
+                    hold<T>();
+                    dk[d] = mma32(lds_cols<DP, true>(tq, 32 * n + 16 * c, 32 * d), ds, dk[d]);
+                    hold<T>();
+                }
+            }
+        }
+    };
+    const auto walks = [&](auto masked, const Score<T, CAP, BIAS>& rule, int from, int to) __attribute__((always_inline)) {
+        for (int i = from; i < to; ++i) {
+            load(sq1, sg1);
+            step(masked, rule, sq0, sg0, 0);
+            landed(sq1, sg1, 1);
+            __syncthreads();
+            const bool more = left > 0;
+            if (more) load(sq0, sg0);
+            step(masked, rule, sq1, sg1, 1);
+            if (more) landed(sq0, sg0, 0);
+            __syncthreads();
+        }
+    };
+    if (left) {
+        load(sq0, sg0);
+        landed(sq0, sg0, 0);
+        __syncthreads();
+        for (int u = u0; u < u1;) {
+            const int g = u / per, i0 = u - g * per, i1 = min(per, i0 + u1 - u);
+            const Score<T, CAP, BIAS> rule(a, kvh * a.G + g);
+            walks(std::true_type{}, rule, i0, min(p0, i1));
+            walks(std::false_type{}, rule, max(i0, p0), min(p1, i1));
+            walks(std::true_type{}, rule, max(i0, p1), i1);
+            u += i1 - i0;
+        }
+    }
+    if (!valid) return;
+    if (b.parts > 1) {
+        float* o = b.part + ((static_cast<long>(part) * a.Hkv + kvh) * a.m.Tk + key) * 2 * a.D;
+#pragma unroll
+        for (int dt = 0; dt < ND; ++dt)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const int d = 32 * dt + 8 * q + 4 * half;
+                store4(o + d, a.D - d, true, dk[dt][4 * q], dk[dt][4 * q + 1], dk[dt][4 * q + 2], dk[dt][4 * q + 3]);
+                store4(o + a.D + d, a.D - d, true, dv[dt][4 * q], dv[dt][4 * q + 1], dv[dt][4 * q + 2], dv[dt][4 * q + 3]);
+            }
+        return;
+    }
+    T* ok = static_cast<T*>(b.dK) + kvh * b.dk_hs + key * b.dk_rs;
+    T* ov = static_cast<T*>(b.dV) + kvh * b.dv_hs + key * b.dv_rs;
+#pragma unroll
+    for (int dt = 0; dt < ND; ++dt)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const int d = 32 * dt + 8 * q + 4 * half;
+            store4(ok + d, b.D_out - d, b.vec_dk, dk[dt][4 * q] * a.scale, dk[dt][4 * q + 1] * a.scale,
+                   dk[dt][4 * q + 2] * a.scale, dk[dt][4 * q + 3] * a.scale);
+            store4(ov + d, b.D_out - d, b.vec_dv, dv[dt][4 * q], dv[dt][4 * q + 1], dv[dt][4 * q + 2], dv[dt][4 * q + 3]);
+        }
+}
+
+// The parts' dK and dV added in their order, four columns a thread.
+template <class T>
+__global__ __launch_bounds__(AT) void attn_dkv_join_k(Bwd b) {
+    const Args& a = b.a;
+    const long n = static_cast<long>(a.Hkv) * a.m.Tk * 2 * a.D;
+    const long e = 4 * (static_cast<long>(blockIdx.x) * AT + threadIdx.x);
+    if (e >= n) return;
+    f32x4 s = f32x4{};
+    for (int i = 0; i < b.parts; ++i) s += *reinterpret_cast<const f32x4*>(b.part + i * n + e);
+    const long r = e / (2 * a.D);
+    int d = static_cast<int>(e - r * 2 * a.D);
+    const long kvh = r / a.m.Tk, key = r - kvh * a.m.Tk;
+    if (d < a.D) {
+        store4(static_cast<T*>(b.dK) + kvh * b.dk_hs + key * b.dk_rs + d, b.D_out - d, b.vec_dk, s[0] * a.scale, s[1] * a.scale,
+               s[2] * a.scale, s[3] * a.scale);
+    } else {
+        d -= a.D;
+        store4(static_cast<T*>(b.dV) + kvh * b.dv_hs + key * b.dv_rs + d, b.D_out - d, b.vec_dv, s[0], s[1], s[2], s[3]);
+    }
+}
+
+struct Launch {
+    template <class T, int DP, bool CAP, bool BIAS>
+    static int run(kdec_ctx* ctx, const Bwd& b, long q_blocks, long k_blocks, size_t part_n) {
+        const auto blocks = [](long n) { return dim3(static_cast<unsigned>(n)); };
+        if (b.a.m.Tq > 0) {
+            hipLaunchKernelGGL(attn_stat_k<T>, blocks(cdiv(static_cast<long>(b.a.m.Tq) * b.a.Hq, AT / 16)), dim3(AT), 0, ctx->stream, b);
+            hipLaunchKernelGGL((attn_dq_k<T, DP, CAP, BIAS>), blocks(q_blocks), dim3(AT), 0, ctx->stream, b);
+        }
+        if (b.a.m.Tk > 0) {
+            hipLaunchKernelGGL((attn_dkv_k<T, DP, CAP, BIAS>), dim3(static_cast<unsigned>(k_blocks), static_cast<unsigned>(b.parts)),
+                               dim3(AT), 0, ctx->stream, b);
+            if (b.parts > 1)
+                hipLaunchKernelGGL(attn_dkv_join_k<T>, blocks(cdiv(part_n / 4, AT)), dim3(AT), 0, ctx->stream, b);
+        }
+        return launch_check(ctx, "kdec_attn_bwd");
+    }
+};
+
+}  // namespace
+}  // namespace attn
+}  // namespace kdec
+
+using namespace kdec;
+using namespace kdec::attn;
+
+extern "C" int kdec_attn_bwd(kdec_ctx* ctx, int dtype, const void* Q, long q_rs, long q_hs, const void* K, long k_rs,
+                             long k_hs, const void* V, long v_rs, long v_hs, const void* O, long o_rs, long o_hs,
+                             const float* lse, const void* dO, long do_rs, long do_hs, const int* q_off, const int* k_off,
+                             const int* k_len, const int* prefix, int docs, int causal, const float* slopes, float scale,
+                             float cap, int Tq, int Tk, int Hq, int Hkv, int D, void* dQ, long dq_rs, long dq_hs, void* dK,
+                             long dk_rs, long dk_hs, void* dV, long dv_rs, long dv_hs) {
+    if (!ctx) return KDEC_EINVAL;
+    if (int rc = check(ctx, "kdec_attn_bwd", dtype, q_off, k_off, docs, scale, cap, Tq, Tk, Hq, Hkv, D)) return rc;
+    KDEC_CHECK(ctx, (Tq == 0 || (Q && O && lse && dO && dQ)) && (Tk == 0 || (K && V && dK && dV)),
+               "kdec_attn_bwd: null tensor");
+    if (Tq == 0 && Tk == 0) return KDEC_OK;
+    const size_t size = dtype == KDEC_F32 ? 4 : 2;
+    const int G = Hq / Hkv;
+    ProfScope ps(ctx, "attn", 0.0, 0.0);
+    Bwd b{};
+    b.a = Args{{Q, q_rs, q_hs}, {K, k_rs, k_hs}, {V, v_rs, v_hs}, {q_off, k_off, k_len, prefix, docs, causal != 0, Tq, Tk},
+               slopes, scale, cap, Hq, Hkv, G, D, Tq * G};
+    b.O = Heads{O, o_rs, o_hs};
+    b.dO = Heads{dO, do_rs, do_hs};
+    b.vec_o = plain(b.O, D, size);
+    std::unique_ptr<Workspace> packed[4];
+    if (!plain(b.a.Q, D, size) || !plain(b.a.K, D, size) || !plain(b.a.V, D, size) || !plain(b.dO, D, size)) {
+        if (int rc = pack(ctx, dtype, b.a.Q, Tq, Hq, D, packed[0])) return rc;
+        if (int rc = pack(ctx, dtype, b.a.K, Tk, Hkv, D, packed[1])) return rc;
+        if (int rc = pack(ctx, dtype, b.a.V, Tk, Hkv, D, packed[2])) return rc;
+        if (int rc = pack(ctx, dtype, b.dO, Tq, Hq, D, packed[3])) return rc;
+        b.a.D = (D + 7) & ~7;
+    }
+    b.lse = lse;
+    b.D_out = D;
+    b.dQ = dQ;
+    b.dK = dK;
+    b.dV = dV;
+    b.dq_rs = dq_rs;
+    b.dq_hs = dq_hs;
+    b.dk_rs = dk_rs;
+    b.dk_hs = dk_hs;
+    b.dv_rs = dv_rs;
+    b.dv_hs = dv_hs;
+    b.vec_dq = D % 4 == 0 && aligned(Heads{dQ, dq_rs, dq_hs}, size, 4 * size);
+    b.vec_dk = D % 4 == 0 && aligned(Heads{dK, dk_rs, dk_hs}, size, 4 * size);
+    b.vec_dv = D % 4 == 0 && aligned(Heads{dV, dv_rs, dv_hs}, size, 4 * size);
+    const size_t stat_bytes = (static_cast<size_t>(Tq) * Hq * sizeof(float2) + 255) & ~size_t(255);
+    const long q_blocks = cdiv(b.a.E, BM) * Hkv, k_blocks = cdiv(Tk, BM) * Hkv;
+    KDEC_CHECK(ctx, k_blocks < INT_MAX, "kdec_attn_bwd: too many keys");
+    // Key tiles too few to fill the device (causal walks differ in length, so
+    // two blocks per CU) share their rows among parts of no fewer than four
+    // turns of 128 rows.
+    const long turns = docs > 0 ? cdiv(Tq / docs, 128) * G : 1;
+    long parts = k_blocks > 0 ? cdiv(2L * ctx->num_cus, k_blocks) : 1;
+    if (parts > turns / 4) parts = turns / 4;
+    if (parts < 1) parts = 1;
+    b.parts = static_cast<int>(parts);
+    const size_t row_bytes = (static_cast<size_t>(Tq) * sizeof(Row) + 255) & ~size_t(255);
+    const size_t part_n = parts > 1 ? static_cast<size_t>(Hkv) * Tk * 2 * b.a.D : 0;
+    Workspace ws(ctx, stat_bytes + row_bytes + parts * part_n * sizeof(float));
+    if (!ws.p) return KDEC_ENOMEM;
+    b.stat = ws.as<float2>();
+    b.rows = reinterpret_cast<Row*>(ws.as<char>() + stat_bytes);
+    b.part = reinterpret_cast<float*>(ws.as<char>() + stat_bytes + row_bytes);
+    return dispatch<Launch>(dtype, D, cap > 0.0f, slopes != nullptr, ctx, b, q_blocks, k_blocks, part_n);
+}

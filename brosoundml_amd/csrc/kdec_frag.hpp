@@ -15,6 +15,8 @@
 
 #include <hip/hip_runtime.h>
 
+#include "kdec_buffer.hpp"
+
 namespace kdec {
 
 typedef __bf16 bf16;
@@ -76,50 +78,158 @@ __device__ inline f32x8 load8(const float* p, int n, bool vec) {
     return f;
 }
 
-// The depth-16 step c of a tile held row-major in shared memory (stride `ls`
-// elements) as an operand whose rows are the tile's rows row0 .. row0 + 31.
-template <class T>
-__device__ inline Frag<T> lds_rows(const T* tile, int ls, int row0, int c) {
+// A tile in shared memory: rows of DP elements in units of 16 bytes. It is
+// read two ways, a unit of each of 16 rows at once (lds_rows) and a stretch of
+// columns of 2 or 4 rows at once (lds_cols); either takes one cycle of the 64
+// banks only if the units fall on different banks. Rows are a multiple or an
+// even part of the banks, so the units of a row are permuted by an exclusive
+// or with bits of the row that set apart the rows of both reads. Float tiles
+// settle for two cycles and simpler addresses: their products take sixteen
+// times as long.
+template <class T, int DP>
+struct Tile {
+    static constexpr int U = 16 / static_cast<int>(sizeof(T)), NU = DP / U;
+    __device__ static inline int swz(int row) {
+        if (sizeof(T) == 2 && NU == 16) return (row & 3) << 2 | (row >> 2 & 3);
+        if (sizeof(T) == 2 && NU == 8) return (row >> 1 & 1) << 2 | (row >> 2 & 3);
+        if (sizeof(T) == 4) return NU == 8 ? row >> 1 & 7 : row & 7;
+        return 0;
+    }
+    __device__ static inline int at(int row, int unit) { return row * DP + U * (unit ^ swz(row)); }
+    // 8 elements from column 8 * chunk
+    __device__ static inline Frag<T> get8(const T* tile, int row, int chunk) {
+        if constexpr (sizeof(T) == 2) {
+            return *reinterpret_cast<const Frag<T>*>(tile + at(row, chunk));
+        } else {
+            const f32x4 a = *reinterpret_cast<const f32x4*>(tile + at(row, 2 * chunk));
+            const f32x4 b = *reinterpret_cast<const f32x4*>(tile + at(row, 2 * chunk + 1));
+            return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+        }
+    }
+    __device__ static inline void put8(T* tile, int row, int chunk, const Frag<T>& f) {
+        if constexpr (sizeof(T) == 2) {
+            *reinterpret_cast<Frag<T>*>(tile + at(row, chunk)) = f;
+        } else {
+            *reinterpret_cast<f32x4*>(tile + at(row, 2 * chunk)) = __builtin_shufflevector(f, f, 0, 1, 2, 3);
+            *reinterpret_cast<f32x4*>(tile + at(row, 2 * chunk + 1)) = __builtin_shufflevector(f, f, 4, 5, 6, 7);
+        }
+    }
+};
+
+// The depth-16 step c of a tile as an operand whose rows are the tile's rows
+// row0 .. row0 + 31, depth along the tile's columns.
+template <class T, int DP>
+__device__ inline Frag<T> lds_rows(const T* tile, int row0, int c) {
     const int l = threadIdx.x & 63;
-    return *reinterpret_cast<const Frag<T>*>(tile + (row0 + (l & 31)) * ls + 16 * c + 8 * (l >> 5));
+    return Tile<T, DP>::get8(tile, row0 + (l & 31), 2 * c + (l >> 5));
 }
 
-// The same tile transposed: an operand whose rows are the tile's columns
-// col0 .. col0 + 31 and whose depth slots are the rows of acc_frag(c) of the
-// 32-row block at row0. bf16 reads it with the transposing LDS read, which
-// hands lane i of 16 the column i of a 4 x 16 block whose row j the lanes
-// 4j .. 4j + 3 address.
-__device__ inline bf16x8 lds_cols(const bf16* tile, int ls, int row0, int col0, int c) {
+// A tile's columns col0 .. col0 + 31 as an operand's rows, depth along the 16
+// tile rows from row0, in the order of acc_frag's slots (ACC) or in their own.
+// bf16 reads it with the transposing LDS read, which hands lane i of 16 the
+// column i of a 4 x 16 block whose row j the lanes 4j .. 4j + 3 address.
+template <int DP, bool ACC>
+__device__ inline bf16x8 lds_cols(const bf16* tile, int row0, int col0) {
     typedef __attribute__((address_space(3))) short4v lds4;
     const int l = threadIdx.x & 63;
-    const bf16* p = tile + (row0 + 16 * c + 4 * (l >> 5) + ((l >> 2) & 3)) * ls + col0 + 16 * ((l >> 4) & 1) + 4 * (l & 3);
+    const int row = row0 + (ACC ? 4 : 8) * (l >> 5) + (l >> 2 & 3), col = col0 + 16 * (l >> 4 & 1) + 4 * (l & 3);
     union { short4v s[2]; bf16x8 v; } u;
-    u.s[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)p);
-    u.s[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(p + 8 * ls));
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+        u.s[i] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+            (lds4*)(tile + Tile<bf16, DP>::at(row + (ACC ? 8 : 4) * i, col >> 3) + (col & 7)));
     return u.v;
 }
-__device__ inline f32x8 lds_cols(const float* tile, int ls, int row0, int col0, int c) {
-    const int l = threadIdx.x & 63;
-    const float* p = tile + (row0 + 16 * c + 4 * (l >> 5)) * ls + col0 + (l & 31);
+template <int DP, bool ACC>
+__device__ inline f32x8 lds_cols(const float* tile, int row0, int col0) {
+    static_assert(DP >= 64, "the permutation below is that of these widths: the low three bits of the row");
+    const int l = threadIdx.x & 63, half = l >> 5;
     f32x8 f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = p[(8 * (i >> 2) + (i & 3)) * ls];
+    for (int i = 0; i < 8; ++i) {
+        const int r = ACC ? 8 * (i >> 2) + (i & 3) : i;  // row0 is a multiple of 16, col0 of 32
+        const int low = ACC ? 4 * half + (i & 3) : i;    // the row's low three bits
+        int at = (ACC ? 4 : 8) * half * DP + 4 * (((l & 31) >> 2) ^ low) + (l & 3);
+        asm("" : "+v"(at));  // one register for every tile row and column: the rest is the read's own offset
+        f[i] = tile[at + (row0 + r) * DP + col0];
+    }
     return f;
 }
 
-// lds_rows with the depth slots of acc_frag, the other operand of lds_cols.
-__device__ inline bf16x8 lds_rows_acc(const bf16* tile, int ls, int row0, int c) {
-    const int l = threadIdx.x & 63;
-    const bf16* p = tile + (row0 + (l & 31)) * ls + 16 * c + 4 * (l >> 5);
-    const bf16x4 a = *reinterpret_cast<const bf16x4*>(p), b = *reinterpret_cast<const bf16x4*>(p + 8);
+// Bounds-checked loads of a tensor's rows: of `rows` rows (any number) from a
+// wave-uniform base, each D columns; what lies past them is zeros. kFar is an
+// offset past every descriptor's end (all are below 2^30 bytes).
+constexpr int kFar = 0x60000000;
+template <class T>
+__device__ inline __amdgpu_buffer_rsrc_t rows_rsrc(const T* base, long rs, int rows, int D) {
+    return uniform_rsrc(base, rows > 0 ? static_cast<int>(((rows - 1) * rs + D) * static_cast<long>(sizeof(T))) : 0);
+}
+__device__ inline bf16x8 buffer_load8(__amdgpu_buffer_rsrc_t r, int off, bf16) {
+    return __builtin_bit_cast(bf16x8, __builtin_amdgcn_raw_buffer_load_b128(r, off, 0, 0));
+}
+__device__ inline f32x8 buffer_load8(__amdgpu_buffer_rsrc_t r, int off, float) {
+    const f32x4 a = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(r, off, 0, 0));
+    const f32x4 b = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(r, off + 16, 0, 0));
     return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
 }
-__device__ inline f32x8 lds_rows_acc(const float* tile, int ls, int row0, int c) {
-    const int l = threadIdx.x & 63;
-    const float* p = tile + (row0 + (l & 31)) * ls + 16 * c + 4 * (l >> 5);
-    const f32x4 a = *reinterpret_cast<const f32x4*>(p), b = *reinterpret_cast<const f32x4*>(p + 8);
-    return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+
+// 16 bytes per lane from the descriptor's offset `off` to shared memory at
+// `to` (wave-uniform) + 16 * lane.
+__device__ inline void copy16(__amdgpu_buffer_rsrc_t r, void* to, int off) {
+    typedef __attribute__((address_space(3))) void Shared;
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (Shared*)to, 16, off, 0, 0, 0);
 }
+
+// Copies a tile of ROWS rows from memory straight into shared memory, 16 bytes
+// per thread at a time: unit u of the tile is written by thread u mod NT, so
+// the permutation of a row's units is made on the side of the memory
+// addresses. A thread's offset stays from tile to tile; those of its further
+// units are whole steps of rows away where the permutation repeats after that
+// many rows, and are kept one by one where it does not.
+template <class T, int DP, int ROWS, int NT>
+struct Copy {
+    typedef Tile<T, DP> Tl;
+    static constexpr int N = ROWS * Tl::NU / NT, STEP = NT / Tl::NU;
+    static constexpr bool SAME = STEP % (sizeof(T) == 4 && Tl::NU > 8 ? 8 : 16) == 0;
+    int off[SAME ? 1 : N], step;
+    __device__ inline void init(long rs, int D, int tid) {
+        step = static_cast<int>(STEP * rs * static_cast<long>(sizeof(T)));
+#pragma unroll
+        for (int i = 0; i < (SAME ? 1 : N); ++i) {
+            const int u = tid + i * NT, row = u / Tl::NU, col = Tl::U * ((u % Tl::NU) ^ Tl::swz(row));
+            off[i] = col < D ? static_cast<int>((row * rs + col) * static_cast<long>(sizeof(T))) : kFar;
+        }
+    }
+    __device__ inline void load(T* tile, const T* base, long rs, int rows, int D, int wave) const {
+        const __amdgpu_buffer_rsrc_t r = rows_rsrc(base, rs, min(rows, ROWS), D);
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            copy16(r, tile + (64 * wave + i * NT) * Tl::U, SAME ? off[0] + i * step : off[SAME ? 0 : i]);
+    }
+    // The thread's own units of the tile (its loads have landed): values that
+    // are not finite become zeros, f(row) is told of their rows. bf16 takes a
+    // unit as it is; float units are half a fragment.
+    template <class F>
+    __device__ static inline void clean(T* tile, int tid, F f) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            typedef T V __attribute__((ext_vector_type(Tl::U)));
+            V* p = reinterpret_cast<V*>(tile + (tid + i * NT) * Tl::U);
+            V v = *p;
+            bool bad = false;
+#pragma unroll
+            for (int x = 0; x < Tl::U; ++x)
+                if (!(__builtin_fabsf(static_cast<float>(v[x])) < __builtin_inff())) {
+                    v[x] = static_cast<T>(0.0f);
+                    bad = true;
+                }
+            if (bad) {
+                *p = v;
+                f((tid + i * NT) / Tl::NU);
+            }
+        }
+    }
+};
 
 // A float fragment as bf16 terms whose sum holds it to 16 (two terms) or 24
 // bits (three): products with a bf16 operand then lose nothing that float
@@ -158,22 +268,6 @@ __device__ inline void store4(T* p, int n, bool vec, float a, float b, float c, 
 #pragma unroll
     for (int i = 0; i < 4; ++i)
         if (i < n) p[i] = v[i];
-}
-
-// Whether any of the fragment's values is not finite.
-template <class T>
-__device__ inline bool any_nonfinite(const Frag<T>& f) {
-    bool bad = false;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) bad |= !(__builtin_fabsf(static_cast<float>(f[i])) < __builtin_inff());
-    return bad;
-}
-template <class T>
-__device__ inline Frag<T> finite_or_zero(Frag<T> f) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-        if (!(__builtin_fabsf(static_cast<float>(f[i])) < __builtin_inff())) f[i] = static_cast<T>(0.0f);
-    return f;
 }
 
 }  // namespace kdec
