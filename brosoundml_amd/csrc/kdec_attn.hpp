@@ -75,18 +75,75 @@ __device__ inline Doc doc_at(const Docs& m, int d) {
     return r;
 }
 
-__device__ inline Row row_at(const Docs& m, int i) {
-    Row r{INT_MAX, INT_MIN, 0};
-    const int d = doc_of(m.q_off, m.docs, i);
-    if (d < 0 || i >= m.q_off[d + 1]) return r;
+__device__ inline Row row_in(const Docs& m, int d, int i) {
     const Doc c = doc_at(m, d);
     const int p = i - c.q0 + c.lk - c.lq;  // position of its last key
     const int n = m.causal ? min(max(max(p + 1, c.prefix), 0), c.lk) : c.lk;
-    if (n <= 0) return r;
-    r.lo = c.k0;
-    r.hi = c.k0 + n;
-    r.pos = c.k0 + p;
-    return r;
+    if (n <= 0) return Row{INT_MAX, INT_MIN, 0};
+    return Row{c.k0, c.k0 + n, c.k0 + p};
+}
+
+// The keys of every lane's row i, `first` the least of the wave's rows (all
+// lanes take part). The wave reads 64 offsets at once, from the document of
+// its first row, and each lane finds its own among them; only rows past 64
+// documents (most of them empty, then) search memory.
+__device__ inline Row row_at(const Docs& m, int i, int first) {
+    const int lane = threadIdx.x & 63;
+    if (m.docs <= 0) return Row{INT_MAX, INT_MIN, 0};
+    int d0 = 0;
+    if (m.docs > 64) d0 = max(doc_of(m.q_off, m.docs, __builtin_amdgcn_readfirstlane(first)), 0);
+    const int off = d0 + lane <= m.docs ? m.q_off[d0 + lane] : INT_MAX;
+    int n = 0;  // how many of the 64 are not past i
+#pragma unroll
+    for (int s = 32; s; s >>= 1) n += __shfl(off, n + s - 1) <= i ? s : 0;
+    n += __shfl(off, min(n, 63)) <= i;
+    int d = d0 + n - 1;
+    if (n == 64) d = doc_of(m.q_off, m.docs, i);
+    if (d < 0 || d >= m.docs || i >= m.q_off[d + 1]) return Row{INT_MAX, INT_MIN, 0};
+    return row_in(m, d, i);
+}
+
+// What a block of 128 entries (32 per wave) walks: keys [lo, hi) in tiles of
+// 64, of which those in [full_lo, full_hi) are seen by every row; a wave's
+// rows see keys of [wlo, whi), and all of them those of [wfull_lo, wfull_hi).
+struct Walk {
+    int lo, hi, full_lo, full_hi, wlo, whi, wfull_lo, wfull_hi;
+};
+__device__ inline Walk walk_of(const Row& me, bool valid, int (&red)[4][4]) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    int lo = me.lo, hi = me.hi, full_lo = valid ? me.lo : INT_MIN, full_hi = valid ? me.hi : INT_MAX;
+    for (int o = 16; o; o >>= 1) {
+        lo = min(lo, __shfl_xor(lo, o));
+        hi = max(hi, __shfl_xor(hi, o));
+        full_lo = max(full_lo, __shfl_xor(full_lo, o));
+        full_hi = min(full_hi, __shfl_xor(full_hi, o));
+    }
+    if (lane == 0) {
+        red[wave][0] = lo;
+        red[wave][1] = hi;
+        red[wave][2] = full_lo;
+        red[wave][3] = full_hi;
+    }
+    __syncthreads();
+    const auto u = [](int x) { return __builtin_amdgcn_readfirstlane(x); };
+    return Walk{u(min(min(red[0][0], red[1][0]), min(red[2][0], red[3][0]))),
+                u(max(max(red[0][1], red[1][1]), max(red[2][1], red[3][1]))),
+                u(max(max(red[0][2], red[1][2]), max(red[2][2], red[3][2]))),
+                u(min(min(red[0][3], red[1][3]), min(red[2][3], red[3][3]))),
+                u(lo), u(hi), u(full_lo), u(full_hi)};
+}
+// Tiles [t0, f0) and [f1, t1) of a walk are masked, those between are seen
+// whole by every row; the first two numbers of tiles are even, so that each
+// loop starts at the first buffer.
+__device__ inline void split_walk(const Walk& w, int t0, int t1, int& f0, int& f1) {
+    f0 = f1 = t0;
+    if (w.full_hi > w.full_lo && w.full_lo <= w.hi) {
+        f0 = min(max((w.full_lo - w.lo + BN - 1) / BN, t0), t1);
+        f0 = min(f0 + ((f0 - t0) & 1), t1);
+        f1 = min(max((w.full_hi - w.lo) / BN, f0), t1);
+        f1 -= (f1 - f0) & 1;
+    }
+    if (f0 >= f1) f0 = f1 = t0;
 }
 
 // Scores in log2 units from raw products. T says how exact the cap's tanh has

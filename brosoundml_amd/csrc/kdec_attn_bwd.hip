@@ -31,36 +31,14 @@ struct Bwd {
     float* part;  // (parts, Hkv, Tk, 2, D): their dK / scale and dV
 };
 
-// delta = dO . O and lse in log2 units of every row and head, and the rows'
-// keys. A row without keys gets lse = +inf, so that its probabilities are
-// zeros; one whose delta is not finite gets NaN, which then marks every
-// gradient that the row reaches. 16 lanes per row and head.
-template <class T>
-__global__ __launch_bounds__(AT) void attn_stat_k(Bwd b) {
-    const Args& a = b.a;
-    const int lane = threadIdx.x & 15;
-    const long w = static_cast<long>(blockIdx.x) * (AT / 16) + (threadIdx.x >> 4);
-    if (w >= static_cast<long>(a.m.Tq) * a.Hq) return;
-    const int row = static_cast<int>(w / a.Hq), head = static_cast<int>(w - static_cast<long>(row) * a.Hq);
-    const int d = 8 * lane;
-    const Frag<T> o = load8(static_cast<const T*>(b.O.p) + row * b.O.rs + head * b.O.hs + d, min(8, b.D_out - d), b.vec_o);
-    const Frag<T> g = load8(static_cast<const T*>(b.dO.p) + row * b.dO.rs + head * b.dO.hs + d, min(8, a.D - d), true);
-    float s = 0.0f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) s += static_cast<float>(o[i]) * static_cast<float>(g[i]);
-    for (int x = 8; x; x >>= 1) s += __shfl_xor(s, x);
-    if (lane) return;
-    const float lse = b.lse[static_cast<long>(head) * a.m.Tq + row];
-    float l2 = lse == -INF ? INF : lse * LOG2E;
-    if (lse != -INF && !(__builtin_fabsf(s) < INF)) l2 = __builtin_nanf("");
-    b.stat[static_cast<long>(head) * a.m.Tq + row] = make_float2(l2, lse == -INF ? 0.0f : s);
-    if (head == 0) b.rows[row] = row_at(a.m, row);
-}
-
 // dQ: the forward's walk over the keys, with dQ^T = K^T dS^T in place of the
-// output.
+// output. Before it a block forms delta = dO . O of its rows and heads and
+// writes what the walk over the rows takes: delta, lse in log2 units, and the
+// rows' keys. A row without keys gets lse = +inf, so that its probabilities
+// are zeros; one whose delta is not finite gets NaN, which then marks every
+// gradient that the row reaches.
 template <class T, int DP, bool CAP, bool BIAS>
-__global__ __launch_bounds__(AT, sizeof(T) == 2 ? 2 : 1) void attn_dq_k(Bwd b) {
+__global__ __launch_bounds__(AT, sizeof(T) == 2 ? (DP == 64 && !BIAS ? 3 : 2) : 1) void attn_dq_k(Bwd b) {
     constexpr int NC = DP / 16, ND = DP / 32;
     __shared__ __align__(16) T sk0[BN * DP], sk1[BN * DP], sv0[BN * DP], sv1[BN * DP];
     __shared__ int red[4][4];
@@ -72,38 +50,37 @@ __global__ __launch_bounds__(AT, sizeof(T) == 2 ? 2 : 1) void attn_dq_k(Bwd b) {
     const int e = tile * BM + wave * 32 + (lane & 31);
     const bool valid = e < a.E;
     const int row = valid ? e / a.G : 0, head = kvh * a.G + (valid ? e - row * a.G : 0);
-    const Row me = valid ? b.rows[row] : Row{INT_MAX, INT_MIN, 0};
-    int lo = me.lo, hi = me.hi, full_lo = valid ? me.lo : INT_MIN, full_hi = valid ? me.hi : INT_MAX;
-    for (int o = 16; o; o >>= 1) {
-        lo = min(lo, __shfl_xor(lo, o));
-        hi = max(hi, __shfl_xor(hi, o));
-        full_lo = max(full_lo, __shfl_xor(full_lo, o));
-        full_hi = min(full_hi, __shfl_xor(full_hi, o));
-    }
-    if (lane == 0) {
-        red[wave][0] = lo;
-        red[wave][1] = hi;
-        red[wave][2] = full_lo;
-        red[wave][3] = full_hi;
-    }
-    const int wlo = __builtin_amdgcn_readfirstlane(lo), whi = __builtin_amdgcn_readfirstlane(hi);
-    __syncthreads();
-    const int blo = __builtin_amdgcn_readfirstlane(min(min(red[0][0], red[1][0]), min(red[2][0], red[3][0])));
-    const int bhi = __builtin_amdgcn_readfirstlane(max(max(red[0][1], red[1][1]), max(red[2][1], red[3][1])));
-    full_lo = __builtin_amdgcn_readfirstlane(max(max(red[0][2], red[1][2]), max(red[2][2], red[3][2])));
-    full_hi = __builtin_amdgcn_readfirstlane(min(min(red[0][3], red[1][3]), min(red[2][3], red[3][3])));
-    const int t1 = bhi > blo ? (bhi - blo + BN - 1) / BN : 0;
+    Row me = row_at(a.m, row, min(tile * BM + wave * 32, a.E - 1) / a.G);
+    if (!valid) me = Row{INT_MAX, INT_MIN, 0};
+    const Walk w = walk_of(me, valid, red);
+    const int t1 = w.hi > w.lo ? (w.hi - w.lo + BN - 1) / BN : 0;
 
     const Score<T, CAP, BIAS> rule(a, head);
-    const float2 stat = valid ? b.stat[static_cast<long>(head) * a.m.Tq + row] : make_float2(INF, 0.0f);
     Frag<T> q[NC], g[NC];
     const T* qp = static_cast<const T*>(a.Q.p) + row * a.Q.rs + head * a.Q.hs;
     const T* gp = static_cast<const T*>(b.dO.p) + row * b.dO.rs + head * b.dO.hs;
+    const T* op = static_cast<const T*>(b.O.p) + row * b.O.rs + head * b.O.hs;
+    float lse2 = INF, delta = 0.0f;
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
         const int d = 16 * c + 8 * half, n = valid ? min(8, a.D - d) : 0;
         q[c] = load8(qp + d, n, true);
         g[c] = load8(gp + d, n, true);
+        const Frag<T> o = load8(op + d, valid ? min(8, b.D_out - d) : 0, b.vec_o);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) delta = __builtin_fmaf(static_cast<float>(o[i]), static_cast<float>(g[c][i]), delta);
+        if (sizeof(T) == 4) __builtin_amdgcn_sched_barrier(0);
+    }
+    delta += __shfl_xor(delta, 32);
+    if (valid) {
+        const float lse = b.lse[static_cast<long>(head) * a.m.Tq + row];
+        lse2 = lse == -INF ? INF : lse * LOG2E;
+        if (lse == -INF) delta = 0.0f;
+        else if (!(__builtin_fabsf(delta) < INF)) lse2 = __builtin_nanf("");
+        if (!half) {
+            b.stat[static_cast<long>(head) * a.m.Tq + row] = make_float2(lse2, delta);
+            if (head == 0) b.rows[row] = me;
+        }
     }
     const T* kb = static_cast<const T*>(a.K.p) + kvh * a.K.hs;
     const T* vb = static_cast<const T*>(a.V.p) + kvh * a.V.hs;
@@ -111,19 +88,12 @@ __global__ __launch_bounds__(AT, sizeof(T) == 2 ? 2 : 1) void attn_dq_k(Bwd b) {
     ks.init(a.K.rs, a.D, tid);
     vs.init(a.V.rs, a.D, tid);
     const auto load = [&](int t, T* tk, T* tv) __attribute__((always_inline)) {
-        const int j = blo + t * BN;
-        ks.load(tk, kb + j * a.K.rs, a.K.rs, bhi - j, a.D, wave);
-        vs.load(tv, vb + j * a.V.rs, a.V.rs, bhi - j, a.D, wave);
+        const int j = w.lo + t * BN;
+        ks.load(tk, kb + j * a.K.rs, a.K.rs, w.hi - j, a.D, wave);
+        vs.load(tv, vb + j * a.V.rs, a.V.rs, w.hi - j, a.D, wave);
     };
-    // Tiles [0, f0) and [f1, t1) are masked, as in the forward.
-    int f0 = 0, f1 = 0;
-    if (full_hi > full_lo && full_lo <= bhi) {
-        f0 = min(max((full_lo - blo + BN - 1) / BN, 0), t1);
-        f0 = min(f0 + (f0 & 1), t1);
-        f1 = min(max((full_hi - blo) / BN, f0), t1);
-        f1 -= (f1 - f0) & 1;
-    }
-    if (f0 >= f1) f0 = f1 = 0;
+    int f0, f1;
+    split_walk(w, 0, t1, f0, f1);
     const auto landed = [&](int t, T* tk) __attribute__((always_inline)) {
         __builtin_amdgcn_s_waitcnt(0);
         if (t < f0 || t >= f1) ks.clean(tk, tid, [](int) {});  // a zero of dS times such a key
@@ -135,6 +105,7 @@ __global__ __launch_bounds__(AT, sizeof(T) == 2 ? 2 : 1) void attn_dq_k(Bwd b) {
         const unsigned at = static_cast<unsigned>(j0 + 4 * half - me.lo);
         const unsigned len = me.hi > me.lo ? static_cast<unsigned>(me.hi - me.lo) : 0u;
         const float dist = static_cast<float>(me.pos - j0 - 4 * half);
+        const bool whole = j0 >= w.wfull_lo && j0 + BN <= w.wfull_hi;
 #pragma unroll
         for (int n = 0; n < 2; ++n) {
             f32x16 s = f32x16{}, dp = f32x16{};
@@ -149,10 +120,12 @@ __global__ __launch_bounds__(AT, sizeof(T) == 2 ? 2 : 1) void attn_dq_k(Bwd b) {
             for (int r = 0; r < 16; ++r) {
                 const int k = 32 * n + acc_row(r, 0);
                 float dt;
-                float p = grad_p(rule, s[r], dist - static_cast<float>(k), stat.x, dt);
-                p *= (dp[r] - stat.y) * dt;
-                if (decltype(masked)::value) p = at + static_cast<unsigned>(k) < len ? p : 0.0f;
-                s[r] = p;
+                s[r] = grad_p(rule, s[r], dist - static_cast<float>(k), lse2, dt) * ((dp[r] - delta) * dt);
+            }
+            if (decltype(masked)::value && !whole) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) s[r] = at + static_cast<unsigned>(32 * n + acc_row(r, 0)) < len ? s[r] : 0.0f;
+                asm volatile("");  // a branch
             }
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
@@ -166,9 +139,9 @@ __global__ __launch_bounds__(AT, sizeof(T) == 2 ? 2 : 1) void attn_dq_k(Bwd b) {
         }
     };
     const auto walk = [&](auto masked, int t, const T* tk, const T* tv, T* nk, T* nv) __attribute__((always_inline)) {
-        const int j0 = blo + t * BN;
+        const int j0 = w.lo + t * BN;
         if (t + 1 < t1) load(t + 1, nk, nv);
-        if (!decltype(masked)::value || (wlo < j0 + BN && whi > j0)) step(masked, j0, tk, tv);
+        if (!decltype(masked)::value || (w.wlo < j0 + BN && w.whi > j0)) step(masked, j0, tk, tv);
         if (t + 1 < t1) landed(t + 1, nk);
         __syncthreads();
     };
@@ -198,24 +171,38 @@ __global__ __launch_bounds__(AT, sizeof(T) == 2 ? 2 : 1) void attn_dq_k(Bwd b) {
         }
 }
 
-// dK and dV: a block holds 128 keys of one key head (32 per wave, keys and
+// dK and dV: a block holds 32 keys for each of its KG pairs of waves (keys and
 // values in registers) and walks the rows that see them, head by head of the
 // group, in tiles of 64 whose queries and output gradients are staged in
-// shared memory, two buffers deep and two tiles a turn. All heads of the group
-// belong to the same walk, so the sums over shared heads need no joining;
-// where the key tiles alone do not fill the device, `parts` blocks share a
-// walk and attn_dkv_join_k adds their sums. Scores are S = Q K^T here, a lane
-// holding one key's column.
+// shared memory, two buffers deep and two tiles a turn. Scores are S = Q K^T
+// here, a lane holding one key's column. The waves of a pair form P and dS of
+// one half of a tile each, hand each other what it takes to keep one sum per
+// wave -- the first gets the other's P and sums dV over the whole tile, the
+// second the other's dS and sums dK -- and so hold half the accumulators
+// each, which leaves room for two waves per SIMD whose arithmetic and
+// products overlap (one wave with both sums: 900 us where two take 630, 8192
+// causal rows of 16 heads on 4, width 128). All heads of the group belong to the
+// same walk, so the sums over shared heads need no joining; where the key
+// tiles alone do not fill the device, `parts` blocks share a walk and
+// attn_dkv_join_k adds their sums.
+// Wide heads in float, or with a bias, take the registers of a whole SIMD per
+// wave: two pairs.
+template <class T, int DP, bool BIAS> constexpr int key_groups() { return DP == 64 ? 2 : sizeof(T) == 4 || BIAS ? 2 : 4; }
+
 template <class T, int DP, bool CAP, bool BIAS>
-__global__ __launch_bounds__(AT, DP == 64 && sizeof(T) == 2 ? 2 : 1) void attn_dkv_k(Bwd b) {
-    constexpr int NC = DP / 16, ND = DP / 32, BE = 64, PAIR = 2 * BE;
-    __shared__ __align__(16) T sq0[BE * DP], sq1[BE * DP], sg0[BE * DP], sg1[BE * DP];
+__global__ __launch_bounds__((128 * key_groups<T, DP, BIAS>()), (sizeof(T) == 2 && DP == 64 ? 3 : key_groups<T, DP, BIAS>() == 4 ? 2 : 1)) void attn_dkv_k(Bwd b) {
+    constexpr int NC = DP / 16, ND = DP / 32, BE = 64, PAIR = 2 * BE, KG = key_groups<T, DP, BIAS>(), NT = 128 * KG, KEYS = 32 * KG;
+    // (aligned to come first: within the reach of the reads' own offsets)
+    __shared__ __align__(256) T sq0[BE * DP], sq1[BE * DP], sg0[BE * DP], sg1[BE * DP];
+    __shared__ Frag<T> pass[KG][2][2][64];  // by pair, half of the tile, step: the other wave's operand
+    __shared__ int some[KG][2];             // whether the half's rows see any of the pair's keys
     __shared__ __align__(16) float slse[2][BE], sdelta[2][BE];
     __shared__ __align__(16) int slo[2][BE], shi[2][BE], spos[2][BE];
     const Args& a = b.a;
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, half = lane >> 5;
-    const int kvh = blockIdx.x % a.Hkv, j0 = (blockIdx.x / a.Hkv) * BM, part = blockIdx.y;
-    const int wkey = j0 + wave * 32, key = wkey + (lane & 31);
+    const int pair = wave % KG, role = wave / KG;
+    const int kvh = blockIdx.x % a.Hkv, j0 = (blockIdx.x / a.Hkv) * KEYS, part = blockIdx.y;
+    const int wkey = j0 + pair * 32, key = wkey + (lane & 31);
     const bool valid = key < a.m.Tk;
 
     // the rows [e0, e1) that may see keys of the block, and those [f0, f1)
@@ -223,17 +210,17 @@ __global__ __launch_bounds__(AT, DP == 64 && sizeof(T) == 2 ? 2 : 1) void attn_d
     int e0 = 0, e1 = 0, f0 = 0, f1 = 0;
     {
         const int d0 = max(doc_of(a.m.k_off, a.m.docs, j0), 0);
-        const int d1 = doc_of(a.m.k_off, a.m.docs, min(j0 + BM, a.m.Tk) - 1);
+        const int d1 = doc_of(a.m.k_off, a.m.docs, min(j0 + KEYS, a.m.Tk) - 1);
         if (d1 >= 0) {
             const Doc c = doc_at(a.m, d0), z = doc_at(a.m, d1);
             const int skip = c.lk - c.lq;  // position of the first row's key
             e0 = c.q0;
             if (a.m.causal && j0 - c.k0 >= c.prefix) e0 = min(max(c.q0 + (j0 - c.k0) - skip, c.q0), c.q0 + c.lq);
             e1 = z.q0 + z.lq;
-            if (d0 == d1 && j0 >= c.k0 && j0 + BM <= c.k0 + c.lk) {
+            if (d0 == d1 && j0 >= c.k0 && j0 + KEYS <= c.k0 + c.lk) {
                 f0 = c.q0;
-                if (a.m.causal && j0 + BM - c.k0 > c.prefix)
-                    f0 = min(max(c.q0 + (j0 + BM - 1 - c.k0) - skip, c.q0), c.q0 + c.lq);
+                if (a.m.causal && j0 + KEYS - c.k0 > c.prefix)
+                    f0 = min(max(c.q0 + (j0 + KEYS - 1 - c.k0) - skip, c.q0), c.q0 + c.lq);
                 f1 = c.q0 + c.lq;
             }
         }
@@ -263,7 +250,7 @@ __global__ __launch_bounds__(AT, DP == 64 && sizeof(T) == 2 ? 2 : 1) void attn_d
         k[c] = load8(kp + d, n, true);
         v[c] = load8(vp + d, n, true);
     }
-    Copy<T, DP, BE, AT> qs, gs;
+    Copy<T, DP, BE, NT> qs, gs;
     qs.init(a.Q.rs, a.D, tid);
     gs.init(b.dO.rs, a.D, tid);
     int left = 2 * (u1 - u0), lg = 0, li = 0;  // tiles to load; the next one's head and place
@@ -302,114 +289,152 @@ __global__ __launch_bounds__(AT, DP == 64 && sizeof(T) == 2 ? 2 : 1) void attn_d
             shi[buf][tid] = r_row.hi;
             spos[buf][tid] = r_row.pos;
         }
-        if (l_masked) {
+        if (l_masked) {  // zeros of P and dS times such values
             qs.clean(tq, tid, [](int) {});
             gs.clean(tg, tid, [](int) {});
         }
     };
-    f32x16 dk[ND], dv[ND];
+    // The two waves of a pair run code of their own, with the same barriers.
+    const auto run = [&](auto which) __attribute__((always_inline)) {
+        constexpr int ROLE = decltype(which)::value;
+        f32x16 acc[ND];  // dV (the pair's first wave) or dK / scale (its second)
 #pragma unroll
-    for (int d = 0; d < ND; ++d) dk[d] = dv[d] = f32x16{};
-    const auto step = [&](auto masked, const Score<T, CAP, BIAS>& rule, const T* tq, const T* tg, int buf)
-        __attribute__((always_inline)) {
-#pragma unroll
-        for (int n = 0; n < 2; ++n) {
-            if (decltype(masked)::value) {  // rows of 32 that see none of the wave's keys
-                const int i = 32 * n + (lane & 31);
-                if (!__builtin_amdgcn_ballot_w64(slo[buf][i] < wkey + 32 && shi[buf][i] > wkey)) continue;
+        for (int d = 0; d < ND; ++d) acc[d] = f32x16{};
+        const auto step = [&](auto masked, const Score<T, CAP, BIAS>& rule, const T* tq, const T* tg, int buf)
+                              __attribute__((always_inline)) {
+            constexpr bool MASKED = decltype(masked)::value;
+            constexpr int n0 = 32 * ROLE;  // the wave's half
+            const T *hq = tq + n0 * DP, *hg = tg + n0 * DP;
+            bool any = true, whole = true;  // some, all of the half's rows and the wave's keys meet
+            if (MASKED) {
+                const int i = n0 + (lane & 31), lo = slo[buf][i], hi = shi[buf][i];
+                any = __builtin_amdgcn_ballot_w64(lo < wkey + 32 && hi > wkey) != 0;
+                whole = __builtin_amdgcn_ballot_w64(!(lo <= wkey && hi >= wkey + 32)) == 0;
+                if (lane == 0) some[pair][ROLE] = any;
             }
-            f32x16 s = f32x16{}, dp = f32x16{}, p;
+            Frag<T> own[2];
+            if (any) {
+                f32x16 s = f32x16{}, p = f32x16{};  // products, then dS and P
 #pragma unroll
-            for (int c = 0; c < NC; ++c) {
-                s = mma32(lds_rows<T, DP>(tq, 32 * n, c), k[c], s);
-                hold<T>();
-                dp = mma32(lds_rows<T, DP>(tg, 32 * n, c), v[c], dp);
-                hold<T>();
-            }
+                for (int c = 0; c < NC; ++c) {
+                    s = mma32(lds_rows<T, DP>(hq, 0, c), k[c], s);
+                    hold<T>();
+                    p = mma32(lds_rows<T, DP>(hg, 0, c), v[c], p);
+                    hold<T>();
+                }
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const int i0 = 32 * n + 8 * q + 4 * half;
-                const f32x4 lse = *reinterpret_cast<const f32x4*>(&slse[buf][i0]);
-                const f32x4 delta = *reinterpret_cast<const f32x4*>(&sdelta[buf][i0]);
+                for (int q = 0; q < 4; ++q) {
+                    const int i0 = n0 + 8 * q + 4 * half;
+                    const f32x4 lse = *reinterpret_cast<const f32x4*>(&slse[buf][i0]);
+                    const f32x4 delta = *reinterpret_cast<const f32x4*>(&sdelta[buf][i0]);
 #pragma unroll
-                for (int x = 0; x < 4; ++x) {
-                    const int r = 4 * q + x, i = i0 + x;
-                    float dt;
-                    float pr = grad_p(rule, s[r], BIAS ? static_cast<float>(spos[buf][i] - key) : 0.0f, lse[x], dt);
-                    float ds = pr * (dp[r] - delta[x]) * dt;
-                    if (decltype(masked)::value) {
-                        const bool seen = key >= slo[buf][i] && key < shi[buf][i];
-                        pr = seen ? pr : 0.0f;
-                        ds = seen ? ds : 0.0f;
+                    for (int x = 0; x < 4; ++x) {
+                        const int r = 4 * q + x, i = i0 + x;
+                        float dt;
+                        float pr = grad_p(rule, s[r], BIAS ? static_cast<float>(spos[buf][i] - key) : 0.0f, lse[x], dt);
+                        s[r] = pr * (p[r] - delta[x]) * dt;
+                        p[r] = pr;
                     }
-                    p[r] = pr;
-                    s[r] = ds;
-                }
-                hold<T>();
-            }
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                const Frag<T> pf = acc_frag<T>(p, c), ds = acc_frag<T>(s, c);
-#pragma unroll
-                for (int d = 0; d < ND; ++d) {
-                    dv[d] = mma32(lds_cols<DP, true>(tg, 32 * n + 16 * c, 32 * d), pf, dv[d]);
-                    hold<T>();
-                    dk[d] = mma32(lds_cols<DP, true>(tq, 32 * n + 16 * c, 32 * d), ds, dk[d]);
+                    if (MASKED || CAP || BIAS) __builtin_amdgcn_sched_barrier(0);
                     hold<T>();
                 }
+                if (MASKED && !whole) {
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        typedef int i32x4 __attribute__((ext_vector_type(4)));
+                        const i32x4 lo = *reinterpret_cast<const i32x4*>(&slo[buf][n0 + 8 * q + 4 * half]);
+                        const i32x4 hi = *reinterpret_cast<const i32x4*>(&shi[buf][n0 + 8 * q + 4 * half]);
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) {
+                            const bool seen = key >= lo[x] && key < hi[x];
+                            p[4 * q + x] = seen ? p[4 * q + x] : 0.0f;
+                            s[4 * q + x] = seen ? s[4 * q + x] : 0.0f;
+                        }
+                        __builtin_amdgcn_sched_barrier(0);
+                    }
+                    asm volatile("");  // a branch
+                }
+                if constexpr (ROLE) {
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) {
+                        own[c] = acc_frag<T>(s, c);
+                        pass[pair][1][c][lane] = acc_frag<T>(p, c);
+                    }
+                } else {
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) {
+                        own[c] = acc_frag<T>(p, c);
+                        pass[pair][0][c][lane] = acc_frag<T>(s, c);
+                    }
+                }
+            }
+            __syncthreads();
+            const T *mine = ROLE ? hq : hg, *other = (ROLE ? tq : tg) + (32 - n0) * DP;
+            if (!MASKED || any) {
+#pragma unroll
+                for (int c = 0; c < 2; ++c)
+#pragma unroll
+                    for (int d = 0; d < ND; ++d) {
+                        acc[d] = mma32(lds_cols<DP, true>(mine, 16 * c, 32 * d), own[c], acc[d]);
+                        hold<T>();
+                    }
+            }
+            if (!MASKED || some[pair][1 - ROLE]) {
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    const Frag<T> f = pass[pair][1 - ROLE][c][lane];
+#pragma unroll
+                    for (int d = 0; d < ND; ++d) {
+                        acc[d] = mma32(lds_cols<DP, true>(other, 16 * c, 32 * d), f, acc[d]);
+                        hold<T>();
+                    }
+                }
+            }
+        };
+        const auto walks = [&](auto masked, const Score<T, CAP, BIAS>& rule, int from, int to) __attribute__((always_inline)) {
+            for (int i = from; i < to; ++i) {
+                load(sq1, sg1);
+                step(masked, rule, sq0, sg0, 0);
+                landed(sq1, sg1, 1);
+                __syncthreads();
+                const bool more = left > 0;
+                if (more) load(sq0, sg0);
+                step(masked, rule, sq1, sg1, 1);
+                if (more) landed(sq0, sg0, 0);
+                __syncthreads();
+            }
+        };
+        if (left) {
+            load(sq0, sg0);
+            landed(sq0, sg0, 0);
+            __syncthreads();
+            for (int u = u0; u < u1;) {
+                const int g = u / per, i0 = u - g * per, i1 = min(per, i0 + u1 - u);
+                const Score<T, CAP, BIAS> rule(a, kvh * a.G + g);
+                walks(std::true_type{}, rule, i0, min(p0, i1));
+                walks(std::false_type{}, rule, max(i0, p0), min(p1, i1));
+                walks(std::true_type{}, rule, max(i0, p1), i1);
+                u += i1 - i0;
             }
         }
-    };
-    const auto walks = [&](auto masked, const Score<T, CAP, BIAS>& rule, int from, int to) __attribute__((always_inline)) {
-        for (int i = from; i < to; ++i) {
-            load(sq1, sg1);
-            step(masked, rule, sq0, sg0, 0);
-            landed(sq1, sg1, 1);
-            __syncthreads();
-            const bool more = left > 0;
-            if (more) load(sq0, sg0);
-            step(masked, rule, sq1, sg1, 1);
-            if (more) landed(sq0, sg0, 0);
-            __syncthreads();
-        }
-    };
-    if (left) {
-        load(sq0, sg0);
-        landed(sq0, sg0, 0);
-        __syncthreads();
-        for (int u = u0; u < u1;) {
-            const int g = u / per, i0 = u - g * per, i1 = min(per, i0 + u1 - u);
-            const Score<T, CAP, BIAS> rule(a, kvh * a.G + g);
-            walks(std::true_type{}, rule, i0, min(p0, i1));
-            walks(std::false_type{}, rule, max(i0, p0), min(p1, i1));
-            walks(std::true_type{}, rule, max(i0, p1), i1);
-            u += i1 - i0;
-        }
-    }
-    if (!valid) return;
-    if (b.parts > 1) {
-        float* o = b.part + ((static_cast<long>(part) * a.Hkv + kvh) * a.m.Tk + key) * 2 * a.D;
+        if (!valid) return;
+        T* out = ROLE ? static_cast<T*>(b.dK) + kvh * b.dk_hs + key * b.dk_rs : static_cast<T*>(b.dV) + kvh * b.dv_hs + key * b.dv_rs;
+        const float f = ROLE ? a.scale : 1.0f;
+        float* o = b.part + (((static_cast<long>(part) * a.Hkv + kvh) * a.m.Tk + key) * 2 + 1 - ROLE) * a.D;
 #pragma unroll
         for (int dt = 0; dt < ND; ++dt)
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
                 const int d = 32 * dt + 8 * q + 4 * half;
-                store4(o + d, a.D - d, true, dk[dt][4 * q], dk[dt][4 * q + 1], dk[dt][4 * q + 2], dk[dt][4 * q + 3]);
-                store4(o + a.D + d, a.D - d, true, dv[dt][4 * q], dv[dt][4 * q + 1], dv[dt][4 * q + 2], dv[dt][4 * q + 3]);
+                if (b.parts > 1)
+                    store4(o + d, a.D - d, true, acc[dt][4 * q], acc[dt][4 * q + 1], acc[dt][4 * q + 2], acc[dt][4 * q + 3]);
+                else
+                    store4(out + d, b.D_out - d, ROLE ? b.vec_dk : b.vec_dv, acc[dt][4 * q] * f, acc[dt][4 * q + 1] * f,
+                           acc[dt][4 * q + 2] * f, acc[dt][4 * q + 3] * f);
             }
-        return;
-    }
-    T* ok = static_cast<T*>(b.dK) + kvh * b.dk_hs + key * b.dk_rs;
-    T* ov = static_cast<T*>(b.dV) + kvh * b.dv_hs + key * b.dv_rs;
-#pragma unroll
-    for (int dt = 0; dt < ND; ++dt)
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            const int d = 32 * dt + 8 * q + 4 * half;
-            store4(ok + d, b.D_out - d, b.vec_dk, dk[dt][4 * q] * a.scale, dk[dt][4 * q + 1] * a.scale,
-                   dk[dt][4 * q + 2] * a.scale, dk[dt][4 * q + 3] * a.scale);
-            store4(ov + d, b.D_out - d, b.vec_dv, dv[dt][4 * q], dv[dt][4 * q + 1], dv[dt][4 * q + 2], dv[dt][4 * q + 3]);
-        }
+    };
+    if (role) run(std::integral_constant<int, 1>{});
+    else run(std::integral_constant<int, 0>{});
 }
 
 // The parts' dK and dV added in their order, four columns a thread.
@@ -438,12 +463,12 @@ struct Launch {
     static int run(kdec_ctx* ctx, const Bwd& b, long q_blocks, long k_blocks, size_t part_n) {
         const auto blocks = [](long n) { return dim3(static_cast<unsigned>(n)); };
         if (b.a.m.Tq > 0) {
-            hipLaunchKernelGGL(attn_stat_k<T>, blocks(cdiv(static_cast<long>(b.a.m.Tq) * b.a.Hq, AT / 16)), dim3(AT), 0, ctx->stream, b);
             hipLaunchKernelGGL((attn_dq_k<T, DP, CAP, BIAS>), blocks(q_blocks), dim3(AT), 0, ctx->stream, b);
         }
         if (b.a.m.Tk > 0) {
+            constexpr int KG = key_groups<T, DP, BIAS>();
             hipLaunchKernelGGL((attn_dkv_k<T, DP, CAP, BIAS>), dim3(static_cast<unsigned>(k_blocks), static_cast<unsigned>(b.parts)),
-                               dim3(AT), 0, ctx->stream, b);
+                               dim3(128 * KG), 0, ctx->stream, b);
             if (b.parts > 1)
                 hipLaunchKernelGGL(attn_dkv_join_k<T>, blocks(cdiv(part_n / 4, AT)), dim3(AT), 0, ctx->stream, b);
         }
@@ -501,7 +526,7 @@ extern "C" int kdec_attn_bwd(kdec_ctx* ctx, int dtype, const void* Q, long q_rs,
     b.vec_dk = D % 4 == 0 && aligned(Heads{dK, dk_rs, dk_hs}, size, 4 * size);
     b.vec_dv = D % 4 == 0 && aligned(Heads{dV, dv_rs, dv_hs}, size, 4 * size);
     const size_t stat_bytes = (static_cast<size_t>(Tq) * Hq * sizeof(float2) + 255) & ~size_t(255);
-    const long q_blocks = cdiv(b.a.E, BM) * Hkv, k_blocks = cdiv(Tk, BM) * Hkv;
+    const long q_blocks = cdiv(b.a.E, BM) * Hkv, k_blocks = cdiv(Tk, D <= 64 || dtype == KDEC_F32 || slopes ? 64 : 128) * Hkv;
     KDEC_CHECK(ctx, k_blocks < INT_MAX, "kdec_attn_bwd: too many keys");
     // Key tiles too few to fill the device (causal walks differ in length, so
     // two blocks per CU) share their rows among parts of no fewer than four

@@ -52,27 +52,37 @@ struct Soft {
 };
 
 // One step of the running softmax of a lane's column over N score blocks of
-// 32 keys from j0. Scores become probabilities; acc is rescaled when the
+// 32 keys from j0 (whole: all of the wave's rows see all of them). Scores become probabilities; acc is rescaled when the
 // wave's maxima move far enough.
 template <bool MASKED, class T, bool CAP, bool BIAS, int N, int ND>
-__device__ inline void soft_step(const Score<T, CAP, BIAS>& rule, const Row& row, int j0, int half, f32x16 (&s)[N],
-                                 f32x16 (&acc)[ND], Soft& st) {
+__device__ inline void soft_step(const Score<T, CAP, BIAS>& rule, const Row& row, bool whole, int j0, int half,
+                                 f32x16 (&s)[N], f32x16 (&acc)[ND], Soft& st) {
     constexpr bool RAW = !CAP && !BIAS;
     const float unit = RAW ? rule.unit : 1.0f;
     const float dist = static_cast<float>(row.pos - j0 - 4 * half);
-    const unsigned at = static_cast<unsigned>(j0 + 4 * half - row.lo);  // seen: at + key's place < len
-    const unsigned len = row.hi > row.lo ? static_cast<unsigned>(row.hi - row.lo) : 0u;
-    float mx = -INF;
 #pragma unroll
     for (int n = 0; n < N; ++n)
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
             float t = s[n][r], dt;
             if (!RAW) t = rule.of(t, dist - static_cast<float>(32 * n + acc_row(r, 0)), dt);
-            if (MASKED) t = at + static_cast<unsigned>(32 * n + acc_row(r, 0)) < len ? t : -INF;
             s[n][r] = t;
-            mx = fmaxf(mx, t);
         }
+    if (MASKED && !whole) {
+        const unsigned at = static_cast<unsigned>(j0 + 4 * half - row.lo);  // seen: at + key's place < len
+        const unsigned len = row.hi > row.lo ? static_cast<unsigned>(row.hi - row.lo) : 0u;
+#pragma unroll
+        for (int n = 0; n < N; ++n)
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+                s[n][r] = at + static_cast<unsigned>(32 * n + acc_row(r, 0)) < len ? s[n][r] : -INF;
+        asm volatile("");  // a branch
+    }
+    float mx = -INF;
+#pragma unroll
+    for (int n = 0; n < N; ++n)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[n][r]);
     mx = fmaxf(mx, __shfl_xor(mx, 32));
     if (__builtin_amdgcn_ballot_w64((mx - st.m) * unit > 8.0f || (st.m == -INF && mx > -INF))) {
         const float m = fmaxf(st.m, mx);
@@ -137,7 +147,7 @@ __device__ inline void finish(const Fwd& p, int kvh, int e, int row, int head, i
 // that its rows see in tiles of 64, staged in shared memory two buffers deep
 // with the tile after next on its way.
 template <class T, int DP, bool CAP, bool BIAS>
-__global__ __launch_bounds__(AT, sizeof(T) == 2 ? 2 : 1) void attn_fwd_k(Fwd p) {
+__global__ __launch_bounds__(AT, sizeof(T) == 2 ? (DP == 64 ? 3 : 2) : 1) void attn_fwd_k(Fwd p) {
     constexpr int NC = DP / 16, ND = DP / 32;
     __shared__ __align__(16) T sk0[BN * DP], sk1[BN * DP], sv0[BN * DP], sv1[BN * DP];
     __shared__ unsigned bad[3][2];  // rows of the tile that hold values that are not finite
@@ -150,30 +160,11 @@ __global__ __launch_bounds__(AT, sizeof(T) == 2 ? 2 : 1) void attn_fwd_k(Fwd p) 
     const int e = tile * BM + wave * 32 + (lane & 31);
     const bool valid = e < a.E;
     const int row = valid ? e / a.G : 0, head = kvh * a.G + (valid ? e - row * a.G : 0);
-    const Row me = valid ? row_at(a.m, row) : Row{INT_MAX, INT_MIN, 0};
-
-    // the wave's and the block's keys, and those that every row sees
-    int lo = me.lo, hi = me.hi, full_lo = valid ? me.lo : INT_MIN, full_hi = valid ? me.hi : INT_MAX;
-    for (int o = 16; o; o >>= 1) {
-        lo = min(lo, __shfl_xor(lo, o));
-        hi = max(hi, __shfl_xor(hi, o));
-        full_lo = max(full_lo, __shfl_xor(full_lo, o));
-        full_hi = min(full_hi, __shfl_xor(full_hi, o));
-    }
-    if (lane == 0) {
-        red[wave][0] = lo;
-        red[wave][1] = hi;
-        red[wave][2] = full_lo;
-        red[wave][3] = full_hi;
-    }
+    Row me = row_at(a.m, row, min(tile * BM + wave * 32, a.E - 1) / a.G);
+    if (!valid) me = Row{INT_MAX, INT_MIN, 0};
     if (tid < 6) bad[tid >> 1][tid & 1] = 0;
-    const int wlo = __builtin_amdgcn_readfirstlane(lo), whi = __builtin_amdgcn_readfirstlane(hi);
-    __syncthreads();
-    const int blo = __builtin_amdgcn_readfirstlane(min(min(red[0][0], red[1][0]), min(red[2][0], red[3][0])));
-    const int bhi = __builtin_amdgcn_readfirstlane(max(max(red[0][1], red[1][1]), max(red[2][1], red[3][1])));
-    full_lo = __builtin_amdgcn_readfirstlane(max(max(red[0][2], red[1][2]), max(red[2][2], red[3][2])));
-    full_hi = __builtin_amdgcn_readfirstlane(min(min(red[0][3], red[1][3]), min(red[2][3], red[3][3])));
-    const int tiles = bhi > blo ? (bhi - blo + BN - 1) / BN : 0;
+    const Walk w = walk_of(me, valid, red);
+    const int tiles = w.hi > w.lo ? (w.hi - w.lo + BN - 1) / BN : 0;
     const int split = blockIdx.y;
     const int t0 = static_cast<int>(static_cast<long>(tiles) * split / p.splits);
     const int t1 = static_cast<int>(static_cast<long>(tiles) * (split + 1) / p.splits);
@@ -192,21 +183,12 @@ __global__ __launch_bounds__(AT, sizeof(T) == 2 ? 2 : 1) void attn_fwd_k(Fwd p) 
     ks.init(a.K.rs, a.D, tid);
     vs.init(a.V.rs, a.D, tid);
     const auto load = [&](int t, T* tk, T* tv) __attribute__((always_inline)) {
-        const int j = blo + t * BN;
-        ks.load(tk, kb + j * a.K.rs, a.K.rs, bhi - j, a.D, wave);
-        vs.load(tv, vb + j * a.V.rs, a.V.rs, bhi - j, a.D, wave);
+        const int j = w.lo + t * BN;
+        ks.load(tk, kb + j * a.K.rs, a.K.rs, w.hi - j, a.D, wave);
+        vs.load(tv, vb + j * a.V.rs, a.V.rs, w.hi - j, a.D, wave);
     };
-    // Tiles [t0, f0) and [f1, t1) are masked, those between are seen whole by
-    // every row; even numbers of the first two, so that each loop starts at
-    // the first buffer.
-    int f0 = t0, f1 = t0;
-    if (full_hi > full_lo && full_lo <= bhi) {
-        f0 = min(max((full_lo - blo + BN - 1) / BN, t0), t1);
-        f0 = min(f0 + ((f0 - t0) & 1), t1);
-        f1 = min(max((full_hi - blo) / BN, f0), t1);
-        f1 -= (f1 - f0) & 1;
-    }
-    if (f0 >= f1) f0 = f1 = t0;
+    int f0, f1;
+    split_walk(w, t0, t1, f0, f1);
     const auto is_masked = [&](int t) { return t < f0 || t >= f1; };
     // Waits for the thread's own loads of tile t. Values that are not finite
     // become zeros where rows are masked: their product with a probability
@@ -215,8 +197,8 @@ __global__ __launch_bounds__(AT, sizeof(T) == 2 ? 2 : 1) void attn_fwd_k(Fwd p) 
     const auto landed = [&](int t, T* tv) __attribute__((always_inline)) {
         __builtin_amdgcn_s_waitcnt(0);
         if (is_masked(t)) {
-            unsigned* w = bad[(t - t0) % 3];
-            vs.clean(tv, tid, [&](int r) { atomicOr(&w[r >> 5], 1u << (r & 31)); });
+            unsigned* m = bad[(t - t0) % 3];
+            vs.clean(tv, tid, [&](int r) { atomicOr(&m[r >> 5], 1u << (r & 31)); });
         }
     };
     f32x16 acc[ND];
@@ -235,7 +217,7 @@ __global__ __launch_bounds__(AT, sizeof(T) == 2 ? 2 : 1) void attn_fwd_k(Fwd p) 
                 hold<T>();
             }
         }
-        soft_step<decltype(masked)::value>(rule, me, j0, half, s, acc, st);
+        soft_step<decltype(masked)::value>(rule, me, j0 >= w.wfull_lo && j0 + BN <= w.wfull_hi, j0, half, s, acc, st);
 #pragma unroll
         for (int n = 0; n < 2; ++n)
 #pragma unroll
@@ -250,14 +232,14 @@ __global__ __launch_bounds__(AT, sizeof(T) == 2 ? 2 : 1) void attn_fwd_k(Fwd p) 
     };
     const auto walk = [&](auto masked, int t, const T* tk, const T* tv, T* nk, T* nv) __attribute__((always_inline)) {
         constexpr bool MASKED = decltype(masked)::value;
-        const int j0 = blo + t * BN;
+        const int j0 = w.lo + t * BN;
         if (t + 1 < t1) load(t + 1, nk, nv);
         if (tid < 2) bad[(t - t0 + 2) % 3][tid] = 0;
-        if (!MASKED || (wlo < j0 + BN && whi > j0)) {
+        if (!MASKED || (w.wlo < j0 + BN && w.whi > j0)) {
             step(masked, j0, tk, tv);
             if (MASKED) {
-                const unsigned* w = bad[(t - t0) % 3];
-                poison |= sees_bad(me.lo, me.hi, j0, w[0] | static_cast<unsigned long long>(w[1]) << 32);
+                const unsigned* m = bad[(t - t0) % 3];
+                poison |= sees_bad(me.lo, me.hi, j0, m[0] | static_cast<unsigned long long>(m[1]) << 32);
             }
         }
         if (t + 1 < t1) landed(t + 1, nv);
@@ -306,7 +288,7 @@ __global__ __launch_bounds__(AT, 1) void attn_rows_k(Fwd p, int chunks) {
     const int nh = min(32, a.G - 32 * chunk);  // heads of this block
     const bool valid = (lane & 31) < nh;
     const int g = 32 * chunk + (valid ? (lane & 31) : 0), head = kvh * a.G + g, e = row * a.G + g;
-    Row me = row_at(a.m, row);
+    Row me = row_at(a.m, row, row);
     me.lo = __builtin_amdgcn_readfirstlane(me.lo);
     me.hi = __builtin_amdgcn_readfirstlane(me.hi);
     const int keys = me.hi > me.lo ? me.hi - me.lo : 0;
@@ -354,8 +336,7 @@ __global__ __launch_bounds__(AT, 1) void attn_rows_k(Fwd p, int chunks) {
             hold<T>();
         }
         if (t + 4 < t1) load_k(t + 4);
-        if (j0 + RN > me.hi) soft_step<true>(rule, me, j0, half, s, acc, st);
-        else soft_step<false>(rule, me, j0, half, s, acc, st);
+        soft_step<true>(rule, me, j0 + RN <= me.hi, j0, half, s, acc, st);
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
             const Frag<T> w = acc_frag<T>(s[0], c);

@@ -116,12 +116,28 @@ struct Tile {
     }
 };
 
+// A lane's place in a tile, in a register of its own: which tile and which of
+// its row blocks then is the read's own offset. (Left alone, the compiler
+// merges the two and keeps a register per tile and block.)
+__device__ inline int own_reg(int at) {
+    asm("" : "+v"(at));
+    return at;
+}
+
 // The depth-16 step c of a tile as an operand whose rows are the tile's rows
 // row0 .. row0 + 31, depth along the tile's columns.
 template <class T, int DP>
 __device__ inline Frag<T> lds_rows(const T* tile, int row0, int c) {
     const int l = threadIdx.x & 63;
-    return Tile<T, DP>::get8(tile, row0 + (l & 31), 2 * c + (l >> 5));
+    typedef Tile<T, DP> Tl;
+    if constexpr (sizeof(T) == 2) {
+        return *reinterpret_cast<const Frag<T>*>(tile + row0 * DP + own_reg(Tl::at(l & 31, 2 * c + (l >> 5))));
+    } else {
+        const float* p = tile + row0 * DP;
+        const f32x4 a = *reinterpret_cast<const f32x4*>(p + own_reg(Tl::at(l & 31, 4 * c + 2 * (l >> 5))));
+        const f32x4 b = *reinterpret_cast<const f32x4*>(p + own_reg(Tl::at(l & 31, 4 * c + 2 * (l >> 5) + 1)));
+        return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+    }
 }
 
 // A tile's columns col0 .. col0 + 31 as an operand's rows, depth along the 16
@@ -132,12 +148,13 @@ template <int DP, bool ACC>
 __device__ inline bf16x8 lds_cols(const bf16* tile, int row0, int col0) {
     typedef __attribute__((address_space(3))) short4v lds4;
     const int l = threadIdx.x & 63;
-    const int row = row0 + (ACC ? 4 : 8) * (l >> 5) + (l >> 2 & 3), col = col0 + 16 * (l >> 4 & 1) + 4 * (l & 3);
+    // row0 is a multiple of 16, after which the permutation repeats
+    const int row = (ACC ? 4 : 8) * (l >> 5) + (l >> 2 & 3), col = col0 + 16 * (l >> 4 & 1) + 4 * (l & 3);
     union { short4v s[2]; bf16x8 v; } u;
 #pragma unroll
     for (int i = 0; i < 2; ++i)
         u.s[i] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-            (lds4*)(tile + Tile<bf16, DP>::at(row + (ACC ? 8 : 4) * i, col >> 3) + (col & 7)));
+            (lds4*)(tile + row0 * DP + own_reg(Tile<bf16, DP>::at(row + (ACC ? 8 : 4) * i, col >> 3) + (col & 7))));
     return u.v;
 }
 template <int DP, bool ACC>
@@ -149,8 +166,7 @@ __device__ inline f32x8 lds_cols(const float* tile, int row0, int col0) {
     for (int i = 0; i < 8; ++i) {
         const int r = ACC ? 8 * (i >> 2) + (i & 3) : i;  // row0 is a multiple of 16, col0 of 32
         const int low = ACC ? 4 * half + (i & 3) : i;    // the row's low three bits
-        int at = (ACC ? 4 : 8) * half * DP + 4 * (((l & 31) >> 2) ^ low) + (l & 3);
-        asm("" : "+v"(at));  // one register for every tile row and column: the rest is the read's own offset
+        const int at = own_reg((ACC ? 4 : 8) * half * DP + 4 * (((l & 31) >> 2) ^ low) + (l & 3));
         f[i] = tile[at + (row0 + r) * DP + col0];
     }
     return f;
