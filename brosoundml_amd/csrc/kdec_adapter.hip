@@ -1,15 +1,17 @@
 // A projection shared by all rows with low-rank adapters that each row
 // chooses, on gfx950, forward and backward.
 //
-// Rows are sorted by adapter first (a counting sort that keeps their order),
-// so a tile of rows meets few adapters. Then
-//   H = A xd        the rows' low-rank inputs, one small product per tile
-//   Y = W x + b + s B H   one matrix product; a tile's own low-rank products
-//                   go into its accumulators before the walk over the depth
+// With many rows they are sorted by adapter first (a counting sort that keeps
+// their order) and cut into pieces of one adapter each. Then
+//   H = s A xd       the rows' low-rank inputs, one small product per piece
+//   Y = W x + b + B H  one matrix product; a tile's own low-rank products
+//                    go into its accumulators before the walk over the depth
 // and backward
-//   dH = s B^T dy,  dX = W^T dy + drop(A^T dH),  dA = dH^T xd,  dB = s H^T dy.
+//   dH = s B^T dy,  dX = W^T dy + drop(A^T dH),  dA = dH^T xd,  dB = H^T dy.
 // Low-rank values H and dH stay float; where they meet a bf16 operand in the
-// matrix units they are split into bf16 terms (kdec_frag.hpp).
+// matrix units they are split into bf16 terms (kdec_frag.hpp). Few rows go
+// without the sort: a row's H is a block's work, and a block of the product
+// holds all rows.
 #include "kdec_frag.hpp"
 #include "kdec_internal.hpp"
 #include "kdec_philox.hpp"
@@ -20,9 +22,18 @@
 namespace kdec {
 namespace {
 
-constexpr int NT = 256;   // threads of a block
-constexpr int ST = 1024;  // threads of the sort
+constexpr int NT = 256;            // threads of a product's block
+constexpr int LT = 512;            // threads of the low-rank kernels' blocks, 8 waves
+constexpr int ST = 1024;           // threads of the sort
 constexpr int GM = 128, GN = 128;  // features and rows of a product tile
+constexpr int PIECE = 32;          // sorted rows of a piece
+constexpr int CHUNK = 256;         // sorted rows of a chunk, the adapters' gradients' unit of work
+constexpr int FEW = 64;            // rows that one block of the product holds whole
+
+// Sorted rows [start, start + count) of one adapter (n: none).
+struct Piece {
+    int start, count, adapter, pad;
+};
 
 struct Adapter {
     const void *X, *W, *bias, *A, *B, *dY;
@@ -32,8 +43,9 @@ struct Adapter {
     int T, in, out, n, units, rank, R;  // R = units * rank
     Drop drop;
     bool dropping;
-    const int *perm, *seg;  // sorted rows; adapter a's are [seg[a], seg[a+1]), those without any from seg[n]
-    float *H, *dH;          // (T, R)
+    const int* perm;              // sorted rows
+    const Piece *pieces, *chunks;
+    float *H, *dH;                // (T, R), with the adapters' scales
     bool vec_x, vec_w, vec_a, vec_b, vec_dy, vec_h;
 };
 
@@ -42,9 +54,23 @@ __device__ inline int adapter_of(const Adapter& p, int row) {
     return a >= 0 && a < p.n ? a : p.n;
 }
 
+// The unit that holds output row m: how many of the offsets 1 .. units - 1 are
+// not past it, 64 at a time (all lanes of the wave take part).
+__device__ inline int unit_at(const int* off, int units, int m) {
+    const int lane = threadIdx.x & 63;
+    int u = 0;
+    for (int b = 1; b < units; b += 64)
+        u += __builtin_popcountll(__builtin_amdgcn_ballot_w64(b + lane < units && off[b + lane] <= m));
+    return u;
+}
+
 // Block a places adapter a's rows (a = n: the rows without one): every thread
-// counts a run of rows, the counts are scanned, and the rows written in order.
-__global__ __launch_bounds__(ST) void adapter_sort_k(const int* idx, int T, int n, int* perm, int* seg) {
+// counts a run of rows, the counts are scanned, and the rows written in
+// order. Its pieces (and chunks) are the windows of PIECE (CHUNK) sorted
+// places that its rows meet. They start at table entry start / window + a,
+// which no other adapter's reach: an adapter of c rows meets at most
+// c / window + 1 windows; entries up to the next adapter's first are empty.
+__global__ __launch_bounds__(ST) void adapter_sort_k(const int* idx, int T, int n, int* perm, Piece* pieces, Piece* chunks) {
     __shared__ int less_sum[ST / 64], eq_sum[ST / 64];
     const int a = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int per = (T + ST - 1) / ST;
@@ -68,15 +94,22 @@ __global__ __launch_bounds__(ST) void adapter_sort_k(const int* idx, int T, int 
         eq_sum[wave] = before;
     }
     __syncthreads();
-    int at = before - eq;
+    int at = before - eq, start = 0, count = 0;
     for (int w = 0; w < ST / 64; ++w) {
-        at += less_sum[w];
+        start += less_sum[w];
+        count += eq_sum[w];
         if (w < wave) at += eq_sum[w];
     }
-    if (tid == 0) {
-        seg[a] = at;
-        if (a == n) seg[n + 1] = T;
-    }
+    at += start;
+    const auto table = [&](Piece* to, int window) {
+        const int first = start / window, next = (start + count) / window + a + 1;
+        for (int i = first + a + tid; i < next; i += ST) {
+            const int w = i - a, s = max(start, w * window);
+            to[i] = Piece{s, max(min(start + count, (w + 1) * window) - s, 0), a, 0};
+        }
+    };
+    table(pieces, PIECE);
+    table(chunks, CHUNK);
     for (int t = t0; t < t1; ++t) {
         int id = idx[t];
         if (id < 0 || id >= n) id = n;
@@ -96,88 +129,137 @@ __device__ inline Frag<T> dropped(const Drop& d, int row, int col, Frag<T> f) {
     return f;
 }
 
-// The sum of the four waves' accumulators over a 32 x 32 block, handed to
-// f(row, column, sum) by all threads.
+// The sum of eight waves' accumulators over a 32 x 32 block, handed to
+// f(row, column, sum) by all threads, rows running fastest.
+typedef float Join8[32][33];
 template <class F>
-__device__ inline void join_waves(float (&buf)[4][32][33], const f32x16& acc, F f) {
+__device__ inline void join8(Join8* buf, const f32x16& acc, F f) {
     const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
 #pragma unroll
     for (int r = 0; r < 16; ++r) buf[wave][acc_row(r, lane >> 5)][lane & 31] = acc[r];
     __syncthreads();
-    for (int e = tid; e < 1024; e += NT) {
+    for (int e = tid; e < 1024; e += LT) {
         const int m = e & 31, c = e >> 5;
-        f(m, c, (buf[0][m][c] + buf[1][m][c]) + (buf[2][m][c] + buf[3][m][c]));
+        float s = buf[0][m][c];
+#pragma unroll
+        for (int w = 1; w < 8; ++w) s += buf[w][m][c];
+        f(m, c, s);
     }
     __syncthreads();
 }
 
-// H: 32 sorted rows by 32 of the R low-rank columns per block, the depth
-// split over its waves; one product per adapter that the rows meet.
-template <class T>
-__global__ __launch_bounds__(NT) void adapter_h_k(Adapter p) {
-    __shared__ float buf[4][32][33];
-    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, half = lane >> 5;
-    const int s0 = blockIdx.x * 32, m0 = blockIdx.y * 32, ns = min(32, p.T - s0);
-    const int col = lane & 31, row = col < ns ? p.perm[s0 + col] : 0;
-    const int m = m0 + col;
-    const T* x = static_cast<const T*>(p.X) + row * p.x_rs;
-    for (int s = s0; s < s0 + ns;) {
-        const int a = adapter_of(p, p.perm[s]), end = min(p.seg[a + 1], s0 + ns);
-        f32x16 acc = f32x16{};
-        if (a < p.n) {
-            const T* w = static_cast<const T*>(p.A) + (static_cast<long>(a) * p.R + (m < p.R ? m : 0)) * p.in;
-            for (int k = 16 * wave; k < p.in; k += 64) {
-                const int d = k + 8 * half;
-                Frag<T> f = load8(x + d, col < ns ? min(8, p.in - d) : 0, p.vec_x);
-                if (p.dropping) f = dropped<T>(p.drop, row, d, f);
-                acc = mma32(load8(w + d, m < p.R ? min(8, p.in - d) : 0, p.vec_a), f, acc);
+// H: a piece's rows (or, unsorted, one row) by 32 MT of the R low-rank columns
+// per block, the depth split over its eight waves, four steps' loads in flight.
+template <class T, int MT>
+__global__ __launch_bounds__(LT) void adapter_h_k(Adapter p) {
+    __shared__ Join8 buf[8];
+    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, half = lane >> 5, col = lane & 31;
+    const int m0 = blockIdx.y * 32 * MT;
+    int start = 0, count = 1, a, row;
+    if (p.pieces) {
+        const Piece pc = p.pieces[blockIdx.x];
+        start = pc.start;
+        count = pc.count;
+        a = pc.adapter;
+        if (!count) return;
+        row = p.perm[start + min(col, count - 1)];
+    } else {
+        row = blockIdx.x;
+        a = adapter_of(p, row);
+    }
+    const auto row_of = [&](int c) { return p.pieces ? p.perm[start + c] : static_cast<int>(blockIdx.x); };
+    f32x16 acc[MT];
+#pragma unroll
+    for (int i = 0; i < MT; ++i) acc[i] = f32x16{};
+    float f = 0.0f;
+    if (a < p.n) {
+        f = p.scale[a] * (p.dropping ? p.drop.keep : 1.0f);
+        const T* x = static_cast<const T*>(p.X) + row * p.x_rs;
+        const T* w[MT];
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+            w[i] = static_cast<const T*>(p.A) + (static_cast<long>(a) * p.R + min(m0 + 32 * i + col, p.R - 1)) * p.in;
+        for (int k = 16 * wave; k < p.in; k += 512) {
+            Frag<T> z[4], g[4][MT];
+#pragma unroll
+            for (int s = 0; s < 4; ++s) {
+                const int d = k + 128 * s + 8 * half, n = min(8, p.in - d);
+                z[s] = load8(x + (n > 0 ? d : 0), col < count ? n : 0, p.vec_x);
+#pragma unroll
+                for (int i = 0; i < MT; ++i) g[s][i] = load8(w[i] + (n > 0 ? d : 0), m0 + 32 * i + col < p.R ? n : 0, p.vec_a);
+            }
+#pragma unroll
+            for (int s = 0; s < 4; ++s) {
+                if (p.dropping) z[s] = dropped<T>(p.drop, row, k + 128 * s + 8 * half, z[s]);
+#pragma unroll
+                for (int i = 0; i < MT; ++i) acc[i] = mma32(g[s][i], z[s], acc[i]);
             }
         }
-        join_waves(buf, acc, [&](int c, int t, float v) {
-            if (t >= s - s0 && t < end - s0 && m0 + c < p.R)
-                p.H[static_cast<long>(p.perm[s0 + t]) * p.R + m0 + c] = p.dropping ? v * p.drop.keep : v;
-        });
-        s = end;
     }
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+        join8(buf, acc[i], [&](int m, int c, float v) {
+            if (c < count && m0 + 32 * i + m < p.R) p.H[static_cast<long>(row_of(c)) * p.R + m0 + 32 * i + m] = v * f;
+        });
 }
 
-// dH: as H, over a unit's output rows; B holds them row by row, so a lane
-// gathers its eight depths.
+// dH: a piece's rows by 32 low-rank columns of one unit per block. The
+// depth is the unit's output rows, RT at a time per wave; B's rows go through
+// the wave's shared memory, from which the product reads their columns.
 template <class T>
-__global__ __launch_bounds__(NT) void adapter_dh_k(Adapter p) {
-    __shared__ float buf[4][32][33];
-    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, half = lane >> 5;
-    const int jt = (p.rank + 31) / 32, unit = blockIdx.y / jt, m0 = 32 * (blockIdx.y % jt);
-    const int s0 = blockIdx.x * 32, ns = min(32, p.T - s0);
-    const int col = lane & 31, row = col < ns ? p.perm[s0 + col] : 0;
-    const int m = m0 + col;
+__global__ __launch_bounds__(LT) void adapter_dh_k(Adapter p) {
+    constexpr int RT = sizeof(T) == 2 ? 64 : 32, DPB = 64, NB = RT * 4 / 64;
+    __shared__ __align__(16) char smem[8 * RT * DPB * sizeof(T)];
+    static_assert(sizeof(smem) >= 8 * sizeof(Join8), "the waves are joined in the tiles' place");
+    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, half = lane >> 5, col = lane & 31;
+    const Piece pc = p.pieces[blockIdx.x];
+    if (!pc.count) return;
+    const int jt = (p.rank + 31) / 32, unit = blockIdx.y / jt, m0 = 32 * (blockIdx.y % jt), a = pc.adapter;
     const int u0 = min(max(p.unit_off[unit], 0), p.out), u1 = min(max(p.unit_off[unit + 1], u0), p.out);
-    const T* y = static_cast<const T*>(p.dY) + row * p.dy_rs;
-    for (int s = s0; s < s0 + ns;) {
-        const int a = adapter_of(p, p.perm[s]), end = min(p.seg[a + 1], s0 + ns);
-        f32x16 acc = f32x16{};
-        float sc = 0.0f;
-        if (a < p.n) {
-            sc = p.scale[a];
-            const T* w = static_cast<const T*>(p.B) + static_cast<long>(a) * p.out * p.rank + (m < p.rank ? m : 0);
-            for (int k = (u0 & ~15) + 16 * wave; k < u1; k += 64) {
-                const int d = k + 8 * half;
-                Frag<T> f = load8(y + d, col < ns ? min(8, p.out - d) : 0, p.vec_dy), g;
+    const int row = p.perm[pc.start + min(col, pc.count - 1)];
+    T* tile = reinterpret_cast<T*>(smem) + wave * RT * DPB;
+    f32x16 acc = f32x16{};
+    float f = 0.0f;
+    if (a < p.n) {
+        f = p.scale[a];
+        const T* y = static_cast<const T*>(p.dY) + row * p.dy_rs;
+        const T* b = static_cast<const T*>(p.B) + static_cast<long>(a) * p.out * p.rank + m0;
+        for (int r0 = (u0 & ~7) + RT * wave; r0 < u1; r0 += 8 * RT) {
+            Frag<T> z[RT / 16], w[NB];
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const bool in = d + i >= u0 && d + i < u1;
-                    g[i] = in && m < p.rank ? w[static_cast<long>(d + i) * p.rank] : static_cast<T>(0.0f);
-                    if (!in) f[i] = static_cast<T>(0.0f);
-                }
-                acc = mma32(g, f, acc);
+            for (int c = 0; c < RT / 16; ++c) {
+                const int d = r0 + 16 * c + 8 * half;
+                z[c] = load8(y + min(d, p.out), col < pc.count ? min(8, p.out - d) : 0, p.vec_dy);
             }
+#pragma unroll
+            for (int i = 0; i < NB; ++i) {
+                const int e = lane + 64 * i, r = r0 + (e >> 2), j = 8 * (e & 3);
+                const bool in = r >= u0 && r < u1 && m0 + j < p.rank;
+                w[i] = load8(b + (in ? static_cast<long>(r) * p.rank + j : 0), in ? min(8, p.rank - m0 - j) : 0, p.vec_b);
+            }
+#pragma unroll
+            for (int i = 0; i < NB; ++i) {
+                const int e = lane + 64 * i;
+                Tile<T, DPB>::put8(tile, e >> 2, e & 3, w[i]);
+            }
+            if (r0 < u0 || r0 + RT > u1) {  // other units' outputs, whatever they hold
+#pragma unroll
+                for (int c = 0; c < RT / 16; ++c)
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const int d = r0 + 16 * c + 8 * half + i;
+                        if (d < u0 || d >= u1) z[c][i] = static_cast<T>(0.0f);
+                    }
+            }
+#pragma unroll
+            for (int c = 0; c < RT / 16; ++c) acc = mma32(lds_cols<DPB, false>(tile, 16 * c, 0), z[c], acc);
         }
-        join_waves(buf, acc, [&](int c, int t, float v) {
-            if (t >= s - s0 && t < end - s0 && m0 + c < p.rank)
-                p.dH[static_cast<long>(p.perm[s0 + t]) * p.R + unit * p.rank + m0 + c] = v * sc;
-        });
-        s = end;
     }
+    __syncthreads();
+    join8(reinterpret_cast<Join8*>(smem), acc, [&](int c, int t, float v) {
+        if (t < pc.count && m0 + c < p.rank)
+            p.dH[static_cast<long>(p.perm[pc.start + t]) * p.R + unit * p.rank + m0 + c] = v * f;
+    });
 }
 
 // The product tile's operands: M features (W's rows forward, its columns
@@ -196,21 +278,94 @@ struct Product {
 
 template <class T> constexpr int depth_of() { return sizeof(T) == 2 ? 64 : 32; }  // of a tile: 128 bytes
 
-// One 128 x 128 tile: forward Y = W X (+ bias + s B H), backward
+// The low-rank products of a wave's 64 features (from wm) and up to 64 rows
+// (a lane each: its row and adapter), into acc: forward B H, backward A^T dH.
+// Adapters and units are taken in turn by `turns` takers of which this is
+// number `turn`.
+template <class T, bool BWD, int MB, int NB>
+__device__ inline void low_rank(const Adapter& p, int M, int wm, int u0, int u1, int row, int id, int turn, int turns,
+                                f32x16 (&acc)[MB][NB]) {
+    const int lane = threadIdx.x & 63, half = lane >> 5, col = lane & 31;
+    const float* H = BWD ? p.dH : p.H;
+    unsigned long long left = __builtin_amdgcn_ballot_w64(id < p.n);
+    int rows[NB], ids[NB];
+#pragma unroll
+    for (int j = 0; j < NB; ++j) {
+        rows[j] = __shfl(row, 32 * j + col);
+        ids[j] = __shfl(id, 32 * j + col);
+    }
+    int item = 0;
+    while (left) {
+        const int a = __shfl(id, __builtin_ctzll(left));
+        const unsigned long long mine = __builtin_amdgcn_ballot_w64(id == a);
+        left &= ~mine;
+        for (int u = u0; u < u1; ++u) {
+            if (item++ % turns != turn) continue;
+            const int lo = BWD ? 0 : p.unit_off[u], hi = BWD ? M : p.unit_off[u + 1];
+            f32x16 tmp[MB][NB];
+#pragma unroll
+            for (int i = 0; i < MB; ++i)
+#pragma unroll
+                for (int j = 0; j < NB; ++j) tmp[i][j] = f32x16{};
+            for (int k = 0; k < p.rank; k += 16) {
+                const int d = k + 8 * half, n = min(8, p.rank - d), dd = n > 0 ? d : 0;
+                Frag<T> w[MB];
+                f32x8 h[NB];
+#pragma unroll
+                for (int j = 0; j < NB; ++j)
+                    h[j] = load8(H + static_cast<long>(rows[j]) * p.R + u * p.rank + dd, ids[j] == a ? n : 0, p.vec_h);
+#pragma unroll
+                for (int i = 0; i < MB; ++i) {
+                    const int m = wm + 32 * i + col;
+                    const bool in = m >= lo && m < hi && m < M;
+                    if (BWD) {  // A's columns
+                        const T* q = static_cast<const T*>(p.A) + (static_cast<long>(a) * p.R + u * p.rank) * p.in + (in ? m : 0);
+#pragma unroll
+                        for (int x = 0; x < 8; ++x)
+                            w[i][x] = in && x < n ? q[static_cast<long>(d + x) * p.in] : static_cast<T>(0.0f);
+                    } else {
+                        const T* q = static_cast<const T*>(p.B) + (static_cast<long>(a) * p.out + (in ? m : 0)) * p.rank;
+                        w[i] = load8(q + dd, in ? n : 0, p.vec_b);
+                    }
+                }
+#pragma unroll
+                for (int j = 0; j < NB; ++j) {
+                    if (!(mine >> (32 * j) & 0xFFFFFFFFull)) continue;
+                    const Terms<T, 2> v(h[j]);
+#pragma unroll
+                    for (int x = 0; x < v.n; ++x)
+#pragma unroll
+                        for (int i = 0; i < MB; ++i) tmp[i][j] = mma32(w[i], v.t[x], tmp[i][j]);
+                }
+            }
+            // only this adapter's rows take the product, whatever another's would be
+#pragma unroll
+            for (int j = 0; j < NB; ++j)
+                if (ids[j] == a)
+#pragma unroll
+                    for (int i = 0; i < MB; ++i)
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) acc[i][j][r] += tmp[i][j][r];
+        }
+    }
+}
+
+// One 128 x 128 tile: forward Y = W X (+ bias + B H), backward
 // dX = W^T dY (+ drop(A^T dH)). Features are the accumulators' rows, so a
 // lane holds one token's run of features. Four waves of 64 x 64. Rows of W
 // lie along the depth forward and across it backward, where the transposing
-// LDS read turns them.
-template <class T, bool BWD>
-__global__ __launch_bounds__(NT, 1) void adapter_gemm_k(Adapter p, Product g) {
-    constexpr int BK = depth_of<T>(), WC = (BWD ? GM : BK) / 8;
+// LDS read turns them. Tiles are copied straight to shared memory, two
+// buffers deep (DIRECT), or go through registers where alignment or size
+// rule that out.
+template <class T, bool BWD, bool DIRECT>
+__global__ __launch_bounds__(NT, DIRECT ? 2 : 1) void adapter_gemm_k(Adapter p, Product g) {
+    constexpr int BK = depth_of<T>(), WC = (BWD ? GM : BK) / 8, WR = BWD ? BK : GM;
     typedef Tile<T, BWD ? GM : BK> Tw;
     typedef Tile<T, BK> Tz;
     constexpr int NZ = GN * BK / 8 / NT, NW = GM * BK / 8 / NT;
-    __shared__ __align__(16) T sw[GM * BK];
-    __shared__ __align__(16) T sz[GN * BK];
+    __shared__ __align__(256) T sw0[GM * BK], sw1[GM * BK], sz0[GN * BK], sz1[GN * BK];
     __shared__ int srow[GN], sid[GN];
-    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, half = lane >> 5, col = lane & 31;
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, half = lane >> 5, col = lane & 31;
     const int mt = (g.M + GM - 1) / GM;
     const int m0 = (blockIdx.x % mt) * GM, s0 = (blockIdx.x / mt) * GN, ns = min(GN, p.T - s0), split = blockIdx.y;
     if (tid < GN) {
@@ -220,74 +375,79 @@ __global__ __launch_bounds__(NT, 1) void adapter_gemm_k(Adapter p, Product g) {
     }
     __syncthreads();
     const int wm = m0 + 64 * (wave & 1), wn = 64 * (wave >> 1);
+    const int steps = (g.K + BK - 1) / BK;
+    const int c0 = static_cast<int>(static_cast<long>(steps) * split / g.splits);
+    const int c1 = static_cast<int>(static_cast<long>(steps) * (split + 1) / g.splits);
+    const T* W = static_cast<const T*>(p.W);
+    const T* Z = static_cast<const T*>(g.Z);
+
+    // direct copies: a thread's units of both tiles
+    Copy<T, BWD ? GM : BK, WR, NT> cw;
+    constexpr int NU = Tz::NU, NZU = GN * NU / NT;
+    unsigned oz[NZU];
+    __amdgpu_buffer_rsrc_t rz = rows_rsrc<T>(Z, 0, 0, 0);
+    const auto z_offsets = [&](int depth) __attribute__((always_inline)) {  // columns of the tile that are there
+#pragma unroll
+        for (int i = 0; i < NZU; ++i) {
+            const int u = tid + i * NT, r = u / NU, c = Tz::U * ((u % NU) ^ Tz::swz(r));
+            oz[i] = r < ns && c < depth ? static_cast<unsigned>((srow[r] * g.z_rs + c) * static_cast<long>(sizeof(T))) : 0xFFFFFFF0u;
+        }
+    };
+    if (DIRECT) {
+        cw.init(BWD ? g.M : g.K, BWD ? g.M - m0 : g.K - c0 * BK, tid);
+        z_offsets(g.K - c0 * BK);
+        rz = uniform_rsrc(Z, static_cast<int>(((p.T - 1) * g.z_rs + g.K) * static_cast<long>(sizeof(T))));
+    }
+    Frag<T> fw[DIRECT ? 1 : NW], fz[DIRECT ? 1 : NZ];
+    const auto load = [&](int c, T* tw, T* tz) __attribute__((always_inline)) {
+        const int k0 = c * BK;
+        if constexpr (DIRECT) {
+            if (c > c0 && k0 + BK > g.K) {  // the last, narrower step
+                if (!BWD) cw.init(g.K, g.K - k0, tid);
+                z_offsets(g.K - k0);
+            }
+            if (BWD) cw.load(tw, W + static_cast<long>(k0) * g.M + m0, g.M, g.K - k0, min(GM, g.M - m0), wave);
+            else cw.load(tw, W + static_cast<long>(m0) * g.K + k0, g.K, g.M - m0, min(BK, g.K - k0), wave);
+#pragma unroll
+            for (int i = 0; i < NZU; ++i)
+                copy16(rz, tz + (64 * wave + i * NT) * Tz::U,
+                       static_cast<int>(oz[i] == 0xFFFFFFF0u ? oz[i] : oz[i] + static_cast<unsigned>(k0 * sizeof(T))));
+        } else {
+#pragma unroll
+            for (int i = 0; i < NZ; ++i) {
+                const int e = tid + i * NT, t = e / (BK / 8), d = k0 + 8 * (e % (BK / 8));
+                fz[i] = load8(Z + srow[t] * g.z_rs + min(d, g.K), t < ns ? min(8, g.K - d) : 0, g.vec_z);
+            }
+#pragma unroll
+            for (int i = 0; i < NW; ++i) {
+                const int e = tid + i * NT, r = e / WC, d = 8 * (e % WC);
+                const bool in = BWD ? k0 + r < g.K : m0 + r < g.M;
+                const long at = BWD ? static_cast<long>(k0 + r) * g.M + m0 + d : static_cast<long>(m0 + r) * g.K + k0 + d;
+                const int n = BWD ? g.M - m0 - d : g.K - k0 - d;
+                fw[i] = load8(W + (in && n > 0 ? at : 0), in ? min(8, n) : 0, p.vec_w);
+            }
+        }
+    };
+    const auto landed = [&](T* tw, T* tz) __attribute__((always_inline)) {
+        if constexpr (DIRECT) {
+            __builtin_amdgcn_s_waitcnt(0);
+        } else {
+#pragma unroll
+            for (int i = 0; i < NZ; ++i) Tz::put8(tz, (tid + i * NT) / (BK / 8), (tid + i * NT) % (BK / 8), fz[i]);
+#pragma unroll
+            for (int i = 0; i < NW; ++i) Tw::put8(tw, (tid + i * NT) / WC, (tid + i * NT) % WC, fw[i]);
+        }
+    };
     f32x16 acc[2][2];
 #pragma unroll
     for (int i = 0; i < 2; ++i)
 #pragma unroll
         for (int j = 0; j < 2; ++j) acc[i][j] = f32x16{};
-
-    // the rows' adapters; splits take them in turn
-    int turn = 0;
-    for (int s = s0; s < s0 + ns;) {
-        const int a = sid[s - s0], end = min(p.seg[a + 1], s0 + ns), s_end = end - s0;
-        const bool mine = a < p.n && turn++ % g.splits == split && s - s0 < wn + 64 && s_end > wn;
-        s = end;
-        if (!mine) continue;
-        const float sc = BWD ? 1.0f : p.scale[a];
-        const float* H = BWD ? p.dH : p.H;
-        int u0 = 0, u1 = p.units;
-        if (!BWD) {  // the units that meet the wave's features
-            while (u0 + 1 < p.units && p.unit_off[u0 + 1] <= wm) ++u0;
-            u1 = u0 + 1;
-            while (u1 < p.units && p.unit_off[u1] < wm + 64) ++u1;
-        }
-        for (int u = u0; u < u1; ++u) {
-            const int lo = BWD ? 0 : p.unit_off[u], hi = BWD ? g.M : p.unit_off[u + 1];
-            f32x16 tmp[2][2];
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-#pragma unroll
-                for (int j = 0; j < 2; ++j) tmp[i][j] = f32x16{};
-            for (int k = 0; k < p.rank; k += 16) {
-                const int d = k + 8 * half;
-                Frag<T> w[2];
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const int m = wm + 32 * i + col;
-                    const bool in = m >= lo && m < hi && m < g.M;
-                    if (BWD) {  // A's columns
-                        const T* q = static_cast<const T*>(p.A) + (static_cast<long>(a) * p.R + u * p.rank) * p.in + (in ? m : 0);
-#pragma unroll
-                        for (int x = 0; x < 8; ++x)
-                            w[i][x] = in && d + x < p.rank ? q[static_cast<long>(d + x) * p.in] : static_cast<T>(0.0f);
-                    } else {
-                        const T* q = static_cast<const T*>(p.B) + (static_cast<long>(a) * p.out + (in ? m : 0)) * p.rank;
-                        w[i] = load8(q + (d < p.rank ? d : 0), in ? min(8, p.rank - d) : 0, p.vec_b);
-                    }
-                }
-#pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    const int t = wn + 32 * j + col;
-                    const float* h = H + static_cast<long>(srow[t]) * p.R + u * p.rank;
-                    f32x8 f = load8(h + (d < p.rank ? d : 0), t < ns ? min(8, p.rank - d) : 0, p.vec_h);
-#pragma unroll
-                    for (int x = 0; x < 8; ++x) f[x] *= sc;
-                    const Terms<T, 2> v(f);
-#pragma unroll
-                    for (int x = 0; x < v.n; ++x)
-#pragma unroll
-                        for (int i = 0; i < 2; ++i) tmp[i][j] = mma32(w[i], v.t[x], tmp[i][j]);
-                }
-            }
-            // only this adapter's rows take the product, whatever another's would be
-#pragma unroll
-            for (int j = 0; j < 2; ++j)
-                if (sid[wn + 32 * j + col] == a)
-#pragma unroll
-                    for (int i = 0; i < 2; ++i)
-#pragma unroll
-                        for (int r = 0; r < 16; ++r) acc[i][j][r] += tmp[i][j][r];
-        }
+    if (c0 < c1) load(c0, sw0, sz0);
+    {
+        const int u0 = BWD ? 0 : unit_at(p.unit_off, p.units, wm);
+        const int u1 = BWD ? p.units : unit_at(p.unit_off, p.units, min(wm + 63, g.M - 1)) + 1;
+        low_rank<T, BWD, 2, 2>(p, g.M, wm, u0, u1, srow[wn + lane], sid[wn + lane], split, g.splits, acc);
     }
     if (BWD && p.dropping) {
 #pragma unroll
@@ -307,62 +467,33 @@ __global__ __launch_bounds__(NT, 1) void adapter_gemm_k(Adapter p, Product g) {
                     }
                 }
     }
-
-    const int steps = (g.K + BK - 1) / BK;
-    const int c0 = static_cast<int>(static_cast<long>(steps) * split / g.splits);
-    const int c1 = static_cast<int>(static_cast<long>(steps) * (split + 1) / g.splits);
-    Frag<T> fw[NW], fz[NZ];
-    const auto load = [&](int c) {
-        const int k0 = c * BK;
-#pragma unroll
-        for (int i = 0; i < NZ; ++i) {
-            const int e = tid + i * NT, t = e / (BK / 8), d = k0 + 8 * (e % (BK / 8));
-            fz[i] = load8(static_cast<const T*>(g.Z) + srow[t] * g.z_rs + d, t < ns ? min(8, g.K - d) : 0, g.vec_z);
-        }
-#pragma unroll
-        for (int i = 0; i < NW; ++i) {
-            const int e = tid + i * NT, r = e / WC, d = 8 * (e % WC);
-            if (BWD) {
-                const bool in = k0 + r < g.K;
-                fw[i] = load8(static_cast<const T*>(p.W) + static_cast<long>(in ? k0 + r : 0) * g.M + m0 + d,
-                              in ? min(8, g.M - m0 - d) : 0, p.vec_w);
-            } else {
-                const bool in = m0 + r < g.M;
-                fw[i] = load8(static_cast<const T*>(p.W) + static_cast<long>(in ? m0 + r : 0) * g.K + k0 + d,
-                              in ? min(8, g.K - k0 - d) : 0, p.vec_w);
-            }
-        }
-    };
-    if (c0 < c1) load(c0);
-    for (int c = c0; c < c1; ++c) {
-#pragma unroll
-        for (int i = 0; i < NZ; ++i) {
-            const int e = tid + i * NT;
-            Tz::put8(sz, e / (BK / 8), e % (BK / 8), fz[i]);
-        }
-#pragma unroll
-        for (int i = 0; i < NW; ++i) {
-            const int e = tid + i * NT;
-            Tw::put8(sw, e / WC, e % WC, fw[i]);
-        }
-        __syncthreads();
-        if (c + 1 < c1) load(c + 1);
+    const auto walk = [&](int c, const T* tw, const T* tz, T* nw, T* nz) __attribute__((always_inline)) {
+        if (c + 1 < c1) load(c + 1, nw, nz);
 #pragma unroll
         for (int k = 0; k < BK / 16; ++k) {
             Frag<T> w[2], z[2];
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
                 const int m = 64 * (wave & 1) + 32 * i;
-                if constexpr (BWD) w[i] = lds_cols<GM, false>(sw, 16 * k, m);
-                else w[i] = lds_rows<T, BK>(sw, m, k);
-                z[i] = lds_rows<T, BK>(sz, wn + 32 * i, k);
+                if constexpr (BWD) w[i] = lds_cols<GM, false>(tw, 16 * k, m);
+                else w[i] = lds_rows<T, BK>(tw, m, k);
+                z[i] = lds_rows<T, BK>(tz, wn + 32 * i, k);
             }
 #pragma unroll
             for (int i = 0; i < 2; ++i)
 #pragma unroll
                 for (int j = 0; j < 2; ++j) acc[i][j] = mma32(w[i], z[j], acc[i][j]);
         }
+        if (c + 1 < c1) landed(nw, nz);
         __syncthreads();
+    };
+    if (c0 < c1) {
+        landed(sw0, sz0);
+        __syncthreads();
+    }
+    for (int c = c0; c < c1; c += 2) {
+        walk(c, sw0, sz0, sw1, sz1);
+        if (c + 1 < c1) walk(c + 1, sw1, sz1, sw0, sz0);
     }
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
@@ -394,72 +525,162 @@ __global__ __launch_bounds__(NT) void adapter_join_k(const float* part, int spli
     const long e = static_cast<long>(blockIdx.x) * NT + threadIdx.x;
     if (e >= n) return;
     float s = 0.0f;
+#pragma unroll 8
     for (int i = 0; i < splits; ++i) s += part[i * n + e];
     const long row = e / M;
     Y[row * y_rs + (e - row * M)] = static_cast<T>(s);
 }
 
-// Sums over an adapter's rows: C[m, c] = f sum_t P[t, m] Z[t, c] for 32
-// columns m of the float matrix P (H or dH, width R) and 128 columns c of X or
-// dY. dA = dH^T drop(X): all of P's columns. dB^T = s H^T dY: the columns of
-// the unit that c lies in. Steps of 32 rows through shared memory.
+// Up to 64 rows, unsorted: a block forms 32 features of all of them, its eight
+// waves taking the depth (and then the adapters) in turn. W is read once, four
+// steps' loads in flight.
+template <class T, int NB>
+__global__ __launch_bounds__(LT) void adapter_few_k(Adapter p, Product g) {
+    __shared__ Join8 buf[8];
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, half = lane >> 5, col = lane & 31;
+    const int m0 = blockIdx.x * 32, m = m0 + col;
+    const T* w = static_cast<const T*>(p.W) + static_cast<long>(min(m, g.M - 1)) * g.K;
+    const T* x[NB];
+#pragma unroll
+    for (int j = 0; j < NB; ++j) x[j] = static_cast<const T*>(g.Z) + min(32 * j + col, p.T - 1) * g.z_rs;
+    f32x16 acc[1][NB];
+#pragma unroll
+    for (int j = 0; j < NB; ++j) acc[0][j] = f32x16{};
+    for (int k = 16 * wave; k < g.K; k += 512) {
+        Frag<T> f[4], z[4][NB];
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+            const int d = k + 128 * s + 8 * half, n = min(8, g.K - d), dd = n > 0 ? d : 0;
+            f[s] = load8(w + dd, m < g.M ? n : 0, p.vec_w);
+#pragma unroll
+            for (int j = 0; j < NB; ++j) z[s][j] = load8(x[j] + dd, 32 * j + col < p.T ? n : 0, g.vec_z);
+        }
+#pragma unroll
+        for (int s = 0; s < 4; ++s)
+#pragma unroll
+            for (int j = 0; j < NB; ++j) acc[0][j] = mma32(f[s], z[s][j], acc[0][j]);
+    }
+    const int id = lane < p.T ? adapter_of(p, lane) : p.n;
+    const int u0 = unit_at(p.unit_off, p.units, m0), u1 = unit_at(p.unit_off, p.units, min(m0 + 31, g.M - 1)) + 1;
+    low_rank<T, false, 1, NB>(p, g.M, m0, u0, u1, min(lane, p.T - 1), id, wave, 8, acc);
+#pragma unroll
+    for (int j = 0; j < NB; ++j)
+        join8(buf, acc[0][j], [&](int r, int c, float v) {
+            const int t = 32 * j + c;
+            if (t >= p.T || m0 + r >= g.M) return;
+            if (p.bias) v += static_cast<float>(static_cast<const T*>(p.bias)[m0 + r]);
+            static_cast<T*>(g.Y)[t * g.y_rs + m0 + r] = static_cast<T>(v);
+        });
+}
+
+// Sums over a chunk's rows: C[m, c] = f sum_t P[t, m] Z[t, c] for 32 columns m
+// of the float matrix P (H or dH, width R) and 128 columns c of X or dY.
+// dA = dH^T drop(X): all of P's columns. dB^T = H^T dY: the columns of the
+// unit that c lies in. Steps of 64 rows through shared memory, the next
+// step's loads in flight. Where every adapter is one chunk (T <= CHUNK) the
+// sums are the gradients; else they go to `part` (chunks, the gradient's
+// adapter) and adapter_grad_k adds them.
 template <class T, bool DB>
 __global__ __launch_bounds__(NT) void adapter_outer_k(Adapter p, const float* P, const T* Z, long z_rs, int C, bool vec_z,
-                                                      float* out, float beta, int mt) {
-    constexpr int NTERM = Terms<T, 3>::n;
-    __shared__ __align__(16) T sz[32 * 128];
-    __shared__ __align__(16) T sp[NTERM][32 * 64];
+                                                      float* out, float beta, float* part, int mt) {
+    constexpr int NTERM = Terms<T, 3>::n, ROWS = 64, NZ = ROWS * 16 / NT;
+    __shared__ __align__(16) T sz[ROWS * 128];
+    __shared__ __align__(16) T sp[NTERM][ROWS * 64];
     const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, half = lane >> 5, col = lane & 31;
     const int ct = (C + 127) / 128;
-    int b = blockIdx.x;
-    const int c0 = (b % ct) * 128;
-    b /= ct;
-    const int m0 = (b % mt) * 32, a = b / mt;
-    const int s0 = p.seg[a], s1 = p.seg[a + 1];
+    const int c0 = (blockIdx.x % ct) * 128, m0 = (blockIdx.x / ct % mt) * 32;
+    const int chunk = blockIdx.x / ct / mt;
+    const Piece pc = p.chunks[chunk];
+    const int a = pc.adapter;
+    if (a >= p.n || (part && !pc.count)) return;
+    if (!part && chunk > 0 && p.chunks[chunk - 1].adapter == a) return;  // the adapter's empty last entry
     const int cols = DB ? p.rank : p.R;  // P's columns that a block's m counts
-    const float f = DB ? p.scale[a] : p.dropping ? p.drop.keep : 1.0f;
-    int u0 = 0, u1 = 1;
-    if (DB) {
-        while (u0 + 1 < p.units && p.unit_off[u0 + 1] <= c0) ++u0;
-        u1 = u0 + 1;
-        while (u1 < p.units && p.unit_off[u1] < c0 + 128) ++u1;
-    }
+    const float f = !DB && p.dropping ? p.drop.keep : 1.0f;
+    const int u0 = DB ? unit_at(p.unit_off, p.units, c0) : 0;
+    const int u1 = DB ? unit_at(p.unit_off, p.units, min(c0 + 127, C - 1)) + 1 : 1;
     for (int u = u0; u < u1; ++u) {
         const float* base = P + (DB ? u * p.rank : 0);
         f32x16 acc = f32x16{};
-        for (int s = s0; s < s1; s += 32) {
-            for (int e = tid; e < 32 * 16; e += NT) {
-                const int t = e >> 4, d = c0 + 8 * (e & 15), row = s + t < s1 ? p.perm[s + t] : 0;
-                Frag<T> z = load8(Z + row * z_rs + d, s + t < s1 ? min(8, C - d) : 0, vec_z);
-                if (!DB && p.dropping) z = dropped<T>(p.drop, row, d, z);
-                Tile<T, 128>::put8(sz, t, e & 15, z);
-            }
-            if (tid < 32 * 4) {
-                const int t = tid >> 2, d = m0 + 8 * (tid & 3), row = s + t < s1 ? p.perm[s + t] : 0;
-                const float* q = base + static_cast<long>(row) * p.R + (d < cols ? d : 0);
-                const Terms<T, 3> v(load8(q, s + t < s1 ? min(8, cols - d) : 0, false));
+        Frag<T> z[NZ];
+        f32x8 h;
+        int rows[NZ];
+        const auto load = [&](int s) {
 #pragma unroll
-                for (int x = 0; x < NTERM; ++x) Tile<T, 64>::put8(sp[x], t, tid & 3, v.t[x]);
+            for (int i = 0; i < NZ; ++i) {
+                const int e = tid + i * NT, t = s + (e >> 4), d = c0 + 8 * (e & 15);
+                rows[i] = t < pc.count ? p.perm[pc.start + t] : 0;
+                z[i] = load8(Z + rows[i] * z_rs + min(d, C), t < pc.count ? min(8, C - d) : 0, vec_z);
             }
+            const int t = s + (tid >> 2), d = m0 + 8 * (tid & 3), row = t < pc.count ? p.perm[pc.start + t] : 0;
+            h = load8(base + static_cast<long>(row) * p.R + min(d, cols), t < pc.count ? min(8, cols - d) : 0, p.vec_h);
+        };
+        if (pc.count) load(0);
+        for (int s = 0; s < pc.count; s += ROWS) {
+#pragma unroll
+            for (int i = 0; i < NZ; ++i) {
+                const int e = tid + i * NT;
+                if (!DB && p.dropping) z[i] = dropped<T>(p.drop, rows[i], c0 + 8 * (e & 15), z[i]);
+                Tile<T, 128>::put8(sz, e >> 4, e & 15, z[i]);
+            }
+            const Terms<T, 3> v(h);
+#pragma unroll
+            for (int x = 0; x < NTERM; ++x) Tile<T, 64>::put8(sp[x], tid >> 2, tid & 3, v.t[x]);
             __syncthreads();
+            if (s + ROWS < pc.count) load(s + ROWS);
 #pragma unroll
-            for (int k = 0; k < 2; ++k) {
-                const Frag<T> z = lds_cols<128, false>(sz, 16 * k, 32 * wave);
+            for (int k = 0; k < ROWS / 16; ++k) {
+                const Frag<T> w = lds_cols<128, false>(sz, 16 * k, 32 * wave);
 #pragma unroll
-                for (int x = 0; x < NTERM; ++x) acc = mma32(lds_cols<64, false>(sp[x], 16 * k, 0), z, acc);
+                for (int x = 0; x < NTERM; ++x) acc = mma32(lds_cols<64, false>(sp[x], 16 * k, 0), w, acc);
             }
             __syncthreads();
         }
         const int c = c0 + 32 * wave + col;
         if (c >= C || (DB && (c < p.unit_off[u] || c >= p.unit_off[u + 1]))) continue;
+        const long size = DB ? static_cast<long>(C) * p.rank : static_cast<long>(p.R) * C;
+        float* to = part ? part + chunk * size : out + a * size;
+        const bool add = !part && beta != 0.0f;
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-            const int m = m0 + acc_row(r, half);
-            if (m >= cols) continue;
-            float* o = DB ? out + (static_cast<long>(a) * C + c) * p.rank + m : out + (static_cast<long>(a) * p.R + m) * C + c;
-            *o = beta == 0.0f ? f * acc[r] : beta * *o + f * acc[r];
+        for (int q = 0; q < 4; ++q) {
+            const int m = m0 + 8 * q + 4 * half;
+            if (DB && p.vec_h && !add) {  // four of a row
+                store4(to + static_cast<long>(c) * p.rank + m, cols - m, true, acc[4 * q], acc[4 * q + 1], acc[4 * q + 2], acc[4 * q + 3]);
+                continue;
+            }
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+                if (m + x >= cols) continue;
+                float* o = DB ? to + static_cast<long>(c) * p.rank + m + x : to + static_cast<long>(m + x) * C + c;
+                *o = add ? beta * *o + f * acc[4 * q + x] : f * acc[4 * q + x];
+            }
         }
     }
+}
+
+// An adapter's chunks' sums in their order; adapters without rows get zeros.
+__global__ __launch_bounds__(NT) void adapter_grad_k(const Piece* chunks, int table, const float* part, long size, float* out,
+                                                     float beta, int a0) {
+    __shared__ int range[2];
+    const int a = a0 + blockIdx.y;
+    if (threadIdx.x == 0) {  // the adapter's entries: [first, next), found by their adapter
+        int lo = 0, hi = table;
+        while (lo < hi) {
+            const int mid = (lo + hi) >> 1;
+            if (chunks[mid].adapter < a) lo = mid + 1;
+            else hi = mid;
+        }
+        range[0] = lo;
+        while (lo < table && chunks[lo].adapter == a && chunks[lo].count) ++lo;
+        range[1] = lo;
+    }
+    __syncthreads();
+    const long e = static_cast<long>(blockIdx.x) * NT + threadIdx.x;
+    if (e >= size) return;
+    float s = 0.0f;
+#pragma unroll 4
+    for (int i = range[0]; i < range[1]; ++i) s += part[i * size + e];
+    float* o = out + a * size + e;
+    *o = beta == 0.0f ? s : beta * *o + s;
 }
 
 // ─── host ───
@@ -475,24 +696,54 @@ int check(kdec_ctx* ctx, const char* who, int dtype, int T, int in, int out, int
     if (T < 0 || in <= 0 || out <= 0 || adapters < 0) return bad("bad sizes");
     if (units < 1 || units > 4096) return bad("units outside 1..4096");
     if (rank < 1 || rank > 128) return bad("rank outside 1..128");
-    if (T > INT_MAX - 256 || in > INT_MAX - 256 || out > INT_MAX - 256 || adapters > (1 << 20)) return bad("sizes too large");
+    if (T > INT_MAX / 2 || in > (1 << 24) || out > (1 << 24) || adapters > (1 << 20)) return bad("sizes too large");
     if (!make_drop(prob, seed, offset, p.drop)) return bad("p must be at least 0 and below 1");
     p.dropping = p.drop.thr != 0;
     return KDEC_OK;
 }
 
-// Launches f(type value) for the call's type.
-template <class F> int typed(int dtype, F f) { return dtype == KDEC_F32 ? f(float{}) : f(bf16{}); }
+size_t up(size_t n) { return (n + 255) & ~size_t(255); }
 
-void sort_rows(kdec_ctx* ctx, const Adapter& p, int* perm, int* seg) {
-    hipLaunchKernelGGL(adapter_sort_k, dim3(p.n + 1), dim3(ST), 0, ctx->stream, p.idx, p.T, p.n, perm, seg);
+// The sort's workspace: rows, pieces, chunks.
+struct Sorted {
+    size_t perm, pieces, chunks;
+    long n_pieces, n_chunks;
+    Sorted(int T, int adapters)
+        : perm(up(T * 4ul)), n_pieces(T / PIECE + adapters + 1), n_chunks(T / CHUNK + adapters + 1) {
+        pieces = up(n_pieces * sizeof(Piece));
+        chunks = up(n_chunks * sizeof(Piece));
+    }
+    size_t bytes() const { return perm + pieces + chunks; }
+    void sort(kdec_ctx* ctx, Adapter& p, char* ws) const {
+        int* rows = reinterpret_cast<int*>(ws);
+        Piece *a = reinterpret_cast<Piece*>(ws + perm), *b = reinterpret_cast<Piece*>(ws + perm + pieces);
+        hipLaunchKernelGGL(adapter_sort_k, dim3(p.n + 1), dim3(ST), 0, ctx->stream, p.idx, p.T, p.n, rows, a, b);
+        p.perm = rows;
+        p.pieces = a;
+        p.chunks = b;
+    }
+};
+
+template <class T>
+void low_inputs(kdec_ctx* ctx, const Adapter& p, long pieces) {
+    const unsigned x = static_cast<unsigned>(p.pieces ? pieces : p.T);
+    if (p.R > 32)
+        hipLaunchKernelGGL((adapter_h_k<T, 2>), dim3(x, static_cast<unsigned>(cdiv(p.R, 64))), dim3(LT), 0, ctx->stream, p);
+    else
+        hipLaunchKernelGGL((adapter_h_k<T, 1>), dim3(x, 1), dim3(LT), 0, ctx->stream, p);
 }
 
 template <class T, bool BWD>
 int product(kdec_ctx* ctx, const Adapter& p, Product g) {
     const long tiles = cdiv(g.M, GM) * cdiv(p.T, GN);
     if (tiles >= INT_MAX) return fail(ctx, KDEC_EINVAL, "kdec_adapter: too many rows");
-    hipLaunchKernelGGL((adapter_gemm_k<T, BWD>), dim3(static_cast<unsigned>(tiles), g.splits), dim3(NT), 0, ctx->stream, p, g);
+    const dim3 grid(static_cast<unsigned>(tiles), g.splits);
+    const long bytes = ((p.T - 1) * g.z_rs + g.K) * static_cast<long>(sizeof(T));
+    const long wide = static_cast<long>(GM) * (BWD ? g.M : g.K) * static_cast<long>(sizeof(T));  // a tile of W, in its offsets
+    if (p.vec_w && g.vec_z && g.z_rs >= 0 && bytes < 0xFFFF0000L && wide < (1L << 30))
+        hipLaunchKernelGGL((adapter_gemm_k<T, BWD, true>), grid, dim3(NT), 0, ctx->stream, p, g);
+    else
+        hipLaunchKernelGGL((adapter_gemm_k<T, BWD, false>), grid, dim3(NT), 0, ctx->stream, p, g);
     if (g.splits > 1) {
         const long n = static_cast<long>(p.T) * g.M;
         hipLaunchKernelGGL(adapter_join_k<T>, dim3(static_cast<unsigned>(cdiv(n, NT))), dim3(NT), 0, ctx->stream, g.part, g.splits,
@@ -501,7 +752,59 @@ int product(kdec_ctx* ctx, const Adapter& p, Product g) {
     return KDEC_OK;
 }
 
-size_t up(size_t n) { return (n + 255) & ~size_t(255); }
+template <class T>
+int forward(kdec_ctx* ctx, const Adapter& p, const Product& g, long pieces) {
+    low_inputs<T>(ctx, p, pieces);
+    if (!p.pieces) {
+        const dim3 grid(static_cast<unsigned>(cdiv(g.M, 32)));
+        if (p.T <= 32) hipLaunchKernelGGL((adapter_few_k<T, 1>), grid, dim3(LT), 0, ctx->stream, p, g);
+        else hipLaunchKernelGGL((adapter_few_k<T, 2>), grid, dim3(LT), 0, ctx->stream, p, g);
+    } else if (int rc = product<T, false>(ctx, p, g)) {
+        return rc;
+    }
+    return launch_check(ctx, "kdec_adapter_fwd");
+}
+
+struct Grads {
+    float *dA, *dB, beta, *part_a, *part_b;  // parts: null where every adapter is one chunk
+    long n_chunks;
+};
+
+template <class T, bool DB>
+int grads(kdec_ctx* ctx, const Adapter& p, const Grads& gr, const float* P, const void* Z, long z_rs, int C, bool vec_z, float* out,
+          float* part, long size) {
+    const long mt = cdiv(DB ? p.rank : p.R, 32), blocks = cdiv(C, 128) * mt * gr.n_chunks;
+    if (blocks >= INT_MAX || cdiv(size, NT) >= INT_MAX) return fail(ctx, KDEC_EINVAL, "kdec_adapter_bwd: too many adapters");
+    hipLaunchKernelGGL((adapter_outer_k<T, DB>), dim3(static_cast<unsigned>(blocks)), dim3(NT), 0, ctx->stream, p, P,
+                       static_cast<const T*>(Z), z_rs, C, vec_z, out, gr.beta, part, static_cast<int>(mt));
+    if (part)
+        for (int a = 0; a < p.n; a += 65535)  // the grid's second dimension ends there
+            hipLaunchKernelGGL(adapter_grad_k, dim3(static_cast<unsigned>(cdiv(size, NT)), static_cast<unsigned>(p.n - a < 65535 ? p.n - a : 65535)),
+                               dim3(NT), 0, ctx->stream, p.chunks, static_cast<int>(gr.n_chunks), part, size, out, gr.beta, a);
+    return KDEC_OK;
+}
+
+template <class T>
+int backward(kdec_ctx* ctx, const Adapter& p, const Product& g, const Grads& gr, long pieces) {
+    if (p.T > 0)
+        hipLaunchKernelGGL(adapter_dh_k<T>, dim3(static_cast<unsigned>(pieces), static_cast<unsigned>(p.units * cdiv(p.rank, 32))),
+                           dim3(LT), 0, ctx->stream, p);
+    if (p.T > 0 && g.Y)
+        if (int rc = product<T, true>(ctx, p, g)) return rc;
+    if (gr.dA && p.n > 0) {
+        if (int rc = grads<T, false>(ctx, p, gr, p.dH, p.X, p.x_rs, p.in, p.vec_x, gr.dA, gr.part_a, static_cast<long>(p.R) * p.in))
+            return rc;
+        if (int rc = grads<T, true>(ctx, p, gr, p.H, p.dY, p.dy_rs, p.out, p.vec_dy, gr.dB, gr.part_b,
+                                    static_cast<long>(p.out) * p.rank))
+            return rc;
+    }
+    return launch_check(ctx, "kdec_adapter_bwd");
+}
+
+// Whether four values of a row of Y can be stored at once.
+bool stores4(const void* Y, long rs, int cols, size_t es) {
+    return cols % 4 == 0 && reinterpret_cast<size_t>(Y) % (4 * es) == 0 && (rs * es) % (4 * es) == 0;
+}
 
 }  // namespace
 }  // namespace kdec
@@ -529,24 +832,15 @@ int kdec_adapter_fwd(kdec_ctx* ctx, int dtype, const void* X, long x_rs, const v
     p.vec_a = in % el == 0 && aligned16(A, 0);
     p.vec_b = rank % 8 == 0 && aligned16(B, 0);
     ProfScope ps(ctx, "adapter", 2.0 * T * in * out, 0.0);
-    const size_t perm_b = up(T * 4ul), seg_b = up((adapters + 2ul) * 4), h_b = H ? 0 : up(static_cast<size_t>(T) * R * 4);
-    Workspace ws(ctx, perm_b + seg_b + h_b);
+    const Sorted sorted(T, adapters);
+    const size_t h_b = H ? 0 : up(static_cast<size_t>(T) * R * 4);
+    Workspace ws(ctx, sorted.bytes() + h_b);
     if (!ws.p) return KDEC_ENOMEM;
-    int *perm = ws.as<int>(), *seg = reinterpret_cast<int*>(ws.as<char>() + perm_b);
-    p.perm = perm;
-    p.seg = seg;
-    p.H = H ? H : reinterpret_cast<float*>(ws.as<char>() + perm_b + seg_b);
+    p.H = H ? H : reinterpret_cast<float*>(ws.as<char>() + sorted.bytes());
     p.vec_h = rank % 8 == 0 && aligned16(p.H, 0);
-    sort_rows(ctx, p, perm, seg);
-    return typed(dtype, [&](auto t) {
-        typedef decltype(t) E;
-        hipLaunchKernelGGL(adapter_h_k<E>, dim3(static_cast<unsigned>(cdiv(T, 32)), static_cast<unsigned>(cdiv(R, 32))), dim3(NT), 0,
-                           ctx->stream, p);
-        Product g{out, in, X, x_rs, p.vec_x, Y, y_rs,
-                  out % 4 == 0 && reinterpret_cast<size_t>(Y) % (4 * es) == 0 && (y_rs * es) % (4 * es) == 0, 1, nullptr};
-        if (int rc = product<E, false>(ctx, p, g)) return rc;
-        return launch_check(ctx, "kdec_adapter_fwd");
-    });
+    if (T > FEW) sorted.sort(ctx, p, ws.as<char>());
+    const Product g{out, in, X, x_rs, p.vec_x, Y, y_rs, stores4(Y, y_rs, out, es), 1, nullptr};
+    return dtype == KDEC_F32 ? forward<float>(ctx, p, g, sorted.n_pieces) : forward<bf16>(ctx, p, g, sorted.n_pieces);
 }
 
 int kdec_adapter_bwd(kdec_ctx* ctx, int dtype, const void* X, long x_rs, const void* W, const void* A, const void* B,
@@ -557,7 +851,7 @@ int kdec_adapter_bwd(kdec_ctx* ctx, int dtype, const void* X, long x_rs, const v
     Adapter p{};
     if (int rc = check(ctx, "kdec_adapter_bwd", dtype, T, in, out, adapters, units, rank, prob, seed, offset, p)) return rc;
     KDEC_CHECK(ctx, !dA == !dB, "kdec_adapter_bwd: dA and dB go together");
-    KDEC_CHECK(ctx, T == 0 || (X && W && H && dY && idx && unit_off), "kdec_adapter_bwd: null tensor");
+    KDEC_CHECK(ctx, T == 0 || (X && W && H && dY && idx), "kdec_adapter_bwd: null tensor");
     KDEC_CHECK(ctx, unit_off && (adapters == 0 || (A && B && scale)), "kdec_adapter_bwd: null tensor");
     KDEC_CHECK(ctx, !dX || T <= 1 || dx_rs >= in, "kdec_adapter_bwd: row stride of dX too small");
     if ((T == 0 || !dX) && (adapters == 0 || !dA)) return KDEC_OK;
@@ -573,45 +867,28 @@ int kdec_adapter_bwd(kdec_ctx* ctx, int dtype, const void* X, long x_rs, const v
     p.vec_dy = out % el == 0 && aligned16(dY, dy_rs * es);
     ProfScope ps(ctx, "adapter", 2.0 * T * in * out, 0.0);
     // Few tiles over a long depth: the depth split over blocks, to no fewer
-    // than 512 deep each.
+    // than 128 deep each.
     const long tiles = cdiv(in, GM) * cdiv(T, GN);
     long splits = dX && T > 0 ? cdiv(2L * ctx->num_cus, tiles) : 1;
-    if (splits > out / 512) splits = out / 512;
+    if (splits > out / 128) splits = out / 128;
     if (splits < 1) splits = 1;
-    const size_t perm_b = up(T * 4ul), seg_b = up((adapters + 2ul) * 4), h_b = up(static_cast<size_t>(T) * R * 4);
-    Workspace ws(ctx, perm_b + seg_b + h_b + (splits > 1 ? static_cast<size_t>(splits) * T * in * 4 : 0));
+    const Sorted sorted(T, adapters);
+    const size_t h_b = up(static_cast<size_t>(T) * R * 4), s_b = splits > 1 ? up(static_cast<size_t>(splits) * T * in * 4) : 0;
+    const bool parts = dA && T > CHUNK;
+    const size_t a_b = parts ? up(static_cast<size_t>(sorted.n_chunks) * R * in * 4) : 0;
+    const size_t b_b = parts ? up(static_cast<size_t>(sorted.n_chunks) * out * rank * 4) : 0;
+    Workspace ws(ctx, sorted.bytes() + h_b + s_b + a_b + b_b);
     if (!ws.p) return KDEC_ENOMEM;
-    int *perm = ws.as<int>(), *seg = reinterpret_cast<int*>(ws.as<char>() + perm_b);
-    p.perm = perm;
-    p.seg = seg;
+    char* at = ws.as<char>() + sorted.bytes();
     p.H = const_cast<float*>(H);
-    p.dH = reinterpret_cast<float*>(ws.as<char>() + perm_b + seg_b);
-    p.vec_h = rank % 8 == 0;
-    sort_rows(ctx, p, perm, seg);
-    return typed(dtype, [&](auto t) {
-        typedef decltype(t) E;
-        if (T > 0) {
-            const long jt = cdiv(rank, 32);
-            hipLaunchKernelGGL(adapter_dh_k<E>, dim3(static_cast<unsigned>(cdiv(T, 32)), static_cast<unsigned>(units * jt)), dim3(NT),
-                               0, ctx->stream, p);
-        }
-        if (T > 0 && dX) {
-            Product g{in, out, dY, dy_rs, p.vec_dy, dX, dx_rs,
-                      in % 4 == 0 && reinterpret_cast<size_t>(dX) % (4 * es) == 0 && (dx_rs * es) % (4 * es) == 0,
-                      static_cast<int>(splits), reinterpret_cast<float*>(ws.as<char>() + perm_b + seg_b + h_b)};
-            if (int rc = product<E, true>(ctx, p, g)) return rc;
-        }
-        if (dA && adapters > 0) {
-            const long at = cdiv(R, 32), bt = cdiv(rank, 32);
-            const long ab = cdiv(in, 128) * at * adapters, bb = cdiv(out, 128) * bt * adapters;
-            KDEC_CHECK(ctx, ab < INT_MAX && bb < INT_MAX, "kdec_adapter_bwd: too many adapters");
-            hipLaunchKernelGGL((adapter_outer_k<E, false>), dim3(static_cast<unsigned>(ab)), dim3(NT), 0, ctx->stream, p, p.dH,
-                               static_cast<const E*>(X), x_rs, in, p.vec_x, dA, beta, static_cast<int>(at));
-            hipLaunchKernelGGL((adapter_outer_k<E, true>), dim3(static_cast<unsigned>(bb)), dim3(NT), 0, ctx->stream, p, p.H,
-                               static_cast<const E*>(dY), dy_rs, out, p.vec_dy, dB, beta, static_cast<int>(bt));
-        }
-        return launch_check(ctx, "kdec_adapter_bwd");
-    });
+    p.dH = reinterpret_cast<float*>(at);
+    p.vec_h = rank % 8 == 0 && aligned16(H, 0) && aligned16(dB, 0);
+    sorted.sort(ctx, p, ws.as<char>());
+    const Product g{in, out, dY, dy_rs, p.vec_dy, dX, dx_rs, dX && stores4(dX, dx_rs, in, es), static_cast<int>(splits),
+                    reinterpret_cast<float*>(at + h_b)};
+    const Grads gr{dA, dB, beta, parts ? reinterpret_cast<float*>(at + h_b + s_b) : nullptr,
+                   parts ? reinterpret_cast<float*>(at + h_b + s_b + a_b) : nullptr, sorted.n_chunks};
+    return dtype == KDEC_F32 ? backward<float>(ctx, p, g, gr, sorted.n_pieces) : backward<bf16>(ctx, p, g, gr, sorted.n_pieces);
 }
 
 }  // extern "C"

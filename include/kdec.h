@@ -494,9 +494,8 @@ int kdec_attn_bwd(kdec_ctx* ctx, int dtype, const void* Q, long q_rs,
 /* A projection shared by all rows and the low-rank adapters that each row
  * chooses beside it: row t takes adapter a = idx[t], none where idx[t] is
  * outside [0, adapters);
- *   H[t, u*rank + j] = sum_i A[a][u*rank + j, i] drop(X)[t, i]
- *   Y[t, r] = W[r, :] . X[t, :] + bias[r]
- *             + scale[a] sum_j B[a][r, j] H[t, u(r)*rank + j]
+ *   H[t, u*rank + j] = scale[a] sum_i A[a][u*rank + j, i] drop(X)[t, i]
+ *   Y[t, r] = W[r, :] . X[t, :] + bias[r] + sum_j B[a][r, j] H[t, u(r)*rank + j]
  * with the output rows cut into `units` units, unit u owning
  * [unit_off[u], unit_off[u+1]) (units+1 ints on the device, from 0 to out:
  * one unit for a plain projection, three for a fused query / key / value,
@@ -506,7 +505,7 @@ int kdec_attn_bwd(kdec_ctx* ctx, int dtype, const void* Q, long q_rs,
  * p > 0 drops inputs of the adapters (not of W) as kdec_dropout does with
  * this seed and offset. H (T, units*rank floats; zero rows where no adapter
  * is chosen) is written when not NULL, for the backward.
- * rank <= 128, units <= 4096. */
+ * rank <= 128, units <= 4096, in and out <= 2^24, adapters <= 2^20. */
 int kdec_adapter_fwd(kdec_ctx* ctx, int dtype, const void* X, long x_rs,
                      const void* W, const void* bias, const void* A,
                      const void* B, const float* scale, const int* idx,
@@ -518,7 +517,7 @@ int kdec_adapter_fwd(kdec_ctx* ctx, int dtype, const void* X, long x_rs,
  *   dX = dY W + drop(A[a]^T dH)
  *   dA[a] = beta dA[a] + sum_{t of a} dH[t]^T drop(X)[t]
  *   dB[a][r, j] = beta dB[a][r, j]
- *                 + scale[a] sum_{t of a} dY[t, r] H[t, u(r)*rank + j]
+ *                 + sum_{t of a} dY[t, r] H[t, u(r)*rank + j]
  * dA and dB are floats of A's and B's shapes; adapters that no row chooses
  * get zeros (beta = 0: overwritten, what they held is not read). dX (T, in)
  * at dx_rs. dX, or dA and dB together, may be NULL. */
