@@ -22,10 +22,10 @@
 namespace kdec {
 namespace {
 
-constexpr int NT = 256;            // threads of a product's block
+constexpr int NT = 256;            // threads of the gradients' blocks
 constexpr int LT = 512;            // threads of the low-rank kernels' blocks, 8 waves
 constexpr int ST = 1024;           // threads of the sort
-constexpr int GM = 128, GN = 128;  // features and rows of a product tile
+constexpr int GN = 128;            // rows of a product tile
 constexpr int PIECE = 32;          // sorted rows of a piece
 constexpr int CHUNK = 256;         // sorted rows of a chunk, the adapters' gradients' unit of work
 constexpr int FEW = 64;            // rows that one block of the product holds whole
@@ -64,38 +64,43 @@ __device__ inline int unit_at(const int* off, int units, int m) {
     return u;
 }
 
-// Block a places adapter a's rows (a = n: the rows without one): every thread
-// counts a run of rows, the counts are scanned, and the rows written in
-// order. Its pieces (and chunks) are the windows of PIECE (CHUNK) sorted
+// Block a places adapter a's rows (a = n: the rows without one): every wave
+// counts a run of rows, and from the counts writes its rows in order. Its pieces (and chunks) are the windows of PIECE (CHUNK) sorted
 // places that its rows meet. They start at table entry start / window + a,
 // which no other adapter's reach: an adapter of c rows meets at most
 // c / window + 1 windows; entries up to the next adapter's first are empty.
 __global__ __launch_bounds__(ST) void adapter_sort_k(const int* idx, int T, int n, int* perm, Piece* pieces, Piece* chunks) {
-    __shared__ int less_sum[ST / 64], eq_sum[ST / 64];
+    constexpr int NW = ST / 64, AHEAD = 8;
+    __shared__ int less_sum[NW], eq_sum[NW];
     const int a = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int per = (T + ST - 1) / ST;
-    const int t0 = static_cast<int>(min(static_cast<long>(tid) * per, static_cast<long>(T)));
+    const int per = ((T + NW - 1) / NW + 63) / 64 * 64;  // rows of a wave, 64 at a time
+    const int t0 = static_cast<int>(min(static_cast<long>(wave) * per, static_cast<long>(T)));
     const int t1 = static_cast<int>(min(static_cast<long>(t0) + per, static_cast<long>(T)));
+    const auto each = [&](auto f) {  // f(row, its adapter or n; -1 past the rows)
+        for (int t = t0; t < t1; t += 64 * AHEAD) {
+            int id[AHEAD];
+#pragma unroll
+            for (int i = 0; i < AHEAD; ++i) {
+                const int row = t + 64 * i + lane;
+                id[i] = row < t1 ? idx[row] : -1;
+                if (row < t1 && (id[i] < 0 || id[i] >= n)) id[i] = n;
+            }
+#pragma unroll
+            for (int i = 0; i < AHEAD; ++i) f(t + 64 * i + lane, id[i]);
+        }
+    };
     int less = 0, eq = 0;
-    for (int t = t0; t < t1; ++t) {
-        int id = idx[t];
-        if (id < 0 || id >= n) id = n;
-        less += id < a;
-        eq += id == a;
-    }
-    for (int o = 32; o; o >>= 1) less += __shfl_xor(less, o);
-    int before = eq;  // inclusive scan within the wave
-    for (int o = 1; o < 64; o <<= 1) {
-        const int v = __shfl_up(before, o);
-        if (lane >= o) before += v;
-    }
-    if (lane == 63) {
+    each([&](int, int id) {
+        less += __builtin_popcountll(__builtin_amdgcn_ballot_w64(id >= 0 && id < a));
+        eq += __builtin_popcountll(__builtin_amdgcn_ballot_w64(id == a));
+    });
+    if (lane == 0) {
         less_sum[wave] = less;
-        eq_sum[wave] = before;
+        eq_sum[wave] = eq;
     }
     __syncthreads();
-    int at = before - eq, start = 0, count = 0;
-    for (int w = 0; w < ST / 64; ++w) {
+    int at = 0, start = 0, count = 0;
+    for (int w = 0; w < NW; ++w) {
         start += less_sum[w];
         count += eq_sum[w];
         if (w < wave) at += eq_sum[w];
@@ -110,11 +115,11 @@ __global__ __launch_bounds__(ST) void adapter_sort_k(const int* idx, int T, int 
     };
     table(pieces, PIECE);
     table(chunks, CHUNK);
-    for (int t = t0; t < t1; ++t) {
-        int id = idx[t];
-        if (id < 0 || id >= n) id = n;
-        if (id == a) perm[at++] = t;
-    }
+    each([&](int row, int id) {
+        const unsigned long long hit = __builtin_amdgcn_ballot_w64(id == a);
+        if (id == a) perm[at + __builtin_popcountll(hit & ((1ull << lane) - 1))] = row;
+        at += __builtin_popcountll(hit);
+    });
 }
 
 // Zeros the fragment's values that the dropout mask drops: columns col .. + 7
@@ -294,13 +299,12 @@ __device__ inline void low_rank(const Adapter& p, int M, int wm, int u0, int u1,
         rows[j] = __shfl(row, 32 * j + col);
         ids[j] = __shfl(id, 32 * j + col);
     }
-    int item = 0;
+    int u = u0 + turn;  // the next unit that is this taker's
     while (left) {
         const int a = __shfl(id, __builtin_ctzll(left));
         const unsigned long long mine = __builtin_amdgcn_ballot_w64(id == a);
         left &= ~mine;
-        for (int u = u0; u < u1; ++u) {
-            if (item++ % turns != turn) continue;
+        for (; u < u1; u += turns) {
             const int lo = BWD ? 0 : p.unit_off[u], hi = BWD ? M : p.unit_off[u + 1];
             f32x16 tmp[MB][NB];
 #pragma unroll
@@ -347,34 +351,42 @@ __device__ inline void low_rank(const Adapter& p, int M, int wm, int u0, int u1,
 #pragma unroll
                         for (int r = 0; r < 16; ++r) acc[i][j][r] += tmp[i][j][r];
         }
+        u -= u1 - u0;
     }
 }
 
-// One 128 x 128 tile: forward Y = W X (+ bias + B H), backward
-// dX = W^T dY (+ drop(A^T dH)). Features are the accumulators' rows, so a
-// lane holds one token's run of features. Four waves of 64 x 64. Rows of W
-// lie along the depth forward and across it backward, where the transposing
-// LDS read turns them. Tiles are copied straight to shared memory, two
-// buffers deep (DIRECT), or go through registers where alignment or size
-// rule that out.
-template <class T, bool BWD, bool DIRECT>
-__global__ __launch_bounds__(NT, DIRECT ? 2 : 1) void adapter_gemm_k(Adapter p, Product g) {
+// One tile of 64 WM features by 128 rows: forward Y = W X (+ bias + B H),
+// backward dX = W^T dY (+ drop(A^T dH)). Features are the accumulators' rows,
+// so a lane holds one token's run of features. 2 WM waves of 64 x 64. Rows of
+// W lie along the depth forward and across it backward, where the transposing
+// LDS read turns them. Tiles are copied straight to shared memory (DIRECT),
+// or go through registers where alignment or size rule that out. WM = 2 has
+// two buffers and two blocks per CU; WM = 4 three buffers, which give a copy
+// two steps to arrive, and takes half the reads of X per feature.
+template <class T, bool BWD, bool DIRECT, int WM>
+__global__ __launch_bounds__(128 * WM, DIRECT ? 2 : 1) void adapter_gemm_k(Adapter p, Product g) {
+    constexpr int GM = 64 * WM, NT = 128 * WM, STAGES = WM == 4 ? 3 : 2;
     constexpr int BK = depth_of<T>(), WC = (BWD ? GM : BK) / 8, WR = BWD ? BK : GM;
     typedef Tile<T, BWD ? GM : BK> Tw;
     typedef Tile<T, BK> Tz;
     constexpr int NZ = GN * BK / 8 / NT, NW = GM * BK / 8 / NT;
     __shared__ __align__(256) T sw0[GM * BK], sw1[GM * BK], sz0[GN * BK], sz1[GN * BK];
+    __shared__ __align__(256) T sw2[STAGES == 3 ? GM * BK : 8], sz2[STAGES == 3 ? GN * BK : 8];
     __shared__ int srow[GN], sid[GN];
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, half = lane >> 5, col = lane & 31;
+    // Blocks go to the eight XCDs in turn: each takes a run of row tiles with
+    // all their features, so its L2 holds few rows of X and one step of W.
+    int tile = blockIdx.x;
+    if (gridDim.x % 8 == 0) tile = (blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3);
     const int mt = (g.M + GM - 1) / GM;
-    const int m0 = (blockIdx.x % mt) * GM, s0 = (blockIdx.x / mt) * GN, ns = min(GN, p.T - s0), split = blockIdx.y;
+    const int m0 = (tile % mt) * GM, s0 = (tile / mt) * GN, ns = min(GN, p.T - s0), split = blockIdx.y;
     if (tid < GN) {
         const int row = tid < ns ? p.perm[s0 + tid] : 0;
         srow[tid] = row;
         sid[tid] = tid < ns ? adapter_of(p, row) : p.n;
     }
     __syncthreads();
-    const int wm = m0 + 64 * (wave & 1), wn = 64 * (wave >> 1);
+    const int wm = m0 + 64 * (wave % WM), wn = 64 * (wave / WM);
     const int steps = (g.K + BK - 1) / BK;
     const int c0 = static_cast<int>(static_cast<long>(steps) * split / g.splits);
     const int c1 = static_cast<int>(static_cast<long>(steps) * (split + 1) / g.splits);
@@ -383,7 +395,7 @@ __global__ __launch_bounds__(NT, DIRECT ? 2 : 1) void adapter_gemm_k(Adapter p, 
 
     // direct copies: a thread's units of both tiles
     Copy<T, BWD ? GM : BK, WR, NT> cw;
-    constexpr int NU = Tz::NU, NZU = GN * NU / NT;
+    constexpr int NU = Tz::NU, NZU = GN * NU / NT, LOADS = NZU + cw.N;  // copies of a step
     unsigned oz[NZU];
     __amdgpu_buffer_rsrc_t rz = rows_rsrc<T>(Z, 0, 0, 0);
     const auto z_offsets = [&](int depth) __attribute__((always_inline)) {  // columns of the tile that are there
@@ -428,9 +440,10 @@ __global__ __launch_bounds__(NT, DIRECT ? 2 : 1) void adapter_gemm_k(Adapter p, 
             }
         }
     };
-    const auto landed = [&](T* tw, T* tz) __attribute__((always_inline)) {
+    const auto landed = [&](T* tw, T* tz, bool last) __attribute__((always_inline)) {
         if constexpr (DIRECT) {
-            __builtin_amdgcn_s_waitcnt(0);
+            if (STAGES == 3 && !last) wait_loads<LOADS>();  // the step after it may be on its way
+            else wait_loads<0>();
         } else {
 #pragma unroll
             for (int i = 0; i < NZ; ++i) Tz::put8(tz, (tid + i * NT) / (BK / 8), (tid + i * NT) % (BK / 8), fz[i]);
@@ -444,6 +457,7 @@ __global__ __launch_bounds__(NT, DIRECT ? 2 : 1) void adapter_gemm_k(Adapter p, 
 #pragma unroll
         for (int j = 0; j < 2; ++j) acc[i][j] = f32x16{};
     if (c0 < c1) load(c0, sw0, sz0);
+    if (STAGES == 3 && c0 + 1 < c1) load(c0 + 1, sw1, sz1);
     {
         const int u0 = BWD ? 0 : unit_at(p.unit_off, p.units, wm);
         const int u1 = BWD ? p.units : unit_at(p.unit_off, p.units, min(wm + 63, g.M - 1)) + 1;
@@ -467,14 +481,16 @@ __global__ __launch_bounds__(NT, DIRECT ? 2 : 1) void adapter_gemm_k(Adapter p, 
                     }
                 }
     }
-    const auto walk = [&](int c, const T* tw, const T* tz, T* nw, T* nz) __attribute__((always_inline)) {
-        if (c + 1 < c1) load(c + 1, nw, nz);
+    // One step on the tiles at tw, tz; the next step's are at nw, nz, and with
+    // three buffers the one after goes to lw, lz.
+    const auto walk = [&](int c, const T* tw, const T* tz, T* nw, T* nz, T* lw, T* lz) __attribute__((always_inline)) {
+        if (c + STAGES - 1 < c1) load(c + STAGES - 1, lw, lz);
 #pragma unroll
         for (int k = 0; k < BK / 16; ++k) {
             Frag<T> w[2], z[2];
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                const int m = 64 * (wave & 1) + 32 * i;
+                const int m = 64 * (wave % WM) + 32 * i;
                 if constexpr (BWD) w[i] = lds_cols<GM, false>(tw, 16 * k, m);
                 else w[i] = lds_rows<T, BK>(tw, m, k);
                 z[i] = lds_rows<T, BK>(tz, wn + 32 * i, k);
@@ -484,16 +500,24 @@ __global__ __launch_bounds__(NT, DIRECT ? 2 : 1) void adapter_gemm_k(Adapter p, 
 #pragma unroll
                 for (int j = 0; j < 2; ++j) acc[i][j] = mma32(w[i], z[j], acc[i][j]);
         }
-        if (c + 1 < c1) landed(nw, nz);
+        if (c + 1 < c1) landed(nw, nz, c + 2 >= c1);
         __syncthreads();
     };
     if (c0 < c1) {
-        landed(sw0, sz0);
+        landed(sw0, sz0, true);
         __syncthreads();
     }
-    for (int c = c0; c < c1; c += 2) {
-        walk(c, sw0, sz0, sw1, sz1);
-        if (c + 1 < c1) walk(c + 1, sw1, sz1, sw0, sz0);
+    if constexpr (STAGES == 3) {
+        for (int c = c0; c < c1; c += 3) {
+            walk(c, sw0, sz0, sw1, sz1, sw2, sz2);
+            if (c + 1 < c1) walk(c + 1, sw1, sz1, sw2, sz2, sw0, sz0);
+            if (c + 2 < c1) walk(c + 2, sw2, sz2, sw0, sz0, sw1, sz1);
+        }
+    } else {
+        for (int c = c0; c < c1; c += 2) {
+            walk(c, sw0, sz0, sw1, sz1, sw1, sz1);
+            if (c + 1 < c1) walk(c + 1, sw1, sz1, sw0, sz0, sw0, sz0);
+        }
     }
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
@@ -519,14 +543,21 @@ __global__ __launch_bounds__(NT, DIRECT ? 2 : 1) void adapter_gemm_k(Adapter p, 
     }
 }
 
-// The splits' sums in their order, rounded once.
+// The splits' sums, rounded once: 64 values per block, its sixteen waves
+// taking the splits in turn and their sums added in order.
 template <class T>
-__global__ __launch_bounds__(NT) void adapter_join_k(const float* part, int splits, long n, int M, T* Y, long y_rs) {
-    const long e = static_cast<long>(blockIdx.x) * NT + threadIdx.x;
-    if (e >= n) return;
+__global__ __launch_bounds__(1024) void adapter_join_k(const float* part, int splits, long n, int M, T* Y, long y_rs) {
+    __shared__ float sum[16][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const long e = static_cast<long>(blockIdx.x) * 64 + lane;
     float s = 0.0f;
-#pragma unroll 8
-    for (int i = 0; i < splits; ++i) s += part[i * n + e];
+    if (e < n)
+#pragma unroll 4
+        for (int i = wave; i < splits; i += 16) s += part[i * n + e];
+    sum[wave][lane] = s;
+    __syncthreads();
+    if (wave || e >= n) return;
+    for (int w = 1; w < 16; ++w) s += sum[w][lane];
     const long row = e / M;
     Y[row * y_rs + (e - row * M)] = static_cast<T>(s);
 }
@@ -657,6 +688,63 @@ __global__ __launch_bounds__(NT) void adapter_outer_k(Adapter p, const float* P,
     }
 }
 
+// The gradients of up to 64 rows: an adapter has few of them, and what counts
+// is writing its gradients. Four values a thread, the rows in turn.
+// dA[m, c] = sum_t dH[t, m] drop(X)[t, c], dB[c, m] = sum_t H[t, u(c) rank + m] dY[t, c].
+template <class T, bool DB>
+__global__ __launch_bounds__(NT) void adapter_outer_few_k(Adapter p, const float* P, const T* Z, long z_rs, int C, bool vec,
+                                                          float* out, float beta) {
+    const int chunk = blockIdx.y;
+    const Piece pc = p.chunks[chunk];
+    const int a = pc.adapter;
+    if (a >= p.n || (chunk > 0 && p.chunks[chunk - 1].adapter == a)) return;  // (the adapter's empty last entry)
+    const int width = DB ? p.rank : C, q = (width + 3) / 4;  // a row of the gradient, in fours
+    const long n = static_cast<long>(DB ? C : p.R) * q;
+    const long e = static_cast<long>(blockIdx.x) * NT + threadIdx.x;
+    if (e >= n) return;
+    const int r = static_cast<int>(e / q), x = 4 * static_cast<int>(e - static_cast<long>(r) * q);
+    int u = 0;
+    if (DB) {
+        int lo = 1, hi = p.units;  // offsets 1 .. units - 1 that are not past r
+        while (lo < hi) {
+            const int mid = (lo + hi) >> 1;
+            if (p.unit_off[mid] <= r) lo = mid + 1;
+            else hi = mid;
+        }
+        u = lo - 1;
+    }
+    float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int t = 0; t < pc.count; ++t) {
+        const int row = p.perm[pc.start + t];
+        float v[4], f;
+        if (DB) {
+            const float* h = P + static_cast<long>(row) * p.R + u * p.rank + x;
+            f = static_cast<float>(Z[row * z_rs + r]);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] = x + i < width ? h[i] : 0.0f;
+        } else {
+            f = P[static_cast<long>(row) * p.R + r];
+            unsigned w[4];
+            if (p.dropping) drop_words(p.drop, static_cast<unsigned>(row), static_cast<unsigned>(x) >> 3, w);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                v[i] = x + i < width ? static_cast<float>(Z[row * z_rs + x + i]) : 0.0f;
+                if (p.dropping) v[i] = kept(p.drop, w, (x & 7) + i) ? v[i] * p.drop.keep : 0.0f;
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[i] = __builtin_fmaf(f, v[i], s[i]);
+    }
+    float* o = out + (static_cast<long>(a) * (DB ? C : p.R) + r) * width + x;
+    if (vec && beta == 0.0f) {
+        *reinterpret_cast<f32x4*>(o) = f32x4{s[0], s[1], s[2], s[3]};
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        if (x + i < width) o[i] = beta == 0.0f ? s[i] : beta * o[i] + s[i];
+}
+
 // An adapter's chunks' sums in their order; adapters without rows get zeros.
 __global__ __launch_bounds__(NT) void adapter_grad_k(const Piece* chunks, int table, const float* part, long size, float* out,
                                                      float beta, int a0) {
@@ -735,18 +823,20 @@ void low_inputs(kdec_ctx* ctx, const Adapter& p, long pieces) {
 
 template <class T, bool BWD>
 int product(kdec_ctx* ctx, const Adapter& p, Product g) {
-    const long tiles = cdiv(g.M, GM) * cdiv(p.T, GN);
+    const long rows = cdiv(p.T, GN), tiles = cdiv(g.M, 128) * rows, wide = cdiv(g.M, 256) * rows;
     if (tiles >= INT_MAX) return fail(ctx, KDEC_EINVAL, "kdec_adapter: too many rows");
-    const dim3 grid(static_cast<unsigned>(tiles), g.splits);
     const long bytes = ((p.T - 1) * g.z_rs + g.K) * static_cast<long>(sizeof(T));
-    const long wide = static_cast<long>(GM) * (BWD ? g.M : g.K) * static_cast<long>(sizeof(T));  // a tile of W, in its offsets
-    if (p.vec_w && g.vec_z && g.z_rs >= 0 && bytes < 0xFFFF0000L && wide < (1L << 30))
-        hipLaunchKernelGGL((adapter_gemm_k<T, BWD, true>), grid, dim3(NT), 0, ctx->stream, p, g);
+    const long reach = 256L * (BWD ? g.M : g.K) * static_cast<long>(sizeof(T));  // of a tile's offsets in W
+    const dim3 grid(static_cast<unsigned>(tiles), g.splits);
+    if (!(p.vec_w && g.vec_z && g.z_rs >= 0 && bytes < 0xFFFF0000L && reach < (1L << 30)))
+        hipLaunchKernelGGL((adapter_gemm_k<T, BWD, false, 2>), grid, dim3(256), 0, ctx->stream, p, g);
+    else if (sizeof(T) == 2 && g.splits == 1 && wide >= ctx->num_cus)  // enough wide tiles for every CU
+        hipLaunchKernelGGL((adapter_gemm_k<bf16, BWD, true, 4>), dim3(static_cast<unsigned>(wide)), dim3(512), 0, ctx->stream, p, g);
     else
-        hipLaunchKernelGGL((adapter_gemm_k<T, BWD, false>), grid, dim3(NT), 0, ctx->stream, p, g);
+        hipLaunchKernelGGL((adapter_gemm_k<T, BWD, true, 2>), grid, dim3(256), 0, ctx->stream, p, g);
     if (g.splits > 1) {
         const long n = static_cast<long>(p.T) * g.M;
-        hipLaunchKernelGGL(adapter_join_k<T>, dim3(static_cast<unsigned>(cdiv(n, NT))), dim3(NT), 0, ctx->stream, g.part, g.splits,
+        hipLaunchKernelGGL(adapter_join_k<T>, dim3(static_cast<unsigned>(cdiv(n, 64))), dim3(1024), 0, ctx->stream, g.part, g.splits,
                            n, g.M, static_cast<T*>(g.Y), g.y_rs);
     }
     return KDEC_OK;
@@ -773,6 +863,15 @@ struct Grads {
 template <class T, bool DB>
 int grads(kdec_ctx* ctx, const Adapter& p, const Grads& gr, const float* P, const void* Z, long z_rs, int C, bool vec_z, float* out,
           float* part, long size) {
+    if (p.T <= FEW && gr.n_chunks <= 65535) {
+        const int width = DB ? p.rank : C;
+        const long n = static_cast<long>(DB ? C : p.R) * cdiv(width, 4);
+        if (cdiv(n, NT) >= INT_MAX) return fail(ctx, KDEC_EINVAL, "kdec_adapter_bwd: too many adapters");
+        hipLaunchKernelGGL((adapter_outer_few_k<T, DB>), dim3(static_cast<unsigned>(cdiv(n, NT)), static_cast<unsigned>(gr.n_chunks)),
+                           dim3(NT), 0, ctx->stream, p, P, static_cast<const T*>(Z), z_rs, C, width % 4 == 0 && aligned16(out, 0), out,
+                           gr.beta);
+        return KDEC_OK;
+    }
     const long mt = cdiv(DB ? p.rank : p.R, 32), blocks = cdiv(C, 128) * mt * gr.n_chunks;
     if (blocks >= INT_MAX || cdiv(size, NT) >= INT_MAX) return fail(ctx, KDEC_EINVAL, "kdec_adapter_bwd: too many adapters");
     hipLaunchKernelGGL((adapter_outer_k<T, DB>), dim3(static_cast<unsigned>(blocks)), dim3(NT), 0, ctx->stream, p, P,
@@ -868,7 +967,7 @@ int kdec_adapter_bwd(kdec_ctx* ctx, int dtype, const void* X, long x_rs, const v
     ProfScope ps(ctx, "adapter", 2.0 * T * in * out, 0.0);
     // Few tiles over a long depth: the depth split over blocks, to no fewer
     // than 128 deep each.
-    const long tiles = cdiv(in, GM) * cdiv(T, GN);
+    const long tiles = cdiv(in, 128) * cdiv(T, GN);
     long splits = dX && T > 0 ? cdiv(2L * ctx->num_cus, tiles) : 1;
     if (splits > out / 128) splits = out / 128;
     if (splits < 1) splits = 1;

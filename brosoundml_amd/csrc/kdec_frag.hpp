@@ -90,7 +90,7 @@ template <class T, int DP>
 struct Tile {
     static constexpr int U = 16 / static_cast<int>(sizeof(T)), NU = DP / U;
     __device__ static inline int swz(int row) {
-        if (sizeof(T) == 2 && NU == 16) return (row & 3) << 2 | (row >> 2 & 3);
+        if (sizeof(T) == 2 && NU >= 16) return (row & 3) << 2 | (row >> 2 & 3);
         if (sizeof(T) == 2 && NU == 8) return (row >> 1 & 1) << 2 | (row >> 2 & 3);
         if (sizeof(T) == 4) return NU == 8 ? row >> 1 & 7 : row & 7;
         return 0;
@@ -187,6 +187,13 @@ __device__ inline f32x8 buffer_load8(__amdgpu_buffer_rsrc_t r, int off, float) {
     const f32x4 a = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(r, off, 0, 0));
     const f32x4 b = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(r, off + 16, 0, 0));
     return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+}
+
+// Waits until at most N of the wave's memory loads (copies among them) are
+// outstanding.
+template <int N>
+__device__ inline void wait_loads() {
+    __builtin_amdgcn_s_waitcnt((N & 15) | (N >> 4) << 14 | 7 << 4 | 15 << 8);
 }
 
 // 16 bytes per lane from the descriptor's offset `off` to shared memory at
