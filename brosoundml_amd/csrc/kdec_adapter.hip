@@ -25,7 +25,6 @@ namespace {
 constexpr int NT = 256;            // threads of the gradients' blocks
 constexpr int LT = 512;            // threads of the low-rank kernels' blocks, 8 waves
 constexpr int ST = 1024;           // threads of the sort
-constexpr int GN = 128;            // rows of a product tile
 constexpr int PIECE = 32;          // sorted rows of a piece
 constexpr int CHUNK = 256;         // sorted rows of a chunk, the adapters' gradients' unit of work
 constexpr int FEW = 64;            // rows that one block of the product holds whole
@@ -283,13 +282,14 @@ struct Product {
 
 template <class T> constexpr int depth_of() { return sizeof(T) == 2 ? 64 : 32; }  // of a tile: 128 bytes
 
-// The low-rank products of a wave's 64 features (from wm) and up to 64 rows
-// (a lane each: its row and adapter), into acc: forward B H, backward A^T dH.
+// The low-rank products of 32 MB of a wave's features (from wm; blocks I0 ..
+// of acc) and its 32 NB rows (a lane each: its row and adapter), into acc:
+// forward B H, backward A^T dH.
 // Adapters and units are taken in turn by `turns` takers of which this is
 // number `turn`.
-template <class T, bool BWD, int MB, int NB>
+template <class T, bool BWD, int I0, int MB, int NA, int NB>
 __device__ inline void low_rank(const Adapter& p, int M, int wm, int u0, int u1, int row, int id, int turn, int turns,
-                                f32x16 (&acc)[MB][NB]) {
+                                f32x16 (&acc)[NA][NB]) {
     const int lane = threadIdx.x & 63, half = lane >> 5, col = lane & 31;
     const float* H = BWD ? p.dH : p.H;
     unsigned long long left = __builtin_amdgcn_ballot_w64(id < p.n);
@@ -349,29 +349,30 @@ __device__ inline void low_rank(const Adapter& p, int M, int wm, int u0, int u1,
 #pragma unroll
                     for (int i = 0; i < MB; ++i)
 #pragma unroll
-                        for (int r = 0; r < 16; ++r) acc[i][j][r] += tmp[i][j][r];
+                        for (int r = 0; r < 16; ++r) acc[I0 + i][j][r] += tmp[i][j][r];
         }
         u -= u1 - u0;
     }
 }
 
-// One tile of 64 WM features by 128 rows: forward Y = W X (+ bias + B H),
-// backward dX = W^T dY (+ drop(A^T dH)). Features are the accumulators' rows,
-// so a lane holds one token's run of features. 2 WM waves of 64 x 64. Rows of
-// W lie along the depth forward and across it backward, where the transposing
-// LDS read turns them. Tiles are copied straight to shared memory (DIRECT),
-// or go through registers where alignment or size rule that out. WM = 2 has
-// two buffers and two blocks per CU; WM = 4 three buffers, which give a copy
-// two steps to arrive, and takes half the reads of X per feature.
-template <class T, bool BWD, bool DIRECT, int WM>
-__global__ __launch_bounds__(128 * WM, DIRECT ? 2 : 1) void adapter_gemm_k(Adapter p, Product g) {
-    constexpr int GM = 64 * WM, NT = 128 * WM, STAGES = WM == 4 ? 3 : 2;
-    constexpr int BK = depth_of<T>(), WC = (BWD ? GM : BK) / 8, WR = BWD ? BK : GM;
+// One tile of features by rows: forward Y = W X (+ bias + B H), backward
+// dX = W^T dY (+ drop(A^T dH)). Features are the accumulators' rows, so a lane
+// holds one token's run of features. Rows of W lie along the depth forward
+// and across it backward, where the transposing LDS read turns them. Tiles
+// are copied straight to shared memory (DIRECT), or go through registers where
+// alignment or size rule that out. BIG: 256 x 256 by eight waves of 128 x 64,
+// steps 32 deep, four buffers (a copy has three steps to arrive, and half the
+// bytes of the small tiles' arrive per product); else 128 x 128 by four waves
+// of 64 x 64, two buffers, two blocks per CU.
+template <class T, bool BWD, bool DIRECT, bool BIG>
+__global__ __launch_bounds__(BIG ? 512 : 256, DIRECT ? 2 : 1) void adapter_gemm_k(Adapter p, Product g) {
+    constexpr int GM = BIG ? 256 : 128, GN = GM, NT = 2 * GM, STAGES = BIG ? 4 : 2, MB = BIG ? 4 : 2;
+    constexpr int BK = BIG ? 32 : depth_of<T>(), WC = (BWD ? GM : BK) / 8, WR = BWD ? BK : GM;
     typedef Tile<T, BWD ? GM : BK> Tw;
     typedef Tile<T, BK> Tz;
     constexpr int NZ = GN * BK / 8 / NT, NW = GM * BK / 8 / NT;
     __shared__ __align__(256) T sw0[GM * BK], sw1[GM * BK], sz0[GN * BK], sz1[GN * BK];
-    __shared__ __align__(256) T sw2[STAGES == 3 ? GM * BK : 8], sz2[STAGES == 3 ? GN * BK : 8];
+    __shared__ __align__(256) T sw2[BIG ? GM * BK : 8], sz2[BIG ? GN * BK : 8], sw3[BIG ? GM * BK : 8], sz3[BIG ? GN * BK : 8];
     __shared__ int srow[GN], sid[GN];
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, half = lane >> 5, col = lane & 31;
     // Blocks go to the eight XCDs in turn: each takes a run of row tiles with
@@ -386,7 +387,7 @@ __global__ __launch_bounds__(128 * WM, DIRECT ? 2 : 1) void adapter_gemm_k(Adapt
         sid[tid] = tid < ns ? adapter_of(p, row) : p.n;
     }
     __syncthreads();
-    const int wm = m0 + 64 * (wave % WM), wn = 64 * (wave / WM);
+    const int wf = 32 * MB * (wave & 1), wm = m0 + wf, wn = 64 * (wave >> 1);  // the wave's features and rows
     const int steps = (g.K + BK - 1) / BK;
     const int c0 = static_cast<int>(static_cast<long>(steps) * split / g.splits);
     const int c1 = static_cast<int>(static_cast<long>(steps) * (split + 1) / g.splits);
@@ -440,9 +441,10 @@ __global__ __launch_bounds__(128 * WM, DIRECT ? 2 : 1) void adapter_gemm_k(Adapt
             }
         }
     };
-    const auto landed = [&](T* tw, T* tz, bool last) __attribute__((always_inline)) {
+    const auto landed = [&](T* tw, T* tz, int ahead) __attribute__((always_inline)) {
         if constexpr (DIRECT) {
-            if (STAGES == 3 && !last) wait_loads<LOADS>();  // the step after it may be on its way
+            if (ahead >= 2) wait_loads<2 * LOADS>();  // the steps after it may be on their way
+            else if (ahead == 1) wait_loads<LOADS>();
             else wait_loads<0>();
         } else {
 #pragma unroll
@@ -451,23 +453,33 @@ __global__ __launch_bounds__(128 * WM, DIRECT ? 2 : 1) void adapter_gemm_k(Adapt
             for (int i = 0; i < NW; ++i) Tw::put8(tw, (tid + i * NT) / WC, (tid + i * NT) % WC, fw[i]);
         }
     };
-    f32x16 acc[2][2];
+    f32x16 acc[MB][2];
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+    for (int i = 0; i < MB; ++i)
 #pragma unroll
         for (int j = 0; j < 2; ++j) acc[i][j] = f32x16{};
     if (c0 < c1) load(c0, sw0, sz0);
-    if (STAGES == 3 && c0 + 1 < c1) load(c0 + 1, sw1, sz1);
-    {
-        const int u0 = BWD ? 0 : unit_at(p.unit_off, p.units, wm);
-        const int u1 = BWD ? p.units : unit_at(p.unit_off, p.units, min(wm + 63, g.M - 1)) + 1;
-        low_rank<T, BWD, 2, 2>(p, g.M, wm, u0, u1, srow[wn + lane], sid[wn + lane], split, g.splits, acc);
+    if (BIG && c0 + 1 < c1) load(c0 + 1, sw1, sz1);
+    if (BIG && c0 + 2 < c1) load(c0 + 2, sw2, sz2);
+    constexpr int LB = BIG && BWD ? 1 : 2;  // 32 LB features at a time, which the registers leave room for
+    const auto low = [&](auto first) __attribute__((always_inline)) {
+        constexpr int I0 = LB * decltype(first)::value;
+        const int m = wm + 32 * I0;
+        const int u0 = BWD ? 0 : unit_at(p.unit_off, p.units, m);
+        const int u1 = BWD ? p.units : unit_at(p.unit_off, p.units, min(m + 32 * LB - 1, g.M - 1)) + 1;
+        low_rank<T, BWD, I0, LB>(p, g.M, m, u0, u1, srow[wn + lane], sid[wn + lane], split, g.splits, acc);
+    };
+    low(std::integral_constant<int, 0>{});
+    if constexpr (MB > LB) low(std::integral_constant<int, 1>{});
+    if constexpr (MB > 2 * LB) {
+        low(std::integral_constant<int, 2>{});
+        low(std::integral_constant<int, 3>{});
     }
     if (BWD && p.dropping) {
 #pragma unroll
         for (int j = 0; j < 2; ++j)
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
+            for (int i = 0; i < MB; ++i)
 #pragma unroll
                 for (int q = 0; q < 4; ++q) {
                     unsigned w[4];
@@ -481,37 +493,38 @@ __global__ __launch_bounds__(128 * WM, DIRECT ? 2 : 1) void adapter_gemm_k(Adapt
                     }
                 }
     }
-    // One step on the tiles at tw, tz; the next step's are at nw, nz, and with
-    // three buffers the one after goes to lw, lz.
+    // One step on the tiles at tw, tz; the next step's are at nw, nz, and a
+    // step's load goes to the buffer that the step before this one used.
     const auto walk = [&](int c, const T* tw, const T* tz, T* nw, T* nz, T* lw, T* lz) __attribute__((always_inline)) {
         if (c + STAGES - 1 < c1) load(c + STAGES - 1, lw, lz);
 #pragma unroll
         for (int k = 0; k < BK / 16; ++k) {
-            Frag<T> w[2], z[2];
+            Frag<T> w[MB], z[2];
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const int m = 64 * (wave % WM) + 32 * i;
-                if constexpr (BWD) w[i] = lds_cols<GM, false>(tw, 16 * k, m);
-                else w[i] = lds_rows<T, BK>(tw, m, k);
-                z[i] = lds_rows<T, BK>(tz, wn + 32 * i, k);
+            for (int i = 0; i < MB; ++i) {
+                if constexpr (BWD) w[i] = lds_cols<GM, false>(tw, 16 * k, wf + 32 * i);
+                else w[i] = lds_rows<T, BK>(tw, wf + 32 * i, k);
             }
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
+            for (int j = 0; j < 2; ++j) z[j] = lds_rows<T, BK>(tz, wn + 32 * j, k);
+#pragma unroll
+            for (int i = 0; i < MB; ++i)
 #pragma unroll
                 for (int j = 0; j < 2; ++j) acc[i][j] = mma32(w[i], z[j], acc[i][j]);
         }
-        if (c + 1 < c1) landed(nw, nz, c + 2 >= c1);
+        if (c + 1 < c1) landed(nw, nz, BIG ? c1 - 2 - c : 0);
         __syncthreads();
     };
     if (c0 < c1) {
-        landed(sw0, sz0, true);
+        landed(sw0, sz0, 0);
         __syncthreads();
     }
-    if constexpr (STAGES == 3) {
-        for (int c = c0; c < c1; c += 3) {
-            walk(c, sw0, sz0, sw1, sz1, sw2, sz2);
+    if constexpr (BIG) {
+        for (int c = c0; c < c1; c += 4) {
+            walk(c, sw0, sz0, sw1, sz1, sw3, sz3);
             if (c + 1 < c1) walk(c + 1, sw1, sz1, sw2, sz2, sw0, sz0);
-            if (c + 2 < c1) walk(c + 2, sw2, sz2, sw0, sz0, sw1, sz1);
+            if (c + 2 < c1) walk(c + 2, sw2, sz2, sw3, sz3, sw1, sz1);
+            if (c + 3 < c1) walk(c + 3, sw3, sz3, sw0, sz0, sw2, sz2);
         }
     } else {
         for (int c = c0; c < c1; c += 2) {
@@ -525,7 +538,7 @@ __global__ __launch_bounds__(128 * WM, DIRECT ? 2 : 1) void adapter_gemm_k(Adapt
         if (t >= ns) continue;
         const long row = srow[t];
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
+        for (int i = 0; i < MB; ++i)
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
                 const int m = wm + 32 * i + 8 * q + 4 * half;
@@ -593,7 +606,7 @@ __global__ __launch_bounds__(LT) void adapter_few_k(Adapter p, Product g) {
     }
     const int id = lane < p.T ? adapter_of(p, lane) : p.n;
     const int u0 = unit_at(p.unit_off, p.units, m0), u1 = unit_at(p.unit_off, p.units, min(m0 + 31, g.M - 1)) + 1;
-    low_rank<T, false, 1, NB>(p, g.M, m0, u0, u1, min(lane, p.T - 1), id, wave, 8, acc);
+    low_rank<T, false, 0, 1>(p, g.M, m0, u0, u1, min(lane, p.T - 1), id, wave, 8, acc);
 #pragma unroll
     for (int j = 0; j < NB; ++j)
         join8(buf, acc[0][j], [&](int r, int c, float v) {
@@ -823,17 +836,17 @@ void low_inputs(kdec_ctx* ctx, const Adapter& p, long pieces) {
 
 template <class T, bool BWD>
 int product(kdec_ctx* ctx, const Adapter& p, Product g) {
-    const long rows = cdiv(p.T, GN), tiles = cdiv(g.M, 128) * rows, wide = cdiv(g.M, 256) * rows;
+    const long tiles = cdiv(g.M, 128) * cdiv(p.T, 128), big = cdiv(g.M, 256) * cdiv(p.T, 256);
     if (tiles >= INT_MAX) return fail(ctx, KDEC_EINVAL, "kdec_adapter: too many rows");
     const long bytes = ((p.T - 1) * g.z_rs + g.K) * static_cast<long>(sizeof(T));
     const long reach = 256L * (BWD ? g.M : g.K) * static_cast<long>(sizeof(T));  // of a tile's offsets in W
     const dim3 grid(static_cast<unsigned>(tiles), g.splits);
     if (!(p.vec_w && g.vec_z && g.z_rs >= 0 && bytes < 0xFFFF0000L && reach < (1L << 30)))
-        hipLaunchKernelGGL((adapter_gemm_k<T, BWD, false, 2>), grid, dim3(256), 0, ctx->stream, p, g);
-    else if (sizeof(T) == 2 && g.splits == 1 && wide >= ctx->num_cus)  // enough wide tiles for every CU
-        hipLaunchKernelGGL((adapter_gemm_k<bf16, BWD, true, 4>), dim3(static_cast<unsigned>(wide)), dim3(512), 0, ctx->stream, p, g);
+        hipLaunchKernelGGL((adapter_gemm_k<T, BWD, false, false>), grid, dim3(256), 0, ctx->stream, p, g);
+    else if (sizeof(T) == 2 && g.splits == 1 && 8 * big >= 7 * ctx->num_cus)  // big tiles for nearly every CU
+        hipLaunchKernelGGL((adapter_gemm_k<bf16, BWD, true, true>), dim3(static_cast<unsigned>(big)), dim3(512), 0, ctx->stream, p, g);
     else
-        hipLaunchKernelGGL((adapter_gemm_k<T, BWD, true, 2>), grid, dim3(256), 0, ctx->stream, p, g);
+        hipLaunchKernelGGL((adapter_gemm_k<T, BWD, true, false>), grid, dim3(256), 0, ctx->stream, p, g);
     if (g.splits > 1) {
         const long n = static_cast<long>(p.T) * g.M;
         hipLaunchKernelGGL(adapter_join_k<T>, dim3(static_cast<unsigned>(cdiv(n, 64))), dim3(1024), 0, ctx->stream, g.part, g.splits,
@@ -967,7 +980,7 @@ int kdec_adapter_bwd(kdec_ctx* ctx, int dtype, const void* X, long x_rs, const v
     ProfScope ps(ctx, "adapter", 2.0 * T * in * out, 0.0);
     // Few tiles over a long depth: the depth split over blocks, to no fewer
     // than 128 deep each.
-    const long tiles = cdiv(in, 128) * cdiv(T, GN);
+    const long tiles = cdiv(in, 128) * cdiv(T, 128);
     long splits = dX && T > 0 ? cdiv(2L * ctx->num_cus, tiles) : 1;
     if (splits > out / 128) splits = out / 128;
     if (splits < 1) splits = 1;

@@ -92,6 +92,7 @@ struct Tile {
     __device__ static inline int swz(int row) {
         if (sizeof(T) == 2 && NU >= 16) return (row & 3) << 2 | (row >> 2 & 3);
         if (sizeof(T) == 2 && NU == 8) return (row >> 1 & 1) << 2 | (row >> 2 & 3);
+        if (sizeof(T) == 2 && NU == 4) return row >> 2 & 3;
         if (sizeof(T) == 4) return NU == 8 ? row >> 1 & 7 : row & 7;
         return 0;
     }

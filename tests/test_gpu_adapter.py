@@ -241,3 +241,31 @@ def test_refusals(ctx):
     # no adapters at all: the plain projection
     y = tokens.adapter_proj(ctx, d["x"], d["w"], d["a"][:0], d["b"][:0], d["scale"][:0], I, edges)
     assert torch.allclose(y, d["x"] @ d["w"].t(), atol=1e-5)
+
+
+@pytest.mark.parametrize("drop", [None, (0.3, 9, 2)], ids=["", "drop"])
+def test_many_rows_equal_few_rows(ctx, drop):
+    """A call of enough rows for the large product tiles gives each row the bits that a call of fewer rows gives it
+    (the same products in the same order), at sizes that end inside a tile in every direction."""
+    from brosoundml_amd import tokens
+    T, cin, sizes, n, rank = 14999, 200, [500, 24, 404], 5, 8
+    d = make(torch.bfloat16, T, cin, sizes, n, rank, bias=True)
+    wide = make(torch.bfloat16, T, 928, [200], n, rank)  # the input grad's large tiles: 928 features
+    for d, out in ((d, 928), (wide, 200)):
+        I = torch.from_numpy(np.random.default_rng(1).integers(-1, n, T).astype(np.int32)).cuda()
+        edges = torch.tensor(d["edges"], dtype=torch.int32).cuda()
+        y, h = tokens.adapter_proj(ctx, d["x"], d["w"], d["a"], d["b"], d["scale"], I, edges, bias=d["bias"], keep_h=True)
+        dx, _, _ = tokens.adapter_proj_bwd(ctx, d["x"], d["w"], d["a"], d["b"], d["scale"], I, edges, h, d["dy"])
+        part = slice(0, 700)
+        args = (d["x"][part], d["w"], d["a"], d["b"], d["scale"], I[part].contiguous(), edges)
+        y2, h2 = tokens.adapter_proj(ctx, *args, bias=d["bias"], keep_h=True)
+        assert torch.equal(h[part], h2) and torch.equal(y[part], y2)
+        dx2, _, _ = tokens.adapter_proj_bwd(ctx, *args, h2, d["dy"][part])
+        if out < 256:  # (a shorter call may split a longer depth)
+            assert torch.equal(dx[part], dx2)
+        if drop:
+            y, h = tokens.adapter_proj(ctx, d["x"], d["w"], d["a"], d["b"], d["scale"], I, edges, drop=drop, keep_h=True)
+            dx, _, _ = tokens.adapter_proj_bwd(ctx, d["x"], d["w"], d["a"], d["b"], d["scale"], I, edges, h, d["dy"], drop=drop)
+            y2, h2 = tokens.adapter_proj(ctx, *args, drop=drop, keep_h=True)  # the mask goes by row: the first rows' is theirs
+            dx2, _, _ = tokens.adapter_proj_bwd(ctx, *args, h2, d["dy"][part], drop=drop)
+            assert torch.equal(y[part], y2) and (out >= 256 or torch.equal(dx[part], dx2))
