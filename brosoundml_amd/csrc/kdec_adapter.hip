@@ -361,18 +361,16 @@ __device__ inline void low_rank(const Adapter& p, int M, int wm, int u0, int u1,
 // and across it backward, where the transposing LDS read turns them. Tiles
 // are copied straight to shared memory (DIRECT), or go through registers where
 // alignment or size rule that out. BIG: 256 x 256 by eight waves of 128 x 64,
-// steps 32 deep, four buffers (a copy has three steps to arrive, and half the
-// bytes of the small tiles' arrive per product); else 128 x 128 by four waves
-// of 64 x 64, two buffers, two blocks per CU.
+// which copies half the bytes per product; else 128 x 128 by four waves of
+// 64 x 64, two blocks per CU. Two buffers each.
 template <class T, bool BWD, bool DIRECT, bool BIG>
 __global__ __launch_bounds__(BIG ? 512 : 256, DIRECT ? 2 : 1) void adapter_gemm_k(Adapter p, Product g) {
-    constexpr int GM = BIG ? 256 : 128, GN = GM, NT = 2 * GM, STAGES = BIG ? 4 : 2, MB = BIG ? 4 : 2;
-    constexpr int BK = BIG ? 32 : depth_of<T>(), WC = (BWD ? GM : BK) / 8, WR = BWD ? BK : GM;
+    constexpr int GM = BIG ? 256 : 128, GN = GM, NT = 2 * GM, MB = BIG ? 4 : 2;
+    constexpr int BK = depth_of<T>(), WC = (BWD ? GM : BK) / 8, WR = BWD ? BK : GM;
     typedef Tile<T, BWD ? GM : BK> Tw;
     typedef Tile<T, BK> Tz;
     constexpr int NZ = GN * BK / 8 / NT, NW = GM * BK / 8 / NT;
     __shared__ __align__(256) T sw0[GM * BK], sw1[GM * BK], sz0[GN * BK], sz1[GN * BK];
-    __shared__ __align__(256) T sw2[BIG ? GM * BK : 8], sz2[BIG ? GN * BK : 8], sw3[BIG ? GM * BK : 8], sz3[BIG ? GN * BK : 8];
     __shared__ int srow[GN], sid[GN];
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, half = lane >> 5, col = lane & 31;
     // Blocks go to the eight XCDs in turn: each takes a run of row tiles with
@@ -396,7 +394,7 @@ __global__ __launch_bounds__(BIG ? 512 : 256, DIRECT ? 2 : 1) void adapter_gemm_
 
     // direct copies: a thread's units of both tiles
     Copy<T, BWD ? GM : BK, WR, NT> cw;
-    constexpr int NU = Tz::NU, NZU = GN * NU / NT, LOADS = NZU + cw.N;  // copies of a step
+    constexpr int NU = Tz::NU, NZU = GN * NU / NT;
     unsigned oz[NZU];
     __amdgpu_buffer_rsrc_t rz = rows_rsrc<T>(Z, 0, 0, 0);
     const auto z_offsets = [&](int depth) __attribute__((always_inline)) {  // columns of the tile that are there
@@ -441,11 +439,9 @@ __global__ __launch_bounds__(BIG ? 512 : 256, DIRECT ? 2 : 1) void adapter_gemm_
             }
         }
     };
-    const auto landed = [&](T* tw, T* tz, int ahead) __attribute__((always_inline)) {
+    const auto landed = [&](T* tw, T* tz) __attribute__((always_inline)) {
         if constexpr (DIRECT) {
-            if (ahead >= 2) wait_loads<2 * LOADS>();  // the steps after it may be on their way
-            else if (ahead == 1) wait_loads<LOADS>();
-            else wait_loads<0>();
+            wait_loads<0>();
         } else {
 #pragma unroll
             for (int i = 0; i < NZ; ++i) Tz::put8(tz, (tid + i * NT) / (BK / 8), (tid + i * NT) % (BK / 8), fz[i]);
@@ -459,9 +455,7 @@ __global__ __launch_bounds__(BIG ? 512 : 256, DIRECT ? 2 : 1) void adapter_gemm_
 #pragma unroll
         for (int j = 0; j < 2; ++j) acc[i][j] = f32x16{};
     if (c0 < c1) load(c0, sw0, sz0);
-    if (BIG && c0 + 1 < c1) load(c0 + 1, sw1, sz1);
-    if (BIG && c0 + 2 < c1) load(c0 + 2, sw2, sz2);
-    constexpr int LB = BIG && BWD ? 1 : 2;  // 32 LB features at a time, which the registers leave room for
+    constexpr int LB = BIG ? 1 : 2;  // 32 LB features at a time, which the registers leave room for
     const auto low = [&](auto first) __attribute__((always_inline)) {
         constexpr int I0 = LB * decltype(first)::value;
         const int m = wm + 32 * I0;
@@ -474,6 +468,10 @@ __global__ __launch_bounds__(BIG ? 512 : 256, DIRECT ? 2 : 1) void adapter_gemm_
     if constexpr (MB > 2 * LB) {
         low(std::integral_constant<int, 2>{});
         low(std::integral_constant<int, 3>{});
+    }
+    if (DIRECT && BIG) {  // formed again rather than held meanwhile
+        asm volatile("" ::: "memory");
+        z_offsets(g.K - c0 * BK);
     }
     if (BWD && p.dropping) {
 #pragma unroll
@@ -491,45 +489,74 @@ __global__ __launch_bounds__(BIG ? 512 : 256, DIRECT ? 2 : 1) void adapter_gemm_
                         const bool keep = ((x & 1) ? v >> 16 : v & 0xFFFFu) >= p.drop.thr;
                         acc[i][j][4 * q + x] = keep ? acc[i][j][4 * q + x] * p.drop.keep : 0.0f;
                     }
+                    __builtin_amdgcn_sched_barrier(0);  // one mask's registers at a time
                 }
     }
-    // One step on the tiles at tw, tz; the next step's are at nw, nz, and a
-    // step's load goes to the buffer that the step before this one used.
-    const auto walk = [&](int c, const T* tw, const T* tz, T* nw, T* nz, T* lw, T* lz) __attribute__((always_inline)) {
-        if (c + STAGES - 1 < c1) load(c + STAGES - 1, lw, lz);
+    const auto operands = [&](int k, const T* tw, const T* tz, Frag<T> (&w)[MB], Frag<T> (&z)[2]) __attribute__((always_inline)) {
 #pragma unroll
-        for (int k = 0; k < BK / 16; ++k) {
-            Frag<T> w[MB], z[2];
-#pragma unroll
-            for (int i = 0; i < MB; ++i) {
-                if constexpr (BWD) w[i] = lds_cols<GM, false>(tw, 16 * k, wf + 32 * i);
-                else w[i] = lds_rows<T, BK>(tw, wf + 32 * i, k);
-            }
-#pragma unroll
-            for (int j = 0; j < 2; ++j) z[j] = lds_rows<T, BK>(tz, wn + 32 * j, k);
-#pragma unroll
-            for (int i = 0; i < MB; ++i)
-#pragma unroll
-                for (int j = 0; j < 2; ++j) acc[i][j] = mma32(w[i], z[j], acc[i][j]);
+        for (int i = 0; i < MB; ++i) {
+            if constexpr (BWD) w[i] = lds_cols<GM, false>(tw, 16 * k, wf + 32 * i);
+            else w[i] = lds_rows<T, BK>(tw, wf + 32 * i, k);
         }
-        if (c + 1 < c1) landed(nw, nz, BIG ? c1 - 2 - c : 0);
-        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < 2; ++j) z[j] = lds_rows<T, BK>(tz, wn + 32 * j, k);
+    };
+    const auto products = [&](const Frag<T> (&w)[MB], const Frag<T> (&z)[2]) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < MB; ++i)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) acc[i][j] = mma32(w[i], z[j], acc[i][j]);
     };
     if (c0 < c1) {
-        landed(sw0, sz0, 0);
-        __syncthreads();
+        landed(sw0, sz0);
+        lds_barrier();
     }
     if constexpr (BIG) {
-        for (int c = c0; c < c1; c += 4) {
-            walk(c, sw0, sz0, sw1, sz1, sw3, sz3);
-            if (c + 1 < c1) walk(c + 1, sw1, sz1, sw2, sz2, sw0, sz0);
-            if (c + 2 < c1) walk(c + 2, sw2, sz2, sw3, sz3, sw1, sz1);
-            if (c + 3 < c1) walk(c + 3, sw3, sz3, sw0, sz0, sw2, sz2);
+        // A step is four products deep. Each one's operands are read under the
+        // one before, across the barrier too: before a step's last products
+        // the next tile is awaited, and the tile after it sent for, to the
+        // place of this step's, whose operands all are in registers by then.
+        Frag<T> w[2][MB], z[2][2];
+        if (c0 < c1) {
+            if (c0 + 1 < c1) load(c0 + 1, sw1, sz1);
+            operands(0, sw0, sz0, w[0], z[0]);
+        }
+        const auto walk = [&](int c, T* tw, T* tz, T* nw, T* nz) __attribute__((always_inline)) {
+#pragma unroll
+            for (int k = 0; k < 3; ++k) {
+                operands(k + 1, tw, tz, w[(k + 1) & 1], z[(k + 1) & 1]);
+                __builtin_amdgcn_sched_barrier(0);
+                products(w[k & 1], z[k & 1]);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            if (c + 1 < c1) {
+                landed(nw, nz);
+                lds_barrier();
+                if (c + 2 < c1) load(c + 2, tw, tz);
+                operands(0, nw, nz, w[0], z[0]);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            products(w[1], z[1]);
+        };
+        for (int c = c0; c < c1; c += 2) {
+            walk(c, sw0, sz0, sw1, sz1);
+            if (c + 1 < c1) walk(c + 1, sw1, sz1, sw0, sz0);
         }
     } else {
+        const auto walk = [&](int c, const T* tw, const T* tz, T* nw, T* nz) __attribute__((always_inline)) {
+            if (c + 1 < c1) load(c + 1, nw, nz);
+#pragma unroll
+            for (int k = 0; k < BK / 16; ++k) {
+                Frag<T> w[MB], z[2];
+                operands(k, tw, tz, w, z);
+                products(w, z);
+            }
+            if (c + 1 < c1) landed(nw, nz);
+            lds_barrier();
+        };
         for (int c = c0; c < c1; c += 2) {
-            walk(c, sw0, sz0, sw1, sz1, sw1, sz1);
-            if (c + 1 < c1) walk(c + 1, sw1, sz1, sw0, sz0, sw0, sz0);
+            walk(c, sw0, sz0, sw1, sz1);
+            if (c + 1 < c1) walk(c + 1, sw1, sz1, sw0, sz0);
         }
     }
 #pragma unroll

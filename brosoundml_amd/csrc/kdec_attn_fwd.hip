@@ -271,7 +271,7 @@ __global__ __launch_bounds__(AT, sizeof(T) == 2 ? (DP == 64 ? 3 : 2) : 1) void a
 // from memory into the product's registers, values through the wave's own
 // shared memory for their transpose, so no wave waits for another.
 template <class T, int DP, bool CAP, bool BIAS>
-__global__ __launch_bounds__(AT, 1) void attn_rows_k(Fwd p, int chunks) {
+__global__ __launch_bounds__(AT, sizeof(T) == 2 ? 2 : 1) void attn_rows_k(Fwd p, int chunks) {
     constexpr int NC = DP / 16, ND = DP / 32;
     constexpr int JE = 8;  // columns joined at a time
     __shared__ __align__(16) T sv0[4][RN * DP], sv1[4][RN * DP];
@@ -390,27 +390,39 @@ __global__ __launch_bounds__(AT, 1) void attn_rows_k(Fwd p, int chunks) {
     if (valid && wave == ((col / JE) & 3)) finish<T, DP>(p, kvh, e, row, head, split, half, acc, m, l);
 }
 
-// Joins the splits of an entry: one wave per entry, lanes over the output.
+// Joins the splits of an entry (at most 64): one wave per entry, a lane for
+// every split's state, then lanes over the output, the splits in order.
 template <class T>
-__global__ __launch_bounds__(AT) void attn_join_k(Fwd p) {
+__global__ __launch_bounds__(64) void attn_join_k(Fwd p) {
     const Args& a = p.a;
-    const int lane = threadIdx.x & 63;
-    const long w = static_cast<long>(blockIdx.x) * (AT / 64) + (threadIdx.x >> 6);
-    const long n = static_cast<long>(a.Hkv) * a.E;
-    if (w >= n) return;
+    const int lane = threadIdx.x;
+    const long w = blockIdx.x, n = static_cast<long>(a.Hkv) * a.E;
     const int kvh = static_cast<int>(w / a.E), e = static_cast<int>(w - static_cast<long>(kvh) * a.E);
     const int row = e / a.G, head = kvh * a.G + e - row * a.G;
-    float m = -INF;
-    for (int s = 0; s < p.splits; ++s) m = fmaxf(m, p.part_ml[2 * (s * n + w)]);
-    const float m0 = m == -INF ? 0.0f : m;
-    float l = 0.0f, o[2] = {0.0f, 0.0f};
-    for (int s = 0; s < p.splits; ++s) {
-        const float f = __builtin_amdgcn_exp2f(p.part_ml[2 * (s * n + w)] - m0);
-        l += f * p.part_ml[2 * (s * n + w) + 1];
+    float m = -INF, l = 0.0f;
+    if (lane < p.splits) {
+        const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + 2 * (lane * n + w));
+        m = ml.x;
+        l = ml.y;
+    }
+    float top = m;
+    for (int o = 32; o; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
+    const float f = __builtin_amdgcn_exp2f(m - (top == -INF ? 0.0f : top));  // zero past the splits
+    l *= f;
+    for (int o = 32; o; o >>= 1) l += __shfl_xor(l, o);
+    float o[2] = {0.0f, 0.0f};
+    for (int s = 0; s < p.splits; s += 8) {  // eight loads in flight
+        float v[8][2];
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const int d = lane + 64 * i;
-            if (d < p.D_out) o[i] += f * p.part_o[(s * n + w) * a.D + d];
+        for (int x = 0; x < 8; ++x)
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+                v[x][i] = s + x < p.splits && lane + 64 * i < p.D_out ? p.part_o[((s + x) * n + w) * a.D + lane + 64 * i] : 0.0f;
+#pragma unroll
+        for (int x = 0; x < 8; ++x) {
+            const float g = __shfl(f, s + x);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) o[i] = __builtin_fmaf(g, v[x][i], o[i]);
         }
     }
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
@@ -420,7 +432,7 @@ __global__ __launch_bounds__(AT) void attn_join_k(Fwd p) {
         const int d = lane + 64 * i;
         if (d < p.D_out) out[d] = static_cast<T>(o[i] * inv);
     }
-    if (lane == 0) p.lse[static_cast<long>(head) * a.m.Tq + row] = l == 0.0f ? -INF : m * LN2 + logf(l);
+    if (lane == 0) p.lse[static_cast<long>(head) * a.m.Tq + row] = l == 0.0f ? -INF : top * LN2 + logf(l);
 }
 
 struct Launch {
@@ -429,8 +441,8 @@ struct Launch {
         if (rows) hipLaunchKernelGGL((attn_rows_k<T, DP, CAP, BIAS>), grid, dim3(AT), 0, ctx->stream, p, chunks);
         else hipLaunchKernelGGL((attn_fwd_k<T, DP, CAP, BIAS>), grid, dim3(AT), 0, ctx->stream, p);
         if (p.splits > 1)
-            hipLaunchKernelGGL(attn_join_k<T>, dim3(static_cast<unsigned>(cdiv(static_cast<long>(p.a.Hkv) * p.a.E, AT / 64))),
-                               dim3(AT), 0, ctx->stream, p);
+            hipLaunchKernelGGL(attn_join_k<T>, dim3(static_cast<unsigned>(static_cast<long>(p.a.Hkv) * p.a.E)), dim3(64), 0,
+                               ctx->stream, p);
         return launch_check(ctx, "kdec_attn_fwd");
     }
 };
@@ -477,10 +489,12 @@ extern "C" int kdec_attn_fwd(kdec_ctx* ctx, int dtype, const void* Q, long q_rs,
     const long blocks = tiles * Hkv;
     KDEC_CHECK(ctx, blocks < INT_MAX, "kdec_attn_fwd: too many rows");
     // Split the keys where the rows alone do not fill the device, to no fewer
-    // than 256 keys a part.
+    // than 256 keys a part. Few rows take twice as many parts: their documents
+    // differ in length, and the longest ends last.
     const long each = docs > 0 ? Tk / docs : 0;
-    long splits = cdiv(2L * ctx->num_cus, blocks);
+    long splits = cdiv((rows ? 4L : 2L) * ctx->num_cus, blocks);
     if (splits > each / 256) splits = each / 256;
+    if (splits > 64) splits = 64;  // what the join holds
     if (splits < 1) splits = 1;
     p.splits = static_cast<int>(splits);
     if (splits > 1) {

@@ -197,6 +197,16 @@ __device__ inline void wait_loads() {
     __builtin_amdgcn_s_waitcnt((N & 15) | (N >> 4) << 14 | 7 << 4 | 15 << 8);
 }
 
+// A barrier for shared memory alone: the wave's own reads and writes of it are
+// done, its copies from memory may still be on their way (__syncthreads would
+// wait for them too).
+__device__ inline void lds_barrier() {
+    __builtin_amdgcn_s_waitcnt(15 | 3 << 14 | 7 << 4);  // lgkmcnt(0)
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+
 // 16 bytes per lane from the descriptor's offset `off` to shared memory at
 // `to` (wave-uniform) + 16 * lane.
 __device__ inline void copy16(__amdgpu_buffer_rsrc_t r, void* to, int off) {
