@@ -44,6 +44,7 @@ struct Args {
     const float* slopes;
     float scale, cap;
     int Hq, Hkv, G, D, E;  // G = Hq / Hkv, E = Tq * G entries per key head
+    bool by_doc;           // blocks of entries end with their document
 };
 
 struct Row {
@@ -101,6 +102,95 @@ __device__ inline Row row_at(const Docs& m, int i, int first) {
     if (n == 64) d = doc_of(m.q_off, m.docs, i);
     if (d < 0 || d >= m.docs || i >= m.q_off[d + 1]) return Row{INT_MAX, INT_MIN, 0};
     return row_in(m, d, i);
+}
+
+// Blocks that end with their document. Documents, and the rows before the
+// first and past the last as two more, are cut into blocks of `size`; a row
+// counts `each` times. Every lane takes one document's number of blocks, a
+// scan over the wave finds block b's: rows [lo, hi) of document doc (-1 and
+// docs are the two others), whose block `place` it is. False past the last.
+struct Piece {
+    int doc, lo, hi, place;
+};
+__device__ inline bool piece_at(const int* off, int docs, int rows, int each, int size, int b, Piece& p) {
+    const int lane = threadIdx.x & 63;
+    const auto at = [&](int d) { return d < 0 ? 0 : docs > 0 && d <= docs ? min(max(off[d], 0), rows) : rows; };
+    int before = 0;
+    for (int base = -1; base <= docs; base += 64) {
+        const int lo = at(base + lane), hi = at(base + lane + 1);
+        const int n = hi > lo ? ((hi - lo) * each + size - 1) / size : 0;
+        int sum = n;
+#pragma unroll
+        for (int o = 1; o < 64; o *= 2) {
+            const int s = __shfl_up(sum, o);
+            sum += lane >= o ? s : 0;
+        }
+        const int all = __builtin_amdgcn_readlane(sum, 63);
+        if (b - before < all) {
+            const int l = __builtin_popcountll(__builtin_amdgcn_ballot_w64(before + sum <= b));
+            if (l > 63) return false;
+            p.doc = base + l;
+            p.lo = __builtin_amdgcn_readlane(lo, l);
+            p.hi = __builtin_amdgcn_readlane(hi, l);
+            p.place = b - before - __builtin_amdgcn_readlane(sum - n, l);
+            return p.place >= 0 && p.place < __builtin_amdgcn_readlane(n, l);
+        }
+        before += all;
+    }
+    return false;
+}
+
+// A lane's entry: row * G + head of the group. `again` hides that the second
+// call gives what the first gave, so that a kernel's end forms it anew and its
+// loops need not hold it.
+struct Entry {
+    int e, row, head, half;
+    bool valid;
+};
+__device__ inline Entry entry_of(const Args& a, int kvh, int first, int end, bool again) {
+    Entry r;
+    int lane = threadIdx.x & 63, G = a.G;
+    if (again) {
+        unsigned ones = ~0u;
+        asm volatile("" : "+s"(ones), "+s"(G));
+        lane = __builtin_amdgcn_mbcnt_hi(ones, __builtin_amdgcn_mbcnt_lo(ones, 0));
+    }
+    r.half = lane >> 5;
+    r.e = first + (lane & 31);
+    r.valid = r.e < end;
+    r.row = r.valid ? r.e / G : 0;
+    r.head = kvh * G + (r.valid ? r.e - r.row * G : 0);
+    return r;
+}
+
+// Block `tile`'s entries of a key head: [first, end), at most BM of them, the
+// wave's from e0, and the document that holds them all (by_doc).
+struct Span {
+    int e0, end, doc;
+};
+__device__ inline bool span_at(const Args& a, int tile, int wave, Span& s) {
+    if (!a.by_doc) {
+        s = Span{tile * BM + wave * 32, a.E, 0};
+        return true;
+    }
+    Piece p;
+    if (!piece_at(a.m.q_off, a.m.docs, a.m.Tq, a.G, BM, tile, p)) return false;
+    s = Span{p.lo * a.G + p.place * BM + wave * 32, p.hi * a.G, p.doc};
+    return true;
+}
+__device__ inline Row row_of(const Args& a, const Span& s, const Entry& e) {
+    Row r{INT_MAX, INT_MIN, 0};
+    if (!a.by_doc) r = row_at(a.m, e.row, min(s.e0, a.E - 1) / a.G);
+    else if (s.doc >= 0 && s.doc < a.m.docs) r = row_in(a.m, s.doc, e.row);
+    return e.valid ? r : Row{INT_MAX, INT_MIN, 0};
+}
+
+// The larger of a value and that of the lane 32 away.
+__device__ inline float max32(float x) {
+    const unsigned u = __float_as_uint(x);
+    const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    const unsigned lo = r[0], hi = r[1];
+    return fmaxf(__uint_as_float(lo), __uint_as_float(hi));
 }
 
 // What a block of 128 entries (32 per wave) walks: keys [lo, hi) in tiles of
@@ -200,6 +290,13 @@ __device__ inline float grad_p(const Score<T, CAP, BIAS>& rule, float s, float d
 }
 
 // ─── host ───
+
+// Whether blocks of `size` entries (or keys) end with their document: where
+// the documents hold a block's worth each. Else blocks of several documents
+// leave fewer waves without rows, though a block then walks the keys of all
+// of them, the most of which a wave does not see.
+inline bool by_document(int docs, long entries, int size) { return docs < 1023 && docs * static_cast<long>(size) <= entries; }
+inline long doc_blocks(bool by_doc, int docs, long entries, int size) { return cdiv(entries, size) + (by_doc ? docs + 2 : 0); }
 
 // Kernels of a call by its type, width and score: L::run<T, DP, CAP, BIAS>.
 template <class L, class T, int DP, class... P>

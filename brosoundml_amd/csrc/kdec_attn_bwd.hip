@@ -27,6 +27,7 @@ struct Bwd {
     bool vec_dq, vec_dk, vec_dv;
     Row* rows;    // (Tq)
     float2* stat; // (Hq, Tq): lse in log2 units, delta = dO . O
+    bool by_doc_k;  // blocks of keys end with their document
     int parts;    // blocks that share a key tile's rows
     float* part;  // (parts, Hkv, Tk, 2, D): their dK / scale and dV
 };
@@ -38,7 +39,7 @@ struct Bwd {
 // are zeros; one whose delta is not finite gets NaN, which then marks every
 // gradient that the row reaches.
 template <class T, int DP, bool CAP, bool BIAS>
-__global__ __launch_bounds__(AT, sizeof(T) == 2 ? (DP == 64 && !BIAS ? 3 : 2) : 1) void attn_dq_k(Bwd b) {
+__global__ __launch_bounds__(AT, sizeof(T) == 2 ? (DP == 64 ? 3 : 2) : 1) void attn_dq_k(Bwd b) {
     constexpr int NC = DP / 16, ND = DP / 32;
     __shared__ __align__(16) T sk0[BN * DP], sk1[BN * DP], sv0[BN * DP], sv1[BN * DP];
     __shared__ int red[4][4];
@@ -47,11 +48,12 @@ __global__ __launch_bounds__(AT, sizeof(T) == 2 ? (DP == 64 && !BIAS ? 3 : 2) : 
     const int kvh = blockIdx.x % a.Hkv;
     int tile = blockIdx.x / a.Hkv;
     if (a.m.causal) tile = gridDim.x / a.Hkv - 1 - tile;  // the longest walks first
-    const int e = tile * BM + wave * 32 + (lane & 31);
-    const bool valid = e < a.E;
-    const int row = valid ? e / a.G : 0, head = kvh * a.G + (valid ? e - row * a.G : 0);
-    Row me = row_at(a.m, row, min(tile * BM + wave * 32, a.E - 1) / a.G);
-    if (!valid) me = Row{INT_MAX, INT_MIN, 0};
+    Span sp;
+    if (!span_at(a, tile, wave, sp)) return;
+    const Entry en = entry_of(a, kvh, sp.e0, sp.end, false);
+    const bool valid = en.valid;
+    const int row = en.row, head = en.head;
+    const Row me = row_of(a, sp, en);
     const Walk w = walk_of(me, valid, red);
     const int t1 = w.hi > w.lo ? (w.hi - w.lo + BN - 1) / BN : 0;
 
@@ -141,7 +143,7 @@ __global__ __launch_bounds__(AT, sizeof(T) == 2 ? (DP == 64 && !BIAS ? 3 : 2) : 
     const auto walk = [&](auto masked, int t, const T* tk, const T* tv, T* nk, T* nv) __attribute__((always_inline)) {
         const int j0 = w.lo + t * BN;
         if (t + 1 < t1) load(t + 1, nk, nv);
-        if (!decltype(masked)::value || (w.wlo < j0 + BN && w.whi > j0)) step(masked, j0, tk, tv);
+        if (w.wlo < j0 + BN && w.whi > j0) step(masked, j0, tk, tv);
         if (t + 1 < t1) landed(t + 1, nk);
         __syncthreads();
     };
@@ -159,13 +161,14 @@ __global__ __launch_bounds__(AT, sizeof(T) == 2 ? (DP == 64 && !BIAS ? 3 : 2) : 
     walks(std::true_type{}, 0, f0);
     walks(std::false_type{}, f0, f1);
     walks(std::true_type{}, f1, t1);
-    if (!valid) return;
-    T* o = static_cast<T*>(b.dQ) + row * b.dq_rs + head * b.dq_hs;
+    const Entry to = entry_of(a, kvh, sp.e0, sp.end, true);
+    if (!to.valid) return;
+    T* o = static_cast<T*>(b.dQ) + to.row * b.dq_rs + to.head * b.dq_hs;
 #pragma unroll
     for (int dt = 0; dt < ND; ++dt)
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
-            const int d = 32 * dt + 8 * x + 4 * half;
+            const int d = 32 * dt + 8 * x + 4 * to.half;
             store4(o + d, b.D_out - d, b.vec_dq, acc[dt][4 * x] * a.scale, acc[dt][4 * x + 1] * a.scale,
                    acc[dt][4 * x + 2] * a.scale, acc[dt][4 * x + 3] * a.scale);
         }
@@ -201,26 +204,42 @@ __global__ __launch_bounds__((128 * key_groups<T, DP, BIAS>()), (sizeof(T) == 2 
     const Args& a = b.a;
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, half = lane >> 5;
     const int pair = wave % KG, role = wave / KG;
-    const int kvh = blockIdx.x % a.Hkv, j0 = (blockIdx.x / a.Hkv) * KEYS, part = blockIdx.y;
+    const int kvh = blockIdx.x % a.Hkv, part = blockIdx.y;
+    int j0 = (blockIdx.x / a.Hkv) * KEYS, end = a.m.Tk;  // the block's keys
+    Piece piece{};
+    if (b.by_doc_k) {
+        if (!piece_at(a.m.k_off, a.m.docs, a.m.Tk, 1, KEYS, blockIdx.x / a.Hkv, piece)) return;
+        j0 = piece.lo + piece.place * KEYS;
+        end = piece.hi;
+    }
     const int wkey = j0 + pair * 32, key = wkey + (lane & 31);
-    const bool valid = key < a.m.Tk;
+    const bool valid = key < end;
 
-    // the rows [e0, e1) that may see keys of the block, and those [f0, f1)
-    // that all see all of them
-    int e0 = 0, e1 = 0, f0 = 0, f1 = 0;
+    // The rows [e0, e1) that may see keys of the block, and those [f0, f1)
+    // that all see all of its keys below `stop`. Where a block ends with its
+    // document, stop is the end of the document's keys: what a lane forms for
+    // keys past it is dropped at the end.
+    int e0 = 0, e1 = 0, f0 = 0, f1 = 0, stop = j0 + KEYS;
     {
-        const int d0 = max(doc_of(a.m.k_off, a.m.docs, j0), 0);
-        const int d1 = doc_of(a.m.k_off, a.m.docs, min(j0 + KEYS, a.m.Tk) - 1);
+        int d0, d1;
+        if (b.by_doc_k) {
+            d0 = piece.doc;
+            d1 = piece.doc < a.m.docs ? piece.doc : -1;
+        } else {
+            d0 = max(doc_of(a.m.k_off, a.m.docs, j0), 0);
+            d1 = doc_of(a.m.k_off, a.m.docs, min(j0 + KEYS, a.m.Tk) - 1);
+        }
         if (d1 >= 0) {
             const Doc c = doc_at(a.m, d0), z = doc_at(a.m, d1);
             const int skip = c.lk - c.lq;  // position of the first row's key
+            if (b.by_doc_k) stop = min(stop, c.k0 + c.lk);
             e0 = c.q0;
             if (a.m.causal && j0 - c.k0 >= c.prefix) e0 = min(max(c.q0 + (j0 - c.k0) - skip, c.q0), c.q0 + c.lq);
             e1 = z.q0 + z.lq;
-            if (d0 == d1 && j0 >= c.k0 && j0 + KEYS <= c.k0 + c.lk) {
+            if (b.by_doc_k && j0 >= stop) e1 = e0;
+            if (d0 == d1 && j0 >= c.k0 && j0 < stop && stop <= c.k0 + c.lk) {
                 f0 = c.q0;
-                if (a.m.causal && j0 + KEYS - c.k0 > c.prefix)
-                    f0 = min(max(c.q0 + (j0 + KEYS - 1 - c.k0) - skip, c.q0), c.q0 + c.lq);
+                if (a.m.causal && stop - c.k0 > c.prefix) f0 = min(max(c.q0 + (stop - 1 - c.k0) - skip, c.q0), c.q0 + c.lq);
                 f1 = c.q0 + c.lq;
             }
         }
@@ -228,14 +247,17 @@ __global__ __launch_bounds__((128 * key_groups<T, DP, BIAS>()), (sizeof(T) == 2 
         e1 = __builtin_amdgcn_readfirstlane(e1);
         f0 = __builtin_amdgcn_readfirstlane(f0);
         f1 = __builtin_amdgcn_readfirstlane(f1);
+        stop = __builtin_amdgcn_readfirstlane(stop);
     }
+    const int wstop = min(wkey + 32, stop);
     // Turns of two tiles, the group's heads one after another; of a head's
-    // `per` turns, [p0, p1) are seen whole.
+    // `per` turns, [p0, p1) are seen whole (rows past e1 are zeros and have
+    // probabilities of zero, so the last turn may end anywhere).
     const int per = e1 > e0 ? (e1 - e0 + PAIR - 1) / PAIR : 0;
     int p0 = 0, p1 = 0;
     if (f1 > f0) {
         p0 = max((f0 - e0 + PAIR - 1) / PAIR, 0);
-        p1 = min((f1 - e0) / PAIR, per);
+        p1 = f1 >= e1 ? per : (f1 - e0) / PAIR;
         if (p0 >= p1) p0 = p1 = 0;
     }
     const long turns = static_cast<long>(per) * a.G;
@@ -305,11 +327,11 @@ __global__ __launch_bounds__((128 * key_groups<T, DP, BIAS>()), (sizeof(T) == 2 
             constexpr bool MASKED = decltype(masked)::value;
             constexpr int n0 = 32 * ROLE;  // the wave's half
             const T *hq = tq + n0 * DP, *hg = tg + n0 * DP;
-            bool any = true, whole = true;  // some, all of the half's rows and the wave's keys meet
+            bool any = wkey < wstop, whole = true;  // some, all of the half's rows and the wave's keys meet
             if (MASKED) {
                 const int i = n0 + (lane & 31), lo = slo[buf][i], hi = shi[buf][i];
-                any = __builtin_amdgcn_ballot_w64(lo < wkey + 32 && hi > wkey) != 0;
-                whole = __builtin_amdgcn_ballot_w64(!(lo <= wkey && hi >= wkey + 32)) == 0;
+                any = __builtin_amdgcn_ballot_w64(lo < wstop && hi > wkey) != 0;
+                whole = __builtin_amdgcn_ballot_w64(!(lo <= wkey && hi >= wstop)) == 0;
                 if (lane == 0) some[pair][ROLE] = any;
             }
             Frag<T> own[2];
@@ -370,7 +392,7 @@ __global__ __launch_bounds__((128 * key_groups<T, DP, BIAS>()), (sizeof(T) == 2 
             }
             __syncthreads();
             const T *mine = ROLE ? hq : hg, *other = (ROLE ? tq : tg) + (32 - n0) * DP;
-            if (!MASKED || any) {
+            if (any) {
 #pragma unroll
                 for (int c = 0; c < 2; ++c)
 #pragma unroll
@@ -379,7 +401,7 @@ __global__ __launch_bounds__((128 * key_groups<T, DP, BIAS>()), (sizeof(T) == 2 
                         hold<T>();
                     }
             }
-            if (!MASKED || some[pair][1 - ROLE]) {
+            if (MASKED ? some[pair][1 - ROLE] : any) {
 #pragma unroll
                 for (int c = 0; c < 2; ++c) {
                     const Frag<T> f = pass[pair][1 - ROLE][c][lane];
@@ -418,6 +440,10 @@ __global__ __launch_bounds__((128 * key_groups<T, DP, BIAS>()), (sizeof(T) == 2 
             }
         }
         if (!valid) return;
+        if (key >= stop) {
+#pragma unroll
+            for (int d = 0; d < ND; ++d) acc[d] = f32x16{};
+        }
         T* out = ROLE ? static_cast<T*>(b.dK) + kvh * b.dk_hs + key * b.dk_rs : static_cast<T*>(b.dV) + kvh * b.dv_hs + key * b.dv_rs;
         const float f = ROLE ? a.scale : 1.0f;
         float* o = b.part + (((static_cast<long>(part) * a.Hkv + kvh) * a.m.Tk + key) * 2 + 1 - ROLE) * a.D;
@@ -499,7 +525,7 @@ extern "C" int kdec_attn_bwd(kdec_ctx* ctx, int dtype, const void* Q, long q_rs,
     ProfScope ps(ctx, "attn", 0.0, 0.0);
     Bwd b{};
     b.a = Args{{Q, q_rs, q_hs}, {K, k_rs, k_hs}, {V, v_rs, v_hs}, {q_off, k_off, k_len, prefix, docs, causal != 0, Tq, Tk},
-               slopes, scale, cap, Hq, Hkv, G, D, Tq * G};
+               slopes, scale, cap, Hq, Hkv, G, D, Tq * G, by_document(docs, static_cast<long>(Tq) * G, BM)};
     b.O = Heads{O, o_rs, o_hs};
     b.dO = Heads{dO, do_rs, do_hs};
     b.vec_o = plain(b.O, D, size);
@@ -526,7 +552,9 @@ extern "C" int kdec_attn_bwd(kdec_ctx* ctx, int dtype, const void* Q, long q_rs,
     b.vec_dk = D % 4 == 0 && aligned(Heads{dK, dk_rs, dk_hs}, size, 4 * size);
     b.vec_dv = D % 4 == 0 && aligned(Heads{dV, dv_rs, dv_hs}, size, 4 * size);
     const size_t stat_bytes = (static_cast<size_t>(Tq) * Hq * sizeof(float2) + 255) & ~size_t(255);
-    const long q_blocks = cdiv(b.a.E, BM) * Hkv, k_blocks = cdiv(Tk, D <= 64 || dtype == KDEC_F32 || slopes ? 64 : 128) * Hkv;
+    const int keys = D <= 64 || dtype == KDEC_F32 || slopes ? 64 : 128;  // of a block
+    b.by_doc_k = by_document(docs, Tk, keys);
+    const long q_blocks = doc_blocks(b.a.by_doc, docs, b.a.E, BM) * Hkv, k_blocks = doc_blocks(b.by_doc_k, docs, Tk, keys) * Hkv;
     KDEC_CHECK(ctx, k_blocks < INT_MAX, "kdec_attn_bwd: too many keys");
     // Key tiles too few to fill the device (causal walks differ in length, so
     // two blocks per CU) share their rows among parts of no fewer than four

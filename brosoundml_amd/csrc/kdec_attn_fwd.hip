@@ -83,7 +83,7 @@ __device__ inline void soft_step(const Score<T, CAP, BIAS>& rule, const Row& row
     for (int n = 0; n < N; ++n)
 #pragma unroll
         for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[n][r]);
-    mx = fmaxf(mx, __shfl_xor(mx, 32));
+    mx = max32(mx);
     if (__builtin_amdgcn_ballot_w64((mx - st.m) * unit > 8.0f || (st.m == -INF && mx > -INF))) {
         const float m = fmaxf(st.m, mx);
         const float f = __builtin_amdgcn_exp2f((st.m - (m == -INF ? 0.0f : m)) * unit);
@@ -143,11 +143,13 @@ __device__ inline void finish(const Fwd& p, int kvh, int e, int row, int head, i
     if (!half) p.lse[static_cast<long>(head) * a.m.Tq + row] = l == 0.0f ? -INF : m * LN2 + logf(l);
 }
 
+template <class T, int DP> constexpr bool narrow() { return sizeof(T) == 2 && DP == 64; }
+
 // A block holds 128 entries of one key head (32 per wave) and walks the keys
 // that its rows see in tiles of 64, staged in shared memory two buffers deep
 // with the tile after next on its way.
 template <class T, int DP, bool CAP, bool BIAS>
-__global__ __launch_bounds__(AT, sizeof(T) == 2 ? (DP == 64 ? 3 : 2) : 1) void attn_fwd_k(Fwd p) {
+__global__ __launch_bounds__(AT, (sizeof(T) == 2 ? (narrow<T, DP>() ? (CAP || BIAS ? 3 : 4) : 2) : 1)) void attn_fwd_k(Fwd p) {
     constexpr int NC = DP / 16, ND = DP / 32;
     __shared__ __align__(16) T sk0[BN * DP], sk1[BN * DP], sv0[BN * DP], sv1[BN * DP];
     __shared__ unsigned bad[3][2];  // rows of the tile that hold values that are not finite
@@ -157,11 +159,12 @@ __global__ __launch_bounds__(AT, sizeof(T) == 2 ? (DP == 64 ? 3 : 2) : 1) void a
     const int kvh = blockIdx.x % a.Hkv;
     int tile = blockIdx.x / a.Hkv;
     if (a.m.causal) tile = gridDim.x / a.Hkv - 1 - tile;  // the longest walks first
-    const int e = tile * BM + wave * 32 + (lane & 31);
-    const bool valid = e < a.E;
-    const int row = valid ? e / a.G : 0, head = kvh * a.G + (valid ? e - row * a.G : 0);
-    Row me = row_at(a.m, row, min(tile * BM + wave * 32, a.E - 1) / a.G);
-    if (!valid) me = Row{INT_MAX, INT_MIN, 0};
+    Span sp;
+    if (!span_at(a, tile, wave, sp)) return;
+    const Entry en = entry_of(a, kvh, sp.e0, sp.end, false);
+    const bool valid = en.valid;
+    const int row = en.row, head = en.head;
+    const Row me = row_of(a, sp, en);
     if (tid < 6) bad[tid >> 1][tid & 1] = 0;
     const Walk w = walk_of(me, valid, red);
     const int tiles = w.hi > w.lo ? (w.hi - w.lo + BN - 1) / BN : 0;
@@ -207,35 +210,42 @@ __global__ __launch_bounds__(AT, sizeof(T) == 2 ? (DP == 64 ? 3 : 2) : 1) void a
     Soft st;
     bool poison = false;
     const auto step = [&](auto masked, int j0, const T* tk, const T* tv) __attribute__((always_inline)) {
-        f32x16 s[2];
+        // Narrow heads take the keys 32 at a time, which leaves room for four
+        // waves per SIMD; wide ones 64, for fewer steps of the softmax.
+        constexpr int N = narrow<T, DP>() ? 1 : 2;
+        const bool whole = j0 >= w.wfull_lo && j0 + BN <= w.wfull_hi;
 #pragma unroll
-        for (int n = 0; n < 2; ++n) {
-            s[n] = f32x16{};
+        for (int n0 = 0; n0 < 2; n0 += N) {
+            f32x16 s[N];
 #pragma unroll
-            for (int c = 0; c < NC; ++c) {
-                s[n] = mma32(lds_rows<T, DP>(tk, 32 * n, c), q[c], s[n]);
-                hold<T>();
-            }
-        }
-        soft_step<decltype(masked)::value>(rule, me, j0 >= w.wfull_lo && j0 + BN <= w.wfull_hi, j0, half, s, acc, st);
+            for (int n = 0; n < N; ++n) {
+                s[n] = f32x16{};
 #pragma unroll
-        for (int n = 0; n < 2; ++n)
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                const Frag<T> w = acc_frag<T>(s[n], c);
-#pragma unroll
-                for (int d = 0; d < ND; ++d) {
-                    acc[d] = mma32(lds_cols<DP, true>(tv, 32 * n + 16 * c, 32 * d), w, acc[d]);
+                for (int c = 0; c < NC; ++c) {
+                    s[n] = mma32(lds_rows<T, DP>(tk, 32 * (n0 + n), c), q[c], s[n]);
                     hold<T>();
                 }
             }
+            soft_step<decltype(masked)::value>(rule, me, whole, j0 + 32 * n0, half, s, acc, st);
+#pragma unroll
+            for (int n = 0; n < N; ++n)
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    const Frag<T> v = acc_frag<T>(s[n], c);
+#pragma unroll
+                    for (int d = 0; d < ND; ++d) {
+                        acc[d] = mma32(lds_cols<DP, true>(tv, 32 * (n0 + n) + 16 * c, 32 * d), v, acc[d]);
+                        hold<T>();
+                    }
+                }
+        }
     };
     const auto walk = [&](auto masked, int t, const T* tk, const T* tv, T* nk, T* nv) __attribute__((always_inline)) {
         constexpr bool MASKED = decltype(masked)::value;
         const int j0 = w.lo + t * BN;
         if (t + 1 < t1) load(t + 1, nk, nv);
         if (tid < 2) bad[(t - t0 + 2) % 3][tid] = 0;
-        if (!MASKED || (w.wlo < j0 + BN && w.whi > j0)) {
+        if (w.wlo < j0 + BN && w.whi > j0) {
             step(masked, j0, tk, tv);
             if (MASKED) {
                 const unsigned* m = bad[(t - t0) % 3];
@@ -259,10 +269,10 @@ __global__ __launch_bounds__(AT, sizeof(T) == 2 ? (DP == 64 ? 3 : 2) : 1) void a
     walks(std::true_type{}, t0, f0);
     walks(std::false_type{}, f0, f1);
     walks(std::true_type{}, f1, t1);
-    if (!valid) return;
     float l = st.l + __shfl_xor(st.l, 32);
     if (poison) l = __builtin_nanf("");
-    finish<T, DP>(p, kvh, e, row, head, split, half, acc, st.m * (CAP || BIAS ? 1.0f : rule.unit), l);
+    const Entry to = entry_of(a, kvh, sp.e0, sp.end, true);
+    if (to.valid) finish<T, DP>(p, kvh, to.e, to.row, to.head, split, to.half, acc, st.m * (CAP || BIAS ? 1.0f : rule.unit), l);
 }
 
 // Few rows over long keys: a block holds the heads of one row that share a
@@ -467,7 +477,7 @@ extern "C" int kdec_attn_fwd(kdec_ctx* ctx, int dtype, const void* Q, long q_rs,
     ProfScope ps(ctx, "attn", 0.0, 0.0);
     Fwd p{};
     p.a = Args{{Q, q_rs, q_hs}, {K, k_rs, k_hs}, {V, v_rs, v_hs}, {q_off, k_off, k_len, prefix, docs, causal != 0, Tq, Tk},
-               slopes, scale, cap, Hq, Hkv, G, D, Tq * G};
+               slopes, scale, cap, Hq, Hkv, G, D, Tq * G, false};
     std::unique_ptr<Workspace> packed[3], ws;
     if (!plain(p.a.Q, D, size) || !plain(p.a.K, D, size) || !plain(p.a.V, D, size)) {
         if (int rc = pack(ctx, dtype, p.a.Q, Tq, Hq, D, packed[0])) return rc;
@@ -485,7 +495,8 @@ extern "C" int kdec_attn_fwd(kdec_ctx* ctx, int dtype, const void* Q, long q_rs,
     // different documents in one block would walk each other's keys.
     const bool rows = static_cast<long>(Tq) <= 8L * docs && static_cast<long>(Tk) >= 8L * Tq;
     const int chunks = static_cast<int>(cdiv(G, 32));
-    const long tiles = rows ? static_cast<long>(Tq) * chunks : cdiv(p.a.E, BM);
+    p.a.by_doc = by_document(docs, p.a.E, BM);
+    const long tiles = rows ? static_cast<long>(Tq) * chunks : doc_blocks(p.a.by_doc, docs, p.a.E, BM);
     const long blocks = tiles * Hkv;
     KDEC_CHECK(ctx, blocks < INT_MAX, "kdec_attn_fwd: too many rows");
     // Split the keys where the rows alone do not fill the device, to no fewer
