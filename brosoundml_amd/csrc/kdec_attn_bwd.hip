@@ -9,7 +9,8 @@
 // adds to: five products would do for seven, but the sums would be made by
 // atomics in an order that changes from call to call.
 //
-// P and dS are rounded to the tensors' type for the products they enter.
+// P and dS are rounded to the tensors' type for the products they enter (dS of
+// masked tiles to twice its bits in dQ).
 #include "kdec_attn.hpp"
 
 namespace kdec {
@@ -35,7 +36,12 @@ struct Bwd {
 // dQ: the forward's walk over the keys, with dQ^T = K^T dS^T in place of the
 // output. Before it a block forms delta = dO . O of its rows and heads and
 // writes what the walk over the rows takes: delta, lse in log2 units, and the
-// rows' keys. A row without keys gets lse = +inf, so that its probabilities
+// rows' keys. O is rounded, and so is delta; but as sum_j P (dP - delta') is
+// delta - delta', the walk's sums of dS give what is missing, and dK gets
+// delta to float. Of dQ the missing part is about 2^-9 / sqrt(keys), so that
+// rows of few keys show it: they only meet masked tiles, where dS enters the
+// product as two terms, which leaves such rows the one error and the others
+// that of dS's rounding. A row without keys gets lse = +inf, so that its probabilities
 // are zeros; one whose delta is not finite gets NaN, which then marks every
 // gradient that the row reaches.
 template <class T, int DP, bool CAP, bool BIAS>
@@ -79,10 +85,7 @@ __global__ __launch_bounds__(AT, sizeof(T) == 2 ? (DP == 64 ? 3 : 2) : 1) void a
         lse2 = lse == -INF ? INF : lse * LOG2E;
         if (lse == -INF) delta = 0.0f;
         else if (!(__builtin_fabsf(delta) < INF)) lse2 = __builtin_nanf("");
-        if (!half) {
-            b.stat[static_cast<long>(head) * a.m.Tq + row] = make_float2(lse2, delta);
-            if (head == 0) b.rows[row] = me;
-        }
+        if (!half && head == 0) b.rows[row] = me;
     }
     const T* kb = static_cast<const T*>(a.K.p) + kvh * a.K.hs;
     const T* vb = static_cast<const T*>(a.V.p) + kvh * a.V.hs;
@@ -103,7 +106,9 @@ __global__ __launch_bounds__(AT, sizeof(T) == 2 ? (DP == 64 ? 3 : 2) : 1) void a
     f32x16 acc[ND];
 #pragma unroll
     for (int d = 0; d < ND; ++d) acc[d] = f32x16{};
+    float rest = 0.0f;
     const auto step = [&](auto masked, int j0, const T* tk, const T* tv) __attribute__((always_inline)) {
+        constexpr bool MASKED = decltype(masked)::value;
         const unsigned at = static_cast<unsigned>(j0 + 4 * half - me.lo);
         const unsigned len = me.hi > me.lo ? static_cast<unsigned>(me.hi - me.lo) : 0u;
         const float dist = static_cast<float>(me.pos - j0 - 4 * half);
@@ -122,19 +127,27 @@ __global__ __launch_bounds__(AT, sizeof(T) == 2 ? (DP == 64 ? 3 : 2) : 1) void a
             for (int r = 0; r < 16; ++r) {
                 const int k = 32 * n + acc_row(r, 0);
                 float dt;
-                s[r] = grad_p(rule, s[r], dist - static_cast<float>(k), lse2, dt) * ((dp[r] - delta) * dt);
+                const float ds = grad_p(rule, s[r], dist - static_cast<float>(k), lse2, dt) * (dp[r] - delta);
+                s[r] = ds * dt;
+                if (CAP) rest += !MASKED || at + static_cast<unsigned>(k) < len ? ds : 0.0f;
             }
-            if (decltype(masked)::value && !whole) {
+            if (MASKED && !whole) {
 #pragma unroll
                 for (int r = 0; r < 16; ++r) s[r] = at + static_cast<unsigned>(32 * n + acc_row(r, 0)) < len ? s[r] : 0.0f;
                 asm volatile("");  // a branch
             }
+            if (!CAP) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) rest += s[r];
+            }
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
-                const Frag<T> ds = acc_frag<T>(s, c);
+                const Terms<T, MASKED ? 2 : 1> ds(acc_floats(s, c));
 #pragma unroll
                 for (int d = 0; d < ND; ++d) {
-                    acc[d] = mma32(lds_cols<DP, true>(tk, 32 * n + 16 * c, 32 * d), ds, acc[d]);
+                    const Frag<T> kt = lds_cols<DP, true>(tk, 32 * n + 16 * c, 32 * d);
+#pragma unroll
+                    for (int x = ds.n - 1; x >= 0; --x) acc[d] = mma32(kt, ds.t[x], acc[d]);
                     hold<T>();
                 }
             }
@@ -163,6 +176,8 @@ __global__ __launch_bounds__(AT, sizeof(T) == 2 ? (DP == 64 ? 3 : 2) : 1) void a
     walks(std::true_type{}, f1, t1);
     const Entry to = entry_of(a, kvh, sp.e0, sp.end, true);
     if (!to.valid) return;
+    rest += __shfl_xor(rest, 32);
+    if (!to.half) b.stat[static_cast<long>(to.head) * a.m.Tq + to.row] = make_float2(lse2, delta + rest);
     T* o = static_cast<T*>(b.dQ) + to.row * b.dq_rs + to.head * b.dq_hs;
 #pragma unroll
     for (int dt = 0; dt < ND; ++dt)

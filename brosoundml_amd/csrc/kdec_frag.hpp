@@ -53,6 +53,13 @@ __device__ inline Frag<T> acc_frag(const f32x16& s, int c) {
     return f;
 }
 
+__device__ inline f32x8 acc_floats(const f32x16& s, int c) {
+    f32x8 f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = s[8 * c + i];
+    return f;
+}
+
 // 8 elements at p, of which the first n are the tensor's (zeros beyond).
 // vec: p is aligned to 16 bytes and n is a multiple of 16 bytes' elements.
 __device__ inline bf16x8 load8(const bf16* p, int n, bool vec) {

@@ -179,6 +179,39 @@ def test_few_rows_over_long_keys(ctx, ty, case):
 
 
 @pytest.mark.parametrize("ty", TYPES, ids=["f32", "bf16"])
+@pytest.mark.parametrize("case", [
+    dict(lq=[300, 0, 200], lk=[290, 130, 10], slots=[320, 140, 400], pad=150, causal=True, hq=2, hkv=1, D=64),
+    dict(lq=[300, 1, 200], lk=[290, 0, 201], slots=[320, 140, 400], pad=3, hq=2, hkv=2, D=128, cap=4.0),
+    dict(lq=[257, 128, 129], lk=[257, 128, 129], hq=3, hkv=1, D=128, causal=True, prefix=[130, 0, 129], slopes=True),
+    dict(lq=[64, 190] * 33, lk=[64, 190] * 33, hq=1, hkv=1, D=64),                # more documents than a wave has lanes
+], ids=lambda c: "-".join(f"{k}{str(v)[:24]}" for k, v in c.items()).replace(" ", ""))
+def test_blocks_that_end_with_their_document(ctx, ty, case):
+    case = dict(case)
+    lq, lk, hq, hkv, D = (case.pop(n) for n in ("lq", "lk", "hq", "hkv", "D"))
+    compare(ctx, ty, lq, lk, hq, hkv, D, spoil=math.nan if "slots" in case else False, **case)
+
+
+@pytest.mark.parametrize("ty", TYPES, ids=["f32", "bf16"])
+def test_rows_before_the_first_document(ctx, ty):
+    """Rows that offsets leave out at either end get zeros, and the documents between them what they get alone."""
+    from brosoundml_amd import tokens
+    rng = np.random.default_rng(9)
+    q, k, v, do = tensors(rng, ty, 700, 700, 2, 2, 64, "packed")
+    for t in (q, k, v, do):
+        t[:150] = math.nan
+        t[680:] = math.nan
+
+    def run(off, *t):
+        off = torch.tensor(off, dtype=torch.int32).cuda()
+        o, lse = tokens.attention(ctx, *t[:3], off)
+        return (o, *tokens.attention_bwd(ctx, *t[:3], o, lse, t[3], off))
+
+    want = run([0, 330, 530], *(t[150:680].contiguous() for t in (q, k, v, do)))
+    for a, b in zip(run([150, 480, 680], q, k, v, do), want):
+        assert torch.equal(a[150:680], b) and not a[:150].any() and not a[680:].any()
+
+
+@pytest.mark.parametrize("ty", TYPES, ids=["f32", "bf16"])
 @pytest.mark.parametrize("spoil", [math.nan, math.inf])
 def test_rows_of_no_document_do_not_matter(ctx, ty, spoil):
     compare(ctx, ty, [20, 70], [17, 64], 2, 2, 64, slots=[40, 100], pad=11, causal=True, spoil=spoil)
