@@ -15,88 +15,104 @@ import torch
 
 from .native import Context
 
+try:  # the current stream's address without an object around it
+    from torch._C import _cuda_getCurrentRawStream as _raw_stream
+except ImportError:
+    def _raw_stream(device):
+        return torch.cuda.current_stream(device).cuda_stream
+
 _TYPES = {torch.float32: 0, torch.bfloat16: 1}
 
 
-def _need(cond, what):
-    if not cond:
-        raise ValueError("brosoundml: " + what)
+# A single token's kernels take a few microseconds, about what these checks
+# do: each reads what it needs of a tensor once, and forms no message that it
+# does not raise.
+
+def _fail(what):
+    raise ValueError("brosoundml: " + what)
 
 
-def _dtype(x, *others):
-    """The C ABI's type of x, which the others must share, all on one HIP device."""
-    _need(x.dtype in _TYPES, "tensors must be float32 or bfloat16")
-    _need(x.is_cuda, "tensors must be on the HIP device")
+def _dtype(ctx, x, *others):
+    """The C ABI's type of x, which the others must share, all on the context's device."""
+    ty, dev = x.dtype, x.device
+    if ty not in _TYPES:
+        _fail("tensors must be float32 or bfloat16")
+    if dev.type != "cuda" or dev.index != ctx.device:
+        _fail("tensors must be on the context's HIP device")
     for t in others:
-        _need(t.dtype == x.dtype and t.device == x.device, "tensors must share one type and device")
-    return _TYPES[x.dtype]
+        if t.dtype != ty or t.device != dev:
+            _fail("tensors must share one type and device")
+    return _TYPES[ty]
 
 
-def _ints(x, n, what):
+def _ints(ctx, x, n, what):
     """Address of an int32 tensor of n values on the device (None passes)."""
     if x is None:
         return None
-    _need(x.dtype == torch.int32 and x.is_cuda and x.is_contiguous() and x.numel() == n,
-          f"{what} must hold {n} contiguous int32 values on the device")
+    if x.dtype != torch.int32 or x.get_device() != ctx.device or x.numel() != n or not x.is_contiguous():
+        _fail(f"{what} must hold {n} contiguous int32 values on the device")
     return x.data_ptr()
 
 
-def _floats(x, shape, what):
+def _floats(ctx, x, shape, what):
     if x is None:
         return None
-    _need(x.dtype == torch.float32 and x.is_cuda and x.is_contiguous() and tuple(x.shape) == tuple(shape),
-          f"{what} must be a contiguous float32 tensor of shape {tuple(shape)}")
+    if x.dtype != torch.float32 or x.get_device() != ctx.device or x.shape != shape or not x.is_contiguous():
+        _fail(f"{what} must be a contiguous float32 tensor of shape {tuple(shape)}")
     return x.data_ptr()
 
 
 def _heads(x, what):
     """Address, row stride and head stride of a (rows, heads, width) tensor with contiguous width."""
-    _need(x.dim() == 3, f"{what} must be (rows, heads, width)")
-    _need(x.stride(2) == 1 or x.shape[2] <= 1, f"{what}: the width must be contiguous")
-    return x.data_ptr(), x.stride(0), x.stride(1)
+    s = x.stride()
+    if len(s) != 3:
+        _fail(f"{what} must be (rows, heads, width)")
+    if s[2] != 1 and x.shape[2] > 1:
+        _fail(f"{what}: the width must be contiguous")
+    return x.data_ptr(), s[0], s[1]
 
 
 def _rows(x, what):
     """Address and row stride of a (rows, columns) tensor with contiguous columns."""
-    _need(x.dim() == 2, f"{what} must be (rows, columns)")
-    _need(x.stride(1) == 1 or x.shape[1] <= 1, f"{what}: the columns must be contiguous")
-    return x.data_ptr(), x.stride(0)
+    s = x.stride()
+    if len(s) != 2:
+        _fail(f"{what} must be (rows, columns)")
+    if s[1] != 1 and x.shape[1] > 1:
+        _fail(f"{what}: the columns must be contiguous")
+    return x.data_ptr(), s[0]
 
 
 def _whole(x, shape, what):
-    _need(tuple(x.shape) == tuple(shape) and x.is_contiguous(), f"{what} must be contiguous, of shape {tuple(shape)}")
+    if x.shape != shape or not x.is_contiguous():
+        _fail(f"{what} must be contiguous, of shape {tuple(shape)}")
     return x.data_ptr()
 
 
-class _on:
-    """Allocations inside belong to the context's stream."""
-
-    def __init__(self, ctx: Context):
-        self.cm = None if torch.cuda.current_stream(ctx.device) == ctx.stream else torch.cuda.stream(ctx.stream)
-
-    def __enter__(self):
-        if self.cm is not None:
-            self.cm.__enter__()
-
-    def __exit__(self, *a):
-        if self.cm is not None:
-            self.cm.__exit__(*a)
+def _empty(ctx, x, shape, dtype=None):
+    """A new tensor of x's type (or dtype) and device that belongs to the context's stream."""
+    if _raw_stream(ctx.device) == ctx.stream.cuda_stream:
+        return x.new_empty(shape, dtype=dtype)
+    with torch.cuda.stream(ctx.stream):
+        return x.new_empty(shape, dtype=dtype)
 
 
-def _attn_args(q, k, v, q_off, k_off, k_len, causal, prefix, scale, cap, slopes):
-    dt = _dtype(q, k, v)
+def _attn_args(ctx, q, k, v, q_off, k_off, k_len, causal, prefix, scale, cap, slopes):
+    dt = _dtype(ctx, q, k, v)
     Q, K, V = _heads(q, "q"), _heads(k, "k"), _heads(v, "v")
     tq, hq, d = q.shape
     tk, hkv, _ = k.shape
-    _need(v.shape == k.shape and k.shape[2] == d, "k and v must share their shape, and q their width")
+    if not (v.shape == k.shape and k.shape[2] == d):
+        _fail("k and v must share their shape, and q their width")
     docs = q_off.numel() - 1
-    _need(docs >= 0, "q_off must hold one offset more than there are documents")
+    if not (docs >= 0):
+        _fail("q_off must hold one offset more than there are documents")
     if k_off is None:
-        _need(tq == tk, "without k_off the keys are the query rows' own")
+        if not (tq == tk):
+            _fail("without k_off the keys are the query rows' own")
         k_off = q_off
     # where / length / mask arguments, in the C ABI's order
-    mask = (_ints(q_off, docs + 1, "q_off"), _ints(k_off, docs + 1, "k_off"), _ints(k_len, docs, "k_len"),
-            _ints(prefix, docs, "prefix"), docs, int(causal), _floats(slopes, (hq,), "slopes"),
+    mask = (_ints(ctx, q_off, docs + 1, "q_off"), _ints(ctx, k_off, docs + 1, "k_off"), _ints(ctx, k_len, docs, "k_len"),
+            _ints(ctx, prefix, docs, "prefix"), docs, int(causal), _floats(ctx, slopes, (hq,), "slopes"),
             float(d ** -0.5 if scale is None else scale), float(cap), tq, tk, hq, hkv, d)
     return dt, Q, K, V, mask
 
@@ -112,12 +128,12 @@ def attention(ctx: Context, q, k, v, q_off, k_off=None, k_len=None, *, causal=Fa
     cap), ``slopes`` (Hq floats) lowers them by slope * distance; ``scale``
     is 1 / sqrt(D) by default. Returns (o, lse): o as q, lse (Hq, Tq) float.
     Single tokens over long caches take a kernel of their own in this call."""
-    dt, Q, K, V, mask = _attn_args(q, k, v, q_off, k_off, k_len, causal, prefix, scale, cap, slopes)
+    dt, Q, K, V, mask = _attn_args(ctx, q, k, v, q_off, k_off, k_len, causal, prefix, scale, cap, slopes)
     tq, hq, _ = q.shape
-    with _on(ctx):
-        o = torch.empty(q.shape, dtype=q.dtype, device=q.device) if out is None else out
-        lse = torch.empty((hq, tq), dtype=torch.float32, device=q.device)
-    _need(o.shape == q.shape and o.dtype == q.dtype, "out must be as q")
+    o = _empty(ctx, q, q.shape) if out is None else out
+    lse = _empty(ctx, q, (hq, tq), torch.float32)
+    if out is not None and (o.shape != q.shape or o.dtype != q.dtype or o.device != q.device):
+        _fail("out must be as q")
     ctx.call("kdec_attn_fwd", dt, *Q, *K, *V, *mask, *_heads(o, "out"), lse.data_ptr())
     return o, lse
 
@@ -127,28 +143,30 @@ def attention_bwd(ctx: Context, q, k, v, o, lse, do, q_off, k_off=None, k_len=No
     """The gradients (dq, dk, dv) of ``attention`` from ``do``, with its o and
     lse and the same mask arguments (kdec_attn_bwd). dq, dk and dv may be
     given, for example as the parts of a fused projection's gradient."""
-    dt, Q, K, V, mask = _attn_args(q, k, v, q_off, k_off, k_len, causal, prefix, scale, cap, slopes)
-    _dtype(q, o, do)
-    _need(o.shape == q.shape and do.shape == q.shape, "o and do must be as q")
-    with _on(ctx):
-        dq = torch.empty(q.shape, dtype=q.dtype, device=q.device) if dq is None else dq
-        dk = torch.empty(k.shape, dtype=k.dtype, device=k.device) if dk is None else dk
-        dv = torch.empty(v.shape, dtype=v.dtype, device=v.device) if dv is None else dv
-    _dtype(q, dq, dk, dv)
-    _need(dq.shape == q.shape and dk.shape == k.shape and dv.shape == v.shape, "dq, dk and dv must be as q, k and v")
-    ctx.call("kdec_attn_bwd", dt, *Q, *K, *V, *_heads(o, "o"), _floats(lse, (q.shape[1], q.shape[0]), "lse"),
+    dt, Q, K, V, mask = _attn_args(ctx, q, k, v, q_off, k_off, k_len, causal, prefix, scale, cap, slopes)
+    _dtype(ctx, q, o, do)
+    if not (o.shape == q.shape and do.shape == q.shape):
+        _fail("o and do must be as q")
+    dq = _empty(ctx, q, q.shape) if dq is None else dq
+    dk = _empty(ctx, k, k.shape) if dk is None else dk
+    dv = _empty(ctx, v, v.shape) if dv is None else dv
+    _dtype(ctx, q, dq, dk, dv)
+    if not (dq.shape == q.shape and dk.shape == k.shape and dv.shape == v.shape):
+        _fail("dq, dk and dv must be as q, k and v")
+    ctx.call("kdec_attn_bwd", dt, *Q, *K, *V, *_heads(o, "o"), _floats(ctx, lse, (q.shape[1], q.shape[0]), "lse"),
              *_heads(do, "do"), *mask, *_heads(dq, "dq"), *_heads(dk, "dk"), *_heads(dv, "dv"))
     return dq, dk, dv
 
 
-def _adapter_args(x, w, a, b, scale, idx, unit_off):
+def _adapter_args(ctx, x, w, a, b, scale, idx, unit_off):
     t, cin = x.shape
     out = w.shape[0]
     n, units = a.shape[0], unit_off.numel() - 1
-    _need(b.dim() == 3 and units >= 1, "b must be (adapters, out, rank), unit_off units + 1 offsets")
+    if not (b.dim() == 3 and units >= 1):
+        _fail("b must be (adapters, out, rank), unit_off units + 1 offsets")
     rank = b.shape[2]
     return (_whole(w, (out, cin), "w"), _whole(a, (n, units * rank, cin), "a"), _whole(b, (n, out, rank), "b"),
-            _floats(scale, (n,), "scale"), _ints(idx, t, "idx"), _ints(unit_off, units + 1, "unit_off"), t, cin, out,
+            _floats(ctx, scale, (n,), "scale"), _ints(ctx, idx, t, "idx"), _ints(ctx, unit_off, units + 1, "unit_off"), t, cin, out,
             n, units, rank)
 
 
@@ -160,17 +178,17 @@ def adapter_proj(ctx: Context, x, w, a, b, scale, idx, unit_off, *, bias=None, d
     into units with adapters of their own. ``drop`` = (p, seed, offset) drops
     inputs of the adapters. Returns y (T, out), and with ``keep_h`` the pair
     (y, h) whose h the backward takes."""
-    dt = _dtype(x, w, a, b)
+    dt = _dtype(ctx, x, w, a, b)
     X = _rows(x, "x")
-    W, A, B, S, I, U, t, cin, cout, n, units, rank = _adapter_args(x, w, a, b, scale, idx, unit_off)
+    W, A, B, S, I, U, t, cin, cout, n, units, rank = _adapter_args(ctx, x, w, a, b, scale, idx, unit_off)
     p, seed, offset = drop if drop is not None else (0.0, 0, 0)
-    with _on(ctx):
-        y = torch.empty((t, cout), dtype=x.dtype, device=x.device) if out is None else out
-        h = torch.empty((t, units * rank), dtype=torch.float32, device=x.device) if keep_h else None
-    _need(y.shape == (t, cout), "out must be (T, out)")
-    _dtype(x, y)
+    y = _empty(ctx, x, (t, cout)) if out is None else out
+    h = _empty(ctx, x, (t, units * rank), torch.float32) if keep_h else None
+    if not (y.shape == (t, cout)):
+        _fail("out must be (T, out)")
+    _dtype(ctx, x, y)
     if bias is not None:
-        _dtype(x, bias)
+        _dtype(ctx, x, bias)
         _whole(bias, (cout,), "bias")
     ctx.call("kdec_adapter_fwd", dt, *X, W, None if bias is None else bias.data_ptr(), A, B, S, I, U, t, cin, cout,
              n, units, rank, p, seed, offset, None if h is None else h.data_ptr(), *_rows(y, "out"))
@@ -183,19 +201,20 @@ def adapter_proj_bwd(ctx: Context, x, w, a, b, scale, idx, unit_off, h, dy, *, d
     w and bias frozen (kdec_adapter_bwd). dx is of x's type (None without
     ``need_dx``); da and db are float and, where given, become beta times
     what they held plus the gradient."""
-    dt = _dtype(x, w, a, b, dy)
+    dt = _dtype(ctx, x, w, a, b, dy)
     X = _rows(x, "x")
-    W, A, B, S, I, U, t, cin, cout, n, units, rank = _adapter_args(x, w, a, b, scale, idx, unit_off)
+    W, A, B, S, I, U, t, cin, cout, n, units, rank = _adapter_args(ctx, x, w, a, b, scale, idx, unit_off)
     p, seed, offset = drop if drop is not None else (0.0, 0, 0)
-    _need(dy.shape == (t, cout), "dy must be (T, out)")
-    _need(beta == 0.0 or (da is not None and db is not None), "beta without da and db to add to")
-    with _on(ctx):
-        dx = torch.empty((t, cin), dtype=x.dtype, device=x.device) if need_dx else None
-        da = torch.empty(a.shape, dtype=torch.float32, device=x.device) if da is None else da
-        db = torch.empty(b.shape, dtype=torch.float32, device=x.device) if db is None else db
+    if not (dy.shape == (t, cout)):
+        _fail("dy must be (T, out)")
+    if not (beta == 0.0 or (da is not None and db is not None)):
+        _fail("beta without da and db to add to")
+    dx = _empty(ctx, x, (t, cin)) if need_dx else None
+    da = _empty(ctx, x, a.shape, torch.float32) if da is None else da
+    db = _empty(ctx, x, b.shape, torch.float32) if db is None else db
     ctx.call("kdec_adapter_bwd", dt, *X, W, A, B, S, I, U, t, cin, cout, n, units, rank, p, seed, offset,
-             _floats(h, (t, units * rank), "h"), *_rows(dy, "dy"), None if dx is None else dx.data_ptr(), cin,
-             _floats(da, a.shape, "da"), _floats(db, b.shape, "db"), beta)
+             _floats(ctx, h, (t, units * rank), "h"), *_rows(dy, "dy"), None if dx is None else dx.data_ptr(), cin,
+             _floats(ctx, da, a.shape, "da"), _floats(ctx, db, b.shape, "db"), beta)
     return dx, da, db
 
 
@@ -204,16 +223,17 @@ def dropout(ctx: Context, x, p, seed, offset=0, *, residual=None, out=None):
     scaled by 1 / (1 - p) (kdec_dropout; p in steps of 1 / 65536). The mask is
     the seed's and offset's alone: the backward is this call on the gradient
     with the same seed and offset and no residual. ``out`` may be x."""
-    dt = _dtype(x)
+    dt = _dtype(ctx, x)
     X = _rows(x, "x")
-    with _on(ctx):
-        y = torch.empty(x.shape, dtype=x.dtype, device=x.device) if out is None else out
-    _dtype(x, y)
-    _need(y.shape == x.shape, "out must be as x")
+    y = _empty(ctx, x, x.shape) if out is None else out
+    _dtype(ctx, x, y)
+    if not (y.shape == x.shape):
+        _fail("out must be as x")
     R = (None, 0)
     if residual is not None:
-        _dtype(x, residual)
-        _need(residual.shape == x.shape, "residual must be as x")
+        _dtype(ctx, x, residual)
+        if not (residual.shape == x.shape):
+            _fail("residual must be as x")
         R = _rows(residual, "residual")
     ctx.call("kdec_dropout", dt, *X, *R, *_rows(y, "out"), x.shape[0], x.shape[1], p, seed, offset)
     return y
