@@ -157,7 +157,7 @@ __device__ inline void join8(Join8* buf, const f32x16& acc, F f) {
 template <class T, int MT>
 __global__ __launch_bounds__(LT) void adapter_h_k(Adapter p) {
     __shared__ Join8 buf[8];
-    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, half = lane >> 5, col = lane & 31;
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, half = lane >> 5, col = lane & 31;
     const int m0 = blockIdx.y * 32 * MT;
     int start = 0, count = 1, a, row;
     if (p.pieces) {
@@ -194,6 +194,7 @@ __global__ __launch_bounds__(LT) void adapter_h_k(Adapter p) {
             }
 #pragma unroll
             for (int s = 0; s < 4; ++s) {
+                if (k + 128 * s >= p.in) break;
                 if (p.dropping) z[s] = dropped<T>(p.drop, row, k + 128 * s + 8 * half, z[s]);
 #pragma unroll
                 for (int i = 0; i < MT; ++i) acc[i] = mma32(g[s][i], z[s], acc[i]);
@@ -208,14 +209,15 @@ __global__ __launch_bounds__(LT) void adapter_h_k(Adapter p) {
 }
 
 // dH: a piece's rows by 32 low-rank columns of one unit per block. The
-// depth is the unit's output rows, RT at a time per wave; B's rows go through
+// depth is the unit's output rows, RT at a time per wave with four steps'
+// loads in flight; B's rows go through
 // the wave's shared memory, from which the product reads their columns.
 template <class T>
 __global__ __launch_bounds__(LT) void adapter_dh_k(Adapter p) {
-    constexpr int RT = sizeof(T) == 2 ? 64 : 32, DPB = 64, NB = RT * 4 / 64;
-    __shared__ __align__(16) char smem[8 * RT * DPB * sizeof(T)];
-    static_assert(sizeof(smem) >= 8 * sizeof(Join8), "the waves are joined in the tiles' place");
-    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, half = lane >> 5, col = lane & 31;
+    constexpr int RT = sizeof(T) == 2 ? 32 : 16, DPB = 64, NB = RT * 4 / 64, AHEAD = 4;
+    __shared__ __align__(16) char smem[8 * sizeof(Join8)];
+    static_assert(sizeof(smem) >= 8 * RT * DPB * sizeof(T), "the waves are joined in the tiles' place");
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, half = lane >> 5, col = lane & 31;
     const Piece pc = p.pieces[blockIdx.x];
     if (!pc.count) return;
     const int jt = (p.rank + 31) / 32, unit = blockIdx.y / jt, m0 = 32 * (blockIdx.y % jt), a = pc.adapter;
@@ -228,8 +230,8 @@ __global__ __launch_bounds__(LT) void adapter_dh_k(Adapter p) {
         f = p.scale[a];
         const T* y = static_cast<const T*>(p.dY) + row * p.dy_rs;
         const T* b = static_cast<const T*>(p.B) + static_cast<long>(a) * p.out * p.rank + m0;
-        for (int r0 = (u0 & ~7) + RT * wave; r0 < u1; r0 += 8 * RT) {
-            Frag<T> z[RT / 16], w[NB];
+        Frag<T> z[AHEAD][RT / 16], w[AHEAD][NB];
+        const auto load = [&](int r0, Frag<T> (&z)[RT / 16], Frag<T> (&w)[NB]) __attribute__((always_inline)) {
 #pragma unroll
             for (int c = 0; c < RT / 16; ++c) {
                 const int d = r0 + 16 * c + 8 * half;
@@ -241,6 +243,8 @@ __global__ __launch_bounds__(LT) void adapter_dh_k(Adapter p) {
                 const bool in = r >= u0 && r < u1 && m0 + j < p.rank;
                 w[i] = load8(b + (in ? static_cast<long>(r) * p.rank + j : 0), in ? min(8, p.rank - m0 - j) : 0, p.vec_b);
             }
+        };
+        const auto step = [&](int r0, Frag<T> (&z)[RT / 16], const Frag<T> (&w)[NB]) __attribute__((always_inline)) {
 #pragma unroll
             for (int i = 0; i < NB; ++i) {
                 const int e = lane + 64 * i;
@@ -257,7 +261,19 @@ __global__ __launch_bounds__(LT) void adapter_dh_k(Adapter p) {
             }
 #pragma unroll
             for (int c = 0; c < RT / 16; ++c) acc = mma32(lds_cols<DPB, false>(tile, 16 * c, 0), z[c], acc);
-        }
+        };
+        const int first = (u0 & ~7) + RT * wave;
+#pragma unroll
+        for (int s = 0; s < AHEAD; ++s)
+            if (first + 8 * RT * s < u1) load(first + 8 * RT * s, z[s], w[s]);
+        for (int r0 = first; r0 < u1; r0 += 8 * RT * AHEAD)
+#pragma unroll
+            for (int s = 0; s < AHEAD; ++s) {
+                const int r = r0 + 8 * RT * s;
+                if (r >= u1) break;
+                step(r, z[s], w[s]);
+                if (r + 8 * RT * AHEAD < u1) load(r + 8 * RT * AHEAD, z[s], w[s]);
+            }
     }
     __syncthreads();
     join8(reinterpret_cast<Join8*>(smem), acc, [&](int c, int t, float v) {
@@ -602,6 +618,81 @@ __global__ __launch_bounds__(1024) void adapter_join_k(const float* part, int sp
     Y[row * y_rs + (e - row * M)] = static_cast<T>(s);
 }
 
+// The same for few rows and 32 features: two of the taker's pairs of adapter
+// and unit at a time, the loads of both in flight.
+template <class T, int NB>
+__device__ inline void low_rank_few(const Adapter& p, int M, int m, int u0, int u1, int id, int turn, int turns, f32x16 (&acc)[NB]) {
+    const int lane = threadIdx.x & 63, half = lane >> 5, col = lane & 31;
+    unsigned long long left = __builtin_amdgcn_ballot_w64(id < p.n);
+    int rows[NB], ids[NB];
+#pragma unroll
+    for (int j = 0; j < NB; ++j) {
+        rows[j] = min(32 * j + col, p.T - 1);
+        ids[j] = __shfl(id, 32 * j + col);
+    }
+    int a = -1, u = u0 + turn;
+    unsigned long long mine = 0;
+    const auto next = [&]() __attribute__((always_inline)) {  // moves to the taker's next pair
+        if (a >= 0) u += turns;
+        while (a < 0 || u >= u1) {
+            if (a >= 0) u -= u1 - u0;
+            if (!left) return false;
+            a = __builtin_amdgcn_readlane(id, __builtin_ctzll(left));
+            mine = __builtin_amdgcn_ballot_w64(id == a);
+            left &= ~mine;
+        }
+        return true;
+    };
+    for (bool more = next(); more;) {
+        int as[2], us[2];
+        unsigned long long mines[2];
+        as[0] = as[1] = a, us[0] = us[1] = u, mines[0] = mine, mines[1] = 0;
+        more = next();
+        if (more) {
+            as[1] = a, us[1] = u, mines[1] = mine;
+            more = next();
+        }
+        f32x16 tmp[2][NB];
+        bool in[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            in[i] = m >= p.unit_off[us[i]] && m < p.unit_off[us[i] + 1] && m < M;
+#pragma unroll
+            for (int j = 0; j < NB; ++j) tmp[i][j] = f32x16{};
+        }
+        for (int k = 0; k < p.rank; k += 16) {
+            const int d = k + 8 * half, n = min(8, p.rank - d), dd = n > 0 ? d : 0;
+            Frag<T> w[2];
+            f32x8 h[2][NB];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                w[i] = load8(static_cast<const T*>(p.B) + (static_cast<long>(as[i]) * p.out + (in[i] ? m : 0)) * p.rank + dd, in[i] ? n : 0,
+                             p.vec_b);
+#pragma unroll
+                for (int j = 0; j < NB; ++j)
+                    h[i][j] = load8(p.H + static_cast<long>(rows[j]) * p.R + us[i] * p.rank + dd, ids[j] == as[i] ? n : 0, p.vec_h);
+            }
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int j = 0; j < NB; ++j) {
+                    if (!(mines[i] >> (32 * j) & 0xFFFFFFFFull)) continue;
+                    const Terms<T, 2> v(h[i][j]);
+#pragma unroll
+                    for (int x = 0; x < v.n; ++x) tmp[i][j] = mma32(w[i], v.t[x], tmp[i][j]);
+                }
+        }
+        // only an adapter's rows take its product, whatever another's would be
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int j = 0; j < NB; ++j)
+                if (mines[i] >> (32 * j + col) & 1)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) acc[j][r] += tmp[i][j][r];
+    }
+}
+
 // Up to 64 rows, unsorted: a block forms 32 features of all of them, its eight
 // waves taking the depth (and then the adapters) in turn. W is read once, four
 // steps' loads in flight.
@@ -610,13 +701,14 @@ __global__ __launch_bounds__(LT) void adapter_few_k(Adapter p, Product g) {
     __shared__ Join8 buf[8];
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, half = lane >> 5, col = lane & 31;
     const int m0 = blockIdx.x * 32, m = m0 + col;
+    const int id = lane < p.T ? adapter_of(p, lane) : p.n;
     const T* w = static_cast<const T*>(p.W) + static_cast<long>(min(m, g.M - 1)) * g.K;
     const T* x[NB];
 #pragma unroll
     for (int j = 0; j < NB; ++j) x[j] = static_cast<const T*>(g.Z) + min(32 * j + col, p.T - 1) * g.z_rs;
-    f32x16 acc[1][NB];
+    f32x16 acc[NB];
 #pragma unroll
-    for (int j = 0; j < NB; ++j) acc[0][j] = f32x16{};
+    for (int j = 0; j < NB; ++j) acc[j] = f32x16{};
     for (int k = 16 * wave; k < g.K; k += 512) {
         Frag<T> f[4], z[4][NB];
 #pragma unroll
@@ -627,16 +719,17 @@ __global__ __launch_bounds__(LT) void adapter_few_k(Adapter p, Product g) {
             for (int j = 0; j < NB; ++j) z[s][j] = load8(x[j] + dd, 32 * j + col < p.T ? n : 0, g.vec_z);
         }
 #pragma unroll
-        for (int s = 0; s < 4; ++s)
+        for (int s = 0; s < 4; ++s) {
+            if (k + 128 * s >= g.K) break;
 #pragma unroll
-            for (int j = 0; j < NB; ++j) acc[0][j] = mma32(f[s], z[s][j], acc[0][j]);
+            for (int j = 0; j < NB; ++j) acc[j] = mma32(f[s], z[s][j], acc[j]);
+        }
     }
-    const int id = lane < p.T ? adapter_of(p, lane) : p.n;
     const int u0 = unit_at(p.unit_off, p.units, m0), u1 = unit_at(p.unit_off, p.units, min(m0 + 31, g.M - 1)) + 1;
-    low_rank<T, false, 0, 1>(p, g.M, m0, u0, u1, min(lane, p.T - 1), id, wave, 8, acc);
+    low_rank_few<T, NB>(p, g.M, m, u0, u1, id, wave, 8, acc);
 #pragma unroll
     for (int j = 0; j < NB; ++j)
-        join8(buf, acc[0][j], [&](int r, int c, float v) {
+        join8(buf, acc[j], [&](int r, int c, float v) {
             const int t = 32 * j + c;
             if (t >= p.T || m0 + r >= g.M) return;
             if (p.bias) v += static_cast<float>(static_cast<const T*>(p.bias)[m0 + r]);
@@ -741,18 +834,13 @@ __global__ __launch_bounds__(NT) void adapter_outer_few_k(Adapter p, const float
     const int width = DB ? p.rank : C, q = (width + 3) / 4;  // a row of the gradient, in fours
     const long n = static_cast<long>(DB ? C : p.R) * q;
     const long e = static_cast<long>(blockIdx.x) * NT + threadIdx.x;
-    if (e >= n) return;
-    const int r = static_cast<int>(e / q), x = 4 * static_cast<int>(e - static_cast<long>(r) * q);
+    const int r = static_cast<int>(min(e, n - 1) / q), x = 4 * static_cast<int>(e - static_cast<long>(r) * q);
     int u = 0;
-    if (DB) {
-        int lo = 1, hi = p.units;  // offsets 1 .. units - 1 that are not past r
-        while (lo < hi) {
-            const int mid = (lo + hi) >> 1;
-            if (p.unit_off[mid] <= r) lo = mid + 1;
-            else hi = mid;
-        }
-        u = lo - 1;
+    if (DB) {  // the wave's first row's unit, and on from there
+        u = unit_at(p.unit_off, p.units, __builtin_amdgcn_readfirstlane(r));
+        while (u + 1 < p.units && p.unit_off[u + 1] <= r) ++u;
     }
+    if (e >= n) return;
     float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
     for (int t = 0; t < pc.count; ++t) {
         const int row = p.perm[pc.start + t];
@@ -1006,10 +1094,10 @@ int kdec_adapter_bwd(kdec_ctx* ctx, int dtype, const void* X, long x_rs, const v
     p.vec_dy = out % el == 0 && aligned16(dY, dy_rs * es);
     ProfScope ps(ctx, "adapter", 2.0 * T * in * out, 0.0);
     // Few tiles over a long depth: the depth split over blocks, to no fewer
-    // than 128 deep each.
+    // than 64 deep each (from 256 on: two blocks' sums cost more to join).
     const long tiles = cdiv(in, 128) * cdiv(T, 128);
     long splits = dX && T > 0 ? cdiv(2L * ctx->num_cus, tiles) : 1;
-    if (splits > out / 128) splits = out / 128;
+    if (splits > out / 64) splits = out < 256 ? 1 : out / 64;
     if (splits < 1) splits = 1;
     const Sorted sorted(T, adapters);
     const size_t h_b = up(static_cast<size_t>(T) * R * 4), s_b = splits > 1 ? up(static_cast<size_t>(splits) * T * in * 4) : 0;
