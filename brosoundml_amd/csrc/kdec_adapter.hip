@@ -298,14 +298,32 @@ struct Product {
 
 template <class T> constexpr int depth_of() { return sizeof(T) == 2 ? 64 : 32; }  // of a tile: 128 bytes
 
-// The low-rank products of 32 MB of a wave's features (from wm; blocks I0 ..
-// of acc) and its 32 NB rows (a lane each: its row and adapter), into acc:
-// forward B H, backward A^T dH.
+// Whether a fragment of this lane's holds a value that is not finite: its
+// largest magnitude as an integer.
+__device__ inline bool not_finite(bf16x8 f) {
+    typedef unsigned short u16x8 __attribute__((ext_vector_type(8)));
+    const u16x8 b = __builtin_bit_cast(u16x8, f) & static_cast<unsigned short>(0x7FFF);
+    const auto m4 = __builtin_elementwise_max(b.lo, b.hi);
+    const auto m2 = __builtin_elementwise_max(m4.lo, m4.hi);
+    return m2[0] >= 0x7F80 || m2[1] >= 0x7F80;
+}
+__device__ inline bool not_finite(f32x8 f) {
+    unsigned m = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(f[i]) & 0x7FFFFFFFu);
+    return m >= 0x7F800000u;
+}
+
+// The low-rank products of 32 MB of a wave's features (from wm) and its 32 NB
+// rows (a lane each: its row and adapter), into acc: forward B H, backward
+// A^T dH. Rows of other adapters take part with zeros. An adapter's values
+// that are not finite would make NaN of those, so they are left out of this
+// product and make one of their own, which only the adapter's rows take.
 // Adapters and units are taken in turn by `turns` takers of which this is
 // number `turn`.
-template <class T, bool BWD, int I0, int MB, int NA, int NB>
+template <class T, bool BWD, int MB, int NB>
 __device__ inline void low_rank(const Adapter& p, int M, int wm, int u0, int u1, int row, int id, int turn, int turns,
-                                f32x16 (&acc)[NA][NB]) {
+                                f32x16 (&acc)[MB][NB]) {
     const int lane = threadIdx.x & 63, half = lane >> 5, col = lane & 31;
     const float* H = BWD ? p.dH : p.H;
     unsigned long long left = __builtin_amdgcn_ballot_w64(id < p.n);
@@ -317,55 +335,72 @@ __device__ inline void low_rank(const Adapter& p, int M, int wm, int u0, int u1,
     }
     int u = u0 + turn;  // the next unit that is this taker's
     while (left) {
-        const int a = __shfl(id, __builtin_ctzll(left));
+        const int a = __builtin_amdgcn_readlane(id, __builtin_ctzll(left));
         const unsigned long long mine = __builtin_amdgcn_ballot_w64(id == a);
         left &= ~mine;
         for (; u < u1; u += turns) {
             const int lo = BWD ? 0 : p.unit_off[u], hi = BWD ? M : p.unit_off[u + 1];
-            f32x16 tmp[MB][NB];
-#pragma unroll
-            for (int i = 0; i < MB; ++i)
-#pragma unroll
-                for (int j = 0; j < NB; ++j) tmp[i][j] = f32x16{};
             for (int k = 0; k < p.rank; k += 16) {
                 const int d = k + 8 * half, n = min(8, p.rank - d), dd = n > 0 ? d : 0;
-                Frag<T> w[MB];
+                Frag<T> w[2];
                 f32x8 h[NB];
 #pragma unroll
                 for (int j = 0; j < NB; ++j)
                     h[j] = load8(H + static_cast<long>(rows[j]) * p.R + u * p.rank + dd, ids[j] == a ? n : 0, p.vec_h);
 #pragma unroll
-                for (int i = 0; i < MB; ++i) {
-                    const int m = wm + 32 * i + col;
-                    const bool in = m >= lo && m < hi && m < M;
-                    if (BWD) {  // A's columns
-                        const T* q = static_cast<const T*>(p.A) + (static_cast<long>(a) * p.R + u * p.rank) * p.in + (in ? m : 0);
+                for (int i0 = 0; i0 < MB; i0 += 2) {  // 64 features at a time, which the registers leave room for
+                    bool bad = false;
 #pragma unroll
-                        for (int x = 0; x < 8; ++x)
-                            w[i][x] = in && x < n ? q[static_cast<long>(d + x) * p.in] : static_cast<T>(0.0f);
-                    } else {
-                        const T* q = static_cast<const T*>(p.B) + (static_cast<long>(a) * p.out + (in ? m : 0)) * p.rank;
-                        w[i] = load8(q + dd, in ? n : 0, p.vec_b);
+                    for (int i = 0; i < 2; ++i) {
+                        const int m = wm + 32 * (i0 + i) + col;
+                        const bool in = m >= lo && m < hi && m < M;
+                        if (BWD) {  // A's columns
+                            const T* q = static_cast<const T*>(p.A) + (static_cast<long>(a) * p.R + u * p.rank) * p.in + (in ? m : 0);
+#pragma unroll
+                            for (int x = 0; x < 8; ++x)
+                                w[i][x] = in && x < n ? q[static_cast<long>(d + x) * p.in] : static_cast<T>(0.0f);
+                        } else {
+                            const T* q = static_cast<const T*>(p.B) + (static_cast<long>(a) * p.out + (in ? m : 0)) * p.rank;
+                            w[i] = load8(q + dd, in ? n : 0, p.vec_b);
+                        }
                     }
-                }
 #pragma unroll
-                for (int j = 0; j < NB; ++j) {
-                    if (!(mine >> (32 * j) & 0xFFFFFFFFull)) continue;
-                    const Terms<T, 2> v(h[j]);
+                    for (int i = 0; i < 2; ++i) bad |= not_finite(w[i]);
+                    if (__builtin_amdgcn_ballot_w64(bad)) {
 #pragma unroll
-                    for (int x = 0; x < v.n; ++x)
+                        for (int i = 0; i < 2; ++i) {
+                            Frag<T> v = w[i];
 #pragma unroll
-                        for (int i = 0; i < MB; ++i) tmp[i][j] = mma32(w[i], v.t[x], tmp[i][j]);
+                            for (int x = 0; x < 8; ++x) {
+                                const bool fine = __builtin_fabsf(static_cast<float>(v[x])) < __builtin_inff();
+                                w[i][x] = fine ? v[x] : static_cast<T>(0.0f);
+                                v[x] = fine ? static_cast<T>(0.0f) : v[x];
+                            }
+#pragma unroll
+                            for (int j = 0; j < NB; ++j) {
+                                const Terms<T, 2> t(h[j]);
+                                f32x16 tmp = f32x16{};
+#pragma unroll
+                                for (int x = 0; x < t.n; ++x) tmp = mma32(v, t.t[x], tmp);
+                                if (ids[j] == a)
+#pragma unroll
+                                    for (int r = 0; r < 16; ++r) acc[i0 + i][j][r] += tmp[r];
+                            }
+                        }
+                        asm volatile("");  // a branch
+                    }
+#pragma unroll
+                    for (int j = 0; j < NB; ++j) {
+                        if (!(mine >> (32 * j) & 0xFFFFFFFFull)) continue;
+                        const Terms<T, 2> v(h[j]);
+#pragma unroll
+                        for (int x = 0; x < v.n; ++x)
+#pragma unroll
+                            for (int i = 0; i < 2; ++i) acc[i0 + i][j] = mma32(w[i], v.t[x], acc[i0 + i][j]);
+                    }
+                    if (MB > 2) __builtin_amdgcn_sched_barrier(0);
                 }
             }
-            // only this adapter's rows take the product, whatever another's would be
-#pragma unroll
-            for (int j = 0; j < NB; ++j)
-                if (ids[j] == a)
-#pragma unroll
-                    for (int i = 0; i < MB; ++i)
-#pragma unroll
-                        for (int r = 0; r < 16; ++r) acc[I0 + i][j][r] += tmp[i][j][r];
         }
         u -= u1 - u0;
     }
@@ -471,19 +506,10 @@ __global__ __launch_bounds__(BIG ? 512 : 256, DIRECT ? 2 : 1) void adapter_gemm_
 #pragma unroll
         for (int j = 0; j < 2; ++j) acc[i][j] = f32x16{};
     if (c0 < c1) load(c0, sw0, sz0);
-    constexpr int LB = BIG ? 1 : 2;  // 32 LB features at a time, which the registers leave room for
-    const auto low = [&](auto first) __attribute__((always_inline)) {
-        constexpr int I0 = LB * decltype(first)::value;
-        const int m = wm + 32 * I0;
-        const int u0 = BWD ? 0 : unit_at(p.unit_off, p.units, m);
-        const int u1 = BWD ? p.units : unit_at(p.unit_off, p.units, min(m + 32 * LB - 1, g.M - 1)) + 1;
-        low_rank<T, BWD, I0, LB>(p, g.M, m, u0, u1, srow[wn + lane], sid[wn + lane], split, g.splits, acc);
-    };
-    low(std::integral_constant<int, 0>{});
-    if constexpr (MB > LB) low(std::integral_constant<int, 1>{});
-    if constexpr (MB > 2 * LB) {
-        low(std::integral_constant<int, 2>{});
-        low(std::integral_constant<int, 3>{});
+    {
+        const int u0 = BWD ? 0 : unit_at(p.unit_off, p.units, wm);
+        const int u1 = BWD ? p.units : unit_at(p.unit_off, p.units, min(wm + 32 * MB - 1, g.M - 1)) + 1;
+        low_rank<T, BWD>(p, g.M, wm, u0, u1, srow[wn + lane], sid[wn + lane], split, g.splits, acc);
     }
     if (DIRECT && BIG) {  // formed again rather than held meanwhile
         asm volatile("" ::: "memory");

@@ -269,3 +269,30 @@ def test_many_rows_equal_few_rows(ctx, drop):
             y2, h2 = tokens.adapter_proj(ctx, *args, drop=drop, keep_h=True)  # the mask goes by row: the first rows' is theirs
             dx2, _, _ = tokens.adapter_proj_bwd(ctx, *args, h2, d["dy"][part], drop=drop)
             assert torch.equal(y[part], y2) and (out >= 256 or torch.equal(dx[part], dx2))
+
+
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("T", [700, 14999])
+def test_adapter_not_finite_among_many_rows(ctx, T, bad):
+    """Values of one adapter that are not finite reach its rows' outputs that they enter, and no bit of any other's."""
+    from brosoundml_amd import tokens
+    cin, sizes, n, rank = 928, [500, 24, 404], 5, 8
+    d = make(torch.bfloat16, T, cin, sizes, n, rank, bias=True)
+    I = torch.from_numpy(np.random.default_rng(2).integers(-1, n, T).astype(np.int32)).cuda()
+    edges = torch.tensor(d["edges"], dtype=torch.int32).cuda()
+
+    def run(a, b):
+        args = (ctx, d["x"], d["w"], a, b, d["scale"], I, edges)
+        y, h = tokens.adapter_proj(*args, bias=d["bias"], keep_h=True)
+        return y, h, tokens.adapter_proj_bwd(*args, h, d["dy"])[0]
+
+    y0, _, dx0 = run(d["a"], d["b"])
+    a, b = d["a"].clone(), d["b"].clone()
+    b[3, 510, 2] = bad
+    a[3, 17, 300] = bad
+    y, h, dx = run(a, b)
+    mine = I == 3
+    assert torch.equal(y[~mine], y0[~mine]) and torch.equal(dx[~mine], dx0[~mine])
+    assert not torch.isfinite(y[mine][:, 510].float()).any()       # (its H is of order one, its x too)
+    assert torch.equal(y[mine][:, :500], y0[mine][:, :500])
+    assert not torch.isfinite(dx[mine][:, 300].float()).any()
