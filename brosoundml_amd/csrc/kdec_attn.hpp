@@ -163,19 +163,20 @@ __device__ inline Entry entry_of(const Args& a, int kvh, int first, int end, boo
     return r;
 }
 
-// Block `tile`'s entries of a key head: [first, end), at most BM of them, the
-// wave's from e0, and the document that holds them all (by_doc).
+// Block `tile`'s entries of a key head, `size` of them at most: its group's
+// 32 from e0, the end of those there are, and the document that holds them all
+// (by_doc).
 struct Span {
     int e0, end, doc;
 };
-__device__ inline bool span_at(const Args& a, int tile, int wave, Span& s) {
+__device__ inline bool span_at(const Args& a, int size, int tile, int group, Span& s) {
     if (!a.by_doc) {
-        s = Span{tile * BM + wave * 32, a.E, 0};
+        s = Span{tile * size + group * 32, a.E, 0};
         return true;
     }
     Piece p;
-    if (!piece_at(a.m.q_off, a.m.docs, a.m.Tq, a.G, BM, tile, p)) return false;
-    s = Span{p.lo * a.G + p.place * BM + wave * 32, p.hi * a.G, p.doc};
+    if (!piece_at(a.m.q_off, a.m.docs, a.m.Tq, a.G, size, tile, p)) return false;
+    s = Span{p.lo * a.G + p.place * size + group * 32, p.hi * a.G, p.doc};
     return true;
 }
 __device__ inline Row row_of(const Args& a, const Span& s, const Entry& e) {
@@ -291,12 +292,23 @@ __device__ inline float grad_p(const Score<T, CAP, BIAS>& rule, float s, float d
 
 // ─── host ───
 
-// Whether blocks of `size` entries (or keys) end with their document: where
-// the documents hold a block's worth each. Else blocks of several documents
-// leave fewer waves without rows, though a block then walks the keys of all
-// of them, the most of which a wave does not see.
-inline bool by_document(int docs, long entries, int size) { return docs < 1023 && docs * static_cast<long>(size) <= entries; }
+// Whether blocks of `size` entries (or keys) end with their document. Else
+// blocks of several documents leave fewer waves without rows, though a block
+// then walks the keys of all of them, the most of which a wave does not see.
+// Documents of half a block or more gain from it (8192 rows, 12 heads of width
+// 64, bf16, forward and backward together: documents of about 1024 rows 311 ->
+// 197 us, 256 132 -> 98, 64 91 -> 89, but 32 89 -> 119), as long as two turns
+// of the scan find them (900 documents of 100 rows: 817 -> 1154).
+inline bool by_document(int docs, long entries, int size) { return docs < 127 && docs * static_cast<long>(size / 2) <= entries; }
 inline long doc_blocks(bool by_doc, int docs, long entries, int size) { return cdiv(entries, size) + (by_doc ? docs + 2 : 0); }
+
+// Waves of a block that share 32 entries: one where blocks of 128 entries fill
+// the device, else two, each with half of every tile's keys. Then twice as
+// many blocks walk half as long (7 documents of up to 333 rows, 8 heads of
+// width 64, float with a bias: forward 33 -> 23 us, dQ 43 -> 29; 2 of 1000
+// rows, 16 heads on 4 of width 128, bf16: forward 51 -> 32). Filled, two lose
+// the join's time and half of a tile's use (2 of 2000 rows: 78 -> 99).
+inline int waves_shared(kdec_ctx* ctx, long blocks) { return blocks < ctx->num_cus ? 2 : 1; }
 
 // Kernels of a call by its type, width and score: L::run<T, DP, CAP, BIAS>.
 template <class L, class T, int DP, class... P>

@@ -44,18 +44,20 @@ struct Bwd {
 // that of dS's rounding. A row without keys gets lse = +inf, so that its probabilities
 // are zeros; one whose delta is not finite gets NaN, which then marks every
 // gradient that the row reaches.
-template <class T, int DP, bool CAP, bool BIAS>
+template <class T, int DP, bool CAP, bool BIAS, int KS>
 __global__ __launch_bounds__(AT, sizeof(T) == 2 ? (DP == 64 ? 3 : 2) : 1) void attn_dq_k(Bwd b) {
     constexpr int NC = DP / 16, ND = DP / 32;
     __shared__ __align__(16) T sk0[BN * DP], sk1[BN * DP], sv0[BN * DP], sv1[BN * DP];
     __shared__ int red[4][4];
+    __shared__ float srest[2][KS == 2 ? 64 : 1];
     const Args& a = b.a;
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, half = lane >> 5;
+    const int group = wave / KS, part = wave % KS;  // of the block's entries, of a tile's keys
     const int kvh = blockIdx.x % a.Hkv;
     int tile = blockIdx.x / a.Hkv;
     if (a.m.causal) tile = gridDim.x / a.Hkv - 1 - tile;  // the longest walks first
     Span sp;
-    if (!span_at(a, tile, wave, sp)) return;
+    if (!span_at(a, BM / KS, tile, group, sp)) return;
     const Entry en = entry_of(a, kvh, sp.e0, sp.end, false);
     const bool valid = en.valid;
     const int row = en.row, head = en.head;
@@ -109,12 +111,13 @@ __global__ __launch_bounds__(AT, sizeof(T) == 2 ? (DP == 64 ? 3 : 2) : 1) void a
     float rest = 0.0f;
     const auto step = [&](auto masked, int j0, const T* tk, const T* tv) __attribute__((always_inline)) {
         constexpr bool MASKED = decltype(masked)::value;
+        const bool whole = j0 >= w.wfull_lo && j0 + BN <= w.wfull_hi;
+        if (KS == 2) j0 += 32 * part, tk += 32 * part * DP, tv += 32 * part * DP;
         const unsigned at = static_cast<unsigned>(j0 + 4 * half - me.lo);
         const unsigned len = me.hi > me.lo ? static_cast<unsigned>(me.hi - me.lo) : 0u;
         const float dist = static_cast<float>(me.pos - j0 - 4 * half);
-        const bool whole = j0 >= w.wfull_lo && j0 + BN <= w.wfull_hi;
 #pragma unroll
-        for (int n = 0; n < 2; ++n) {
+        for (int n = 0; n < 2 / KS; ++n) {
             f32x16 s = f32x16{}, dp = f32x16{};
 #pragma unroll
             for (int c = 0; c < NC; ++c) {
@@ -174,6 +177,24 @@ __global__ __launch_bounds__(AT, sizeof(T) == 2 ? (DP == 64 ? 3 : 2) : 1) void a
     walks(std::true_type{}, 0, f0);
     walks(std::false_type{}, f0, f1);
     walks(std::true_type{}, f1, t1);
+    if constexpr (KS == 2) {  // the walk's last barrier is behind the tiles' last reads
+        float* other = reinterpret_cast<float*>(group ? sk1 : sk0);
+        static_assert(sizeof(sk0) >= DP * 32 * sizeof(float), "a wave's sums take a tile's place");
+        if (part) {
+#pragma unroll
+            for (int d = 0; d < ND; ++d)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) other[(16 * d + r) * 64 + lane] = acc[d][r];
+            srest[group][lane] = rest;
+        }
+        __syncthreads();
+        if (part) return;
+        rest += srest[group][lane];
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) acc[d][r] += other[(16 * d + r) * 64 + lane];
+    }
     const Entry to = entry_of(a, kvh, sp.e0, sp.end, true);
     if (!to.valid) return;
     rest += __shfl_xor(rest, 32);
@@ -501,10 +522,11 @@ __global__ __launch_bounds__(AT) void attn_dkv_join_k(Bwd b) {
 
 struct Launch {
     template <class T, int DP, bool CAP, bool BIAS>
-    static int run(kdec_ctx* ctx, const Bwd& b, long q_blocks, long k_blocks, size_t part_n) {
+    static int run(kdec_ctx* ctx, const Bwd& b, int shared, long q_blocks, long k_blocks, size_t part_n) {
         const auto blocks = [](long n) { return dim3(static_cast<unsigned>(n)); };
         if (b.a.m.Tq > 0) {
-            hipLaunchKernelGGL((attn_dq_k<T, DP, CAP, BIAS>), blocks(q_blocks), dim3(AT), 0, ctx->stream, b);
+            if (shared == 2) hipLaunchKernelGGL((attn_dq_k<T, DP, CAP, BIAS, 2>), blocks(q_blocks), dim3(AT), 0, ctx->stream, b);
+            else hipLaunchKernelGGL((attn_dq_k<T, DP, CAP, BIAS, 1>), blocks(q_blocks), dim3(AT), 0, ctx->stream, b);
         }
         if (b.a.m.Tk > 0) {
             constexpr int KG = key_groups<T, DP, BIAS>();
@@ -540,7 +562,7 @@ extern "C" int kdec_attn_bwd(kdec_ctx* ctx, int dtype, const void* Q, long q_rs,
     ProfScope ps(ctx, "attn", 0.0, 0.0);
     Bwd b{};
     b.a = Args{{Q, q_rs, q_hs}, {K, k_rs, k_hs}, {V, v_rs, v_hs}, {q_off, k_off, k_len, prefix, docs, causal != 0, Tq, Tk},
-               slopes, scale, cap, Hq, Hkv, G, D, Tq * G, by_document(docs, static_cast<long>(Tq) * G, BM)};
+               slopes, scale, cap, Hq, Hkv, G, D, Tq * G, false};
     b.O = Heads{O, o_rs, o_hs};
     b.dO = Heads{dO, do_rs, do_hs};
     b.vec_o = plain(b.O, D, size);
@@ -569,7 +591,9 @@ extern "C" int kdec_attn_bwd(kdec_ctx* ctx, int dtype, const void* Q, long q_rs,
     const size_t stat_bytes = (static_cast<size_t>(Tq) * Hq * sizeof(float2) + 255) & ~size_t(255);
     const int keys = D <= 64 || dtype == KDEC_F32 || slopes ? 64 : 128;  // of a block
     b.by_doc_k = by_document(docs, Tk, keys);
-    const long q_blocks = doc_blocks(b.a.by_doc, docs, b.a.E, BM) * Hkv, k_blocks = doc_blocks(b.by_doc_k, docs, Tk, keys) * Hkv;
+    const int shared = waves_shared(ctx, cdiv(b.a.E, BM) * Hkv), held = BM / shared;
+    b.a.by_doc = by_document(docs, b.a.E, held);
+    const long q_blocks = doc_blocks(b.a.by_doc, docs, b.a.E, held) * Hkv, k_blocks = doc_blocks(b.by_doc_k, docs, Tk, keys) * Hkv;
     KDEC_CHECK(ctx, k_blocks < INT_MAX, "kdec_attn_bwd: too many keys");
     // Key tiles too few to fill the device (causal walks differ in length, so
     // two blocks per CU) share their rows among parts of no fewer than four
@@ -586,5 +610,5 @@ extern "C" int kdec_attn_bwd(kdec_ctx* ctx, int dtype, const void* Q, long q_rs,
     b.stat = ws.as<float2>();
     b.rows = reinterpret_cast<Row*>(ws.as<char>() + stat_bytes);
     b.part = reinterpret_cast<float*>(ws.as<char>() + stat_bytes + row_bytes);
-    return dispatch<Launch>(dtype, D, cap > 0.0f, slopes != nullptr, ctx, b, q_blocks, k_blocks, part_n);
+    return dispatch<Launch>(dtype, D, cap > 0.0f, slopes != nullptr, ctx, b, shared, q_blocks, k_blocks, part_n);
 }

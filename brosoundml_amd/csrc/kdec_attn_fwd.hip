@@ -145,22 +145,25 @@ __device__ inline void finish(const Fwd& p, int kvh, int e, int row, int head, i
 
 template <class T, int DP> constexpr bool narrow() { return sizeof(T) == 2 && DP == 64; }
 
-// A block holds 128 entries of one key head (32 per wave) and walks the keys
-// that its rows see in tiles of 64, staged in shared memory two buffers deep
-// with the tile after next on its way.
-template <class T, int DP, bool CAP, bool BIAS>
+// A block holds 128 / KS entries of one key head (32 per KS waves) and walks
+// the keys that its rows see in tiles of 64, staged in shared memory two
+// buffers deep with the next tile on its way. Two waves that share entries
+// (KS) take 32 keys of each tile and are joined at the end.
+template <class T, int DP, bool CAP, bool BIAS, int KS>
 __global__ __launch_bounds__(AT, (sizeof(T) == 2 ? (narrow<T, DP>() ? (CAP || BIAS ? 3 : 4) : 2) : 1)) void attn_fwd_k(Fwd p) {
     constexpr int NC = DP / 16, ND = DP / 32;
     __shared__ __align__(16) T sk0[BN * DP], sk1[BN * DP], sv0[BN * DP], sv1[BN * DP];
     __shared__ unsigned bad[3][2];  // rows of the tile that hold values that are not finite
     __shared__ int red[4][4];
+    __shared__ float sml[2][2][KS == 2 ? 64 : 1];
     const Args& a = p.a;
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, half = lane >> 5;
+    const int group = wave / KS, part = wave % KS;  // of the block's entries, of a tile's keys
     const int kvh = blockIdx.x % a.Hkv;
     int tile = blockIdx.x / a.Hkv;
     if (a.m.causal) tile = gridDim.x / a.Hkv - 1 - tile;  // the longest walks first
     Span sp;
-    if (!span_at(a, tile, wave, sp)) return;
+    if (!span_at(a, BM / KS, tile, group, sp)) return;
     const Entry en = entry_of(a, kvh, sp.e0, sp.end, false);
     const bool valid = en.valid;
     const int row = en.row, head = en.head;
@@ -212,10 +215,11 @@ __global__ __launch_bounds__(AT, (sizeof(T) == 2 ? (narrow<T, DP>() ? (CAP || BI
     const auto step = [&](auto masked, int j0, const T* tk, const T* tv) __attribute__((always_inline)) {
         // Narrow heads take the keys 32 at a time, which leaves room for four
         // waves per SIMD; wide ones 64, for fewer steps of the softmax.
-        constexpr int N = narrow<T, DP>() ? 1 : 2;
+        constexpr int N = narrow<T, DP>() || KS == 2 ? 1 : 2;
         const bool whole = j0 >= w.wfull_lo && j0 + BN <= w.wfull_hi;
+        if (KS == 2) j0 += 32 * part, tk += 32 * part * DP, tv += 32 * part * DP;
 #pragma unroll
-        for (int n0 = 0; n0 < 2; n0 += N) {
+        for (int n0 = 0; n0 < 2 / KS; n0 += N) {
             f32x16 s[N];
 #pragma unroll
             for (int n = 0; n < N; ++n) {
@@ -271,6 +275,28 @@ __global__ __launch_bounds__(AT, (sizeof(T) == 2 ? (narrow<T, DP>() ? (CAP || BI
     walks(std::true_type{}, f1, t1);
     float l = st.l + __shfl_xor(st.l, 32);
     if (poison) l = __builtin_nanf("");
+    if constexpr (KS == 2) {  // the walk's last barrier is behind the tiles' last reads
+        float* other = reinterpret_cast<float*>(group ? sk1 : sk0);
+        static_assert(sizeof(sk0) >= DP * 32 * sizeof(float), "a wave's sums take a tile's place");
+        if (part) {
+#pragma unroll
+            for (int d = 0; d < ND; ++d)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) other[(16 * d + r) * 64 + lane] = acc[d][r];
+            sml[group][0][lane] = st.m;
+            sml[group][1][lane] = l;
+        }
+        __syncthreads();
+        if (part) return;
+        const float unit = CAP || BIAS ? 1.0f : rule.unit, om = sml[group][0][lane], m = fmaxf(st.m, om), m0 = m == -INF ? 0.0f : m;
+        const float f = __builtin_amdgcn_exp2f((st.m - m0) * unit), of = __builtin_amdgcn_exp2f((om - m0) * unit);
+        l = l * f + sml[group][1][lane] * of;
+        st.m = m;
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) acc[d][r] = acc[d][r] * f + other[(16 * d + r) * 64 + lane] * of;
+    }
     const Entry to = entry_of(a, kvh, sp.e0, sp.end, true);
     if (to.valid) finish<T, DP>(p, kvh, to.e, to.row, to.head, split, to.half, acc, st.m * (CAP || BIAS ? 1.0f : rule.unit), l);
 }
@@ -447,9 +473,10 @@ __global__ __launch_bounds__(64) void attn_join_k(Fwd p) {
 
 struct Launch {
     template <class T, int DP, bool CAP, bool BIAS>
-    static int run(kdec_ctx* ctx, const Fwd& p, dim3 grid, bool rows, int chunks) {
+    static int run(kdec_ctx* ctx, const Fwd& p, dim3 grid, bool rows, int chunks, int shared) {
         if (rows) hipLaunchKernelGGL((attn_rows_k<T, DP, CAP, BIAS>), grid, dim3(AT), 0, ctx->stream, p, chunks);
-        else hipLaunchKernelGGL((attn_fwd_k<T, DP, CAP, BIAS>), grid, dim3(AT), 0, ctx->stream, p);
+        else if (shared == 2) hipLaunchKernelGGL((attn_fwd_k<T, DP, CAP, BIAS, 2>), grid, dim3(AT), 0, ctx->stream, p);
+        else hipLaunchKernelGGL((attn_fwd_k<T, DP, CAP, BIAS, 1>), grid, dim3(AT), 0, ctx->stream, p);
         if (p.splits > 1)
             hipLaunchKernelGGL(attn_join_k<T>, dim3(static_cast<unsigned>(static_cast<long>(p.a.Hkv) * p.a.E)), dim3(64), 0,
                                ctx->stream, p);
@@ -495,8 +522,9 @@ extern "C" int kdec_attn_fwd(kdec_ctx* ctx, int dtype, const void* Q, long q_rs,
     // different documents in one block would walk each other's keys.
     const bool rows = static_cast<long>(Tq) <= 8L * docs && static_cast<long>(Tk) >= 8L * Tq;
     const int chunks = static_cast<int>(cdiv(G, 32));
-    p.a.by_doc = by_document(docs, p.a.E, BM);
-    const long tiles = rows ? static_cast<long>(Tq) * chunks : doc_blocks(p.a.by_doc, docs, p.a.E, BM);
+    const int shared = waves_shared(ctx, cdiv(p.a.E, BM) * Hkv), held = BM / shared;
+    p.a.by_doc = by_document(docs, p.a.E, held);
+    const long tiles = rows ? static_cast<long>(Tq) * chunks : doc_blocks(p.a.by_doc, docs, p.a.E, held);
     const long blocks = tiles * Hkv;
     KDEC_CHECK(ctx, blocks < INT_MAX, "kdec_attn_fwd: too many rows");
     // Split the keys where the rows alone do not fill the device, to no fewer
@@ -516,5 +544,5 @@ extern "C" int kdec_attn_fwd(kdec_ctx* ctx, int dtype, const void* Q, long q_rs,
         p.part_ml = p.part_o + n * p.a.D;
     }
     const dim3 grid(static_cast<unsigned>(blocks), static_cast<unsigned>(splits));
-    return dispatch<Launch>(dtype, D, cap > 0.0f, slopes != nullptr, ctx, p, grid, rows, chunks);
+    return dispatch<Launch>(dtype, D, cap > 0.0f, slopes != nullptr, ctx, p, grid, rows, chunks, shared);
 }
