@@ -18,6 +18,14 @@
 //
 // Entries: the rows of the heads that share a key head, entry e = row * G +
 // head within the group, so keys and values are staged once for the group.
+//
+// Long walks are bound by the matrix units and the exponentials between their
+// products: 8192 causal rows, 16 heads on 4 of width 128, bf16, take 330 us
+// (833 TFLOP/s of what the mask leaves; a large library product reaches 1320),
+// 12012 rows with a prefix and capped scores 375 (410 TFLOP/s: the cap's
+// exponential and reciprocal come on top). Packed texts of 20 to 510 tokens, 12
+// heads of width 64, take 33 us: their walks are a few tiles long, so that the
+// way to the first tile and the longest documents count.
 #include "kdec_attn.hpp"
 
 namespace kdec {
@@ -52,8 +60,8 @@ struct Soft {
 };
 
 // One step of the running softmax of a lane's column over N score blocks of
-// 32 keys from j0 (whole: all of the wave's rows see all of them). Scores become probabilities; acc is rescaled when the
-// wave's maxima move far enough.
+// 32 keys from j0 (whole: all of the wave's rows see all of them). Scores
+// become probabilities; acc is rescaled when the wave's maxima move far enough.
 template <bool MASKED, class T, bool CAP, bool BIAS, int N, int ND>
 __device__ inline void soft_step(const Score<T, CAP, BIAS>& rule, const Row& row, bool whole, int j0, int half,
                                  f32x16 (&s)[N], f32x16 (&acc)[ND], Soft& st) {
@@ -143,14 +151,14 @@ __device__ inline void finish(const Fwd& p, int kvh, int e, int row, int head, i
     if (!half) p.lse[static_cast<long>(head) * a.m.Tq + row] = l == 0.0f ? -INF : m * LN2 + logf(l);
 }
 
-template <class T, int DP> constexpr bool narrow() { return sizeof(T) == 2 && DP == 64; }
-
 // A block holds 128 / KS entries of one key head (32 per KS waves) and walks
 // the keys that its rows see in tiles of 64, staged in shared memory two
 // buffers deep with the next tile on its way. Two waves that share entries
 // (KS) take 32 keys of each tile and are joined at the end.
-template <class T, int DP, bool CAP, bool BIAS, int KS>
-__global__ __launch_bounds__(AT, (sizeof(T) == 2 ? (narrow<T, DP>() ? (CAP || BIAS ? 3 : 4) : 2) : 1)) void attn_fwd_k(Fwd p) {
+// FOUR: the two halves of a tile one after the other, which leaves registers
+// for a fourth wave per SIMD.
+template <class T, int DP, bool CAP, bool BIAS, int KS, bool FOUR = false>
+__global__ __launch_bounds__(AT, sizeof(T) == 2 ? (FOUR ? 4 : DP == 64 ? 3 : 2) : 1) void attn_fwd_k(Fwd p) {
     constexpr int NC = DP / 16, ND = DP / 32;
     __shared__ __align__(16) T sk0[BN * DP], sk1[BN * DP], sv0[BN * DP], sv1[BN * DP];
     __shared__ unsigned bad[3][2];  // rows of the tile that hold values that are not finite
@@ -213,9 +221,7 @@ __global__ __launch_bounds__(AT, (sizeof(T) == 2 ? (narrow<T, DP>() ? (CAP || BI
     Soft st;
     bool poison = false;
     const auto step = [&](auto masked, int j0, const T* tk, const T* tv) __attribute__((always_inline)) {
-        // Narrow heads take the keys 32 at a time, which leaves room for four
-        // waves per SIMD; wide ones 64, for fewer steps of the softmax.
-        constexpr int N = narrow<T, DP>() || KS == 2 ? 1 : 2;
+        constexpr int N = FOUR || KS == 2 ? 1 : 2;  // 32 keys each, of a step of the softmax
         const bool whole = j0 >= w.wfull_lo && j0 + BN <= w.wfull_hi;
         if (KS == 2) j0 += 32 * part, tk += 32 * part * DP, tv += 32 * part * DP;
 #pragma unroll
@@ -305,7 +311,11 @@ __global__ __launch_bounds__(AT, (sizeof(T) == 2 ? (narrow<T, DP>() ? (CAP || BI
 // key head (up to 32) and its waves take the keys in turn, 32 at a time, each
 // with a softmax state of its own; the four are joined at the end. Keys go
 // from memory into the product's registers, values through the wave's own
-// shared memory for their transpose, so no wave waits for another.
+// shared memory for their transpose, so no wave waits for another. Bound by
+// memory: 48 requests over caches of up to 4096 tokens, 16 heads on 4 of width
+// 128, bf16, take 50 us for 206 MB (4.1 TB/s; a large copy 4.7); one request
+// over 6000 tokens of 12 heads of width 64 in float takes 21 us for 37 MB, most
+// of it the offsets', the first keys' and the join's latency.
 template <class T, int DP, bool CAP, bool BIAS>
 __global__ __launch_bounds__(AT, sizeof(T) == 2 ? 2 : 1) void attn_rows_k(Fwd p, int chunks) {
     constexpr int NC = DP / 16, ND = DP / 32;
@@ -471,11 +481,17 @@ __global__ __launch_bounds__(64) void attn_join_k(Fwd p) {
     if (lane == 0) p.lse[static_cast<long>(head) * a.m.Tq + row] = l == 0.0f ? -INF : top * LN2 + logf(l);
 }
 
+// Whether a fourth wave per SIMD fits (a cap or a bias takes its registers).
+template <class T, int DP>
+constexpr bool four_fit(bool shaped) { return sizeof(T) == 2 && DP == 64 && !shaped; }
+
 struct Launch {
     template <class T, int DP, bool CAP, bool BIAS>
-    static int run(kdec_ctx* ctx, const Fwd& p, dim3 grid, bool rows, int chunks, int shared) {
+    static int run(kdec_ctx* ctx, const Fwd& p, dim3 grid, bool rows, int chunks, int shared, bool four) {
         if (rows) hipLaunchKernelGGL((attn_rows_k<T, DP, CAP, BIAS>), grid, dim3(AT), 0, ctx->stream, p, chunks);
         else if (shared == 2) hipLaunchKernelGGL((attn_fwd_k<T, DP, CAP, BIAS, 2>), grid, dim3(AT), 0, ctx->stream, p);
+        else if (four_fit<T, DP>(CAP || BIAS) && four)
+            hipLaunchKernelGGL((attn_fwd_k<T, DP, CAP, BIAS, 1, four_fit<T, DP>(CAP || BIAS)>), grid, dim3(AT), 0, ctx->stream, p);
         else hipLaunchKernelGGL((attn_fwd_k<T, DP, CAP, BIAS, 1>), grid, dim3(AT), 0, ctx->stream, p);
         if (p.splits > 1)
             hipLaunchKernelGGL(attn_join_k<T>, dim3(static_cast<unsigned>(static_cast<long>(p.a.Hkv) * p.a.E)), dim3(64), 0,
@@ -518,9 +534,12 @@ extern "C" int kdec_attn_fwd(kdec_ctx* ctx, int dtype, const void* Q, long q_rs,
     p.vec_o = D % 4 == 0 && aligned(Heads{O, o_rs, o_hs}, size, 4 * size);
     p.lse = lse;
     p.D_out = D;
-    // Few rows per document over many keys: a block per row. Rows of
-    // different documents in one block would walk each other's keys.
-    const bool rows = static_cast<long>(Tq) <= 8L * docs && static_cast<long>(Tk) >= 8L * Tq;
+    // One or two rows per document over many keys: a block per row. Rows of
+    // different documents in one block would walk each other's keys; from
+    // three on that costs less than reading the keys for each row (bf16, 16
+    // heads on 4 of width 128, 48 documents of 2000 keys: 1 row 43 us for 135,
+    // 2 68 for 74, 3 74 for 61, 4 77 for 52).
+    const bool rows = static_cast<long>(Tq) <= 2L * docs && static_cast<long>(Tk) >= 8L * Tq;
     const int chunks = static_cast<int>(cdiv(G, 32));
     const int shared = waves_shared(ctx, cdiv(p.a.E, BM) * Hkv), held = BM / shared;
     p.a.by_doc = by_document(docs, p.a.E, held);
@@ -528,8 +547,9 @@ extern "C" int kdec_attn_fwd(kdec_ctx* ctx, int dtype, const void* Q, long q_rs,
     const long blocks = tiles * Hkv;
     KDEC_CHECK(ctx, blocks < INT_MAX, "kdec_attn_fwd: too many rows");
     // Split the keys where the rows alone do not fill the device, to no fewer
-    // than 256 keys a part. Few rows take twice as many parts: their documents
-    // differ in length, and the longest ends last.
+    // than 256 keys a part (of 128, one float token over 6000 keys of 12 heads
+    // takes 29 us with the join, of 256 it takes 26). Few rows take twice as
+    // many parts: their documents differ in length, and the longest ends last.
     const long each = docs > 0 ? Tk / docs : 0;
     long splits = cdiv((rows ? 4L : 2L) * ctx->num_cus, blocks);
     if (splits > each / 256) splits = each / 256;
@@ -543,6 +563,14 @@ extern "C" int kdec_attn_fwd(kdec_ctx* ctx, int dtype, const void* Q, long q_rs,
         p.part_o = ws->as<float>();
         p.part_ml = p.part_o + n * p.a.D;
     }
+    // Four waves per SIMD where three do not hold all blocks at once and walks
+    // are short and differ, so that more of them side by side even out; long
+    // ones lose more to the shorter steps (bf16, 12 heads of width 64: 32 texts
+    // of 20 to 510 rows 38 -> 33 us, 64 of about 256 47 -> 45, 40 of 280 34 ->
+    // 36, 100 of 500 151 -> 153, but 8 of 1024 54 -> 58, 1 of 8192 262 -> 283).
+    // A document's last block counts half.
+    const long real = (cdiv(p.a.E, BM) + docs / 2) * Hkv;
+    const bool four = shared == 1 && real > 3L * ctx->num_cus && each <= 512;
     const dim3 grid(static_cast<unsigned>(blocks), static_cast<unsigned>(splits));
-    return dispatch<Launch>(dtype, D, cap > 0.0f, slopes != nullptr, ctx, p, grid, rows, chunks, shared);
+    return dispatch<Launch>(dtype, D, cap > 0.0f, slopes != nullptr, ctx, p, grid, rows, chunks, shared, four);
 }
