@@ -22,8 +22,8 @@
 // Long walks are bound by the matrix units and the exponentials between their
 // products: 8192 causal rows, 16 heads on 4 of width 128, bf16, take 330 us
 // (833 TFLOP/s of what the mask leaves; a large library product reaches 1320),
-// 12012 rows with a prefix and capped scores 375 (410 TFLOP/s: the cap's
-// exponential and reciprocal come on top). Packed texts of 20 to 510 tokens, 12
+// 4 causal texts of 1900 to 4099 rows with a prefix and capped scores 375 (410
+// TFLOP/s: the cap's exponential and reciprocal come on top). Packed texts of 20 to 510 tokens, 12
 // heads of width 64, take 33 us: their walks are a few tiles long, so that the
 // way to the first tile and the longest documents count.
 #include "kdec_attn.hpp"
