@@ -298,8 +298,14 @@ __device__ inline float grad_p(const Score<T, CAP, BIAS>& rule, float s, float d
 // Documents of half a block or more gain from it (8192 rows, 12 heads of width
 // 64, bf16, forward and backward together: documents of about 1024 rows 311 ->
 // 197 us, 256 132 -> 98, 64 91 -> 89, but 32 89 -> 119), as long as two turns
-// of the scan find them (900 documents of 100 rows: 817 -> 1154).
-inline bool by_document(int docs, long entries, int size) { return docs < 127 && docs * static_cast<long>(size / 2) <= entries; }
+// of the scan find them (900 documents of 100 rows: 817 -> 1154). So do
+// shorter ones where blocks of several would not fill the device, since a
+// block walks one document's keys then (54 documents of 3 rows over 120 keys, 12
+// heads of width 128: forward 83 -> 22 us, backward 136 -> 71; 48 of 4 rows over
+// 2000, 16 heads on 4: backward 566 -> 379).
+inline bool by_document(kdec_ctx* ctx, int docs, long entries, int heads, int size) {
+    return docs < 127 && (docs * static_cast<long>(size / 2) <= entries || cdiv(entries, size) * heads < ctx->num_cus);
+}
 inline long doc_blocks(bool by_doc, int docs, long entries, int size) { return cdiv(entries, size) + (by_doc ? docs + 2 : 0); }
 
 // Waves of a block that share 32 entries: one where blocks of 128 entries fill
