@@ -223,6 +223,14 @@ __device__ inline Walk walk_of(const Row& me, bool valid, int (&red)[4][4]) {
                 u(min(min(red[0][3], red[1][3]), min(red[2][3], red[3][3]))),
                 u(lo), u(hi), u(full_lo), u(full_hi)};
 }
+// Whether [lo, hi) holds a marked key of the 64 at j0.
+__device__ inline bool sees_bad(int lo, int hi, int j0, unsigned long long bad) {
+    const int a = min(max(lo - j0, 0), 64), b = min(max(hi - j0, 0), 64);
+    if (b <= a) return false;
+    const unsigned long long upto = b == 64 ? ~0ull : (1ull << b) - 1;
+    return (upto & ~((1ull << a) - 1) & bad) != 0;
+}
+
 // Tiles [t0, f0) and [f1, t1) of a walk are masked, those between are seen
 // whole by every row; the first two numbers of tiles are even, so that each
 // loop starts at the first buffer.

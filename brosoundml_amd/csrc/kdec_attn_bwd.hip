@@ -48,11 +48,14 @@ struct Bwd {
 // product as two terms, which leaves such rows the one error and the others
 // that of dS's rounding. A row without keys gets lse = +inf, so that its probabilities
 // are zeros; one whose delta is not finite gets NaN, which then marks every
-// gradient that the row reaches.
+// gradient that the row reaches. So does one that sees a key that is not
+// finite: masked tiles clean such keys and note which they were, and in whole
+// tiles they make a sum of dQ that is not finite.
 template <class T, int DP, bool CAP, bool BIAS, int KS>
-__global__ __launch_bounds__(AT, sizeof(T) == 2 ? (DP == 64 ? 3 : 2) : 1) void attn_dq_k(Bwd b) {
+__global__ __launch_bounds__(AT, (sizeof(T) == 2 ? 2 : 1) + (DP == 64)) void attn_dq_k(Bwd b) {
     constexpr int NC = DP / 16, ND = DP / 32;
     __shared__ __align__(16) T sk0[BN * DP], sk1[BN * DP], sv0[BN * DP], sv1[BN * DP];
+    __shared__ unsigned bad[3][2];  // keys of the tile that are not finite
     __shared__ int red[4][4];
     __shared__ float srest[2][KS == 2 ? 64 : 1];
     const Args& a = b.a;
@@ -67,6 +70,7 @@ __global__ __launch_bounds__(AT, sizeof(T) == 2 ? (DP == 64 ? 3 : 2) : 1) void a
     const bool valid = en.valid;
     const int row = en.row, head = en.head;
     const Row me = row_of(a, sp, en);
+    if (tid < 6) bad[tid >> 1][tid & 1] = 0;
     const Walk w = walk_of(me, valid, red);
     const int t1 = w.hi > w.lo ? (w.hi - w.lo + BN - 1) / BN : 0;
 
@@ -108,7 +112,10 @@ __global__ __launch_bounds__(AT, sizeof(T) == 2 ? (DP == 64 ? 3 : 2) : 1) void a
     split_walk(w, 0, t1, f0, f1);
     const auto landed = [&](int t, T* tk) __attribute__((always_inline)) {
         __builtin_amdgcn_s_waitcnt(0);
-        if (t < f0 || t >= f1) ks.clean(tk, tid, [](int) {});  // a zero of dS times such a key
+        if (t < f0 || t >= f1) {  // a zero of dS times such a key
+            unsigned* m = bad[t % 3];
+            ks.clean(tk, tid, [&](int r) { atomicOr(&m[r >> 5], 1u << (r & 31)); });
+        }
     };
     f32x16 acc[ND];
 #pragma unroll
@@ -164,7 +171,14 @@ __global__ __launch_bounds__(AT, sizeof(T) == 2 ? (DP == 64 ? 3 : 2) : 1) void a
     const auto walk = [&](auto masked, int t, const T* tk, const T* tv, T* nk, T* nv) __attribute__((always_inline)) {
         const int j0 = w.lo + t * BN;
         if (t + 1 < t1) load(t + 1, nk, nv);
-        if (w.wlo < j0 + BN && w.whi > j0) step(masked, j0, tk, tv);
+        if (tid < 2) bad[(t + 2) % 3][tid] = 0;
+        if (w.wlo < j0 + BN && w.whi > j0) {
+            step(masked, j0, tk, tv);
+            if (decltype(masked)::value) {
+                const unsigned* m = bad[t % 3];
+                if (sees_bad(me.lo, me.hi, j0, m[0] | static_cast<unsigned long long>(m[1]) << 32)) rest = __builtin_nanf("");
+            }
+        }
         if (t + 1 < t1) landed(t + 1, nk);
         __syncthreads();
     };
@@ -203,6 +217,12 @@ __global__ __launch_bounds__(AT, sizeof(T) == 2 ? (DP == 64 ? 3 : 2) : 1) void a
     const Entry to = entry_of(a, kvh, sp.e0, sp.end, true);
     if (!to.valid) return;
     rest += __shfl_xor(rest, 32);
+    unsigned top = 0;
+#pragma unroll
+    for (int d = 0; d < ND; ++d) top = magnitude(acc[d], top);
+    top = max(top, static_cast<unsigned>(__shfl_xor(static_cast<int>(top), 32)));
+    float scale = a.scale;
+    if (top >= kNotFinite || !(__builtin_fabsf(rest) < INF)) scale = lse2 = __builtin_nanf("");
     if (!to.half) b.stat[static_cast<long>(to.head) * a.m.Tq + to.row] = make_float2(lse2, delta + rest);
     T* o = static_cast<T*>(b.dQ) + to.row * b.dq_rs + to.head * b.dq_hs;
 #pragma unroll
@@ -210,8 +230,8 @@ __global__ __launch_bounds__(AT, sizeof(T) == 2 ? (DP == 64 ? 3 : 2) : 1) void a
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
             const int d = 32 * dt + 8 * x + 4 * to.half;
-            store4(o + d, b.D_out - d, b.vec_dq, acc[dt][4 * x] * a.scale, acc[dt][4 * x + 1] * a.scale,
-                   acc[dt][4 * x + 2] * a.scale, acc[dt][4 * x + 3] * a.scale);
+            store4(o + d, b.D_out - d, b.vec_dq, acc[dt][4 * x] * scale, acc[dt][4 * x + 1] * scale, acc[dt][4 * x + 2] * scale,
+                   acc[dt][4 * x + 3] * scale);
         }
 }
 

@@ -45,14 +45,6 @@ struct Fwd {
     float *part_o, *part_ml;  // (splits, Hkv, E, D) and (splits, Hkv, E, 2)
 };
 
-// Whether [lo, hi) holds a marked key of the 64 at j0.
-__device__ inline bool sees_bad(int lo, int hi, int j0, unsigned long long bad) {
-    const int a = min(max(lo - j0, 0), 64), b = min(max(hi - j0, 0), 64);
-    if (b <= a) return false;
-    const unsigned long long upto = b == 64 ? ~0ull : (1ull << b) - 1;
-    return (upto & ~((1ull << a) - 1) & bad) != 0;
-}
-
 // Running softmax state of one lane's column, in the units of m: raw products
 // (times `unit` they are log2) without cap and bias, log2 with either.
 struct Soft {

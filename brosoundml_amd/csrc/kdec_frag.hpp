@@ -53,6 +53,15 @@ __device__ inline Frag<T> acc_frag(const f32x16& s, int c) {
     return f;
 }
 
+// The largest magnitude of an accumulator's values, and of `top`, as an
+// integer: kNotFinite or more where one of them is not finite.
+constexpr unsigned kNotFinite = 0x7F800000u;
+__device__ inline unsigned magnitude(const f32x16& s, unsigned top) {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) top = max(top, __float_as_uint(s[r]) & 0x7FFFFFFFu);
+    return top;
+}
+
 __device__ inline f32x8 acc_floats(const f32x16& s, int c) {
     f32x8 f;
 #pragma unroll
