@@ -299,22 +299,6 @@ struct Product {
 
 template <class T> constexpr int depth_of() { return sizeof(T) == 2 ? 64 : 32; }  // of a tile: 128 bytes
 
-// Whether a fragment of this lane's holds a value that is not finite: its
-// largest magnitude as an integer.
-__device__ inline bool not_finite(bf16x8 f) {
-    typedef unsigned short u16x8 __attribute__((ext_vector_type(8)));
-    const u16x8 b = __builtin_bit_cast(u16x8, f) & static_cast<unsigned short>(0x7FFF);
-    const auto m4 = __builtin_elementwise_max(b.lo, b.hi);
-    const auto m2 = __builtin_elementwise_max(m4.lo, m4.hi);
-    return m2[0] >= 0x7F80 || m2[1] >= 0x7F80;
-}
-__device__ inline bool not_finite(f32x8 f) {
-    unsigned m = 0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(f[i]) & 0x7FFFFFFFu);
-    return m >= 0x7F800000u;
-}
-
 // The low-rank products of 32 MB of a wave's features (from wm) and its 32 NB
 // rows (a lane each: its row and adapter), into acc: forward B H, backward
 // A^T dH. Rows of other adapters take part with zeros. An adapter's values

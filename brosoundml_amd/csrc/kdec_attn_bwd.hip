@@ -47,8 +47,8 @@ struct Bwd {
 // rows of few keys show it: they only meet masked tiles, where dS enters the
 // product as two terms, which leaves such rows the one error and the others
 // that of dS's rounding. A row without keys gets lse = +inf, so that its probabilities
-// are zeros; one whose delta is not finite gets NaN, which then marks every
-// gradient that the row reaches. So does one that sees a key that is not
+// are zeros; one whose query or delta is not finite gets NaN, which then marks
+// every gradient that the row reaches. So does one that sees a key that is not
 // finite: masked tiles clean such keys and note which they were, and in whole
 // tiles they make a sum of dQ that is not finite.
 template <class T, int DP, bool CAP, bool BIAS, int KS>
@@ -80,22 +80,25 @@ __global__ __launch_bounds__(AT, (sizeof(T) == 2 ? 2 : 1) + (DP == 64)) void att
     const T* gp = static_cast<const T*>(b.dO.p) + row * b.dO.rs + head * b.dO.hs;
     const T* op = static_cast<const T*>(b.O.p) + row * b.O.rs + head * b.O.hs;
     float lse2 = INF, delta = 0.0f;
+    bool wild = false;  // (capped scores of such a query are finite)
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
         const int d = 16 * c + 8 * half, n = valid ? min(8, a.D - d) : 0;
         q[c] = load8(qp + d, n, true);
         g[c] = load8(gp + d, n, true);
+        wild |= not_finite(q[c]);
         const Frag<T> o = load8(op + d, valid ? min(8, b.D_out - d) : 0, b.vec_o);
 #pragma unroll
         for (int i = 0; i < 8; ++i) delta = __builtin_fmaf(static_cast<float>(o[i]), static_cast<float>(g[c][i]), delta);
         if (sizeof(T) == 4) __builtin_amdgcn_sched_barrier(0);
     }
     delta += __shfl_xor(delta, 32);
+    wild |= __shfl_xor(wild, 32) != 0;
     if (valid) {
         const float lse = b.lse[static_cast<long>(head) * a.m.Tq + row];
         lse2 = lse == -INF ? INF : lse * LOG2E;
-        if (lse == -INF) delta = 0.0f;
-        else if (!(__builtin_fabsf(delta) < INF)) lse2 = __builtin_nanf("");
+        if (me.hi <= me.lo) delta = 0.0f;
+        else if (wild || !(__builtin_fabsf(delta) < INF)) lse2 = __builtin_nanf("");
         if (!half && head == 0) b.rows[row] = me;
     }
     const T* kb = static_cast<const T*>(a.K.p) + kvh * a.K.hs;

@@ -69,6 +69,22 @@ __device__ inline f32x8 acc_floats(const f32x16& s, int c) {
     return f;
 }
 
+// Whether a fragment of this lane's holds a value that is not finite: its
+// largest magnitude as an integer.
+__device__ inline bool not_finite(bf16x8 f) {
+    typedef unsigned short u16x8 __attribute__((ext_vector_type(8)));
+    const u16x8 b = __builtin_bit_cast(u16x8, f) & static_cast<unsigned short>(0x7FFF);
+    const auto m4 = __builtin_elementwise_max(b.lo, b.hi);
+    const auto m2 = __builtin_elementwise_max(m4.lo, m4.hi);
+    return m2[0] >= 0x7F80 || m2[1] >= 0x7F80;
+}
+__device__ inline bool not_finite(f32x8 f) {
+    unsigned m = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(f[i]) & 0x7FFFFFFFu);
+    return m >= kNotFinite;
+}
+
 // 8 elements at p, of which the first n are the tensor's (zeros beyond).
 // vec: p is aligned to 16 bytes and n is a multiple of 16 bytes' elements.
 __device__ inline bf16x8 load8(const bf16* p, int n, bool vec) {

@@ -479,9 +479,9 @@ int kdec_attn_fwd(kdec_ctx* ctx, int dtype, const void* Q, long q_rs,
 /* Its backward from dO, with the forward's O and lse: dQ, dK and dV are
  * overwritten (zeros in rows that nothing sees), dK and dV summed over the
  * query heads of a key head in a fixed order. Scores are formed again; the
- * slopes are constants. A row whose O or dO is not finite, or that sees a key
- * row that is not, has a dQ of NaN, and so have dK and dV of the keys that
- * it sees. */
+ * slopes are constants. A row whose Q, O or dO is not finite, or that sees a
+ * key row that is not, has a dQ of NaN, and so have dK and dV of the keys
+ * that it sees. */
 int kdec_attn_bwd(kdec_ctx* ctx, int dtype, const void* Q, long q_rs,
                   long q_hs, const void* K, long k_rs, long k_hs,
                   const void* V, long v_rs, long v_hs, const void* O,

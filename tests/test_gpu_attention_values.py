@@ -1,7 +1,7 @@
 """Attention (kdec_attn_fwd / kdec_attn_bwd) where tensors hold values that are not finite in places that rows see:
 what a row gets does not depend on the kernel or the tile in which a key comes up. A key that is not finite enters
 the scores by the formula (the oracle in 64 bits tells which) and makes every gradient NaN that the rows seeing it
-reach, and so does an output gradient."""
+reach, and so does a query or an output gradient."""
 import math
 
 import numpy as np
@@ -57,6 +57,9 @@ CASES = {  # name: rows, keys, causal, cap; what holds which value
     "key-capped-masked-tile": (200, 200, False, 5.0, "k", 170, INF),
     "key-capped-whole-tile": (200, 200, False, 5.0, "k", 5, -INF),
     "key-nan": (200, 200, True, 0.0, "k", 150, math.nan),
+    "query-capped": (200, 200, False, 5.0, "q", 150, INF),
+    "query-capped-causal": (200, 200, True, 5.0, "q", 90, -INF),
+    "query": (200, 200, True, 0.0, "q", 90, INF),
     "grad": (200, 200, True, 0.0, "do", 90, INF),
     "key-low-one-row": (1, 2500, False, 0.0, "k", 700, -INF),
 }
