@@ -194,6 +194,19 @@ __device__ inline float max32(float x) {
     return fmaxf(__uint_as_float(lo), __uint_as_float(hi));
 }
 
+// Whether one of a column's sums is not finite, in either lane half: they are
+// times zero added to one register, which costs one instruction a sum and no
+// registers at the kernels' ends.
+template <int ND>
+__device__ inline bool sums_not_finite(const f32x16 (&acc)[ND]) {
+    float zero = 0.0f;
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) zero = __builtin_fmaf(acc[d][r], 0.0f, zero);
+    return !(zero + __shfl_xor(zero, 32) == 0.0f);
+}
+
 // What a block of 128 entries (32 per wave) walks: keys [lo, hi) in tiles of
 // 64, of which those in [full_lo, full_hi) are seen by every row; a wave's
 // rows see keys of [wlo, whi), and all of them those of [wfull_lo, wfull_hi).

@@ -220,12 +220,8 @@ __global__ __launch_bounds__(AT, (sizeof(T) == 2 ? 2 : 1) + (DP == 64)) void att
     const Entry to = entry_of(a, kvh, sp.e0, sp.end, true);
     if (!to.valid) return;
     rest += __shfl_xor(rest, 32);
-    unsigned top = 0;
-#pragma unroll
-    for (int d = 0; d < ND; ++d) top = magnitude(acc[d], top);
-    top = max(top, static_cast<unsigned>(__shfl_xor(static_cast<int>(top), 32)));
     float scale = a.scale;
-    if (top >= kNotFinite || !(__builtin_fabsf(rest) < INF)) scale = lse2 = __builtin_nanf("");
+    if (sums_not_finite(acc) || !(__builtin_fabsf(rest) < INF)) scale = lse2 = __builtin_nanf("");
     if (!to.half) b.stat[static_cast<long>(to.head) * a.m.Tq + to.row] = make_float2(lse2, delta + rest);
     T* o = static_cast<T*>(b.dQ) + to.row * b.dq_rs + to.head * b.dq_hs;
 #pragma unroll

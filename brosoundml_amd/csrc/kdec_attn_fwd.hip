@@ -272,7 +272,9 @@ __global__ __launch_bounds__(AT, sizeof(T) == 2 ? (FOUR ? 4 : DP == 64 ? 3 : 2) 
     walks(std::false_type{}, f0, f1);
     walks(std::true_type{}, f1, t1);
     float l = st.l + __shfl_xor(st.l, 32);
-    if (poison) l = __builtin_nanf("");
+    // A row that sees a value that is not finite becomes NaN whole, whichever
+    // tile brings the value.
+    if (poison || sums_not_finite(acc)) l = __builtin_nanf("");
     if constexpr (KS == 2) {  // the walk's last barrier is behind the tiles' last reads
         float* other = reinterpret_cast<float*>(group ? sk1 : sk0);
         static_assert(sizeof(sk0) >= DP * 32 * sizeof(float), "a wave's sums take a tile's place");
@@ -396,6 +398,7 @@ __global__ __launch_bounds__(AT, sizeof(T) == 2 ? 2 : 1) void attn_rows_k(Fwd p,
     // join the waves: their states' common maximum, then the sums in order
     const float unit = CAP || BIAS ? 1.0f : rule.unit;
     float l = st.l + __shfl_xor(st.l, 32);
+    if (sums_not_finite(acc)) l = __builtin_nanf("");
     if (!half) {
         sml[wave][0][lane] = st.m * unit;
         sml[wave][1][lane] = l;

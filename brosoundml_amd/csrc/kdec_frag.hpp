@@ -53,15 +53,6 @@ __device__ inline Frag<T> acc_frag(const f32x16& s, int c) {
     return f;
 }
 
-// The largest magnitude of an accumulator's values, and of `top`, as an
-// integer: kNotFinite or more where one of them is not finite.
-constexpr unsigned kNotFinite = 0x7F800000u;
-__device__ inline unsigned magnitude(const f32x16& s, unsigned top) {
-#pragma unroll
-    for (int r = 0; r < 16; ++r) top = max(top, __float_as_uint(s[r]) & 0x7FFFFFFFu);
-    return top;
-}
-
 __device__ inline f32x8 acc_floats(const f32x16& s, int c) {
     f32x8 f;
 #pragma unroll
@@ -82,7 +73,7 @@ __device__ inline bool not_finite(f32x8 f) {
     unsigned m = 0;
 #pragma unroll
     for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(f[i]) & 0x7FFFFFFFu);
-    return m >= kNotFinite;
+    return m >= 0x7F800000u;
 }
 
 // 8 elements at p, of which the first n are the tensor's (zeros beyond).

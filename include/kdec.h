@@ -466,8 +466,10 @@ int kdec_dropout(kdec_ctx* ctx, int dtype, const void* X, long x_rs,
  * exp s. A row that sees nothing, or that no document holds, gets O = 0 and
  * lse = -inf. Query head h reads key head h / (Hq / Hkv). Offsets must not
  * decrease; they are clamped to the Tq and Tk rows. Key and value rows that
- * a row does not see do not reach it, whatever they hold; one that it sees
- * and that is not finite makes it NaN.
+ * a row does not see do not reach it, whatever they hold. A value row that it
+ * sees and that is not finite makes its O and lse NaN; a key row that is not
+ * finite enters its score by the formula (a score of -inf has probability 0,
+ * one of +inf or NaN makes the row NaN).
  * D <= 128, Hq a multiple of Hkv, scale > 0. */
 int kdec_attn_fwd(kdec_ctx* ctx, int dtype, const void* Q, long q_rs,
                   long q_hs, const void* K, long k_rs, long k_hs,

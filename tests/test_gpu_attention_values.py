@@ -1,7 +1,7 @@
 """Attention (kdec_attn_fwd / kdec_attn_bwd) where tensors hold values that are not finite in places that rows see:
-what a row gets does not depend on the kernel or the tile in which a key comes up. A key that is not finite enters
-the scores by the formula (the oracle in 64 bits tells which) and makes every gradient NaN that the rows seeing it
-reach, and so does a query or an output gradient."""
+what a row gets does not depend on the kernel or the tile in which a key comes up. A value that is not finite makes
+the rows that see it NaN, o and lse; a key that is not finite enters the scores by the formula (the oracle in 64 bits
+tells which) and makes every gradient NaN that the rows seeing it reach, and so does a query or an output gradient."""
 import math
 
 import numpy as np
@@ -48,6 +48,12 @@ def forward(q, k, v, see, cap):
 
 
 CASES = {  # name: rows, keys, causal, cap; what holds which value
+    "value-masked-tile": (200, 200, False, 0.0, "v", 170, INF),
+    "value-whole-tile": (200, 200, False, 0.0, "v", 5, INF),
+    "value-causal": (200, 200, True, 0.0, "v", 5, -INF),
+    "value-nan-whole-tile": (200, 200, False, 0.0, "v", 70, math.nan),
+    "value-one-row": (1, 3000, False, 0.0, "v", 1234, INF),
+    "value-one-row-short": (1, 100, False, 0.0, "v", 99, INF),
     "key-low-masked-tile": (200, 200, False, 0.0, "k", 170, -INF),
     "key-low-whole-tile": (200, 200, False, 0.0, "k", 5, -INF),
     "key-low-causal-last": (200, 200, True, 0.0, "k", 199, -INF),
@@ -119,3 +125,19 @@ def test_rows_that_see_values_not_finite(ctx, ty, name, D, heads, many):
         assert torch.equal(g[~r], w[~r]), n
     for n in ("o", "lse"):
         assert torch.equal(got[n].cpu()[~reached[n]], want[n].cpu()[~reached[n]]), n
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_more_requests_than_a_wave_has_lanes(ctx, D):
+    """One row each for 70 requests, one request's cache with an infinite value: its row is NaN, the others keep their bits."""
+    from brosoundml_amd import tokens
+    q, k, v, _ = inputs(torch.bfloat16, 70, 70 * 50, 4, 1, D, 1)
+    q_off, k_off = torch.arange(71, dtype=torch.int32).cuda(), (torch.arange(71) * 50).int().cuda()
+    k_len = torch.from_numpy(np.random.default_rng(4).integers(30, 50, 70)).int().cuda()
+    want, wl = tokens.attention(ctx, q, k, v, q_off, k_off, k_len, causal=True)
+    v[33 * 50 + 20, 0, 9] = INF
+    v[34 * 50 + 49] = math.nan  # past what is filled
+    got, gl = tokens.attention(ctx, q, k, v, q_off, k_off, k_len, causal=True)
+    other = torch.arange(70) != 33
+    assert torch.isnan(got[33].float()).all() and torch.isnan(gl[:, 33]).all()
+    assert torch.equal(got.cpu()[other], want.cpu()[other]) and torch.equal(gl.cpu()[:, other], wl.cpu()[:, other])
