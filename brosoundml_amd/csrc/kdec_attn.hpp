@@ -258,11 +258,16 @@ __device__ inline void split_walk(const Walk& w, int t0, int t1, int& f0, int& f
     if (f0 >= f1) f0 = f1 = t0;
 }
 
-// Scores in log2 units from raw products. T says how exact the cap's tanh has
-// to be: 1 - 2 / (1 + e^2x) is off by 2^-24 absolutely, which a bf16 score
-// cannot show; for float the odd series takes over near zero (its next term,
-// 62/2835 x^9, is below 2^-25 of x up to 0.15).
-template <class T, bool CAP, bool BIAS>
+// Scores in log2 units from raw products. CAP is how the cap's tanh is formed:
+// 1 - 2 / (1 + e^2x) is off by 2^-23 absolutely, and the score by cap times
+// that; up to caps of NEAR_CAP that is 2^-17, which a bf16 probability cannot
+// show. Beyond, and for float, the odd series takes over near zero (its next
+// term, 62/2835 x^9, is below 2^-25 of x up to 0.15), which takes a fifth
+// longer (4 causal texts of 3000 rows, 16 heads on 4 of width 128, bf16, cap
+// 100: forward 230 -> 278 us, backward 854 -> 1005).
+enum Cap { NO_CAP, QUICK_CAP, FINE_CAP };
+constexpr float NEAR_CAP = 64.0f;
+template <class T, int CAP, bool BIAS>
 struct Score {
     float unit;   // product to log2 units
     float k, c2;  // cap: tanh's argument is s k / (2 log2 e), the score c2 tanh
@@ -276,7 +281,7 @@ struct Score {
     __device__ inline float tanh_(float s) const {
         const float x2 = s * k;
         float th = __builtin_fmaf(-2.0f, __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x2)), 1.0f);
-        if (sizeof(T) == 4) {
+        if (CAP == FINE_CAP) {
             const float x = x2 * (0.5f / LOG2E), q = x * x;
             const float near = x * (1.0f + q * (-1.0f / 3 + q * (2.0f / 15 + q * (-17.0f / 315))));
             th = __builtin_fabsf(x) < 0.15f ? near : th;
@@ -302,7 +307,7 @@ struct Score {
 
 // A probability formed again from a raw product and the row's lse in log2
 // units; dt is the score's derivative by scale * product.
-template <class T, bool CAP, bool BIAS>
+template <class T, int CAP, bool BIAS>
 __device__ inline float grad_p(const Score<T, CAP, BIAS>& rule, float s, float dist, float lse2, float& dt) {
     if (!CAP && !BIAS) {
         dt = 1.0f;
@@ -338,13 +343,17 @@ inline long doc_blocks(bool by_doc, int docs, long entries, int size) { return c
 inline int waves_shared(kdec_ctx* ctx, long blocks) { return blocks < ctx->num_cus ? 2 : 1; }
 
 // Kernels of a call by its type, width and score: L::run<T, DP, CAP, BIAS>.
+template <class L, class T, int DP, int CAP, class... P>
+int by_bias(bool bias, P&&... p) {
+    return bias ? L::template run<T, DP, CAP, true>(p...) : L::template run<T, DP, CAP, false>(p...);
+}
 template <class L, class T, int DP, class... P>
-int by_score(bool cap, bool bias, P&&... p) {
-    if (cap) return bias ? L::template run<T, DP, true, true>(p...) : L::template run<T, DP, true, false>(p...);
-    return bias ? L::template run<T, DP, false, true>(p...) : L::template run<T, DP, false, false>(p...);
+int by_score(float cap, bool bias, P&&... p) {
+    if (cap > 0.0f && sizeof(T) == 2 && cap <= NEAR_CAP) return by_bias<L, T, DP, sizeof(T) == 2 ? QUICK_CAP : FINE_CAP>(bias, p...);
+    return cap > 0.0f ? by_bias<L, T, DP, FINE_CAP>(bias, p...) : by_bias<L, T, DP, NO_CAP>(bias, p...);
 }
 template <class L, class... P>
-int dispatch(int dtype, int D, bool cap, bool bias, P&&... p) {
+int dispatch(int dtype, int D, float cap, bool bias, P&&... p) {
     if (dtype == KDEC_F32) return D <= 64 ? by_score<L, float, 64>(cap, bias, p...) : by_score<L, float, 128>(cap, bias, p...);
     return D <= 64 ? by_score<L, bf16, 64>(cap, bias, p...) : by_score<L, bf16, 128>(cap, bias, p...);
 }

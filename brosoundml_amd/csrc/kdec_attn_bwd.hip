@@ -51,8 +51,8 @@ struct Bwd {
 // every gradient that the row reaches. So does one that sees a key that is not
 // finite: masked tiles clean such keys and note which they were, and in whole
 // tiles they make a sum of dQ that is not finite.
-template <class T, int DP, bool CAP, bool BIAS, int KS>
-__global__ __launch_bounds__(AT, (sizeof(T) == 2 ? 2 : 1) + (DP == 64)) void attn_dq_k(Bwd b) {
+template <class T, int DP, int CAP, bool BIAS, int KS>
+__global__ __launch_bounds__(AT, (sizeof(T) == 2 ? 2 : 1) + (DP == 64 && !(sizeof(T) == 2 && CAP == FINE_CAP && BIAS))) void attn_dq_k(Bwd b) {
     constexpr int NC = DP / 16, ND = DP / 32;
     __shared__ __align__(16) T sk0[BN * DP], sk1[BN * DP], sv0[BN * DP], sv1[BN * DP];
     __shared__ unsigned bad[3][2];  // keys of the tile that are not finite
@@ -252,7 +252,7 @@ __global__ __launch_bounds__(AT, (sizeof(T) == 2 ? 2 : 1) + (DP == 64)) void att
 // wave: two pairs.
 template <class T, int DP, bool BIAS> constexpr int key_groups() { return DP == 64 ? 2 : sizeof(T) == 4 || BIAS ? 2 : 4; }
 
-template <class T, int DP, bool CAP, bool BIAS>
+template <class T, int DP, int CAP, bool BIAS>
 __global__ __launch_bounds__((128 * key_groups<T, DP, BIAS>()), (sizeof(T) == 2 && DP == 64 ? 3 : key_groups<T, DP, BIAS>() == 4 ? 2 : 1)) void attn_dkv_k(Bwd b) {
     constexpr int NC = DP / 16, ND = DP / 32, BE = 64, PAIR = 2 * BE, KG = key_groups<T, DP, BIAS>(), NT = 128 * KG, KEYS = 32 * KG;
     // (aligned to come first: within the reach of the reads' own offsets)
@@ -545,7 +545,7 @@ __global__ __launch_bounds__(AT) void attn_dkv_join_k(Bwd b) {
 }
 
 struct Launch {
-    template <class T, int DP, bool CAP, bool BIAS>
+    template <class T, int DP, int CAP, bool BIAS>
     static int run(kdec_ctx* ctx, const Bwd& b, int shared, long q_blocks, long k_blocks, size_t part_n) {
         const auto blocks = [](long n) { return dim3(static_cast<unsigned>(n)); };
         if (b.a.m.Tq > 0) {
@@ -634,5 +634,5 @@ extern "C" int kdec_attn_bwd(kdec_ctx* ctx, int dtype, const void* Q, long q_rs,
     b.stat = ws.as<float2>();
     b.rows = reinterpret_cast<Row*>(ws.as<char>() + stat_bytes);
     b.part = reinterpret_cast<float*>(ws.as<char>() + stat_bytes + row_bytes);
-    return dispatch<Launch>(dtype, D, cap > 0.0f, slopes != nullptr, ctx, b, shared, q_blocks, k_blocks, part_n);
+    return dispatch<Launch>(dtype, D, cap, slopes != nullptr, ctx, b, shared, q_blocks, k_blocks, part_n);
 }

@@ -54,7 +54,7 @@ struct Soft {
 // One step of the running softmax of a lane's column over N score blocks of
 // 32 keys from j0 (whole: all of the wave's rows see all of them). Scores
 // become probabilities; acc is rescaled when the wave's maxima move far enough.
-template <bool MASKED, class T, bool CAP, bool BIAS, int N, int ND>
+template <bool MASKED, class T, int CAP, bool BIAS, int N, int ND>
 __device__ inline void soft_step(const Score<T, CAP, BIAS>& rule, const Row& row, bool whole, int j0, int half,
                                  f32x16 (&s)[N], f32x16 (&acc)[ND], Soft& st) {
     constexpr bool RAW = !CAP && !BIAS;
@@ -149,7 +149,7 @@ __device__ inline void finish(const Fwd& p, int kvh, int e, int row, int head, i
 // (KS) take 32 keys of each tile and are joined at the end.
 // FOUR: the two halves of a tile one after the other, which leaves registers
 // for a fourth wave per SIMD.
-template <class T, int DP, bool CAP, bool BIAS, int KS, bool FOUR = false>
+template <class T, int DP, int CAP, bool BIAS, int KS, bool FOUR = false>
 __global__ __launch_bounds__(AT, sizeof(T) == 2 ? (FOUR ? 4 : DP == 64 ? 3 : 2) : 1) void attn_fwd_k(Fwd p) {
     constexpr int NC = DP / 16, ND = DP / 32;
     __shared__ __align__(16) T sk0[BN * DP], sk1[BN * DP], sv0[BN * DP], sv1[BN * DP];
@@ -310,7 +310,7 @@ __global__ __launch_bounds__(AT, sizeof(T) == 2 ? (FOUR ? 4 : DP == 64 ? 3 : 2) 
 // 128, bf16, take 50 us for 206 MB (4.1 TB/s; a large copy 4.7); one request
 // over 6000 tokens of 12 heads of width 64 in float takes 21 us for 37 MB, most
 // of it the offsets', the first keys' and the join's latency.
-template <class T, int DP, bool CAP, bool BIAS>
+template <class T, int DP, int CAP, bool BIAS>
 __global__ __launch_bounds__(AT, sizeof(T) == 2 ? 2 : 1) void attn_rows_k(Fwd p, int chunks) {
     constexpr int NC = DP / 16, ND = DP / 32;
     constexpr int JE = 8;  // columns joined at a time
@@ -481,7 +481,7 @@ template <class T, int DP>
 constexpr bool four_fit(bool shaped) { return sizeof(T) == 2 && DP == 64 && !shaped; }
 
 struct Launch {
-    template <class T, int DP, bool CAP, bool BIAS>
+    template <class T, int DP, int CAP, bool BIAS>
     static int run(kdec_ctx* ctx, const Fwd& p, dim3 grid, bool rows, int chunks, int shared, bool four) {
         if (rows) hipLaunchKernelGGL((attn_rows_k<T, DP, CAP, BIAS>), grid, dim3(AT), 0, ctx->stream, p, chunks);
         else if (shared == 2) hipLaunchKernelGGL((attn_fwd_k<T, DP, CAP, BIAS, 2>), grid, dim3(AT), 0, ctx->stream, p);
@@ -567,5 +567,5 @@ extern "C" int kdec_attn_fwd(kdec_ctx* ctx, int dtype, const void* Q, long q_rs,
     const long real = (cdiv(p.a.E, BM) + docs / 2) * Hkv;
     const bool four = shared == 1 && real > 3L * ctx->num_cus && each <= 512;
     const dim3 grid(static_cast<unsigned>(blocks), static_cast<unsigned>(splits));
-    return dispatch<Launch>(dtype, D, cap > 0.0f, slopes != nullptr, ctx, p, grid, rows, chunks, shared, four);
+    return dispatch<Launch>(dtype, D, cap, slopes != nullptr, ctx, p, grid, rows, chunks, shared, four);
 }
