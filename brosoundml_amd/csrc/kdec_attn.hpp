@@ -332,6 +332,21 @@ __device__ inline float grad_p(const Score<T, CAP, BIAS>& rule, float s, float d
 inline bool by_document(kdec_ctx* ctx, int docs, long entries, int heads, int size) {
     return docs < 127 && (docs * static_cast<long>(size / 2) <= entries || cdiv(entries, size) * heads < ctx->num_cus);
 }
+// The same for blocks of rows, which walk keys: past two turns of the scan they
+// end with their document as well where a document's walk is long against the
+// scan. A turn takes about as long as half a tile of 64 keys, and blocks of
+// several documents walk as many tiles in all, but on B of the 2 num_cus places
+// that the others fill: (keys / 64 + docs / 128) B < keys / 64 * 2 num_cus.
+// (Causal forward, bf16, 16 heads on 4 of width 128, of several documents and of
+// one: 128 requests of 2 rows over 1000 keys 87 and 48 us, 200 of 4 126 and 89,
+// 256 of 2 over 200 52 and 35, 512 of 8 over 300 75 and 98, 512 of 2 over 60 25
+// and 48; 12 heads of width 64: 200 of 2 over 1000 220 and 117, 1000 of 2 over
+// 200 162 and 216.)
+inline bool rows_by_document(kdec_ctx* ctx, int docs, long keys, long entries, int heads, int size) {
+    if (docs < 127) return by_document(ctx, docs, entries, heads, size);
+    const long each = keys / docs, all = 2L * ctx->num_cus, blocks = cdiv(entries, size) * heads;
+    return (2 * each + docs) * (blocks < all ? blocks : all) < 2 * each * all;
+}
 inline long doc_blocks(bool by_doc, int docs, long entries, int size) { return cdiv(entries, size) + (by_doc ? docs + 2 : 0); }
 
 // Waves of a block that share 32 entries: one where blocks of 128 entries fill

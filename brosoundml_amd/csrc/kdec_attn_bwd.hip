@@ -616,7 +616,7 @@ extern "C" int kdec_attn_bwd(kdec_ctx* ctx, int dtype, const void* Q, long q_rs,
     const int keys = D <= 64 || dtype == KDEC_F32 || slopes ? 64 : 128;  // of a block
     b.by_doc_k = by_document(ctx, docs, Tk, Hkv, keys);
     const int shared = waves_shared(ctx, cdiv(b.a.E, BM) * Hkv), held = BM / shared;
-    b.a.by_doc = by_document(ctx, docs, b.a.E, Hkv, held);
+    b.a.by_doc = rows_by_document(ctx, docs, Tk, b.a.E, Hkv, held);
     const long q_blocks = doc_blocks(b.a.by_doc, docs, b.a.E, held) * Hkv, k_blocks = doc_blocks(b.by_doc_k, docs, Tk, keys) * Hkv;
     KDEC_CHECK(ctx, k_blocks < INT_MAX, "kdec_attn_bwd: too many keys");
     // Key tiles too few to fill the device (causal walks differ in length, so

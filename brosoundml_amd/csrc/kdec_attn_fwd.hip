@@ -529,15 +529,17 @@ extern "C" int kdec_attn_fwd(kdec_ctx* ctx, int dtype, const void* Q, long q_rs,
     p.vec_o = D % 4 == 0 && aligned(Heads{O, o_rs, o_hs}, size, 4 * size);
     p.lse = lse;
     p.D_out = D;
+    const int chunks = static_cast<int>(cdiv(G, 32));
+    const int shared = waves_shared(ctx, cdiv(p.a.E, BM) * Hkv), held = BM / shared;
+    p.a.by_doc = rows_by_document(ctx, docs, Tk, p.a.E, Hkv, held);
     // One row per document over many keys: a block per row. From two on, blocks
     // that end with their document read the keys once for all rows (bf16, 16
     // heads on 4 of width 128, 48 documents of 2000 keys: 2 rows 68 us for 48, 3
     // 74 for 48, 4 77 for 49), and where these would hold several documents, each
-    // other's keys as well (1 row 43 for 135).
-    const bool rows = Tq <= docs && static_cast<long>(Tk) >= 8L * Tq;
-    const int chunks = static_cast<int>(cdiv(G, 32));
-    const int shared = waves_shared(ctx, cdiv(p.a.E, BM) * Hkv), held = BM / shared;
-    p.a.by_doc = by_document(ctx, docs, p.a.E, Hkv, held);
+    // other's keys as well (1 row 43 for 135). A few rows of padding leave it at
+    // that: their blocks end at once (1000 documents of 200 keys, 12 heads of
+    // width 64, 24 rows more: 128 us, in blocks of several 259).
+    const bool rows = static_cast<long>(Tk) >= 8L * Tq && Tq <= (p.a.by_doc ? docs : docs + docs / 4);
     const long tiles = rows ? static_cast<long>(Tq) * chunks : doc_blocks(p.a.by_doc, docs, p.a.E, held);
     const long blocks = tiles * Hkv;
     KDEC_CHECK(ctx, blocks < INT_MAX, "kdec_attn_fwd: too many rows");
