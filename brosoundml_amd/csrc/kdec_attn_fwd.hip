@@ -561,10 +561,12 @@ extern "C" int kdec_attn_fwd(kdec_ctx* ctx, int dtype, const void* Q, long q_rs,
         p.part_ml = p.part_o + n * p.a.D;
     }
     // Four waves per SIMD where three do not hold all blocks at once and walks
-    // are short and differ, so that more of them side by side even out; long
-    // ones lose more to the shorter steps (bf16, 12 heads of width 64: 32 texts
-    // of 20 to 510 rows 38 -> 33 us, 64 of about 256 47 -> 45, 40 of 280 34 ->
-    // 36, 100 of 500 151 -> 153, but 8 of 1024 54 -> 58, 1 of 8192 262 -> 283).
+    // are short, so that more of them side by side even out; long ones lose more
+    // to the shorter steps (bf16, 12 heads of width 64, three and four waves: 32
+    // texts of 20 to 510 rows 28.8 and 26.1 us, 64 of 256 37.2 and 33.7, 120 of
+    // 128 27.7 and 25.2, 40 of 280 33.9 and 33.7, of 200 to 360 33.7 and 35.3, 100
+    // of 500 151 and 143, 60 of 520 101 and 98, but 24 of 700 62.7 and 64.1, 8 of
+    // 1024 42.8 and 45.2, 1 of 8192 246 and 262). The host knows the lengths' mean.
     // A document's last block counts half.
     const long real = (cdiv(p.a.E, BM) + docs / 2) * Hkv;
     const bool four = shared == 1 && real > 3L * ctx->num_cus && each <= 512;
