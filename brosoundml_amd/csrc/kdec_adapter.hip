@@ -301,14 +301,13 @@ template <class T> constexpr int depth_of() { return sizeof(T) == 2 ? 64 : 32; }
 
 // The low-rank products of 32 MB of a wave's features (from wm) and its 32 NB
 // rows (a lane each: its row and adapter), into acc: forward B H, backward
-// A^T dH. Rows of other adapters take part with zeros. An adapter's values
-// that are not finite would make NaN of those, so they are left out of this
-// product and make one of their own, which only the adapter's rows take.
-// Adapters and units are taken in turn by `turns` takers of which this is
-// number `turn`.
+// A^T dH. Rows of other adapters and features of other units take part with
+// zeros, which values that are not finite would make NaN: such values of either
+// side are left out, and `wild` gets the rows that they belong to. Adapters and
+// units are taken in turn by `turns` takers of which this is number `turn`.
 template <class T, bool BWD, int MB, int NB>
 __device__ inline void low_rank(const Adapter& p, int M, int wm, int u0, int u1, int row, int id, int turn, int turns,
-                                f32x16 (&acc)[MB][NB]) {
+                                f32x16 (&acc)[MB][NB], unsigned long long& wild) {
     const int lane = threadIdx.x & 63, half = lane >> 5, col = lane & 31;
     const float* H = BWD ? p.dH : p.H;
     unsigned long long left = __builtin_amdgcn_ballot_w64(id < p.n);
@@ -329,12 +328,21 @@ __device__ inline void low_rank(const Adapter& p, int M, int wm, int u0, int u1,
                 const int d = k + 8 * half, n = min(8, p.rank - d), dd = n > 0 ? d : 0;
                 Frag<T> w[2];
                 f32x8 h[NB];
+                bool bad = false;
 #pragma unroll
-                for (int j = 0; j < NB; ++j)
+                for (int j = 0; j < NB; ++j) {
                     h[j] = load8(H + static_cast<long>(rows[j]) * p.R + u * p.rank + dd, ids[j] == a ? n : 0, p.vec_h);
+                    bad |= not_finite(h[j]);
+                }
+                if (__builtin_amdgcn_ballot_w64(bad)) {
+#pragma unroll
+                    for (int j = 0; j < NB; ++j) h[j] = finite_part(h[j]);
+                    wild |= mine;
+                    asm volatile("");  // a branch
+                }
 #pragma unroll
                 for (int i0 = 0; i0 < MB; i0 += 2) {  // 64 features at a time, which the registers leave room for
-                    bool bad = false;
+                    bad = false;
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
                         const int m = wm + 32 * (i0 + i) + col;
@@ -353,25 +361,8 @@ __device__ inline void low_rank(const Adapter& p, int M, int wm, int u0, int u1,
                     for (int i = 0; i < 2; ++i) bad |= not_finite(w[i]);
                     if (__builtin_amdgcn_ballot_w64(bad)) {
 #pragma unroll
-                        for (int i = 0; i < 2; ++i) {
-                            Frag<T> v = w[i];
-#pragma unroll
-                            for (int x = 0; x < 8; ++x) {
-                                const bool fine = __builtin_fabsf(static_cast<float>(v[x])) < __builtin_inff();
-                                w[i][x] = fine ? v[x] : static_cast<T>(0.0f);
-                                v[x] = fine ? static_cast<T>(0.0f) : v[x];
-                            }
-#pragma unroll
-                            for (int j = 0; j < NB; ++j) {
-                                const Terms<T, 2> t(h[j]);
-                                f32x16 tmp = f32x16{};
-#pragma unroll
-                                for (int x = 0; x < t.n; ++x) tmp = mma32(v, t.t[x], tmp);
-                                if (ids[j] == a)
-#pragma unroll
-                                    for (int r = 0; r < 16; ++r) acc[i0 + i][j][r] += tmp[r];
-                            }
-                        }
+                        for (int i = 0; i < 2; ++i) w[i] = finite_part(w[i]);
+                        wild |= mine;
                         asm volatile("");  // a branch
                     }
 #pragma unroll
@@ -388,6 +379,42 @@ __device__ inline void low_rank(const Adapter& p, int M, int wm, int u0, int u1,
             }
         }
         u -= u1 - u0;
+    }
+}
+
+// What low_rank left out of the `wild` rows: their low-rank sums over a wave's
+// `features` from wm, one by one, of which those that are not finite are added
+// to what the wave has written. (Splits that share such a sum all add it, which
+// changes neither an infinity nor NaN.)
+template <class T, bool BWD, class O>
+__device__ inline void wild_sums(const Adapter& p, int M, int wm, int features, int u0, int u1, int row, int id,
+                                 unsigned long long wild, O* Y, long y_rs) {
+    const int lane = threadIdx.x & 63;
+    __threadfence();  // a lane takes what others wrote
+    for (; wild; wild &= wild - 1) {
+        const int l = __builtin_ctzll(wild);
+        const int t = __builtin_amdgcn_readlane(row, l), a = __builtin_amdgcn_readlane(id, l);
+        for (int m = wm + lane; m < min(wm + features, M); m += 64) {
+            float low = 0.0f;
+            for (int u = u0; u < u1; ++u) {
+                if (!BWD && (m < p.unit_off[u] || m >= p.unit_off[u + 1])) continue;
+                const float* h = (BWD ? p.dH : p.H) + static_cast<long>(t) * p.R + u * p.rank;
+                const T* w = BWD ? static_cast<const T*>(p.A) + (static_cast<long>(a) * p.R + u * p.rank) * p.in + m
+                                 : static_cast<const T*>(p.B) + (static_cast<long>(a) * p.out + m) * p.rank;
+                for (int j = 0; j < p.rank; ++j) low = __builtin_fmaf(static_cast<float>(w[BWD ? static_cast<long>(j) * p.in : j]), h[j], low);
+                if (!__builtin_amdgcn_ballot_w64(low == low)) break;  // NaN whatever follows
+            }
+            if (BWD && p.dropping) {
+                unsigned w[4];
+                drop_words(p.drop, static_cast<unsigned>(t), static_cast<unsigned>(m) >> 3, w);
+                unsigned v = w[0];
+#pragma unroll
+                for (int i = 1; i < 4; ++i) v = (m >> 1 & 3) == i ? w[i] : v;
+                if (((m & 1) ? v >> 16 : v & 0xFFFFu) < p.drop.thr) low = 0.0f;
+            }
+            O* y = Y + t * y_rs + m;
+            if (!(__builtin_fabsf(low) < __builtin_inff())) *y = static_cast<O>(static_cast<float>(*y) + low);
+        }
     }
 }
 
@@ -491,11 +518,10 @@ __global__ __launch_bounds__(BIG ? 512 : 256, DIRECT ? 2 : 1) void adapter_gemm_
 #pragma unroll
         for (int j = 0; j < 2; ++j) acc[i][j] = f32x16{};
     if (c0 < c1) load(c0, sw0, sz0);
-    {
-        const int u0 = BWD ? 0 : unit_at(p.unit_off, p.units, wm);
-        const int u1 = BWD ? p.units : unit_at(p.unit_off, p.units, min(wm + 32 * MB - 1, g.M - 1)) + 1;
-        low_rank<T, BWD>(p, g.M, wm, u0, u1, srow[wn + lane], sid[wn + lane], split, g.splits, acc);
-    }
+    const int u0 = BWD ? 0 : unit_at(p.unit_off, p.units, wm);
+    const int u1 = BWD ? p.units : unit_at(p.unit_off, p.units, min(wm + 32 * MB - 1, g.M - 1)) + 1;
+    unsigned long long wild = 0;
+    low_rank<T, BWD>(p, g.M, wm, u0, u1, srow[wn + lane], sid[wn + lane], split, g.splits, acc, wild);
     if (DIRECT && BIG) {  // formed again rather than held meanwhile
         asm volatile("" ::: "memory");
         z_offsets(g.K - c0 * BK);
@@ -608,6 +634,13 @@ __global__ __launch_bounds__(BIG ? 512 : 256, DIRECT ? 2 : 1) void adapter_gemm_
                     store4(static_cast<T*>(g.Y) + row * g.y_rs + m, g.M - m, g.vec_y, v[0], v[1], v[2], v[3]);
             }
     }
+    if (wild) {
+        const int row = srow[wn + lane], id = sid[wn + lane];
+        if (g.splits > 1)
+            wild_sums<T, BWD>(p, g.M, wm, 32 * MB, u0, u1, row, id, wild, g.part + split * static_cast<long>(p.T) * g.M, g.M);
+        else
+            wild_sums<T, BWD>(p, g.M, wm, 32 * MB, u0, u1, row, id, wild, static_cast<T*>(g.Y), g.y_rs);
+    }
 }
 
 // The splits' sums, rounded once: 64 values per block, its sixteen waves
@@ -632,8 +665,9 @@ __global__ __launch_bounds__(1024) void adapter_join_k(const float* part, int sp
 // The same for few rows and 32 features: two of the taker's pairs of adapter
 // and unit at a time, the loads of both in flight.
 template <class T, int NB>
-__device__ inline void low_rank_few(const Adapter& p, int M, int m, int u0, int u1, int id, int turn, int turns, f32x16 (&acc)[NB]) {
-    const int lane = threadIdx.x & 63, half = lane >> 5, col = lane & 31;
+__device__ inline void low_rank_few(const Adapter& p, int M, int m0, int u0, int u1, int id, int turn, int turns, f32x16 (&acc)[NB],
+                                    unsigned long long& wild) {
+    const int lane = threadIdx.x & 63, half = lane >> 5, col = lane & 31, m = m0 + col;
     unsigned long long left = __builtin_amdgcn_ballot_w64(id < p.n);
     int rows[NB], ids[NB];
 #pragma unroll
@@ -663,14 +697,9 @@ __device__ inline void low_rank_few(const Adapter& p, int M, int m, int u0, int 
             as[1] = a, us[1] = u, mines[1] = mine;
             more = next();
         }
-        f32x16 tmp[2][NB];
         bool in[2];
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            in[i] = m >= p.unit_off[us[i]] && m < p.unit_off[us[i] + 1] && m < M;
-#pragma unroll
-            for (int j = 0; j < NB; ++j) tmp[i][j] = f32x16{};
-        }
+        for (int i = 0; i < 2; ++i) in[i] = m >= p.unit_off[us[i]] && m < p.unit_off[us[i] + 1] && m < M;
         for (int k = 0; k < p.rank; k += 16) {
             const int d = k + 8 * half, n = min(8, p.rank - d), dd = n > 0 ? d : 0;
             Frag<T> w[2];
@@ -684,23 +713,26 @@ __device__ inline void low_rank_few(const Adapter& p, int M, int m, int u0, int 
                     h[i][j] = load8(p.H + static_cast<long>(rows[j]) * p.R + us[i] * p.rank + dd, ids[j] == as[i] ? n : 0, p.vec_h);
             }
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
+            for (int i = 0; i < 2; ++i) {
+                bool bad = not_finite(w[i]);
+#pragma unroll
+                for (int j = 0; j < NB; ++j) bad |= not_finite(h[i][j]);
+                if (__builtin_amdgcn_ballot_w64(bad)) {
+                    w[i] = finite_part(w[i]);
+#pragma unroll
+                    for (int j = 0; j < NB; ++j) h[i][j] = finite_part(h[i][j]);
+                    wild |= mines[i];
+                    asm volatile("");  // a branch
+                }
 #pragma unroll
                 for (int j = 0; j < NB; ++j) {
                     if (!(mines[i] >> (32 * j) & 0xFFFFFFFFull)) continue;
                     const Terms<T, 2> v(h[i][j]);
 #pragma unroll
-                    for (int x = 0; x < v.n; ++x) tmp[i][j] = mma32(w[i], v.t[x], tmp[i][j]);
+                    for (int x = 0; x < v.n; ++x) acc[j] = mma32(w[i], v.t[x], acc[j]);
                 }
+            }
         }
-        // only an adapter's rows take its product, whatever another's would be
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-            for (int j = 0; j < NB; ++j)
-                if (mines[i] >> (32 * j + col) & 1)
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) acc[j][r] += tmp[i][j][r];
     }
 }
 
@@ -710,6 +742,7 @@ __device__ inline void low_rank_few(const Adapter& p, int M, int m, int u0, int 
 template <class T, int NB>
 __global__ __launch_bounds__(LT) void adapter_few_k(Adapter p, Product g) {
     __shared__ Join8 buf[8];
+    __shared__ unsigned long long swild[8];
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, half = lane >> 5, col = lane & 31;
     const int m0 = blockIdx.x * 32, m = m0 + col;
     const int id = lane < p.T ? adapter_of(p, lane) : p.n;
@@ -737,7 +770,9 @@ __global__ __launch_bounds__(LT) void adapter_few_k(Adapter p, Product g) {
         }
     }
     const int u0 = unit_at(p.unit_off, p.units, m0), u1 = unit_at(p.unit_off, p.units, min(m0 + 31, g.M - 1)) + 1;
-    low_rank_few<T, NB>(p, g.M, m, u0, u1, id, wave, 8, acc);
+    unsigned long long wild = 0;
+    low_rank_few<T, NB>(p, g.M, m0, u0, u1, id, wave, 8, acc, wild);
+    if (lane == 0) swild[wave] = wild;
 #pragma unroll
     for (int j = 0; j < NB; ++j)
         join8(buf, acc[j], [&](int r, int c, float v) {
@@ -746,6 +781,12 @@ __global__ __launch_bounds__(LT) void adapter_few_k(Adapter p, Product g) {
             if (p.bias) v += static_cast<float>(static_cast<const T*>(p.bias)[m0 + r]);
             static_cast<T*>(g.Y)[t * g.y_rs + m0 + r] = static_cast<T>(v);
         });
+#pragma unroll
+    for (int w = 0; w < 8; ++w) wild |= swild[w];
+    if (!wild) return;  // all waves or none
+    __threadfence();
+    __syncthreads();
+    if (!wave) wild_sums<T, false>(p, g.M, m0, 32, u0, u1, lane, id, wild, static_cast<T*>(g.Y), g.y_rs);
 }
 
 // Sums over a chunk's rows: C[m, c] = f sum_t P[t, m] Z[t, c] for 32 columns m
@@ -758,7 +799,7 @@ __global__ __launch_bounds__(LT) void adapter_few_k(Adapter p, Product g) {
 template <class T, bool DB>
 __global__ __launch_bounds__(NT) void adapter_outer_k(Adapter p, const float* P, const T* Z, long z_rs, int C, bool vec_z,
                                                       float* out, float beta, float* part, int mt) {
-    constexpr int NTERM = Terms<T, 3>::n, ROWS = 64, NZ = ROWS * 16 / NT;
+    constexpr int NTERM = Terms<T, 3, true>::n, ROWS = 64, NZ = ROWS * 16 / NT;
     __shared__ __align__(16) T sz[ROWS * 128];
     __shared__ __align__(16) T sp[NTERM][ROWS * 64];
     const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, half = lane >> 5, col = lane & 31;
@@ -797,16 +838,20 @@ __global__ __launch_bounds__(NT) void adapter_outer_k(Adapter p, const float* P,
                 if (!DB && p.dropping) z[i] = dropped<T>(p.drop, rows[i], c0 + 8 * (e & 15), z[i]);
                 Tile<T, 128>::put8(sz, e >> 4, e & 15, z[i]);
             }
-            const Terms<T, 3> v(h);
+            const Terms<T, 3, true> v(h);
 #pragma unroll
             for (int x = 0; x < NTERM; ++x) Tile<T, 64>::put8(sp[x], tid >> 2, tid & 3, v.t[x]);
             __syncthreads();
             if (s + ROWS < pc.count) load(s + ROWS);
 #pragma unroll
             for (int k = 0; k < ROWS / 16; ++k) {
-                const Frag<T> w = lds_cols<128, false>(sz, 16 * k, 32 * wave);
+                Frag<T> w = lds_cols<128, false>(sz, 16 * k, 32 * wave);
 #pragma unroll
-                for (int x = 0; x < NTERM; ++x) acc = mma32(lds_cols<64, false>(sp[x], 16 * k, 0), w, acc);
+                for (int x = 0; x < NTERM; ++x) {
+                    acc = mma32(lds_cols<64, false>(sp[x], 16 * k, 0), w, acc);
+                    // values that are not finite meet P's first term alone
+                    if (NTERM > 1 && x == 0 && __builtin_amdgcn_ballot_w64(not_finite(w))) w = finite_part(w);
+                }
             }
             __syncthreads();
         }

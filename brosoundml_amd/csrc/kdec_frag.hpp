@@ -61,7 +61,7 @@ __device__ inline f32x8 acc_floats(const f32x16& s, int c) {
 }
 
 // Whether a fragment of this lane's holds a value that is not finite: its
-// largest magnitude as an integer.
+// largest magnitude as an integer (bf16), zero times its values (float).
 __device__ inline bool not_finite(bf16x8 f) {
     typedef unsigned short u16x8 __attribute__((ext_vector_type(8)));
     const u16x8 b = __builtin_bit_cast(u16x8, f) & static_cast<unsigned short>(0x7FFF);
@@ -70,10 +70,18 @@ __device__ inline bool not_finite(bf16x8 f) {
     return m2[0] >= 0x7F80 || m2[1] >= 0x7F80;
 }
 __device__ inline bool not_finite(f32x8 f) {
-    unsigned m = 0;
+    float zero = 0.0f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(f[i]) & 0x7FFFFFFFu);
-    return m >= 0x7F800000u;
+    for (int i = 0; i < 8; ++i) zero = __builtin_fmaf(f[i], 0.0f, zero);
+    return !(zero == 0.0f);
+}
+
+// A fragment with zeros for its values that are not finite.
+template <class F>
+__device__ inline F finite_part(F f) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = __builtin_fabsf(static_cast<float>(f[i])) < __builtin_inff() ? f[i] : 0.0f;
+    return f;
 }
 
 // 8 elements at p, of which the first n are the tensor's (zeros beyond).
@@ -290,9 +298,10 @@ struct Copy {
 
 // A float fragment as bf16 terms whose sum holds it to 16 (two terms) or 24
 // bits (three): products with a bf16 operand then lose nothing that float
-// sums would keep. Float operands are one term.
-template <class T, int N> struct Terms;
-template <int N> struct Terms<bf16, N> {
+// sums would keep. Float operands are one term. WILD: a value that is not
+// finite is the first term alone.
+template <class T, int N, bool WILD = false> struct Terms;
+template <int N, bool WILD> struct Terms<bf16, N, WILD> {
     static constexpr int n = N;
     bf16x8 t[N];
     __device__ explicit Terms(f32x8 f) {
@@ -301,11 +310,13 @@ template <int N> struct Terms<bf16, N> {
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 t[k][i] = static_cast<bf16>(f[i]);
+                if (k + 1 == N) continue;
                 f[i] -= static_cast<float>(t[k][i]);
+                if (WILD && k == 0) f[i] = f[i] == f[i] ? f[i] : 0.0f;  // infinity less infinity, or NaN
             }
     }
 };
-template <int N> struct Terms<float, N> {
+template <int N, bool WILD> struct Terms<float, N, WILD> {
     static constexpr int n = 1;
     f32x8 t[1];
     __device__ explicit Terms(f32x8 f) { t[0] = f; }

@@ -509,6 +509,8 @@ int kdec_attn_bwd(kdec_ctx* ctx, int dtype, const void* Q, long q_rs,
  * p > 0 drops inputs of the adapters (not of W) as kdec_dropout does with
  * this seed and offset. H (T, units*rank floats; zero rows where no adapter
  * is chosen) is written when not NULL, for the backward.
+ * An adapter's values reach the rows that choose it and their unit's outputs,
+ * whatever they hold; an infinity comes out infinite.
  * rank <= 128, units <= 4096, in and out <= 2^24, adapters <= 2^20. */
 int kdec_adapter_fwd(kdec_ctx* ctx, int dtype, const void* X, long x_rs,
                      const void* W, const void* bias, const void* A,
