@@ -448,7 +448,8 @@ int kdec_length_regulate(kdec_ctx* ctx, const float* t_en, long te_bs,
  * Philox4x32-10 under key `seed` and counter (col / 8, row, offset's low and
  * high word): the same seed, offset, row and column give the same mask, so
  * the backward is this call on dY with R = NULL. Y may be X or R.
- * 0 <= p, and p and its rounding below 1. r_rs = 0 broadcasts one row. */
+ * 0 <= p, and p and its rounding below 1. A row stride of 0 broadcasts one row
+ * of X or R (a mask of its own for every row). */
 int kdec_dropout(kdec_ctx* ctx, int dtype, const void* X, long x_rs,
                  const void* R, long r_rs, void* Y, long y_rs, long rows,
                  int cols, float p, long seed, long offset);
