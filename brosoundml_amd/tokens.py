@@ -5,6 +5,10 @@ and makes one C ABI call on the context's stream; nothing synchronises. A
 tensor made on another stream has to be ordered before the context's by the
 caller, as for every call of the library.
 
+The calls make no autograd graph: a gradient is its own call. So a tensor that
+requires grad is refused where grad mode is on; pass ``t.detach()``, or call
+under ``torch.no_grad()`` or from an autograd function.
+
 Tensors are float32 or bfloat16 (one type per call), on the context's device;
 offsets and adapter choices are int32 tensors there. Errors are
 ``native.KdecError`` (what the library refuses) and ``ValueError`` (tensors
@@ -32,6 +36,11 @@ def _fail(what):
     raise ValueError("brosoundml: " + what)
 
 
+def _no_graph(x):
+    if x.requires_grad and torch.is_grad_enabled():
+        _fail("a tensor requires grad, and these calls make no autograd graph: detach it or call under torch.no_grad()")
+
+
 def _dtype(ctx, x, *others):
     """The C ABI's type of x, which the others must share, all on the context's device."""
     ty, dev = x.dtype, x.device
@@ -39,7 +48,11 @@ def _dtype(ctx, x, *others):
         _fail("tensors must be float32 or bfloat16")
     if dev.type != "cuda" or dev.index != ctx.device:
         _fail("tensors must be on the context's HIP device")
+    if x.requires_grad:
+        _no_graph(x)
     for t in others:
+        if t.requires_grad:
+            _no_graph(t)
         if t.dtype != ty or t.device != dev:
             _fail("tensors must share one type and device")
     return _TYPES[ty]
@@ -59,6 +72,8 @@ def _floats(ctx, x, shape, what):
         return None
     if x.dtype != torch.float32 or x.get_device() != ctx.device or x.shape != shape or not x.is_contiguous():
         _fail(f"{what} must be a contiguous float32 tensor of shape {tuple(shape)}")
+    if x.requires_grad:
+        _no_graph(x)
     return x.data_ptr()
 
 
