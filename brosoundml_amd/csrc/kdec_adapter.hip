@@ -26,7 +26,8 @@ constexpr int NT = 256;            // threads of the gradients' blocks
 constexpr int LT = 512;            // threads of the low-rank kernels' blocks, 8 waves
 constexpr int ST = 1024;           // threads of the sort
 constexpr int PIECE = 32;          // sorted rows of a piece
-constexpr int CHUNK = 256;         // sorted rows of a chunk, the adapters' gradients' unit of work
+constexpr int CHUNK = 256;         // least sorted rows of a chunk, the adapters' gradients' unit of work
+constexpr int CHUNKS = 512;        // cuts of the rows: each holds a gradient of its own until they are added
 constexpr int FEW = 64;            // rows that one block of the product holds whole
 
 // Sorted rows [start, start + count) of one adapter (n: none).
@@ -65,11 +66,11 @@ __device__ inline int unit_at(const int* off, int units, int m) {
 
 // Block a places adapter a's rows (a = n: the rows without one): every wave
 // counts a run of rows, and from the counts writes its rows in order. Its
-// pieces (and chunks) are the windows of PIECE (CHUNK) sorted places that its
+// pieces (and chunks) are the windows of PIECE (`chunk`) sorted places that its
 // rows meet. They start at table entry start / window + a,
 // which no other adapter's reach: an adapter of c rows meets at most
 // c / window + 1 windows; entries up to the next adapter's first are empty.
-__global__ __launch_bounds__(ST) void adapter_sort_k(const int* idx, int T, int n, int* perm, Piece* pieces, Piece* chunks) {
+__global__ __launch_bounds__(ST) void adapter_sort_k(const int* idx, int T, int n, int chunk, int* perm, Piece* pieces, Piece* chunks) {
     constexpr int NW = ST / 64, AHEAD = 8;
     __shared__ int less_sum[NW], eq_sum[NW];
     const int a = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -114,7 +115,7 @@ __global__ __launch_bounds__(ST) void adapter_sort_k(const int* idx, int T, int 
         }
     };
     table(pieces, PIECE);
-    table(chunks, CHUNK);
+    table(chunks, chunk);
     each([&](int row, int id) {
         const unsigned long long hit = __builtin_amdgcn_ballot_w64(id == a);
         if (id == a) perm[at + __builtin_popcountll(hit & ((1ull << lane) - 1))] = row;
@@ -980,9 +981,11 @@ size_t up(size_t n) { return (n + 255) & ~size_t(255); }
 // The sort's workspace: rows, pieces, chunks.
 struct Sorted {
     size_t perm, pieces, chunks;
+    int chunk;  // rows of a chunk
     long n_pieces, n_chunks;
     Sorted(int T, int adapters)
-        : perm(up(T * 4ul)), n_pieces(T / PIECE + adapters + 1), n_chunks(T / CHUNK + adapters + 1) {
+        : perm(up(T * 4ul)), chunk(static_cast<int>(cdiv(T > 0 ? T : 1, static_cast<long>(CHUNK) * CHUNKS)) * CHUNK),
+          n_pieces(T / PIECE + adapters + 1), n_chunks(T / chunk + adapters + 1) {
         pieces = up(n_pieces * sizeof(Piece));
         chunks = up(n_chunks * sizeof(Piece));
     }
@@ -990,7 +993,7 @@ struct Sorted {
     void sort(kdec_ctx* ctx, Adapter& p, char* ws) const {
         int* rows = reinterpret_cast<int*>(ws);
         Piece *a = reinterpret_cast<Piece*>(ws + perm), *b = reinterpret_cast<Piece*>(ws + perm + pieces);
-        hipLaunchKernelGGL(adapter_sort_k, dim3(p.n + 1), dim3(ST), 0, ctx->stream, p.idx, p.T, p.n, rows, a, b);
+        hipLaunchKernelGGL(adapter_sort_k, dim3(p.n + 1), dim3(ST), 0, ctx->stream, p.idx, p.T, p.n, chunk, rows, a, b);
         p.perm = rows;
         p.pieces = a;
         p.chunks = b;
@@ -1161,7 +1164,7 @@ int kdec_adapter_bwd(kdec_ctx* ctx, int dtype, const void* X, long x_rs, const v
     if (splits < 1) splits = 1;
     const Sorted sorted(T, adapters);
     const size_t h_b = up(static_cast<size_t>(T) * R * 4), s_b = splits > 1 ? up(static_cast<size_t>(splits) * T * in * 4) : 0;
-    const bool parts = dA && T > CHUNK;
+    const bool parts = dA && T > sorted.chunk;
     const size_t a_b = parts ? up(static_cast<size_t>(sorted.n_chunks) * R * in * 4) : 0;
     const size_t b_b = parts ? up(static_cast<size_t>(sorted.n_chunks) * out * rank * 4) : 0;
     Workspace ws(ctx, sorted.bytes() + h_b + s_b + a_b + b_b);

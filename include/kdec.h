@@ -512,6 +512,8 @@ int kdec_attn_bwd(kdec_ctx* ctx, int dtype, const void* Q, long q_rs,
  * is chosen) is written when not NULL, for the backward.
  * An adapter's values reach the rows that choose it and their unit's outputs,
  * whatever they hold; an infinity comes out infinite.
+ * More than 64 rows are sorted by adapter, by one block per adapter that looks
+ * at all of them.
  * rank <= 128, units <= 4096, in and out <= 2^24, adapters <= 2^20. */
 int kdec_adapter_fwd(kdec_ctx* ctx, int dtype, const void* X, long x_rs,
                      const void* W, const void* bias, const void* A,
@@ -527,7 +529,9 @@ int kdec_adapter_fwd(kdec_ctx* ctx, int dtype, const void* X, long x_rs,
  *                 + sum_{t of a} dY[t, r] H[t, u(r)*rank + j]
  * dA and dB are floats of A's and B's shapes; adapters that no row chooses
  * get zeros (beta = 0: overwritten, what they held is not read). dX (T, in)
- * at dx_rs. dX, or dA and dB together, may be NULL. */
+ * at dx_rs. dX, or dA and dB together, may be NULL. The rows' shares of dA and
+ * dB (more than 256 rows) take the room of up to 513 adapters' gradients beside
+ * that of dA and dB themselves. */
 int kdec_adapter_bwd(kdec_ctx* ctx, int dtype, const void* X, long x_rs,
                      const void* W, const void* A, const void* B,
                      const float* scale, const int* idx, const int* unit_off,
