@@ -128,16 +128,7 @@ struct Tile {
         return 0;
     }
     __device__ static inline int at(int row, int unit) { return row * DP + U * (unit ^ swz(row)); }
-    // 8 elements from column 8 * chunk
-    __device__ static inline Frag<T> get8(const T* tile, int row, int chunk) {
-        if constexpr (sizeof(T) == 2) {
-            return *reinterpret_cast<const Frag<T>*>(tile + at(row, chunk));
-        } else {
-            const f32x4 a = *reinterpret_cast<const f32x4*>(tile + at(row, 2 * chunk));
-            const f32x4 b = *reinterpret_cast<const f32x4*>(tile + at(row, 2 * chunk + 1));
-            return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
-        }
-    }
+    // 8 elements to column 8 * chunk
     __device__ static inline void put8(T* tile, int row, int chunk, const Frag<T>& f) {
         if constexpr (sizeof(T) == 2) {
             *reinterpret_cast<Frag<T>*>(tile + at(row, chunk)) = f;
