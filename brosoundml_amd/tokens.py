@@ -236,8 +236,10 @@ def adapter_proj_bwd(ctx: Context, x, w, a, b, scale, idx, unit_off, h, dy, *, d
 def dropout(ctx: Context, x, p, seed, offset=0, *, residual=None, out=None):
     """residual + x with values dropped with probability p and the kept ones
     scaled by 1 / (1 - p) (kdec_dropout; p in steps of 1 / 65536). The mask is
-    the seed's and offset's alone: the backward is this call on the gradient
-    with the same seed and offset and no residual. ``out`` may be x."""
+    the seed's, the offset's and the place's alone: the backward is this call on
+    the gradient with the same seed and offset and no residual, and dropouts
+    whose masks are to differ, ``drop`` of ``adapter_proj`` among them, take
+    offsets of their own. ``out`` may be x."""
     dt = _dtype(ctx, x)
     X = _rows(x, "x")
     y = _empty(ctx, x, x.shape) if out is None else out
