@@ -9,10 +9,10 @@
 // adds to: five products would do for seven, but the sums would be made by
 // atomics in an order that changes from call to call.
 //
-// 8192 causal rows, 16 heads on 4 of width 128, bf16: dQ 430 us (960 TFLOP/s of
-// its three products), dK and dV 640 (860 of four), bound by the matrix units
+// 8192 causal rows, 16 heads on 4 of width 128, bf16: dQ 434 us (950 TFLOP/s of
+// its three products), dK and dV 565 (970 of four), bound by the matrix units
 // and the exponentials between the products. Packed texts of 20 to 510 tokens,
-// 12 heads of width 64: 50 and 51 us.
+// 12 heads of width 64: 49 and 46 us.
 //
 // P and dS are rounded to the tensors' type for the products they enter (dS of
 // masked tiles to twice its bits in dQ).

@@ -20,12 +20,12 @@
 // head within the group, so keys and values are staged once for the group.
 //
 // Long walks are bound by the matrix units and the exponentials between their
-// products: 8192 causal rows, 16 heads on 4 of width 128, bf16, take 330 us
-// (833 TFLOP/s of what the mask leaves; a large library product reaches 1320),
-// 4 causal texts of 1900 to 4099 rows with a prefix and capped scores 375 (410
-// TFLOP/s: the cap's exponential and reciprocal come on top). Packed texts of 20 to 510 tokens, 12
-// heads of width 64, take 33 us: their walks are a few tiles long, so that the
-// way to the first tile and the longest documents count.
+// products: 8192 causal rows, 16 heads on 4 of width 128, bf16, take 304 us
+// (905 TFLOP/s of what the mask leaves; a large library product reaches 1320),
+// 4 causal texts of 1900 to 4099 rows with a prefix and capped scores 318 (485
+// TFLOP/s: the cap's exponential and reciprocal come on top). Packed texts of
+// 20 to 510 tokens, 12 heads of width 64, take 31 us: their walks are a few
+// tiles long, so that the way to the first tile and the longest documents count.
 #include "kdec_attn.hpp"
 
 namespace kdec {
@@ -307,7 +307,7 @@ __global__ __launch_bounds__(AT, sizeof(T) == 2 ? (FOUR ? 4 : DP == 64 ? 3 : 2) 
 // from memory into the product's registers, values through the wave's own
 // shared memory for their transpose, so no wave waits for another. Bound by
 // memory: 48 requests over caches of up to 4096 tokens, 16 heads on 4 of width
-// 128, bf16, take 50 us for 206 MB (4.1 TB/s; a large copy 4.7); one request
+// 128, bf16, take 48 us for 206 MB (4.3 TB/s; a large copy 4.7); one request
 // over 6000 tokens of 12 heads of width 64 in float takes 21 us for 37 MB, most
 // of it the offsets', the first keys' and the join's latency.
 template <class T, int DP, int CAP, bool BIAS>

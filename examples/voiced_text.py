@@ -90,7 +90,7 @@ class TextBlock:
 
     def step(self, x, voice, cache, filled, slot):
         """One new token (x: a row per utterance) over the (utterances * slot, 2, heads, head) cache, of which
-        ``filled`` holds how many tokens of every slot there are; they become one more."""
+        ``filled`` holds how many tokens of every slot there are, fewer than `slot`; they become one more."""
         n = x.shape[0]
         q, k, v = self._split(self._qkv(x, voice))
         at = torch.arange(n, device=x.device) * slot + filled

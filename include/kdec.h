@@ -432,11 +432,16 @@ int kdec_length_regulate(kdec_ctx* ctx, const float* t_en, long te_bs,
  * each have adapters of their own. They have no counterpart on the
  * reference's path. Tensors are FP32 or bf16 (`dtype`, one type for all of a
  * call's tensors unless noted), sums and softmax statistics are float, and
- * each output is rounded once. Rows are tokens; a row stride (`_rs`, in
- * elements) is the distance of two tokens, a head stride (`_hs`) that of two
- * heads; the innermost axis is contiguous. Any alignment and any stride is
- * taken; tensors whose base, strides and widths are multiples of 16 bytes
- * take the wide loads. Offsets and adapter choices are int32 on the device.
+ * each output is rounded once. Besides, bf16 calls round to bf16 what enters a
+ * matrix product: attention's probabilities (for O and dV) and dS (for dK and
+ * dQ; in dQ to 16 bits where a tile is masked); the adapters' H and dH enter Y
+ * and dX to 16 bits, dA and dB to 24. Float calls round nothing on the way.
+ * Rows are tokens; a row stride (`_rs`, in elements) is the distance of two
+ * tokens, a head stride (`_hs`) that of two heads; the innermost axis is
+ * contiguous. Inputs take any alignment and any stride; tensors whose base,
+ * strides and widths are multiples of 16 bytes take the wide loads. Offsets and
+ * adapter choices are int32 on the device. The rows of an output must not
+ * overlap.
  * Outputs must not overlap inputs unless noted.
  */
 #define KDEC_F32 0
