@@ -4,6 +4,7 @@
 
 #include <climits>
 #include <cmath>
+#include <cstdlib>
 #include <memory>
 #include <type_traits>
 
@@ -385,6 +386,12 @@ inline int check(kdec_ctx* ctx, const char* who, int dtype, const void* q_off, c
     if (!(cap >= 0.0f) || !(cap < HUGE_VALF)) return bad("cap must be at least 0");
     if (docs > 0 && (!q_off || !k_off)) return bad("null offsets");
     return KDEC_OK;
+}
+
+// Whether an output's rows and heads can lie apart (none repeated, no steps
+// shorter than a row).
+inline bool apart(long rs, long hs, long rows, int heads, int D) {
+    return (rows <= 1 || std::labs(rs) >= D) && (heads == 1 || std::labs(hs) >= D);
 }
 
 // Whether a tensor's rows and heads start on multiples of `to` bytes.

@@ -580,6 +580,8 @@ extern "C" int kdec_attn_bwd(kdec_ctx* ctx, int dtype, const void* Q, long q_rs,
     if (int rc = check(ctx, "kdec_attn_bwd", dtype, q_off, k_off, docs, scale, cap, Tq, Tk, Hq, Hkv, D)) return rc;
     KDEC_CHECK(ctx, (Tq == 0 || (Q && O && lse && dO && dQ)) && (Tk == 0 || (K && V && dK && dV)),
                "kdec_attn_bwd: null tensor");
+    KDEC_CHECK(ctx, apart(dq_rs, dq_hs, Tq, Hq, D) && apart(dk_rs, dk_hs, Tk, Hkv, D) && apart(dv_rs, dv_hs, Tk, Hkv, D),
+               "kdec_attn_bwd: rows of a gradient overlap");
     if (Tq == 0 && Tk == 0) return KDEC_OK;
     const size_t size = dtype == KDEC_F32 ? 4 : 2;
     const int G = Hq / Hkv;

@@ -510,6 +510,7 @@ extern "C" int kdec_attn_fwd(kdec_ctx* ctx, int dtype, const void* Q, long q_rs,
     if (int rc = check(ctx, "kdec_attn_fwd", dtype, q_off, k_off, docs, scale, cap, Tq, Tk, Hq, Hkv, D)) return rc;
     if (Tq == 0) return KDEC_OK;
     KDEC_CHECK(ctx, Q && O && lse && (Tk == 0 || (K && V)), "kdec_attn_fwd: null tensor");
+    KDEC_CHECK(ctx, apart(o_rs, o_hs, Tq, Hq, D), "kdec_attn_fwd: rows of O overlap");
     const size_t size = dtype == KDEC_F32 ? 4 : 2;
     const int G = Hq / Hkv;
     ProfScope ps(ctx, "attn", 0.0, 0.0);

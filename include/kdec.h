@@ -441,8 +441,7 @@ int kdec_length_regulate(kdec_ctx* ctx, const float* t_en, long te_bs,
  * contiguous. Inputs take any alignment and any stride; tensors whose base,
  * strides and widths are multiples of 16 bytes take the wide loads. Offsets and
  * adapter choices are int32 on the device. The rows of an output must not
- * overlap.
- * Outputs must not overlap inputs unless noted.
+ * overlap (repeated ones are refused), nor outputs inputs unless noted.
  */
 #define KDEC_F32 0
 #define KDEC_BF16 1
