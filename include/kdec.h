@@ -434,7 +434,8 @@ int kdec_length_regulate(kdec_ctx* ctx, const float* t_en, long te_bs,
  * call's tensors unless noted), sums and softmax statistics are float, and
  * each output is rounded once. Besides, bf16 calls round to bf16 what enters a
  * matrix product: attention's probabilities (for O and dV) and dS (for dK and
- * dQ; in dQ to 16 bits where a tile is masked); the adapters' H and dH enter Y
+ * dQ; in dQ to 16 bits where a tile is masked), and dQ takes dO . O from the
+ * rounded O (dK from the exact sums); the adapters' H and dH enter Y
  * and dX to 16 bits, dA and dB to 24. Float calls round nothing on the way.
  * Rows are tokens; a row stride (`_rs`, in elements) is the distance of two
  * tokens, a head stride (`_hs`) that of two heads; the innermost axis is
