@@ -48,6 +48,9 @@ struct Args {
     bool by_doc;           // blocks of entries end with their document
 };
 
+// Bytes that a token takes in one head of a cache of 8-bit codes.
+__host__ __device__ constexpr int code_width(int D) { return (D + 15) & ~15; }
+
 struct Row {
     int lo, hi, pos;  // keys [lo, hi), the key row at the row's own position
 };
@@ -85,24 +88,29 @@ __device__ inline Row row_in(const Docs& m, int d, int i) {
     return Row{c.k0, c.k0 + n, c.k0 + p};
 }
 
-// The keys of every lane's row i, `first` the least of the wave's rows (all
-// lanes take part). The wave reads 64 offsets at once, from the document of
-// its first row, and each lane finds its own among them; only rows past 64
-// documents (most of them empty, then) search memory.
-__device__ inline Row row_at(const Docs& m, int i, int first) {
+// The document of every lane's row i, or -1; `first` is the least of the wave's
+// rows (all lanes take part). The wave reads 64 offsets at once, from the
+// document of its first row, and each lane finds its own among them; only rows
+// past 64 documents (most of them empty, then) search memory.
+__device__ inline int doc_of_row(const int* q_off, int docs, int i, int first) {
     const int lane = threadIdx.x & 63;
-    if (m.docs <= 0) return Row{INT_MAX, INT_MIN, 0};
+    if (docs <= 0) return -1;
     int d0 = 0;
-    if (m.docs > 64) d0 = max(doc_of(m.q_off, m.docs, __builtin_amdgcn_readfirstlane(first)), 0);
-    const int off = d0 + lane <= m.docs ? m.q_off[d0 + lane] : INT_MAX;
+    if (docs > 64) d0 = max(doc_of(q_off, docs, __builtin_amdgcn_readfirstlane(first)), 0);
+    const int off = d0 + lane <= docs ? q_off[d0 + lane] : INT_MAX;
     int n = 0;  // how many of the 64 are not past i
 #pragma unroll
     for (int s = 32; s; s >>= 1) n += __shfl(off, n + s - 1) <= i ? s : 0;
     n += __shfl(off, min(n, 63)) <= i;
     int d = d0 + n - 1;
-    if (n == 64) d = doc_of(m.q_off, m.docs, i);
-    if (d < 0 || d >= m.docs || i >= m.q_off[d + 1]) return Row{INT_MAX, INT_MIN, 0};
-    return row_in(m, d, i);
+    if (n == 64) d = doc_of(q_off, docs, i);
+    return d < 0 || d >= docs || i >= q_off[d + 1] ? -1 : d;
+}
+
+// The keys of every lane's row i, `first` the least of the wave's rows.
+__device__ inline Row row_at(const Docs& m, int i, int first) {
+    const int d = doc_of_row(m.q_off, m.docs, i, first);
+    return d < 0 ? Row{INT_MAX, INT_MIN, 0} : row_in(m, d, i);
 }
 
 // Blocks that end with their document. Documents, and the rows before the
@@ -317,6 +325,69 @@ __device__ inline float grad_p(const Score<T, CAP, BIAS>& rule, float s, float d
     return __builtin_amdgcn_exp2f(rule.of(s, dist, dt) - lse2);
 }
 
+// Running softmax state of one lane's column, in the units of m: raw products
+// (times `unit` they are log2) without cap and bias, log2 with either.
+struct Soft {
+    float m = -INF, l = 0.0f;
+};
+
+// One step of the running softmax of a lane's column over N score blocks of
+// 32 keys from j0 (whole: all of the wave's rows see all of them). Scores
+// become probabilities; acc is rescaled when the wave's maxima move far enough.
+template <bool MASKED, class T, int CAP, bool BIAS, int N, int ND>
+__device__ inline void soft_step(const Score<T, CAP, BIAS>& rule, const Row& row, bool whole, int j0, int half,
+                                 f32x16 (&s)[N], f32x16 (&acc)[ND], Soft& st) {
+    constexpr bool RAW = !CAP && !BIAS;
+    const float unit = RAW ? rule.unit : 1.0f;
+    const float dist = static_cast<float>(row.pos - j0 - 4 * half);
+#pragma unroll
+    for (int n = 0; n < N; ++n)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            float t = s[n][r], dt;
+            if (!RAW) t = rule.of(t, dist - static_cast<float>(32 * n + acc_row(r, 0)), dt);
+            s[n][r] = t;
+        }
+    if (MASKED && !whole) {
+        const unsigned at = static_cast<unsigned>(j0 + 4 * half - row.lo);  // seen: at + key's place < len
+        const unsigned len = row.hi > row.lo ? static_cast<unsigned>(row.hi - row.lo) : 0u;
+#pragma unroll
+        for (int n = 0; n < N; ++n)
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+                s[n][r] = at + static_cast<unsigned>(32 * n + acc_row(r, 0)) < len ? s[n][r] : -INF;
+        asm volatile("");  // a branch
+    }
+    float mx = -INF;
+#pragma unroll
+    for (int n = 0; n < N; ++n)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[n][r]);
+    mx = max32(mx);
+    if (__builtin_amdgcn_ballot_w64((mx - st.m) * unit > 8.0f || (st.m == -INF && mx > -INF))) {
+        const float m = fmaxf(st.m, mx);
+        const float f = __builtin_amdgcn_exp2f((st.m - (m == -INF ? 0.0f : m)) * unit);
+        st.l *= f;
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) acc[d][r] *= f;
+        st.m = m;
+        asm volatile("");  // a branch, not sixty-four selects
+    }
+    const float m0 = (st.m == -INF ? 0.0f : st.m) * unit;
+    float sum = 0.0f;
+#pragma unroll
+    for (int n = 0; n < N; ++n)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            const float p = __builtin_amdgcn_exp2f(RAW ? __builtin_fmaf(s[n][r], unit, -m0) : s[n][r] - m0);
+            s[n][r] = p;
+            sum += p;
+        }
+    st.l += sum;
+}
+
 // ─── host ───
 
 // Whether blocks of `size` entries (or keys) end with their document. Else
@@ -397,6 +468,18 @@ inline bool apart(long rs, long hs, long rows, int heads, int D) {
 // Whether a tensor's rows and heads start on multiples of `to` bytes.
 inline bool aligned(const Heads& h, size_t size, size_t to) {
     return reinterpret_cast<size_t>(h.p) % to == 0 && (h.rs * size) % to == 0 && (h.hs * size) % to == 0;
+}
+// A cache of 8-bit codes: its tensors have to be what the kernels' loads take
+// (16 bytes of a row at once, a tile's offsets below 2^30).
+inline int check_codes(kdec_ctx* ctx, const char* who, const Heads& k, const Heads& v, const float* ks, const float* vs, int Tk, int H,
+                       int D) {
+    const auto bad = [&](const char* why) { return fail(ctx, KDEC_EINVAL, std::string(who) + ": " + why); };
+    if (Tk > 0 && !(k.p && v.p && ks && vs)) return bad("null cache");
+    for (const Heads* h : {&k, &v}) {
+        if (!aligned(*h, 1, 16)) return bad("the cache's rows and heads must start on multiples of 16 bytes");
+        if (h->rs < 0 || h->rs >= (1L << 24) || h->hs < 0) return bad("the cache's strides are outside what the kernels take");
+    }
+    return KDEC_OK;
 }
 // Whether the kernels' loads take a tensor as it stands: 16 bytes at a time,
 // a tile's offsets below 2^30 bytes.

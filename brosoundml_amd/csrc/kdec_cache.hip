@@ -1,0 +1,175 @@
+// A key and value cache in 8 bits on gfx950: written as its tokens come, read
+// back as floats. The attention over it is kdec_attn_cache.hip.
+//
+// A token's values in one head share a scale, s = max(max |x| / 127, 2^-126) in
+// float, and are held as the integers nearest to x / s. Nearest is decided
+// exactly (the product with 1 / s may be one off near a half, the remainder
+// x - q s is exact and says so; ties go to the even integer), so the codes are
+// those of the definition on every machine. A token with a value that is not
+// finite gets the scale NaN and codes of zero.
+//
+// 8 or 16 lanes take the values of a token in a head, eight each; bound by
+// memory, or for single tokens by the launch and three dependent loads.
+#include "kdec_attn.hpp"
+
+namespace kdec {
+namespace {
+
+using attn::Docs;
+using attn::Heads;
+
+constexpr int CT = 256;
+typedef signed char i8x8 __attribute__((ext_vector_type(8)));
+
+struct Codes {
+    signed char *k, *v;
+    long k_rs, k_hs, v_rs, v_hs;  // bytes
+    float *ks, *vs;               // (heads, rows)
+};
+
+// The cache row of query row i, or -1: the document's last row is its last
+// filled key.
+__device__ inline long cache_row(const Docs& m, int i, int first) {
+    const int d = attn::doc_of_row(m.q_off, m.docs, min(i, m.Tq - 1), first);
+    if (d < 0 || i >= m.Tq) return -1;
+    const attn::Doc c = attn::doc_at(m, d);
+    const int p = i - c.q0 + c.lk - c.lq;
+    return p < 0 ? -1 : static_cast<long>(c.k0) + p;
+}
+
+__device__ inline int nearest(float x, float s, float inv) {
+    float q = rintf(x * inv);
+    const float r = __builtin_fmaf(-q, s, x), r2 = 2.0f * __builtin_fabsf(r);
+    const bool odd = static_cast<int>(q) & 1;
+    if (r2 > s || (r2 == s && odd)) q += r > 0.0f ? 1.0f : -1.0f;
+    return static_cast<int>(q);
+}
+
+template <class T, int L>
+__global__ __launch_bounds__(CT) void cache_write_k(Docs m, Heads K, Heads V, Codes o, int H, int D, int W, bool vec) {
+    const int per = CT / L, lane = threadIdx.x % L, row = blockIdx.x * per + threadIdx.x / L;
+    const int head = blockIdx.y % H, c = 8 * lane, n = max(min(8, D - c), 0);
+    const bool keys = static_cast<int>(blockIdx.y) < H;
+    const long at = cache_row(m, row, __builtin_amdgcn_readfirstlane(row));
+    const Heads& h = keys ? K : V;
+    const T* p = static_cast<const T*>(h.p) + min(row, m.Tq - 1) * h.rs + head * h.hs + c;
+    const Frag<T> f = load8(p, at < 0 ? 0 : n, vec);
+    float x[8], top = 0.0f, zero = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        x[i] = static_cast<float>(f[i]);
+        top = fmaxf(top, __builtin_fabsf(x[i]));
+        zero = __builtin_fmaf(x[i], 0.0f, zero);
+    }
+#pragma unroll
+    for (int s = 1; s < L; s *= 2) {
+        top = fmaxf(top, __shfl_xor(top, s));
+        zero += __shfl_xor(zero, s);
+    }
+    const bool bad = !(zero == 0.0f);
+    const float s = bad ? __builtin_nanf("") : fmaxf(top / 127.0f, 0x1p-126f), inv = 1.0f / s;
+    if (at < 0) return;
+    i8x8 q;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) q[i] = static_cast<signed char>(bad ? 0 : nearest(x[i], s, inv));
+    signed char* to = (keys ? o.k + at * o.k_rs + head * o.k_hs : o.v + at * o.v_rs + head * o.v_hs) + c;
+    if (c < W) *reinterpret_cast<i8x8*>(to) = q;
+    if (lane == 0) (keys ? o.ks : o.vs)[static_cast<long>(head) * m.Tk + at] = s;
+}
+
+template <class T, int L>
+__global__ __launch_bounds__(CT) void cache_read_k(Docs m, Codes o, int H, int D, int W, T* K, long k_rs, long k_hs, T* V, long v_rs,
+                                                   long v_hs, bool vec) {
+    const int per = CT / L, lane = threadIdx.x % L, row = blockIdx.x * per + threadIdx.x / L;
+    const int head = blockIdx.y % H, c = 8 * lane, n = max(min(8, D - c), 0);
+    const bool keys = static_cast<int>(blockIdx.y) < H;
+    const long at = cache_row(m, row, __builtin_amdgcn_readfirstlane(row));
+    if (row >= m.Tq) return;
+    i8x8 q = i8x8{};
+    float s = 0.0f;
+    if (at >= 0) {
+        const signed char* from = (keys ? o.k + at * o.k_rs + head * o.k_hs : o.v + at * o.v_rs + head * o.v_hs) + c;
+        if (c < W) q = *reinterpret_cast<const i8x8*>(from);
+        s = (keys ? o.ks : o.vs)[static_cast<long>(head) * m.Tk + at];
+    }
+    T* to = (keys ? K + row * k_rs + head * k_hs : V + row * v_rs + head * v_hs) + c;
+    Frag<T> f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = static_cast<T>(s * static_cast<float>(q[i]));
+    if (vec) {
+        if (n > 0) *reinterpret_cast<Frag<T>*>(to) = f;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (i < n) to[i] = f[i];
+    }
+}
+
+// Whether eight elements of a tensor's rows can be moved at once.
+bool wide(const Heads& h, int D, int es) { return D % 8 == 0 && attn::aligned(h, es, 16); }
+
+int check(kdec_ctx* ctx, const char* who, int dtype, const void* q_off, const void* k_off, int docs, int Tq, int Tk, int H, int D,
+          const Codes& o) {
+    if (int rc = attn::check(ctx, who, dtype, q_off, k_off, docs, 1.0f, 0.0f, Tq, Tk, H, H, D)) return rc;
+    return attn::check_codes(ctx, who, {o.k, o.k_rs, o.k_hs}, {o.v, o.v_rs, o.v_hs}, o.ks, o.vs, Tk, H, D);
+}
+
+}  // namespace
+}  // namespace kdec
+
+using namespace kdec;
+
+extern "C" {
+
+int kdec_cache_write(kdec_ctx* ctx, int dtype, const void* K, long k_rs, long k_hs, const void* V, long v_rs, long v_hs,
+                     const int* q_off, const int* k_off, const int* k_len, int docs, int Tq, int Tk, int H, int D, void* Kc, long kc_rs,
+                     long kc_hs, void* Vc, long vc_rs, long vc_hs, float* k_scale, float* v_scale) {
+    if (!ctx) return KDEC_EINVAL;
+    const Codes o{static_cast<signed char*>(Kc), static_cast<signed char*>(Vc), kc_rs, kc_hs, vc_rs, vc_hs, k_scale, v_scale};
+    if (int rc = check(ctx, "kdec_cache_write", dtype, q_off, k_off, docs, Tq, Tk, H, D, o)) return rc;
+    const int W = attn::code_width(D);
+    KDEC_CHECK(ctx, attn::apart(kc_rs, kc_hs, Tk, H, W) && attn::apart(vc_rs, vc_hs, Tk, H, W), "kdec_cache_write: rows of the cache overlap");
+    if (Tq == 0 || Tk == 0 || docs == 0) return KDEC_OK;
+    KDEC_CHECK(ctx, K && V, "kdec_cache_write: null tensor");
+    const int es = dtype == KDEC_F32 ? 4 : 2;
+    const Docs m{q_off, k_off, k_len, nullptr, docs, 0, Tq, Tk};
+    const Heads k{K, k_rs, k_hs}, v{V, v_rs, v_hs};
+    const bool vec = wide(k, D, es) && wide(v, D, es);
+    ProfScope ps(ctx, "cache", 0.0, 2.0 * Tq * H * (static_cast<double>(es) * D + W + 4));
+    const int L = W <= 64 ? 8 : 16;
+    const dim3 grid(static_cast<unsigned>(cdiv(Tq, CT / L)), static_cast<unsigned>(2 * H));
+    KDEC_CHECK(ctx, 2L * H <= 65535, "kdec_cache_write: too many heads");
+    const auto run = [&](auto k_) { hipLaunchKernelGGL(k_, grid, dim3(CT), 0, ctx->stream, m, k, v, o, H, D, W, vec); };
+    if (dtype == KDEC_F32) run(L == 8 ? cache_write_k<float, 8> : cache_write_k<float, 16>);
+    else run(L == 8 ? cache_write_k<bf16, 8> : cache_write_k<bf16, 16>);
+    return launch_check(ctx, "kdec_cache_write");
+}
+
+int kdec_cache_read(kdec_ctx* ctx, int dtype, const void* Kc, long kc_rs, long kc_hs, const void* Vc, long vc_rs, long vc_hs,
+                    const float* k_scale, const float* v_scale, const int* q_off, const int* k_off, const int* k_len, int docs, int Tq,
+                    int Tk, int H, int D, void* K, long k_rs, long k_hs, void* V, long v_rs, long v_hs) {
+    if (!ctx) return KDEC_EINVAL;
+    const auto bytes = [](const void* p) { return static_cast<signed char*>(const_cast<void*>(p)); };
+    const Codes o{bytes(Kc), bytes(Vc), kc_rs, kc_hs, vc_rs, vc_hs, const_cast<float*>(k_scale), const_cast<float*>(v_scale)};
+    if (int rc = check(ctx, "kdec_cache_read", dtype, q_off, k_off, docs, Tq, Tk, H, D, o)) return rc;
+    if (Tq == 0) return KDEC_OK;
+    KDEC_CHECK(ctx, K && V, "kdec_cache_read: null tensor");
+    KDEC_CHECK(ctx, attn::apart(k_rs, k_hs, Tq, H, D) && attn::apart(v_rs, v_hs, Tq, H, D), "kdec_cache_read: rows of an output overlap");
+    const int es = dtype == KDEC_F32 ? 4 : 2, W = attn::code_width(D);
+    const Docs m{q_off, k_off, k_len, nullptr, docs, 0, Tq, Tk};
+    const bool vec = wide({K, k_rs, k_hs}, D, es) && wide({V, v_rs, v_hs}, D, es);
+    ProfScope ps(ctx, "cache", 0.0, 2.0 * Tq * H * (static_cast<double>(es) * D + W + 4));
+    const int L = W <= 64 ? 8 : 16;
+    const dim3 grid(static_cast<unsigned>(cdiv(Tq, CT / L)), static_cast<unsigned>(2 * H));
+    KDEC_CHECK(ctx, 2L * H <= 65535, "kdec_cache_read: too many heads");
+    const auto run = [&](auto k_, auto ty) {
+        typedef decltype(ty) E;
+        hipLaunchKernelGGL(k_, grid, dim3(CT), 0, ctx->stream, m, o, H, D, W, static_cast<E*>(K), k_rs, k_hs, static_cast<E*>(V), v_rs, v_hs,
+                           vec);
+    };
+    if (dtype == KDEC_F32) run(L == 8 ? cache_read_k<float, 8> : cache_read_k<float, 16>, 0.0f);
+    else run(L == 8 ? cache_read_k<bf16, 8> : cache_read_k<bf16, 16>, bf16{});
+    return launch_check(ctx, "kdec_cache_read");
+}
+
+}  // extern "C"

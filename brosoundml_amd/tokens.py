@@ -1,6 +1,7 @@
-"""Token operators on torch tensors: attention over packed documents, the
-projection with low-rank adapters chosen per row, and dropout (the last
-section of kdec.h). Each call checks its tensors, allocates what it returns
+"""Token operators on torch tensors: attention over packed documents and over
+a cache in 8 bits, the projection with low-rank adapters chosen per row,
+dropout, embedding, and the norms around a block with gate and residual (the
+last section of kdec.h). Each call checks its tensors, allocates what it returns
 and makes one C ABI call on the context's stream; nothing synchronises. A
 tensor made on another stream has to be ordered before the context's by the
 caller, as for every call of the library.
@@ -14,6 +15,8 @@ offsets and adapter choices are int32 tensors there. Errors are
 ``native.KdecError`` (what the library refuses) and ``ValueError`` (tensors
 that do not fit each other)."""
 from __future__ import annotations
+
+from typing import NamedTuple
 
 import torch
 
@@ -254,3 +257,234 @@ def dropout(ctx: Context, x, p, seed, offset=0, *, residual=None, out=None):
         R = _rows(residual, "residual")
     ctx.call("kdec_dropout", dt, *X, *R, *_rows(y, "out"), x.shape[0], x.shape[1], p, seed, offset)
     return y
+
+
+def embedding(ctx: Context, table, ids, *, scale=1.0, out=None):
+    """scale * table[ids] (kdec_embed_fwd): table (vocab, columns), ids (T
+    int32); an id outside the table gives a row of zeros."""
+    dt = _dtype(ctx, table)
+    W = _rows(table, "table")
+    vocab, cols = table.shape
+    if ids.dim() != 1:
+        _fail("ids must be (T)")
+    t = ids.shape[0]
+    I = _ints(ctx, ids, t, "ids")
+    y = _empty(ctx, table, (t, cols)) if out is None else out
+    if out is not None:
+        _dtype(ctx, table, y)
+        if y.shape != (t, cols):
+            _fail("out must be (T, columns)")
+    ctx.call("kdec_embed_fwd", dt, *W, I, t, vocab, cols, float(scale), *_rows(y, "out"))
+    return y
+
+
+def embedding_bwd(ctx: Context, ids, dy, vocab, *, scale=1.0, dtable=None, beta=0.0):
+    """The gradient of ``embedding``'s table from ``dy`` (kdec_embed_bwd), float
+    (vocab, columns): beta times what ``dtable`` held, where it is given, plus
+    scale times the sum of every id's rows, in one order."""
+    dt = _dtype(ctx, dy)
+    Y = _rows(dy, "dy")
+    t, cols = dy.shape
+    if ids.dim() != 1:
+        _fail("ids must be (T)")
+    I = _ints(ctx, ids, t, "ids")
+    if not (beta == 0.0 or dtable is not None):
+        _fail("beta without dtable to add to")
+    g = _empty(ctx, dy, (vocab, cols), torch.float32) if dtable is None else dtable
+    ctx.call("kdec_embed_bwd", dt, *Y, I, t, vocab, cols, float(scale), _floats(ctx, g, (vocab, cols), "dtable"), float(beta))
+    return g
+
+
+def _norm_args(ctx, x, z, gate, post, pre, kind, eps, scale, x_scale):
+    dt = _dtype(ctx, x)
+    X = _rows(x, "x")
+    t, c = x.shape
+    if kind not in ("rms", "layer"):
+        _fail("kind must be 'rms' or 'layer'")
+
+    def rows(v, what):
+        if v is None:
+            return None, 0
+        _dtype(ctx, x, v)
+        if v.shape != x.shape:
+            _fail(f"{what} must be as x")
+        return _rows(v, what)
+
+    def norm(wb, what):
+        if wb is None:
+            return 0, None, None
+        if not isinstance(wb, (tuple, list)):
+            wb = (wb, None)
+        if len(wb) != 2:
+            _fail(f"{what} must be a weight or (weight, bias)")
+        for v in wb:
+            if v is not None:
+                _dtype(ctx, x, v)
+                _whole(v, (c,), what)
+        return (1, *(None if v is None else v.data_ptr() for v in wb))
+
+    if gate is not None and gate.dim() == 1:
+        _dtype(ctx, x, gate)
+        G = _whole(gate, (c,), "gate"), 0
+    else:
+        G = rows(gate, "gate")
+        if gate is not None and G[1] == 0:  # which the C ABI takes for one gate for all rows
+            if t > 1:
+                _fail("one gate for all rows must be (columns)")
+            G = G[0], c
+    if z is None and (post is not None or gate is not None or x_scale != 1.0 or pre is None):
+        _fail("without z there is the norm of x alone")
+    args = (dt, int(kind == "layer"), *X, *rows(z, "z"), *G, *norm(post, "post"), *norm(pre, "pre"), float(eps), float(scale), float(x_scale),
+            t, c)
+    return args, rows
+
+
+def residual_norm(ctx: Context, x, z=None, *, gate=None, post=None, pre=None, kind="rms", eps=1e-5, scale=1.0, x_scale=1.0, keep=False,
+                  out=None):
+    """What stands between two blocks, in one pass (kdec_resnorm_fwd): the
+    block's output z (T, C) through its norm ``post``, its ``gate`` ((C), or
+    (T, C) with a gate for each row) and ``scale`` onto the residual x, and the
+    next block's norm ``pre``:
+
+        r = x_scale x + scale gate N_post(z),   y = N_pre(r)
+
+    ``post`` and ``pre`` are None (no norm), a weight, or (weight, bias) of
+    which either may be None; ``kind`` is "rms" or "layer". Without z it is y =
+    N_pre(x), and r is x. ``out`` may give r and y, (r, y). Returns (r, y), y
+    None without ``pre``, and with ``keep`` also the statistics that the
+    backward takes."""
+    args, rows = _norm_args(ctx, x, z, gate, post, pre, kind, eps, scale, x_scale)
+    t, c = x.shape
+    r, y = out if out is not None else (None, None)
+    if z is None:
+        r = x
+    elif r is None:
+        r = _empty(ctx, x, (t, c))
+    if pre is None:
+        y = None
+    elif y is None:
+        y = _empty(ctx, x, (t, c))
+    stats = _empty(ctx, x, (t, 4), torch.float32) if keep else None
+    R = (None, 0) if z is None else rows(r, "r")
+    ctx.call("kdec_resnorm_fwd", *args, *R, *rows(y, "y"), None if stats is None else stats.data_ptr())
+    return (r, y, stats) if keep else (r, y)
+
+
+def residual_norm_bwd(ctx: Context, x, z, dr, dy, stats, *, gate=None, post=None, pre=None, kind="rms", eps=1e-5, scale=1.0, x_scale=1.0):
+    """The gradients (dx, dz, dgate, dpost, dpre) of ``residual_norm`` from
+    those of r (None: none) and y, with its inputs, arguments and statistics
+    (kdec_resnorm_bwd). dx, dz and the gate's of each row are of x's type; the
+    gradients of (C) vectors are float, dpost and dpre (weight's, bias's) with
+    None where there is none."""
+    args, rows = _norm_args(ctx, x, z, gate, post, pre, kind, eps, scale, x_scale)
+    t, c = x.shape
+    if (dy is None) != (pre is None):
+        _fail("dy comes with pre")
+    st = _floats(ctx, stats, (t, 4), "stats")
+    DR, DY = rows(dr, "dr"), rows(dy, "dy")
+    new = lambda *s: _empty(ctx, x, s)  # noqa: E731
+    floats = lambda: _empty(ctx, x, (c,), torch.float32)  # noqa: E731
+    dx, dz = new(t, c), None if z is None else new(t, c)
+    dgate = None if gate is None else floats() if gate.dim() == 1 else new(t, c)
+
+    def grads(wb):
+        if wb is None:
+            return None
+        wb = wb if isinstance(wb, (tuple, list)) else (wb, None)
+        return tuple(None if v is None else floats() for v in wb)
+
+    dpost, dpre = grads(post), grads(pre)
+    at = lambda v: None if v is None else v.data_ptr()  # noqa: E731
+    ctx.call("kdec_resnorm_bwd", *args, st, *DR, *DY, at(dx), at(dz), at(dgate), *map(at, dpost or (None, None)), *map(at, dpre or (None, None)))
+    return dx, dz, dgate, dpost, dpre
+
+
+class Cache(NamedTuple):
+    """A key and value cache in 8 bits (kdec_cache_write): codes k and v (rows,
+    heads, width rounded up to 16), int8, and their scales (heads, rows), float."""
+    k: torch.Tensor
+    v: torch.Tensor
+    k_scale: torch.Tensor
+    v_scale: torch.Tensor
+
+
+def new_cache(ctx: Context, rows, heads, width):
+    """An empty ``Cache`` of `rows` tokens (of all requests' slots together)."""
+    with torch.cuda.stream(ctx.stream):
+        codes = torch.zeros(rows, 2, heads, (width + 15) // 16 * 16, dtype=torch.int8, device=f"cuda:{ctx.device}")
+        scales = torch.zeros(2, heads, rows, device=codes.device)
+    return Cache(codes[:, 0], codes[:, 1], scales[0], scales[1])
+
+
+def _cache_args(ctx, cache, width):
+    """Addresses and strides of a cache for the C ABI (codes, scales), its rows and heads."""
+    k, v = cache.k, cache.v
+    for t, what in ((k, "the cache's k"), (v, "the cache's v")):
+        if t.dtype != torch.int8 or t.get_device() != ctx.device:
+            _fail(f"{what} must be int8 on the device")
+    K, V = _heads(k, "the cache's k"), _heads(v, "the cache's v")
+    rows, heads, wide = k.shape
+    if v.shape != k.shape or wide != (width + 15) // 16 * 16:
+        _fail(f"the cache's k and v must be (rows, heads, {(width + 15) // 16 * 16})")
+    return K, V, (_floats(ctx, cache.k_scale, (heads, rows), "k_scale"), _floats(ctx, cache.v_scale, (heads, rows), "v_scale")), rows, heads
+
+
+def _places(ctx, q_off, k_off, k_len):
+    docs = q_off.numel() - 1
+    if docs < 0:
+        _fail("q_off must hold one offset more than there are documents")
+    return _ints(ctx, q_off, docs + 1, "q_off"), _ints(ctx, k_off, docs + 1, "k_off"), _ints(ctx, k_len, docs, "k_len"), docs
+
+
+def cache_write(ctx: Context, k, v, cache, q_off, k_off, k_len=None):
+    """Writes new tokens' k and v (T, heads, width) into ``cache``
+    (kdec_cache_write): the rows q_off[d]:q_off[d+1] become the last of the
+    k_len[d] filled tokens in the slot k_off[d]:k_off[d+1] (of the whole slot
+    without k_len), where ``cache_attention`` with the same arguments expects
+    them. Rows outside a document or before its slot are left out."""
+    dt = _dtype(ctx, k, v)
+    K, V = _heads(k, "k"), _heads(v, "v")
+    t, h, d = k.shape
+    Kc, Vc, scales, rows, heads = _cache_args(ctx, cache, d)
+    if v.shape != k.shape or heads != h:
+        _fail("k and v must share their shape, and the cache's heads")
+    ctx.call("kdec_cache_write", dt, *K, *V, *_places(ctx, q_off, k_off, k_len), t, rows, h, d, *Kc, *Vc, *scales)
+
+
+def cache_read(ctx: Context, cache, q_off, k_off, k_len=None, *, rows, width, dtype=torch.bfloat16, out=None):
+    """The tokens that ``cache_write`` with the same arguments wrote, as (k, v)
+    of `rows` rows: (rows, heads, width) of ``dtype`` (kdec_cache_read). Rows
+    that it would not have written are zeros."""
+    Kc, Vc, scales, tk, heads = _cache_args(ctx, cache, width)
+    if out is None:
+        k, v = (_empty(ctx, cache.k, (rows, heads, width), dtype) for _ in range(2))
+    else:
+        k, v = out
+    dt = _dtype(ctx, k, v)
+    if k.shape != (rows, heads, width) or v.shape != k.shape:
+        _fail("out must be two tensors (rows, heads, width)")
+    ctx.call("kdec_cache_read", dt, *Kc, *Vc, *scales, *_places(ctx, q_off, k_off, k_len), rows, tk, heads, width, *_heads(k, "k"),
+             *_heads(v, "v"))
+    return k, v
+
+
+def cache_attention(ctx: Context, q, cache, q_off, k_off, k_len=None, *, causal=False, prefix=None, scale=None, cap=0.0, slopes=None,
+                    out=None):
+    """``attention`` over a ``Cache`` (kdec_attn_cache_fwd): q (Tq, Hq, D) and
+    the documents' keys and values k_off, k_len in the cache, the same masks,
+    scores and results (o, lse). One row for a request or many."""
+    dt = _dtype(ctx, q)
+    Q = _heads(q, "q")
+    tq, hq, d = q.shape
+    Kc, Vc, scales, tk, hkv = _cache_args(ctx, cache, d)
+    qo, ko, kl, docs = _places(ctx, q_off, k_off, k_len)
+    o = _empty(ctx, q, q.shape) if out is None else out
+    if out is not None:
+        _dtype(ctx, q, o)
+        if o.shape != q.shape:
+            _fail("out must be as q")
+    lse = _empty(ctx, q, (hq, tq), torch.float32)
+    ctx.call("kdec_attn_cache_fwd", dt, *Q, *Kc, *Vc, *scales, qo, ko, kl, _ints(ctx, prefix, docs, "prefix"), docs, int(causal),
+             _floats(ctx, slopes, (hq,), "slopes"), float(d ** -0.5 if scale is None else scale), float(cap), tq, tk, hq, hkv, d,
+             *_heads(o, "out"), lse.data_ptr())
+    return o, lse

@@ -545,6 +545,90 @@ int kdec_adapter_bwd(kdec_ctx* ctx, int dtype, const void* X, long x_rs,
                      const float* H, const void* dY, long dy_rs, void* dX,
                      long dx_rs, float* dA, float* dB, float beta);
 
+/* Embedding: Y[t] = scale * table[ids[t]] (table (vocab, cols) at row stride
+ * t_rs, Y (T, cols) at y_rs); an id outside [0, vocab) gives a row of zeros. */
+int kdec_embed_fwd(kdec_ctx* ctx, int dtype, const void* table, long t_rs,
+                   const int* ids, int T, int vocab, int cols, float scale,
+                   void* Y, long y_rs);
+/* Its table's gradient, dtable (vocab, cols) floats:
+ *   dtable[v] = beta dtable[v] + scale sum_{t: ids[t] = v} dY[t]
+ * (beta = 0: overwritten, what it held is not read). Every sum has one order,
+ * the tokens sorted by id and cut into pieces: the same bits every time. */
+int kdec_embed_bwd(kdec_ctx* ctx, int dtype, const void* dY, long dy_rs,
+                   const int* ids, int T, int vocab, int cols, float scale,
+                   float* dtable, float beta);
+
+/* The norms before and after a block with its gate and residual, rows of C:
+ *   u = N_post(Z) if `post`, else Z;  R = x_scale X + scale gate u
+ *   Y = N_pre(R) if `pre`
+ * N(v) = v / sqrt(mean(v^2) + eps) * w + b, or where `layer` that of v less
+ * its mean; w1, b1 are N_post's (NULL: ones, zeros), w2, b2 N_pre's. gate is
+ * NULL (ones), a row for all (gate_rs 0) or a row each. Z may be NULL: then
+ * Y = N_pre(X) alone, without post, gate and R. stats (T, 4 floats, aligned to
+ * 16 bytes) is written when not NULL, for the backward. R enters N_pre before
+ * its rounding. R may be X or Z, and Y either of them. Sums are floats: squares
+ * past 2^127 overflow. C <= 8192, eps > 0. */
+int kdec_resnorm_fwd(kdec_ctx* ctx, int dtype, int layer, const void* X,
+                     long x_rs, const void* Z, long z_rs, const void* gate,
+                     long gate_rs, int post, const void* w1, const void* b1,
+                     int pre, const void* w2, const void* b2, float eps,
+                     float scale, float x_scale, int T, int C, void* R,
+                     long r_rs, void* Y, long y_rs, float* stats);
+/* Its backward from dR (NULL: none) and dY (with `pre`) and the forward's
+ * inputs and stats. dX, dZ (with Z) and, where each row has a gate of its own,
+ * dgate are (T, C) without gaps, of the tensors' type; the gradient of one row
+ * of gates for all, dw1, db1, dw2 and db2 (each may be NULL) are C floats,
+ * overwritten, their sums over the rows in one order. R is formed again from X
+ * and Z, so these must hold what the forward read. */
+int kdec_resnorm_bwd(kdec_ctx* ctx, int dtype, int layer, const void* X,
+                     long x_rs, const void* Z, long z_rs, const void* gate,
+                     long gate_rs, int post, const void* w1, const void* b1,
+                     int pre, const void* w2, const void* b2, float eps,
+                     float scale, float x_scale, int T, int C,
+                     const float* stats, const void* dR, long dr_rs,
+                     const void* dY, long dy_rs, void* dX, void* dZ,
+                     void* dgate, float* dw1, float* db1, float* dw2,
+                     float* db2);
+
+/* A key and value cache in 8 bits. A token's values in one head are held as
+ * integers: scale s = max(max|x| / 127, 2^-126) in float, codes x / s to the
+ * nearest, ties to even; a token with a value that is not finite has the scale
+ * NaN. Codes Kc, Vc: Tk rows of H heads, strides in bytes, each row of a head
+ * code_width = D rounded up to 16 bytes (those past D are written as zeros);
+ * base and strides are multiples of 16, a row stride is below 2^24. k_scale and
+ * v_scale: (H, Tk) floats.
+ *
+ * Writes the rows of K and V (Tq, H, D): document d's rows
+ * [q_off[d], q_off[d+1]) are the last of its k_len[d] filled keys in the slot
+ * [k_off[d], k_off[d+1]), as kdec_attn_fwd sees them. Rows that no document
+ * holds, or that lie before the slot's first key, are not written. */
+int kdec_cache_write(kdec_ctx* ctx, int dtype, const void* K, long k_rs,
+                     long k_hs, const void* V, long v_rs, long v_hs,
+                     const int* q_off, const int* k_off, const int* k_len,
+                     int docs, int Tq, int Tk, int H, int D, void* Kc,
+                     long kc_rs, long kc_hs, void* Vc, long vc_rs, long vc_hs,
+                     float* k_scale, float* v_scale);
+/* Reads them back: the rows that the same arguments wrote, scale times code,
+ * into K and V (Tq, H, D); zeros in rows that it would not have written. */
+int kdec_cache_read(kdec_ctx* ctx, int dtype, const void* Kc, long kc_rs,
+                    long kc_hs, const void* Vc, long vc_rs, long vc_hs,
+                    const float* k_scale, const float* v_scale,
+                    const int* q_off, const int* k_off, const int* k_len,
+                    int docs, int Tq, int Tk, int H, int D, void* K, long k_rs,
+                    long k_hs, void* V, long v_rs, long v_hs);
+/* kdec_attn_fwd over such a cache: the same documents, masks, scores and
+ * outputs, keys and values scale times code (Q, O of `dtype`). A row that sees
+ * a token whose key or value scale is not finite becomes NaN. */
+int kdec_attn_cache_fwd(kdec_ctx* ctx, int dtype, const void* Q, long q_rs,
+                        long q_hs, const void* Kc, long kc_rs, long kc_hs,
+                        const void* Vc, long vc_rs, long vc_hs,
+                        const float* k_scale, const float* v_scale,
+                        const int* q_off, const int* k_off, const int* k_len,
+                        const int* prefix, int docs, int causal,
+                        const float* slopes, float scale, float cap, int Tq,
+                        int Tk, int Hq, int Hkv, int D, void* O, long o_rs,
+                        long o_hs, float* lse);
+
 #ifdef __cplusplus
 }
 #endif
