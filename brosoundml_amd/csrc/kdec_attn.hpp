@@ -281,12 +281,13 @@ struct Score {
     float unit;   // product to log2 units
     float k, c2;  // cap: tanh's argument is s k / (2 log2 e), the score c2 tanh
     float slope;  // bias per step of distance, log2 units
-    __device__ inline Score(const Args& a, int head) {
+    __device__ inline explicit Score(const Args& a) {  // without a head's slope
         unit = a.scale * LOG2E;
         k = CAP ? 2.0f * LOG2E * a.scale / a.cap : 0.0f;
         c2 = a.cap * LOG2E;
-        slope = BIAS ? a.slopes[head] * LOG2E : 0.0f;
+        slope = 0.0f;
     }
+    __device__ inline Score(const Args& a, int head) : Score(a) { slope = BIAS ? a.slopes[head] * LOG2E : 0.0f; }
     __device__ inline float tanh_(float s) const {
         const float x2 = s * k;
         float th = __builtin_fmaf(-2.0f, __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x2)), 1.0f);
@@ -323,69 +324,6 @@ __device__ inline float grad_p(const Score<T, CAP, BIAS>& rule, float s, float d
         return __builtin_amdgcn_exp2f(__builtin_fmaf(s, rule.unit, -lse2));
     }
     return __builtin_amdgcn_exp2f(rule.of(s, dist, dt) - lse2);
-}
-
-// Running softmax state of one lane's column, in the units of m: raw products
-// (times `unit` they are log2) without cap and bias, log2 with either.
-struct Soft {
-    float m = -INF, l = 0.0f;
-};
-
-// One step of the running softmax of a lane's column over N score blocks of
-// 32 keys from j0 (whole: all of the wave's rows see all of them). Scores
-// become probabilities; acc is rescaled when the wave's maxima move far enough.
-template <bool MASKED, class T, int CAP, bool BIAS, int N, int ND>
-__device__ inline void soft_step(const Score<T, CAP, BIAS>& rule, const Row& row, bool whole, int j0, int half,
-                                 f32x16 (&s)[N], f32x16 (&acc)[ND], Soft& st) {
-    constexpr bool RAW = !CAP && !BIAS;
-    const float unit = RAW ? rule.unit : 1.0f;
-    const float dist = static_cast<float>(row.pos - j0 - 4 * half);
-#pragma unroll
-    for (int n = 0; n < N; ++n)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-            float t = s[n][r], dt;
-            if (!RAW) t = rule.of(t, dist - static_cast<float>(32 * n + acc_row(r, 0)), dt);
-            s[n][r] = t;
-        }
-    if (MASKED && !whole) {
-        const unsigned at = static_cast<unsigned>(j0 + 4 * half - row.lo);  // seen: at + key's place < len
-        const unsigned len = row.hi > row.lo ? static_cast<unsigned>(row.hi - row.lo) : 0u;
-#pragma unroll
-        for (int n = 0; n < N; ++n)
-#pragma unroll
-            for (int r = 0; r < 16; ++r)
-                s[n][r] = at + static_cast<unsigned>(32 * n + acc_row(r, 0)) < len ? s[n][r] : -INF;
-        asm volatile("");  // a branch
-    }
-    float mx = -INF;
-#pragma unroll
-    for (int n = 0; n < N; ++n)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[n][r]);
-    mx = max32(mx);
-    if (__builtin_amdgcn_ballot_w64((mx - st.m) * unit > 8.0f || (st.m == -INF && mx > -INF))) {
-        const float m = fmaxf(st.m, mx);
-        const float f = __builtin_amdgcn_exp2f((st.m - (m == -INF ? 0.0f : m)) * unit);
-        st.l *= f;
-#pragma unroll
-        for (int d = 0; d < ND; ++d)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) acc[d][r] *= f;
-        st.m = m;
-        asm volatile("");  // a branch, not sixty-four selects
-    }
-    const float m0 = (st.m == -INF ? 0.0f : st.m) * unit;
-    float sum = 0.0f;
-#pragma unroll
-    for (int n = 0; n < N; ++n)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-            const float p = __builtin_amdgcn_exp2f(RAW ? __builtin_fmaf(s[n][r], unit, -m0) : s[n][r] - m0);
-            s[n][r] = p;
-            sum += p;
-        }
-    st.l += sum;
 }
 
 // ─── host ───

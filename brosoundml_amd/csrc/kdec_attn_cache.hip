@@ -6,21 +6,23 @@
 // roundings are those of p vs (bf16 tensors); float tensors enter as three bf16
 // terms, which hold their 24 bits.
 //
-// A block holds 32 entries (rows of one document times the heads that share a
-// key head) and its four waves take tiles of 32 keys in turn, each with a
-// softmax state of its own, joined at the end; long caches are split over
-// blocks as well and joined by a second launch. Codes go from memory into the
-// products' registers, the next tile's on their way: a lane holds a key's half
-// row (depth slots stand for the lane's own bytes, the query's fragments
-// follow), and of the values ND neighbouring columns at a time, so that row m of
-// the output's block dt is column ND m + dt and no byte moves between lanes.
+// A block holds 16 or 32 entries (rows of one document times the heads that share
+// a key head) and its four waves take tiles of 32 keys in turn, each with a
+// softmax state of its own, joined at the end; long caches are split over blocks
+// as well and joined by a second launch. Codes go from memory into the products'
+// registers, the next tile's on their way. Depth slots and output rows stand for
+// whatever bytes a lane has: of a key 16 bytes in each 64, the query's fragments
+// following, and of a value ND neighbouring columns, so that row m of the
+// output's block dt is column ND m + dt and no byte moves between lanes.
 #include "kdec_attn.hpp"
 
 namespace kdec {
 namespace attn {
 namespace {
 
-constexpr int CN = 32;  // keys of a wave's tile, entries of a block
+constexpr int CN = 32;  // keys of a wave's tile
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
 
 struct Cached {
     Args a;  // K, V: bytes
@@ -29,35 +31,88 @@ struct Cached {
     long o_rs, o_hs;
     bool vec_o, vec_q;
     float* lse;
-    int rows, pieces;  // rows of a block; blocks that the heads of a row take (more than 32 of them)
+    int rows, pieces;  // rows of a block; blocks that the heads of a row take (where a block holds fewer)
     int splits;
     float *part_o, *part_ml;  // (splits, Hkv, E, DP) and (splits, Hkv, E, 2)
 };
 
-// Four signed bytes of each of two registers as bf16, exact.
-__device__ inline bf16 code(unsigned x, int i) {
-    return static_cast<bf16>(static_cast<float>(static_cast<signed char>(x >> (8 * i))));
+// Bytes i and j of two registers, signed numbers, as two bf16: a float of at most
+// eight bits is its upper half.
+__device__ inline unsigned codes2(unsigned x, int i, unsigned y, int j) {
+    const auto one = [](unsigned v, int b) { return __float_as_uint(static_cast<float>(static_cast<int>(v << (24 - 8 * b)) >> 24)); };
+    return __builtin_amdgcn_perm(one(y, j), one(x, i), 0x07060302);
 }
 
-typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
-template <int DP>
-struct Keys {
-    static constexpr int N = DP / 32;
-    u32x4 k[N];   // the lane's key: bytes DP / 2 * half ..
-    float scale;  // lanes below 32: the key's, above: the value's
-};
-struct Values {
-    unsigned v[16];  // columns ND * (lane % 32) .. of the keys 8 (i / 4) + 4 half + i % 4
-};
+__device__ inline f32x4 mma16(bf16x8 a, bf16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
 
-template <class T, int DP, int CAP, bool BIAS>
-__global__ __launch_bounds__(AT, sizeof(T) == 2 ? 2 : 1) void attn_cache_k(Cached p) {
-    constexpr int NC = DP / 16, ND = DP / 32, TERMS = sizeof(T) == 2 ? 1 : 3, PITCH = DP + 4;
-    __shared__ __align__(16) float so[4][CN][PITCH];
+// The larger of the values of the four lanes that share a column.
+__device__ inline float max_column(float x) {
+    const unsigned u = __float_as_uint(x);
+    const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+    const unsigned lo = r[0], hi = r[1];
+    return max32(fmaxf(__uint_as_float(lo), __uint_as_float(hi)));
+}
+
+// The document that holds a row, the same in all lanes, or -1.
+__device__ inline int doc_holding(const Docs& m, int row) {
+    const int lane = threadIdx.x & 63;
+    if (m.docs <= 0) return -1;
+    const int d0 = m.docs > 64 ? max(doc_of(m.q_off, m.docs, row), 0) : 0;
+    const int off = d0 + lane <= m.docs ? m.q_off[d0 + lane] : INT_MAX;
+    const int d = d0 + __builtin_popcountll(__builtin_amdgcn_ballot_w64(off <= row)) - 1;
+    return __builtin_amdgcn_readfirstlane(d >= 0 && d < m.docs && row < m.q_off[d + 1] ? d : -1);
+}
+
+// One step of the running softmax of a lane's column over the scores of 32 keys
+// from j0, `at` the lane's first: s become probabilities, acc is rescaled when
+// the wave's maxima move far enough. As soft_step of the float keys.
+struct Soft {
+    float m = -INF, l = 0.0f;
+};
+template <bool MASKED, class T, int CAP, bool BIAS, int ND>
+__device__ inline void cache_soft(const Score<T, CAP, BIAS>& rule, int pos, unsigned seen, int at, f32x4 (&s)[2], f32x4 (&acc)[ND], Soft& st) {
+    constexpr bool RAW = !CAP && !BIAS;
+    const float unit = RAW ? rule.unit : 1.0f, dist = static_cast<float>(pos - at);
+    float mx = -INF;
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            float t = s[b][r], dt;
+            if (!RAW) t = rule.of(t, dist - static_cast<float>(16 * b + r), dt);
+            if (MASKED) t = static_cast<unsigned>(at + 16 * b + r) < seen ? t : -INF;
+            s[b][r] = t;
+            mx = fmaxf(mx, t);
+        }
+    mx = max_column(mx);
+    if (__builtin_amdgcn_ballot_w64((mx - st.m) * unit > 8.0f || (st.m == -INF && mx > -INF))) {
+        const float m = fmaxf(st.m, mx), f = __builtin_amdgcn_exp2f((st.m - (m == -INF ? 0.0f : m)) * unit);
+        st.l *= f;
+#pragma unroll
+        for (int d = 0; d < ND; ++d) acc[d] *= f;
+        st.m = m;
+        asm volatile("");  // a branch
+    }
+    const float m0 = (st.m == -INF ? 0.0f : st.m) * unit;
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const float p = __builtin_amdgcn_exp2f(RAW ? __builtin_fmaf(s[b][r], unit, -m0) : s[b][r] - m0);
+            s[b][r] = p;
+            st.l += p;
+        }
+}
+
+// CB: blocks of 16 entries that a wave holds.
+template <class T, int DP, int CAP, bool BIAS, int CB>
+__global__ __launch_bounds__(AT, sizeof(T) == 2 ? (CB == 1 ? 3 : 2) : 1) void attn_cache_k(Cached p) {
+    constexpr int NC = DP / 32, NK = DP / 64, ND = DP / 16, TERMS = sizeof(T) == 2 ? 1 : 3, PITCH = DP + 4, COLS = 16 * CB;
+    __shared__ __align__(16) float so[4][COLS][PITCH];
     __shared__ __align__(16) float scales[4][2][CN];
-    __shared__ float sml[4][2][CN];
+    __shared__ float sml[4][2][COLS];
     const Args& a = p.a;
-    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, half = lane >> 5, col = lane & 31;
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, col = lane & 15, quarter = lane >> 4;
     int b = blockIdx.x;
     const int kvh = b % a.Hkv;
     b /= a.Hkv;
@@ -68,187 +123,236 @@ __global__ __launch_bounds__(AT, sizeof(T) == 2 ? 2 : 1) void attn_cache_k(Cache
     const signed char* vb = static_cast<const signed char*>(a.V.p) + kvh * a.V.hs;
     const float* ks = p.ks + static_cast<long>(kvh) * a.m.Tk;
     const float* vs = p.vs + static_cast<long>(kvh) * a.m.Tk;
-    int k_at[Keys<DP>::N], v_at[4];
+    int k_at[NK], v_at[4];
 #pragma unroll
-    for (int i = 0; i < Keys<DP>::N; ++i) {
-        const int byte = DP / 2 * half + 16 * i;
-        k_at[i] = byte < W ? static_cast<int>(col * a.K.rs) + byte : kFar;
-    }
+    for (int i = 0; i < NK; ++i) k_at[i] = 64 * i + 16 * quarter < W ? static_cast<int>(col * a.K.rs) + 64 * i + 16 * quarter : kFar;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) v_at[j] = ND * col < W ? static_cast<int>((4 * half + j) * a.V.rs) + ND * col : kFar;
+    for (int r = 0; r < 4; ++r) v_at[r] = ND * col < W ? static_cast<int>((4 * quarter + r) * a.V.rs) + ND * col : kFar;
 
     // the documents that the block's rows belong to, one after the other
     while (row0 < end) {
-        const int doc = __builtin_amdgcn_readfirstlane(doc_of_row(a.m.q_off, a.m.docs, row0, row0));
+        const int d = doc_holding(a.m, row0);
         int stop = end;  // of this document's rows, or of rows that belong to none
-        if (doc >= 0) {
-            stop = min(a.m.q_off[doc + 1], end);
+        Doc doc{0, 0, 0, 0, 0};
+        if (d >= 0) {
+            doc = doc_at(a.m, d);
+            stop = min(a.m.q_off[d + 1], end);
         } else if (a.m.docs > 0 && row0 < a.m.q_off[0]) {
             stop = min(a.m.q_off[0], end);
         }
         stop = __builtin_amdgcn_readfirstlane(max(stop, row0 + 1));
-        const int e0 = row0 * a.G + CN * piece, e1 = min(stop * a.G, p.pieces > 1 ? min(e0 + CN, (row0 + 1) * a.G) : INT_MAX);
-        const int e = e0 + col;
-        const bool valid = e < e1;
-        const int row = valid ? e / a.G : row0, head = kvh * a.G + (valid ? e - row * a.G : 0);
-        Row me{INT_MAX, INT_MIN, 0};
-        if (doc >= 0) me = row_in(a.m, doc, row);
-        if (!valid) me = Row{INT_MAX, INT_MIN, 0};
-        // keys that any of the rows sees, and that all of them see
-        int lo = me.lo, hi = me.hi, all_lo = valid ? me.lo : INT_MIN, all_hi = valid ? me.hi : INT_MAX;
-        for (int o = 16; o; o >>= 1) {
-            lo = min(lo, __shfl_xor(lo, o));
-            hi = max(hi, __shfl_xor(hi, o));
-            all_lo = max(all_lo, __shfl_xor(all_lo, o));
-            all_hi = min(all_hi, __shfl_xor(all_hi, o));
-        }
-        lo = __builtin_amdgcn_readfirstlane(lo);
-        hi = __builtin_amdgcn_readfirstlane(hi);
-        all_lo = __builtin_amdgcn_readfirstlane(all_lo);
-        all_hi = __builtin_amdgcn_readfirstlane(all_hi);
-        const int tiles = hi > lo ? (hi - lo + CN - 1) / CN : 0;
+        const int e0 = row0 * a.G + COLS * piece, e1 = min(stop * a.G, p.pieces > 1 ? min(e0 + COLS, (row0 + 1) * a.G) : INT_MAX);
+        // keys that a row sees, of its document's: more of them from row to row
+        const auto position = [&](int row) { return row - doc.q0 + doc.lk - doc.lq; };
+        const auto sees = [&](int row) { return a.m.causal ? min(max(max(position(row) + 1, doc.prefix), 0), doc.lk) : doc.lk; };
+        const int k0 = doc.k0, all = sees(row0), keys = sees((e1 - 1) / a.G);
+        const int tiles = (keys + CN - 1) / CN;
         const int t0 = static_cast<int>(static_cast<long>(tiles) * split / p.splits);
         const int t1 = static_cast<int>(static_cast<long>(tiles) * (split + 1) / p.splits);
-
-        const Score<T, CAP, BIAS> rule(a, head);
-        bf16x8 q[NC][TERMS];
-        const T* qp = static_cast<const T*>(a.Q.p) + row * a.Q.rs + head * a.Q.hs;
+        int pos[CB];
+        unsigned seen[CB];
+        float slope[CB];
 #pragma unroll
-        for (int c = 0; c < NC; ++c) {
-            const int d = DP / 2 * half + 8 * c;
-            const Frag<T> f = load8(qp + d, valid ? max(min(8, a.D - d), 0) : 0, p.vec_q);
-            if constexpr (TERMS == 1) {
-                q[c][0] = f;
-            } else {
-                const Terms<bf16, TERMS> t(f);
-#pragma unroll
-                for (int k = 0; k < TERMS; ++k) q[c][k] = t.t[k];
-            }
+        for (int x = 0; x < CB; ++x) {
+            const int e = e0 + 16 * x + col, row = e < e1 ? e / a.G : row0;
+            pos[x] = position(row);
+            seen[x] = e < e1 ? static_cast<unsigned>(sees(row)) : 0u;
+            slope[x] = BIAS && e < e1 ? a.slopes[kvh * a.G + e - row * a.G] : 0.0f;
         }
-        Keys<DP> x;
+        Score<T, CAP, BIAS> rule(a);
+
+        // Loads past the part's last tile find empty descriptors: without a branch
+        // around them the products wait for their own operand's loads alone.
+        u32x4 kr[2][NK];
+        float kscale, vscale;
         const auto load_k = [&](int t) __attribute__((always_inline)) {
-            const int j = lo + t * CN, n = min(hi - j, CN);
-            const __amdgpu_buffer_rsrc_t kr = rows_rsrc(kb + j * a.K.rs, a.K.rs, n, W);
+            const long j = k0 + static_cast<long>(t) * CN;
+            const int n = t < t1 ? min(keys - t * CN, CN) : 0;
 #pragma unroll
-            for (int i = 0; i < Keys<DP>::N; ++i)
-                x.k[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(kr, k_at[i], 0, 0));
-            x.scale = col < n ? (half ? vs : ks)[j + col] : 0.0f;
+            for (int g = 0; g < 2; ++g) {
+                const __amdgpu_buffer_rsrc_t r = rows_rsrc(kb + (j + 16 * g) * a.K.rs, a.K.rs, n - 16 * g, W);
+#pragma unroll
+                for (int i = 0; i < NK; ++i)
+                    kr[g][i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, k_at[i], 0, 0));
+            }
+            const __amdgpu_buffer_rsrc_t kr_ = rows_rsrc(ks + j, 1, n, 1), vr_ = rows_rsrc(vs + j, 1, n, 1);
+            kscale = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(kr_, 4 * (lane & 31), 0, 0));
+            vscale = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(vr_, 4 * (lane & 31), 0, 0));
         };
-        Values y;
+        unsigned vr[8][ND / 4];  // ND columns of key 16 g + 4 quarter + r at 4 g + r
         const auto load_v = [&](int t) __attribute__((always_inline)) {
-            const int j = lo + t * CN, n = min(hi - j, CN);
+            const long j = k0 + static_cast<long>(t) * CN;
+            const int n = t < t1 ? min(keys - t * CN, CN) : 0;
 #pragma unroll
-            for (int g = 0; g < 4; ++g) {
-                const __amdgpu_buffer_rsrc_t vr = rows_rsrc(vb + (j + 8 * g) * a.V.rs, a.V.rs, n - 8 * g, W);
+            for (int g = 0; g < 2; ++g) {
+                const __amdgpu_buffer_rsrc_t s = rows_rsrc(vb + (j + 16 * g) * a.V.rs, a.V.rs, n - 16 * g, W);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    if constexpr (DP == 128) y.v[4 * g + i] = __builtin_amdgcn_raw_buffer_load_b32(vr, v_at[i], 0, 0);
-                    else y.v[4 * g + i] = __builtin_amdgcn_raw_buffer_load_b16(vr, v_at[i], 0, 0);
+                for (int r = 0; r < 4; ++r) {
+                    if constexpr (ND == 8) {
+                        const u32x2 w = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(s, v_at[r], 0, 0));
+                        vr[4 * g + r][0] = w[0];
+                        vr[4 * g + r][1] = w[1];
+                    } else {
+                        vr[4 * g + r][0] = __builtin_amdgcn_raw_buffer_load_b32(s, v_at[r], 0, 0);
+                    }
                 }
             }
         };
-        f32x16 acc[ND];
+        f32x4 acc[CB][ND];
+        Soft st[CB];
 #pragma unroll
-        for (int d = 0; d < ND; ++d) acc[d] = f32x16{};
-        Soft st;
-        const auto step = [&](int t) __attribute__((always_inline)) {
-            const int j0 = lo + t * CN;
-            const bool whole = j0 >= all_lo && j0 + CN <= all_hi;
-            scales[wave][half][col] = x.scale;
-            f32x16 s[1];
-            s[0] = f32x16{};
+        for (int x = 0; x < CB; ++x)
 #pragma unroll
-            for (int c = 0; c < NC; ++c) {
-                bf16x8 k;
+            for (int i = 0; i < ND; ++i) acc[x][i] = f32x4{};
+        bf16x8 q[CB][NC][TERMS];
+        const auto step = [&](auto masked, int t) __attribute__((always_inline)) {
+            constexpr bool MASKED = decltype(masked)::value;
+            scales[wave][lane >> 5][lane & 31] = lane >> 5 ? vscale : kscale;
+            f32x4 s[CB][2];
 #pragma unroll
-                for (int i = 0; i < 8; ++i) k[i] = code(x.k[c >> 1][2 * (c & 1) + (i >> 2)], i & 3);
+            for (int g = 0; g < 2; ++g) {
 #pragma unroll
-                for (int m = 0; m < TERMS; ++m) s[0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k, q[c][m], s[0], 0, 0, 0);
+                for (int x = 0; x < CB; ++x) s[x][g] = f32x4{};
+#pragma unroll
+                for (int c = 0; c < NC; ++c) {
+                    u32x4 w;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const unsigned u = kr[g][c >> 1][2 * (c & 1) + (i >> 1)];
+                        w[i] = codes2(u, 2 * (i & 1), u, 2 * (i & 1) + 1);
+                    }
+                    const bf16x8 k = __builtin_bit_cast(bf16x8, w);
+#pragma unroll
+                    for (int x = 0; x < CB; ++x)
+#pragma unroll
+                        for (int m = 0; m < TERMS; ++m) s[x][g] = mma16(k, q[x][c][m], s[x][g]);
+                }
             }
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-            if (t + 4 < t1) load_k(t + 4);
+            load_k(t + 4);
+            f32x4 f[2];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const f32x4 f = *reinterpret_cast<const f32x4*>(&scales[wave][0][8 * i + 4 * half]);
+            for (int g = 0; g < 2; ++g) f[g] = *reinterpret_cast<const f32x4*>(&scales[wave][0][16 * g + 4 * quarter]);
+            const int at = t * CN + 4 * quarter;
 #pragma unroll
-                for (int r = 0; r < 4; ++r) s[0][4 * i + r] *= f[r];
+            for (int x = 0; x < CB; ++x) {
+#pragma unroll
+                for (int g = 0; g < 2; ++g) s[x][g] *= f[g];
+                rule.slope = slope[x] * LOG2E;
+                cache_soft<MASKED>(rule, pos[x], seen[x], at, s[x], acc[x], st[x]);
             }
-            soft_step<true>(rule, me, whole, j0, half, s, acc, st);
-            f32x4 f[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) f[i] = *reinterpret_cast<const f32x4*>(&scales[wave][1][8 * i + 4 * half]);
-            if (whole) {
+            for (int g = 0; g < 2; ++g) f[g] = *reinterpret_cast<const f32x4*>(&scales[wave][1][16 * g + 4 * quarter]);
 #pragma unroll
-                for (int r = 0; r < 16; ++r) s[0][r] *= f[r >> 2][r & 3];
-            } else {  // a value that the row does not see stays out whatever its scale
-                const unsigned at = static_cast<unsigned>(j0 + 4 * half - me.lo), len = me.hi > me.lo ? static_cast<unsigned>(me.hi - me.lo) : 0u;
+            for (int x = 0; x < CB; ++x)
 #pragma unroll
-                for (int r = 0; r < 16; ++r)
-                    s[0][r] = at + static_cast<unsigned>(acc_row(r, 0)) < len ? s[0][r] * f[r >> 2][r & 3] : 0.0f;
-            }
+                for (int g = 0; g < 2; ++g) {
+                    s[x][g] *= f[g];
+                    if (MASKED)  // a value that the row does not see stays out whatever its scale
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) s[x][g][r] = static_cast<unsigned>(at + 16 * g + r) < seen[x] ? s[x][g][r] : 0.0f;
+                }
             __builtin_amdgcn_sched_barrier(0);  // the values' floats come after the scores'
+            bf16x8 w[CB][TERMS];
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                const Terms<bf16, TERMS> w(acc_floats(s[0], c));
+            for (int x = 0; x < CB; ++x) {
+                const Terms<bf16, TERMS> terms(__builtin_shufflevector(s[x][0], s[x][1], 0, 1, 2, 3, 4, 5, 6, 7));
 #pragma unroll
-                for (int d = 0; d < ND; ++d) {
-                    bf16x8 v;
+                for (int m = 0; m < TERMS; ++m) w[x][m] = terms.t[m];
+            }
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) v[i] = code(y.v[8 * c + i], d);
+            for (int i = 0; i < ND; ++i) {
+                u32x4 u;
 #pragma unroll
-                    for (int m = 0; m < TERMS; ++m) acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v, w.t[m], acc[d], 0, 0, 0);
+                for (int j = 0; j < 4; ++j) u[j] = codes2(vr[2 * j][i >> 2], i & 3, vr[2 * j + 1][i >> 2], i & 3);
+                const bf16x8 v = __builtin_bit_cast(bf16x8, u);
+#pragma unroll
+                for (int x = 0; x < CB; ++x)
+#pragma unroll
+                    for (int m = 0; m < TERMS; ++m) acc[x][i] = mma16(v, w[x][m], acc[x][i]);
+            }
+            load_v(t + 4);
+        };
+        load_k(t0 + wave);
+        load_v(t0 + wave);
+#pragma unroll
+        for (int x = 0; x < CB; ++x) {
+            const int e = e0 + 16 * x + col, row = e < e1 ? e / a.G : row0, head = e < e1 ? kvh * a.G + e - row * a.G : 0;
+            const T* qp = static_cast<const T*>(a.Q.p) + row * a.Q.rs + head * a.Q.hs;
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+                const int at = 64 * (c >> 1) + 16 * quarter + 8 * (c & 1);
+                const Frag<T> f = load8(qp + at, e < e1 ? max(min(8, a.D - at), 0) : 0, p.vec_q);
+                if constexpr (TERMS == 1) {
+                    q[x][c][0] = f;
+                    asm volatile("" : "+v"(q[x][c][0]));  // here, not behind the loop's loads
+                } else {
+                    const Terms<bf16, TERMS> t(f);
+#pragma unroll
+                    for (int m = 0; m < TERMS; ++m) q[x][c][m] = t.t[m];
                 }
             }
-            if (t + 4 < t1) load_v(t + 4);
-        };
-        if (t0 + wave < t1) {
-            load_k(t0 + wave);
-            load_v(t0 + wave);
         }
-        for (int t = t0 + wave; t < t1; t += 4) step(t);
+        // tiles that every row sees whole, then the others
+        const int whole = min(all / CN, t1);
+        int t = t0 + wave;
+        for (; t < whole; t += 4) step(std::false_type{}, t);
+        for (; t < t1; t += 4) step(std::true_type{}, t);
+
         // join the waves: their states' common maximum, then the sums in order
         // (the thread's number anew, so that no address of this is held above)
         int thread = tid;
         asm volatile("" : "+v"(thread));
-        const int c1 = thread & 31, h1 = thread >> 5 & 1;
+        const int c1 = thread & 15, q1 = thread >> 4 & 3;
         const float unit = CAP || BIAS ? 1.0f : rule.unit;
-        float l = st.l + __shfl_xor(st.l, 32);
-        if (sums_not_finite(acc)) l = __builtin_nanf("");
-        if (!h1) {
-            sml[wave][0][c1] = st.m * unit;
-            sml[wave][1][c1] = l;
+#pragma unroll
+        for (int x = 0; x < CB; ++x) {
+            float l = st[x].l, zero = 0.0f;
+#pragma unroll
+            for (int i = 0; i < ND; ++i)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) zero = __builtin_fmaf(acc[x][i][r], 0.0f, zero);
+            l += zero == 0.0f ? 0.0f : __builtin_nanf("");  // a value that is not finite makes the whole row NaN
+            l += __shfl_xor(l, 16);
+            l += __shfl_xor(l, 32);
+            if (q1 == 0) {
+                sml[wave][0][16 * x + c1] = st[x].m * unit;
+                sml[wave][1][16 * x + c1] = l;
+            }
+            if (e0 + 16 * x + c1 < e1)
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+#pragma unroll
+                    for (int i = 0; i < ND; i += 4)
+                        *reinterpret_cast<f32x4*>(&so[wave][16 * x + c1][ND * (4 * q1 + r) + i]) =
+                            f32x4{acc[x][i][r], acc[x][i + 1][r], acc[x][i + 2][r], acc[x][i + 3][r]};
         }
         __syncthreads();
-        const float m = fmaxf(fmaxf(sml[0][0][c1], sml[1][0][c1]), fmaxf(sml[2][0][c1], sml[3][0][c1]));
-        const float m0 = m == -INF ? 0.0f : m, f = __builtin_amdgcn_exp2f(st.m * unit - m0);
-        if (e0 + c1 < e1)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                float* to = &so[wave][c1][ND * acc_row(r, h1)];
-#pragma unroll
-                for (int d = 0; d < ND; ++d) to[d] = acc[d][r] * f;
-            }
-        __syncthreads();
-        const int n = max(min(e1 - e0, CN), 0);
+        const int n = max(min(e1 - e0, COLS), 0);
         for (int i = thread; i < n * (DP / 4); i += AT) {
-            const int cc = i / (DP / 4), d = 4 * (i - cc * (DP / 4));
-            float mm = -INF, ll = 0.0f;
-            for (int w = 0; w < 4; ++w) mm = fmaxf(mm, sml[w][0][cc]);
-            for (int w = 0; w < 4; ++w) ll += sml[w][1][cc] * __builtin_amdgcn_exp2f(sml[w][0][cc] - (mm == -INF ? 0.0f : mm));
+            const int cc = i / (DP / 4), d4 = 4 * (i - cc * (DP / 4));
+            float m = -INF, l = 0.0f;
+#pragma unroll
+            for (int w = 0; w < 4; ++w) m = fmaxf(m, sml[w][0][cc]);
             f32x4 v = f32x4{};
-            for (int w = 0; w < 4; ++w) v += *reinterpret_cast<const f32x4*>(&so[w][cc][d]);
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                const float f = __builtin_amdgcn_exp2f(sml[w][0][cc] - (m == -INF ? 0.0f : m));
+                l += sml[w][1][cc] * f;
+                v += *reinterpret_cast<const f32x4*>(&so[w][cc][d4]) * f;
+            }
             const int at = e0 + cc, r = at / a.G, h = kvh * a.G + at - r * a.G;
             if (p.splits > 1) {
                 const long to = (static_cast<long>(split) * a.Hkv + kvh) * a.E + at;
-                *reinterpret_cast<f32x4*>(p.part_o + to * DP + d) = v;
-                if (d == 0) {
-                    p.part_ml[2 * to] = mm;
-                    p.part_ml[2 * to + 1] = ll;
+                *reinterpret_cast<f32x4*>(p.part_o + to * DP + d4) = v;
+                if (d4 == 0) {
+                    p.part_ml[2 * to] = m;
+                    p.part_ml[2 * to + 1] = l;
                 }
             } else {
-                const float inv = ll == 0.0f ? 0.0f : 1.0f / ll;
-                store4(static_cast<T*>(p.O) + r * p.o_rs + h * p.o_hs + d, a.D - d, p.vec_o, v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv);
-                if (d == 0) p.lse[static_cast<long>(h) * a.m.Tq + r] = ll == 0.0f ? -INF : mm * LN2 + logf(ll);
+                const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+                store4(static_cast<T*>(p.O) + r * p.o_rs + h * p.o_hs + d4, a.D - d4, p.vec_o, v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv);
+                if (d4 == 0) p.lse[static_cast<long>(h) * a.m.Tq + r] = l == 0.0f ? -INF : m * LN2 + logf(l);
             }
         }
         __syncthreads();
@@ -304,8 +408,9 @@ __global__ __launch_bounds__(64) void attn_cache_join_k(Cached p) {
 
 struct Launch {
     template <class T, int DP, int CAP, bool BIAS>
-    static int run(kdec_ctx* ctx, const Cached& p, dim3 grid) {
-        hipLaunchKernelGGL((attn_cache_k<T, DP, CAP, BIAS>), grid, dim3(AT), 0, ctx->stream, p);
+    static int run(kdec_ctx* ctx, const Cached& p, dim3 grid, int cols) {
+        if (cols == 16) hipLaunchKernelGGL((attn_cache_k<T, DP, CAP, BIAS, 1>), grid, dim3(AT), 0, ctx->stream, p);
+        else hipLaunchKernelGGL((attn_cache_k<T, DP, CAP, BIAS, 2>), grid, dim3(AT), 0, ctx->stream, p);
         if (p.splits > 1)
             hipLaunchKernelGGL((attn_cache_join_k<T, DP>), dim3(static_cast<unsigned>(static_cast<long>(p.a.Hkv) * p.a.E)), dim3(64), 0,
                                ctx->stream, p);
@@ -346,10 +451,12 @@ extern "C" int kdec_attn_cache_fwd(kdec_ctx* ctx, int dtype, const void* Q, long
     p.vec_o = D % 4 == 0 && aligned(Heads{O, o_rs, o_hs}, size, 4 * size);
     p.vec_q = D % 8 == 0 && aligned(p.a.Q, size, 16);
     p.lse = lse;
-    p.pieces = static_cast<int>(cdiv(G, CN));
-    // Rows of a block: what 32 entries hold, fewer where documents have fewer.
+    // Entries of a block: 16 where a document's rows have no more, else 32. Rows:
+    // what these hold, fewer where documents have fewer.
     const long mean = docs > 0 ? cdiv(Tq, docs) : Tq;
-    p.rows = static_cast<int>(G >= CN ? 1 : mean < CN / G ? mean : CN / G);
+    const int cols = mean * G <= 16 ? 16 : 32;
+    p.pieces = static_cast<int>(cdiv(G, cols));
+    p.rows = static_cast<int>(G >= cols ? 1 : mean < cols / G ? mean : cols / G);
     const long blocks = cdiv(Tq, p.rows) * p.pieces * Hkv;
     KDEC_CHECK(ctx, blocks < INT_MAX && static_cast<long>(Hkv) * p.a.E < INT_MAX, "kdec_attn_cache_fwd: too many rows");
     // Split the keys where the rows alone do not fill the device.
@@ -364,5 +471,6 @@ extern "C" int kdec_attn_cache_fwd(kdec_ctx* ctx, int dtype, const void* Q, long
     if (!ws.p) return KDEC_ENOMEM;
     p.part_o = ws.as<float>();
     p.part_ml = p.part_o + n * DP;
-    return dispatch<Launch>(dtype, D, cap, slopes != nullptr, ctx, p, dim3(static_cast<unsigned>(blocks), static_cast<unsigned>(splits)));
+    return dispatch<Launch>(dtype, D, cap, slopes != nullptr, ctx, p, dim3(static_cast<unsigned>(blocks), static_cast<unsigned>(splits)),
+                            cols);
 }

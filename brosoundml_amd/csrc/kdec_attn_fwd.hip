@@ -45,6 +45,69 @@ struct Fwd {
     float *part_o, *part_ml;  // (splits, Hkv, E, D) and (splits, Hkv, E, 2)
 };
 
+// Running softmax state of one lane's column, in the units of m: raw products
+// (times `unit` they are log2) without cap and bias, log2 with either.
+struct Soft {
+    float m = -INF, l = 0.0f;
+};
+
+// One step of the running softmax of a lane's column over N score blocks of
+// 32 keys from j0 (whole: all of the wave's rows see all of them). Scores
+// become probabilities; acc is rescaled when the wave's maxima move far enough.
+template <bool MASKED, class T, int CAP, bool BIAS, int N, int ND>
+__device__ inline void soft_step(const Score<T, CAP, BIAS>& rule, const Row& row, bool whole, int j0, int half,
+                                 f32x16 (&s)[N], f32x16 (&acc)[ND], Soft& st) {
+    constexpr bool RAW = !CAP && !BIAS;
+    const float unit = RAW ? rule.unit : 1.0f;
+    const float dist = static_cast<float>(row.pos - j0 - 4 * half);
+#pragma unroll
+    for (int n = 0; n < N; ++n)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            float t = s[n][r], dt;
+            if (!RAW) t = rule.of(t, dist - static_cast<float>(32 * n + acc_row(r, 0)), dt);
+            s[n][r] = t;
+        }
+    if (MASKED && !whole) {
+        const unsigned at = static_cast<unsigned>(j0 + 4 * half - row.lo);  // seen: at + key's place < len
+        const unsigned len = row.hi > row.lo ? static_cast<unsigned>(row.hi - row.lo) : 0u;
+#pragma unroll
+        for (int n = 0; n < N; ++n)
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+                s[n][r] = at + static_cast<unsigned>(32 * n + acc_row(r, 0)) < len ? s[n][r] : -INF;
+        asm volatile("");  // a branch
+    }
+    float mx = -INF;
+#pragma unroll
+    for (int n = 0; n < N; ++n)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[n][r]);
+    mx = max32(mx);
+    if (__builtin_amdgcn_ballot_w64((mx - st.m) * unit > 8.0f || (st.m == -INF && mx > -INF))) {
+        const float m = fmaxf(st.m, mx);
+        const float f = __builtin_amdgcn_exp2f((st.m - (m == -INF ? 0.0f : m)) * unit);
+        st.l *= f;
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) acc[d][r] *= f;
+        st.m = m;
+        asm volatile("");  // a branch, not sixty-four selects
+    }
+    const float m0 = (st.m == -INF ? 0.0f : st.m) * unit;
+    float sum = 0.0f;
+#pragma unroll
+    for (int n = 0; n < N; ++n)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            const float p = __builtin_amdgcn_exp2f(RAW ? __builtin_fmaf(s[n][r], unit, -m0) : s[n][r] - m0);
+            s[n][r] = p;
+            sum += p;
+        }
+    st.l += sum;
+}
+
 // A column's output and lse, or its unfinished state where the keys are
 // split. m in log2 units.
 template <class T, int DP>

@@ -45,63 +45,84 @@ __device__ inline int nearest(float x, float s, float inv) {
     return static_cast<int>(q);
 }
 
+// L lanes take UNITS heads' keys or values of a row (unit u: head u / 2, keys or
+// values), their loads together behind one search for the row's place.
+constexpr int UNITS = 4;
 template <class T, int L>
 __global__ __launch_bounds__(CT) void cache_write_k(Docs m, Heads K, Heads V, Codes o, int H, int D, int W, bool vec) {
     const int per = CT / L, lane = threadIdx.x % L, row = blockIdx.x * per + threadIdx.x / L;
-    const int head = blockIdx.y % H, c = 8 * lane, n = max(min(8, D - c), 0);
-    const bool keys = static_cast<int>(blockIdx.y) < H;
+    const int c = 8 * lane, n = max(min(8, D - c), 0), u0 = blockIdx.y * UNITS;
+    Frag<T> f[UNITS];
+#pragma unroll
+    for (int j = 0; j < UNITS; ++j) {
+        const Heads& h = (u0 + j) & 1 ? V : K;
+        const T* p = static_cast<const T*>(h.p) + min(row, m.Tq - 1) * h.rs + min((u0 + j) >> 1, H - 1) * h.hs + c;
+        f[j] = load8(p, n, vec);
+    }
     const long at = cache_row(m, row, __builtin_amdgcn_readfirstlane(row));
-    const Heads& h = keys ? K : V;
-    const T* p = static_cast<const T*>(h.p) + min(row, m.Tq - 1) * h.rs + head * h.hs + c;
-    const Frag<T> f = load8(p, at < 0 ? 0 : n, vec);
-    float x[8], top = 0.0f, zero = 0.0f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        x[i] = static_cast<float>(f[i]);
-        top = fmaxf(top, __builtin_fabsf(x[i]));
-        zero = __builtin_fmaf(x[i], 0.0f, zero);
+    for (int j = 0; j < UNITS; ++j) {
+        const bool keys = !((u0 + j) & 1);
+        const int head = (u0 + j) >> 1;
+        float x[8], top = 0.0f, zero = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            x[i] = static_cast<float>(f[j][i]);
+            top = fmaxf(top, __builtin_fabsf(x[i]));
+            zero = __builtin_fmaf(x[i], 0.0f, zero);
+        }
+#pragma unroll
+        for (int s = 1; s < L; s *= 2) {
+            top = fmaxf(top, __shfl_xor(top, s));
+            zero += __shfl_xor(zero, s);
+        }
+        if (at < 0 || head >= H) continue;
+        const bool bad = !(zero == 0.0f);
+        const float s = bad ? __builtin_nanf("") : fmaxf(top / 127.0f, 0x1p-126f), inv = 1.0f / s;
+        i8x8 q;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) q[i] = static_cast<signed char>(bad ? 0 : nearest(x[i], s, inv));
+        signed char* to = (keys ? o.k + at * o.k_rs + head * o.k_hs : o.v + at * o.v_rs + head * o.v_hs) + c;
+        if (c < W) *reinterpret_cast<i8x8*>(to) = q;
+        if (lane == 0) (keys ? o.ks : o.vs)[static_cast<long>(head) * m.Tk + at] = s;
     }
-#pragma unroll
-    for (int s = 1; s < L; s *= 2) {
-        top = fmaxf(top, __shfl_xor(top, s));
-        zero += __shfl_xor(zero, s);
-    }
-    const bool bad = !(zero == 0.0f);
-    const float s = bad ? __builtin_nanf("") : fmaxf(top / 127.0f, 0x1p-126f), inv = 1.0f / s;
-    if (at < 0) return;
-    i8x8 q;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) q[i] = static_cast<signed char>(bad ? 0 : nearest(x[i], s, inv));
-    signed char* to = (keys ? o.k + at * o.k_rs + head * o.k_hs : o.v + at * o.v_rs + head * o.v_hs) + c;
-    if (c < W) *reinterpret_cast<i8x8*>(to) = q;
-    if (lane == 0) (keys ? o.ks : o.vs)[static_cast<long>(head) * m.Tk + at] = s;
 }
 
 template <class T, int L>
 __global__ __launch_bounds__(CT) void cache_read_k(Docs m, Codes o, int H, int D, int W, T* K, long k_rs, long k_hs, T* V, long v_rs,
                                                    long v_hs, bool vec) {
     const int per = CT / L, lane = threadIdx.x % L, row = blockIdx.x * per + threadIdx.x / L;
-    const int head = blockIdx.y % H, c = 8 * lane, n = max(min(8, D - c), 0);
-    const bool keys = static_cast<int>(blockIdx.y) < H;
+    const int c = 8 * lane, n = max(min(8, D - c), 0), u0 = blockIdx.y * UNITS;
     const long at = cache_row(m, row, __builtin_amdgcn_readfirstlane(row));
     if (row >= m.Tq) return;
-    i8x8 q = i8x8{};
-    float s = 0.0f;
-    if (at >= 0) {
+    i8x8 q[UNITS];
+    float s[UNITS];
+#pragma unroll
+    for (int j = 0; j < UNITS; ++j) {
+        const bool keys = !((u0 + j) & 1);
+        const int head = min((u0 + j) >> 1, H - 1);
         const signed char* from = (keys ? o.k + at * o.k_rs + head * o.k_hs : o.v + at * o.v_rs + head * o.v_hs) + c;
-        if (c < W) q = *reinterpret_cast<const i8x8*>(from);
-        s = (keys ? o.ks : o.vs)[static_cast<long>(head) * m.Tk + at];
+        q[j] = i8x8{};
+        s[j] = 0.0f;
+        if (at >= 0 && c < W) q[j] = *reinterpret_cast<const i8x8*>(from);
+        if (at >= 0) s[j] = (keys ? o.ks : o.vs)[static_cast<long>(head) * m.Tk + at];
     }
-    T* to = (keys ? K + row * k_rs + head * k_hs : V + row * v_rs + head * v_hs) + c;
-    Frag<T> f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = static_cast<T>(s * static_cast<float>(q[i]));
-    if (vec) {
-        if (n > 0) *reinterpret_cast<Frag<T>*>(to) = f;
-    } else {
+    for (int j = 0; j < UNITS; ++j) {
+        const bool keys = !((u0 + j) & 1);
+        const int head = (u0 + j) >> 1;
+        if (head >= H) break;
+        T* to = (keys ? K + row * k_rs + head * k_hs : V + row * v_rs + head * v_hs) + c;
+        Frag<T> f;
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if (i < n) to[i] = f[i];
+        for (int i = 0; i < 8; ++i) f[i] = static_cast<T>(s[j] * static_cast<float>(q[j][i]));
+        if (vec) {
+            if (n > 0) *reinterpret_cast<Frag<T>*>(to) = f;
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (i < n) to[i] = f[i];
+        }
     }
 }
 
@@ -137,8 +158,8 @@ int kdec_cache_write(kdec_ctx* ctx, int dtype, const void* K, long k_rs, long k_
     const bool vec = wide(k, D, es) && wide(v, D, es);
     ProfScope ps(ctx, "cache", 0.0, 2.0 * Tq * H * (static_cast<double>(es) * D + W + 4));
     const int L = W <= 64 ? 8 : 16;
-    const dim3 grid(static_cast<unsigned>(cdiv(Tq, CT / L)), static_cast<unsigned>(2 * H));
-    KDEC_CHECK(ctx, 2L * H <= 65535, "kdec_cache_write: too many heads");
+    const dim3 grid(static_cast<unsigned>(cdiv(Tq, CT / L)), static_cast<unsigned>(cdiv(2L * H, UNITS)));
+    KDEC_CHECK(ctx, cdiv(2L * H, UNITS) <= 65535, "kdec_cache_write: too many heads");
     const auto run = [&](auto k_) { hipLaunchKernelGGL(k_, grid, dim3(CT), 0, ctx->stream, m, k, v, o, H, D, W, vec); };
     if (dtype == KDEC_F32) run(L == 8 ? cache_write_k<float, 8> : cache_write_k<float, 16>);
     else run(L == 8 ? cache_write_k<bf16, 8> : cache_write_k<bf16, 16>);
@@ -160,8 +181,8 @@ int kdec_cache_read(kdec_ctx* ctx, int dtype, const void* Kc, long kc_rs, long k
     const bool vec = wide({K, k_rs, k_hs}, D, es) && wide({V, v_rs, v_hs}, D, es);
     ProfScope ps(ctx, "cache", 0.0, 2.0 * Tq * H * (static_cast<double>(es) * D + W + 4));
     const int L = W <= 64 ? 8 : 16;
-    const dim3 grid(static_cast<unsigned>(cdiv(Tq, CT / L)), static_cast<unsigned>(2 * H));
-    KDEC_CHECK(ctx, 2L * H <= 65535, "kdec_cache_read: too many heads");
+    const dim3 grid(static_cast<unsigned>(cdiv(Tq, CT / L)), static_cast<unsigned>(cdiv(2L * H, UNITS)));
+    KDEC_CHECK(ctx, cdiv(2L * H, UNITS) <= 65535, "kdec_cache_read: too many heads");
     const auto run = [&](auto k_, auto ty) {
         typedef decltype(ty) E;
         hipLaunchKernelGGL(k_, grid, dim3(CT), 0, ctx->stream, m, o, H, D, W, static_cast<E*>(K), k_rs, k_hs, static_cast<E*>(V), v_rs, v_hs,

@@ -1,22 +1,26 @@
 // Embedding lookup on gfx950, and the gradient of its table by sorted tokens.
 //
 // Forward: Y[t] = scale * table[ids[t]], a row of zeros where the id is outside
-// the table. One lane copies eight columns; bound by memory.
+// the table. Sixteen bytes a lane; bound by memory.
 //
 // Backward: dtable[v] = beta dtable[v] + scale * sum of dY[t] over the tokens t
-// of id v, in ascending t. Tokens are sorted by id first (a stable radix sort:
-// ranks within 64 tokens from ballots over the digit's bits, counts by wave and
-// digit, one scan), cut into pieces of a fixed number of sorted tokens, and a
-// wave walks a piece for a stretch of columns: a run of one id that lies inside
-// the piece goes to the table, what a run leaves at a piece's ends goes to a
-// partial row, and the partial rows of a run are added in the pieces' order.
-// So every piece is the same work however often an id occurs, and every sum has
-// one order. The table is cleared (or scaled by beta) by the blocks that the
-// sort leaves idle.
+// of id v, in ascending t. Tokens are sorted by id first, cut into pieces of a
+// fixed number of sorted tokens, and a wave walks a piece for a stretch of
+// columns: a run of one id that lies inside the piece goes to the table, what a
+// run leaves at a piece's ends goes to a partial row, and the partial rows of a
+// run are added in the pieces' order. So every piece is the same work however
+// often an id occurs, and every sum has one order.
+//
+// The sort is one launch: block b owns a range of ids, looks at all tokens,
+// counts those of lower ids and ranks its own (within 64 tokens by ballots over
+// the id's bits, then by wave and id with one scan). It also clears the table's
+// rows that no token has, which the sums leave alone. More tokens than a block
+// holds take a radix sort over several blocks.
 #include "kdec_frag.hpp"
 #include "kdec_internal.hpp"
 
 #include <climits>
+#include <type_traits>
 
 namespace kdec {
 namespace {
@@ -28,25 +32,68 @@ constexpr int CHUNK = ST * SI;  // tokens a sorting block holds
 constexpr int WAVES = ST / 64;
 constexpr int DIGITS = 256;
 
+// A lane's part of a row: 16 bytes.
+template <class T> constexpr int PART = 16 / sizeof(T);
+template <class T> struct PartOf;
+template <> struct PartOf<float> { typedef f32x4 type; };
+template <> struct PartOf<bf16> { typedef bf16x8 type; };
+template <class T> using Part = typename PartOf<T>::type;
+
 template <class T>
-__global__ __launch_bounds__(ET) void embed_k(const T* table, long t_rs, const int* ids, T* Y, long y_rs, int rows, int vocab,
-                                              int cols, unsigned groups, bool vec, float scale) {
+__device__ inline Part<T> load_part(const T* p, int n, bool vec) {
+    Part<T> f = Part<T>{};
+    if (vec) {
+        if (n > 0) f = *reinterpret_cast<const Part<T>*>(p);
+        return f;
+    }
+#pragma unroll
+    for (int i = 0; i < PART<T>; ++i) f[i] = i < n ? p[i] : static_cast<T>(0.0f);
+    return f;
+}
+
+// J parts a thread, a block's width apart: their ids, then their rows are on
+// their way together.
+template <class T, int J>
+__global__ __launch_bounds__(ET) void embed_k(const T* __restrict__ table, long t_rs, const int* __restrict__ ids, T* __restrict__ Y,
+                                              long y_rs, int rows, int vocab, int cols, unsigned groups, bool vec, float scale) {
+    constexpr int E = PART<T>;
     const unsigned long long total = static_cast<unsigned long long>(rows) * groups;
-    for (unsigned long long e = static_cast<unsigned long long>(blockIdx.x) * ET + threadIdx.x; e < total;
-         e += static_cast<unsigned long long>(gridDim.x) * ET) {
-        const unsigned row = static_cast<unsigned>(e / groups), g = static_cast<unsigned>(e - static_cast<unsigned long long>(row) * groups);
-        const int c = 8 * static_cast<int>(g), n = min(8, cols - c), id = ids[row];
-        Frag<T> f = Frag<T>{};
-        if (static_cast<unsigned>(id) < static_cast<unsigned>(vocab)) f = load8(table + id * t_rs + c, n, vec);
-        T* y = Y + row * y_rs + c;
+    for (unsigned long long e0 = static_cast<unsigned long long>(blockIdx.x) * (ET * J) + threadIdx.x; e0 < total;
+         e0 += static_cast<unsigned long long>(gridDim.x) * (ET * J)) {
+        long row[J];
+        int c[J], id[J];
+        Part<T> f[J];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) f[i] = static_cast<T>(scale * static_cast<float>(f[i]));
-        if (vec) {
-            *reinterpret_cast<Frag<T>*>(y) = f;
-        } else {
+        for (int j = 0; j < J; ++j) {
+            const unsigned long long e = min(e0 + static_cast<unsigned long long>(j) * ET, total - 1);
+            if (total <= 0xFFFFFFFFull) {
+                const unsigned r = static_cast<unsigned>(e) / groups;
+                row[j] = r;
+                c[j] = E * static_cast<int>(static_cast<unsigned>(e) - r * groups);
+            } else {
+                row[j] = static_cast<long>(e / groups);
+                c[j] = E * static_cast<int>(e - static_cast<unsigned long long>(row[j]) * groups);
+            }
+            id[j] = ids[row[j]];
+        }
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-                if (i < n) y[i] = f[i];
+        for (int j = 0; j < J; ++j) {
+            const bool in = static_cast<unsigned>(id[j]) < static_cast<unsigned>(vocab);
+            f[j] = load_part(table + (in ? id[j] * t_rs + c[j] : 0), in ? min(E, cols - c[j]) : 0, vec);
+        }
+#pragma unroll
+        for (int j = 0; j < J; ++j) {
+            if (e0 + static_cast<unsigned long long>(j) * ET >= total) break;
+            T* y = Y + row[j] * y_rs + c[j];
+#pragma unroll
+            for (int i = 0; i < E; ++i) f[j][i] = static_cast<T>(scale * static_cast<float>(f[j][i]));
+            if (vec) {
+                *reinterpret_cast<Part<T>*>(y) = f[j];
+            } else {
+#pragma unroll
+                for (int i = 0; i < E; ++i)
+                    if (i < cols - c[j]) y[i] = f[j][i];
+            }
         }
     }
 }
@@ -92,12 +139,34 @@ struct Ranks {
 __device__ inline void rank64(int digit, int bits, int& place) {
     const int lane = threadIdx.x & 63;
     unsigned long long same = __builtin_amdgcn_ballot_w64(digit >= 0);
+    place = 0;
+    if (!same) return;
     for (int b = 0; b < bits; ++b) {
         const unsigned long long one = __builtin_amdgcn_ballot_w64(digit >> b & 1);
         same &= (digit >> b & 1) ? one : ~one;
     }
     const int before = __builtin_popcountll(same & ((1ull << lane) - 1));
     place = before | __builtin_popcountll(same) << 8;
+}
+
+// The sum over a wave's lanes up to each lane's own.
+__device__ inline int wave_scan(int x) {
+    const auto add = [&](auto ctrl, auto rows) __attribute__((always_inline)) {
+        x += __builtin_amdgcn_update_dpp(0, x, decltype(ctrl)::value, decltype(rows)::value, 15, false);
+    };
+    typedef std::integral_constant<int, 15> All;
+    add(std::integral_constant<int, 0x111>{}, All{});  // lanes of 16 to the right by 1, 2, 4, 8
+    add(std::integral_constant<int, 0x112>{}, All{});
+    add(std::integral_constant<int, 0x114>{}, All{});
+    add(std::integral_constant<int, 0x118>{}, All{});
+    add(std::integral_constant<int, 0x142>{}, std::integral_constant<int, 10>{});  // the 16's last lane to the next 16
+    add(std::integral_constant<int, 0x143>{}, std::integral_constant<int, 12>{});  // lane 31 to the upper half
+    return x;
+}
+// The sum of the first n of the block's waves' values.
+__device__ inline int first_waves(const int* sums, int n) {
+    const int lane = threadIdx.x & 63;
+    return __builtin_amdgcn_readlane(wave_scan(lane < n ? sums[min(lane, WAVES - 1)] : 0), 63);
 }
 
 // Counts cnt[wave][digit], then their exclusive sums, digits first: where each
@@ -121,16 +190,10 @@ __device__ inline void block_offsets(Ranks& r, int bits, int (*cnt)[DIGITS], int
         v[i] = cnt[w + i][d];
         sum += v[i];
     }
-    int upto = sum;
-#pragma unroll
-    for (int o = 1; o < 64; o *= 2) {
-        const int x = __shfl_up(upto, o);
-        upto += lane >= o ? x : 0;
-    }
+    const int upto = wave_scan(sum);
     if (lane == 63) sums[wave] = upto;
     __syncthreads();
-    int at = upto - sum;
-    for (int i = 0; i < wave; ++i) at += sums[i];
+    int at = upto - sum + first_waves(sums, wave);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         cnt[w + i][d] = at;
@@ -145,7 +208,7 @@ __device__ inline void place_all(const Ranks& r, int (*cnt)[DIGITS], F f) {
     const int wave = threadIdx.x >> 6;
 #pragma unroll
     for (int g = 0; g < SI; ++g)
-        if (g < r.n) {
+        if (g < r.n && __builtin_amdgcn_ballot_w64(r.digit[g] >= 0)) {
             const int d = r.digit[g];
             if (d >= 0) {
                 const int base = cnt[wave][d];
@@ -157,48 +220,86 @@ __device__ inline void place_all(const Ranks& r, int (*cnt)[DIGITS], F f) {
         }
 }
 
-// One block sorts up to CHUNK tokens, digit by digit, through shared memory.
-// The other blocks begin the table.
-__global__ __launch_bounds__(ST) void sort_one_k(Sort s, int passes, Tokens out) {
-    __shared__ int cnt[WAVES][DIGITS], sums[WAVES];
-    __shared__ int sid[CHUNK], sat[CHUNK];
-    if (blockIdx.x > 0) {
-        begin_table(s, blockIdx.x - 1, gridDim.x - 1);
-        return;
-    }
-    const int tid = threadIdx.x;
+// Block b's ids, `per` of them from b * per (those outside the table count as
+// one more, vocab), of up to CHUNK tokens. FEW tokens are summed right here, a
+// thread's columns over every run in order.
+constexpr int FEW = 256;
+template <class T, bool SUM>
+__global__ __launch_bounds__(ST) void sort_range_k(Sort s, int per, Tokens out, const T* __restrict__ dY, long rs, int cols, float scale) {
+    __shared__ int cnt[WAVES][DIGITS], sums[WAVES], start[DIGITS + 1], lower[WAVES], owned[WAVES], list[SUM ? FEW : 1];
+    const int tid = threadIdx.x, wave = tid >> 6, lo = blockIdx.x * per;
     Ranks r;
     r.n = (s.T + ST - 1) / ST;
-    const int first = (tid >> 6) * 64 * r.n + (tid & 63);
-    int id[SI], at[SI];
+    const int first = wave * 64 * r.n + (tid & 63);
+    int id[SI], less = 0, mine = 0;
 #pragma unroll
     for (int g = 0; g < SI; ++g) {
-        at[g] = first + 64 * g;
-        id[g] = g < r.n && at[g] < s.T ? key_of(s.ids[at[g]], s.vocab) : -1;
-    }
-    for (int p = 0; p < passes; ++p) {
-#pragma unroll
-        for (int g = 0; g < SI; ++g) r.digit[g] = id[g] < 0 ? -1 : id[g] >> (p * s.bits) & ((1 << s.bits) - 1);
-        block_offsets(r, s.bits, cnt, sums);
-        place_all(r, cnt, [&](int g, int to) {
-            sid[to] = id[g];
-            sat[to] = at[g];
-        });
-        __syncthreads();
-#pragma unroll
-        for (int g = 0; g < SI; ++g)
-            if (g < r.n && first + 64 * g < s.T) {
-                id[g] = sid[first + 64 * g];
-                at[g] = sat[first + 64 * g];
-            }
-        __syncthreads();
+        const int i = first + 64 * g;
+        id[g] = g < r.n && i < s.T ? key_of(s.ids[i], s.vocab) : INT_MAX;
     }
 #pragma unroll
-    for (int g = 0; g < SI; ++g)
-        if (g < r.n && first + 64 * g < s.T) {
-            out.id[first + 64 * g] = id[g];
-            out.at[first + 64 * g] = at[g];
+    for (int g = 0; g < SI; ++g) {
+        less += id[g] < lo;
+        const bool in = id[g] >= lo && id[g] - lo < per;
+        r.digit[g] = in ? id[g] - lo : -1;
+        mine += in;
+    }
+    block_offsets(r, s.bits, cnt, sums);
+    if (tid < DIGITS) start[tid] = cnt[0][tid];
+    less = wave_scan(less);
+    mine = wave_scan(mine);
+    if ((tid & 63) == 63) {
+        lower[wave] = less;
+        owned[wave] = mine;
+    }
+    __syncthreads();
+    const int base = first_waves(lower, WAVES);
+    if (wave == 0) start[DIGITS] = first_waves(owned, WAVES);
+    place_all(r, cnt, [&](int g, int to) {
+        if (SUM) {
+            list[to] = first + 64 * g;
+        } else {
+            out.id[base + to] = id[g];
+            out.at[base + to] = first + 64 * g;
         }
+    });
+    __syncthreads();
+    // rows that no token has, a wave 64 places of a row at a time
+    const int n = min(per, s.vocab - lo);
+    const bool vec = cols % 4 == 0 && reinterpret_cast<size_t>(s.table) % 16 == 0;
+    const int width = vec ? cols / 4 : cols, each = (width + 63) / 64;
+    if (s.beta != 1.0f)
+        for (int u = __builtin_amdgcn_readfirstlane(wave); u < n * each; u += WAVES) {
+            const int row = u / each, c = 64 * (u - row * each) + (tid & 63);
+            if ((s.beta == 0.0f && start[row] != start[row + 1]) || c >= width) continue;
+            float* to = s.table + static_cast<long>(lo + row) * cols;
+            if (vec) {
+                f32x4* q = reinterpret_cast<f32x4*>(to) + c;
+                *q = s.beta == 0.0f ? f32x4{} : *q * s.beta;
+            } else {
+                to[c] = s.beta == 0.0f ? 0.0f : to[c] * s.beta;
+            }
+        }
+    if (!SUM) return;
+    __syncthreads();
+    for (int row = 0; row < n; ++row) {
+        const int i0 = start[row], i1 = start[row + 1];
+        if (i0 == i1) continue;
+        for (int c = tid; c < cols; c += ST) {
+            float acc = 0.0f;
+            int i = i0;
+            for (; i + 8 <= i1; i += 8) {
+                float f[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) f[j] = static_cast<float>(dY[list[i + j] * rs + c]);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) acc += f[j];
+            }
+            for (; i < i1; ++i) acc += static_cast<float>(dY[list[i] * rs + c]);
+            float* to = s.table + static_cast<long>(lo + row) * cols + c;
+            *to = s.beta == 0.0f ? scale * acc : *to + scale * acc;
+        }
+    }
 }
 
 // More tokens: a digit's counts by chunk, then every chunk's tokens to their
@@ -276,18 +377,21 @@ struct Sums {
     float* part;  // (pieces, 2, cols): a run that began before the piece, one that goes on behind it
 };
 
-// A wave walks a piece's tokens for 512 columns, eight rows' loads at a time.
+// A wave walks a piece's tokens for 64 parts of a row, sixteen rows' loads at a time.
 template <class T>
-__global__ __launch_bounds__(ET) void embed_sums_k(Sums s, const T* dY, long rs, bool vec) {
+__global__ __launch_bounds__(ET) void embed_sums_k(Sums s, const T* __restrict__ dY, long rs, bool vec) {
+    constexpr int E = PART<T>, N = 16;
     const int lane = threadIdx.x & 63;
     const long unit = static_cast<long>(blockIdx.x) * (ET / 64) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int piece = static_cast<int>(unit / s.chunks), chunk = static_cast<int>(unit - static_cast<long>(piece) * s.chunks);
     if (piece >= s.pieces) return;
     const int s0 = piece * s.piece, n = min(s.piece, s.T - s0);
-    const int c = 512 * chunk + 8 * lane, nc = max(min(8, s.cols - c), 0);
+    const int c = E * (64 * chunk + lane), nc = max(min(E, s.cols - c), 0);
     const int ids = lane < n ? s.id[s0 + lane] : s.vocab, ats = lane < n ? s.at[s0 + lane] : 0;
     const int prev = s0 > 0 ? s.id[s0 - 1] : -1, next = s0 + n < s.T ? s.id[s0 + n] : -1;
-    f32x8 acc = f32x8{};
+    float acc[E];
+#pragma unroll
+    for (int k = 0; k < E; ++k) acc[k] = 0.0f;
     int cur = __builtin_amdgcn_readlane(ids, 0);
     bool left = prev == cur;  // the run began before the piece
     const auto put = [&](bool right) __attribute__((always_inline)) {
@@ -297,41 +401,42 @@ __global__ __launch_bounds__(ET) void embed_sums_k(Sums s, const T* dY, long rs,
         } else {
             to = s.table + static_cast<long>(cur) * s.cols + c;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) acc[i] *= s.scale;
+            for (int i = 0; i < E; ++i) acc[i] *= s.scale;
             if (s.add)
 #pragma unroll
-                for (int i = 0; i < 8; ++i)
+                for (int i = 0; i < E; ++i)
                     if (i < nc) acc[i] += to[i];
         }
-        if (nc == 8 && (s.cols & 3) == 0 && (reinterpret_cast<size_t>(to) & 15) == 0) {
-            *reinterpret_cast<f32x4*>(to) = acc.lo;
-            *reinterpret_cast<f32x4*>(to + 4) = acc.hi;
+        if (nc == E && (s.cols & 3) == 0 && (reinterpret_cast<size_t>(to) & 15) == 0) {
+#pragma unroll
+            for (int i = 0; i < E; i += 4) *reinterpret_cast<f32x4*>(to + i) = f32x4{acc[i], acc[i + 1], acc[i + 2], acc[i + 3]};
         } else {
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
+            for (int i = 0; i < E; ++i)
                 if (i < nc) to[i] = acc[i];
         }
     };
-    for (int i0 = 0; i0 < n; i0 += 8) {
-        Frag<T> f[8];
+    for (int i0 = 0; i0 < n; i0 += N) {
+        Part<T> f[N];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
+        for (int j = 0; j < N; ++j) {
             const int i = min(i0 + j, n - 1);
-            f[j] = load8(dY + __builtin_amdgcn_readlane(ats, i) * rs + c, __builtin_amdgcn_readlane(ids, i) < s.vocab ? nc : 0, vec);
+            f[j] = load_part(dY + __builtin_amdgcn_readlane(ats, i) * rs + c, __builtin_amdgcn_readlane(ids, i) < s.vocab ? nc : 0, vec);
         }
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
+        for (int j = 0; j < N; ++j) {
             if (i0 + j >= n) break;
             const int id = __builtin_amdgcn_readlane(ids, i0 + j);
             if (id != cur) {
                 put(false);
                 cur = id;
                 left = false;
-                acc = f32x8{};
+#pragma unroll
+                for (int k = 0; k < E; ++k) acc[k] = 0.0f;
             }
             if (id == s.vocab) return;  // what follows is outside the table
 #pragma unroll
-            for (int k = 0; k < 8; ++k) acc[k] += static_cast<float>(f[j][k]);
+            for (int k = 0; k < E; ++k) acc[k] += static_cast<float>(f[j][k]);
         }
     }
     put(next == cur);
@@ -390,13 +495,16 @@ __global__ __launch_bounds__(ET) void embed_join_k(Sums s) {
 template <class T>
 void lookup(kdec_ctx* ctx, const void* table, long t_rs, const int* ids, void* Y, long y_rs, int rows, int vocab, int cols,
             float scale) {
-    const int el = 16 / static_cast<int>(sizeof(T));  // elements per 16 bytes
-    const auto ok = [&](const void* p, long rs) { return reinterpret_cast<size_t>(p) % 16 == 0 && rs % el == 0; };
-    const bool vec = cols % 8 == 0 && ok(table, t_rs) && ok(Y, y_rs);
-    const unsigned groups = static_cast<unsigned>(cdiv(cols, 8));
-    long blocks = cdiv(static_cast<long>(rows) * groups, ET);
-    if (blocks > 32L * ctx->num_cus) blocks = 32L * ctx->num_cus;
-    hipLaunchKernelGGL(embed_k<T>, dim3(static_cast<unsigned>(blocks)), dim3(ET), 0, ctx->stream, static_cast<const T*>(table), t_rs, ids,
+    constexpr int E = PART<T>;
+    const auto ok = [&](const void* p, long rs) { return reinterpret_cast<size_t>(p) % 16 == 0 && rs % E == 0; };
+    const bool vec = cols % E == 0 && ok(table, t_rs) && ok(Y, y_rs);
+    const unsigned groups = static_cast<unsigned>(cdiv(cols, E));
+    const long threads = static_cast<long>(rows) * groups;
+    const bool many = threads >= 4L * ET * 4 * ctx->num_cus;  // four parts a thread where that leaves four blocks a CU
+    long blocks = cdiv(threads, ET * (many ? 4 : 1));
+    if (blocks > 64L * ctx->num_cus) blocks = 64L * ctx->num_cus;
+    const auto k = many ? embed_k<T, 4> : embed_k<T, 1>;
+    hipLaunchKernelGGL(k, dim3(static_cast<unsigned>(blocks)), dim3(ET), 0, ctx->stream, static_cast<const T*>(table), t_rs, ids,
                        static_cast<T*>(Y), y_rs, rows, vocab, cols, groups, vec, scale);
 }
 
@@ -434,22 +542,40 @@ int kdec_embed_bwd(kdec_ctx* ctx, int dtype, const void* dY, long dy_rs, const i
     const long n = static_cast<long>(vocab) * cols;
     ProfScope ps(ctx, "embed", 0.0, es * static_cast<double>(T) * cols + 4.0 * n);
 
-    int bits = 32 - __builtin_clz(static_cast<unsigned>(vocab));  // of the keys 0 .. vocab
-    const int passes = (bits + 7) / 8;
-    bits = (bits + passes - 1) / passes;
+    const auto bits_of = [](unsigned last) { return last ? 32 - __builtin_clz(last) : 0; };  // of the numbers 0 .. last
     const int chunks = static_cast<int>(cdiv(T, CHUNK));
+    Sort so{ids, T, vocab, 0, dtable, n, beta};
+    // Ids of a block of the one-launch sort: two blocks a CU, up to a digit's.
+    long per = cdiv(static_cast<long>(vocab) + 1, 2L * ctx->num_cus);
+    if (per > DIGITS) per = DIGITS;
+    const dim3 ranges(static_cast<unsigned>(cdiv(static_cast<long>(vocab) + 1, per)));
+    if (T <= FEW) {
+        so.bits = bits_of(static_cast<unsigned>(per - 1));
+        if (dtype == KDEC_F32)
+            hipLaunchKernelGGL((sort_range_k<float, true>), ranges, dim3(ST), 0, ctx->stream, so, static_cast<int>(per), Tokens{},
+                               static_cast<const float*>(dY), dy_rs, cols, scale);
+        else
+            hipLaunchKernelGGL((sort_range_k<bf16, true>), ranges, dim3(ST), 0, ctx->stream, so, static_cast<int>(per), Tokens{},
+                               static_cast<const bf16*>(dY), dy_rs, cols, scale);
+        return launch_check(ctx, "kdec_embed_bwd");
+    }
     Sums s{};
     s.T = T;
     s.vocab = vocab;
     s.cols = cols;
-    s.piece = 32;
+    s.chunks = static_cast<int>(cdiv(cols, 64 * el));
+    // Tokens of a piece: the partial rows cost up to a piece's worth of two rows,
+    // eight waves a CU are what the loads need.
+    s.piece = 64;
+    while (s.piece > 16 && cdiv(T, s.piece) * s.chunks < 8L * ctx->num_cus) s.piece /= 2;
     s.pieces = static_cast<int>(cdiv(T, s.piece));
-    s.chunks = static_cast<int>(cdiv(cols, 512));
     s.scale = scale;
     s.table = dtable;
     s.add = beta != 0.0f;
     const long units = static_cast<long>(s.pieces) * s.chunks;
     KDEC_CHECK(ctx, cdiv(units, ET / 64) < INT_MAX && cdiv(cols, 256) <= 65535, "kdec_embed_bwd: bad sizes");
+    int bits = bits_of(static_cast<unsigned>(vocab));
+    const int passes = (bits + 7) / 8;
     const bool two = chunks > 1 && passes > 1;  // passes that read what the last one wrote
     const size_t part = cdiv(static_cast<long>(s.pieces) * 2 * cols, 4) * 4, ints = cdiv(T, 4) * 4;
     Workspace ws(ctx, (part + (two ? 4 : 2) * ints + static_cast<size_t>(DIGITS) * chunks) * 4);
@@ -458,35 +584,35 @@ int kdec_embed_bwd(kdec_ctx* ctx, int dtype, const void* dY, long dy_rs, const i
     int* room = reinterpret_cast<int*>(s.part + part);
     const Tokens to[2] = {{room, room + ints}, {room + 2 * ints, room + 3 * ints}};
     int* counts = room + (two ? 4 : 2) * ints;
-
-    Sort so{ids, T, vocab, bits, dtable, n, beta};
-    long fill = beta == 1.0f ? 0 : cdiv(n, 16L * ST);  // blocks beside the sort's
-    if (fill > ctx->num_cus - 1) fill = ctx->num_cus - 1;
     Tokens from{const_cast<int*>(ids), nullptr};
-    if (chunks <= 1) {
+    if (chunks == 1) {
+        so.bits = bits_of(static_cast<unsigned>(per - 1));
         from = to[0];
-        hipLaunchKernelGGL(sort_one_k, dim3(static_cast<unsigned>(1 + fill)), dim3(ST), 0, ctx->stream, so, passes, from);
-    }
-    for (int p = 0; chunks > 1 && p < passes; ++p) {
-        hipLaunchKernelGGL(sort_count_k, dim3(static_cast<unsigned>(chunks + (p == 0 ? fill : 0))), dim3(ST), 0, ctx->stream, so, p, chunks,
-                           from.id, counts);
-        hipLaunchKernelGGL(sort_place_k, dim3(static_cast<unsigned>(chunks)), dim3(ST), 0, ctx->stream, so, p, chunks, from.id, from.at,
-                           counts, to[p & 1]);
-        from = to[p & 1];
+        hipLaunchKernelGGL((sort_range_k<float, false>), ranges, dim3(ST), 0, ctx->stream, so, static_cast<int>(per), from, nullptr, 0, cols,
+                           scale);
+    } else {
+        so.bits = (bits + passes - 1) / passes;
+        long fill = beta == 1.0f ? 0 : cdiv(n, 16L * ST);  // blocks beside the first count's
+        if (fill > 2L * ctx->num_cus) fill = 2L * ctx->num_cus;
+        for (int p = 0; p < passes; ++p) {
+            hipLaunchKernelGGL(sort_count_k, dim3(static_cast<unsigned>(chunks + (p == 0 ? fill : 0))), dim3(ST), 0, ctx->stream, so, p,
+                               chunks, from.id, counts);
+            hipLaunchKernelGGL(sort_place_k, dim3(static_cast<unsigned>(chunks)), dim3(ST), 0, ctx->stream, so, p, chunks, from.id, from.at,
+                               counts, to[p & 1]);
+            from = to[p & 1];
+        }
     }
     s.id = from.id;
     s.at = from.at;
-    if (T > 0) {
-        const bool vec = cols % 8 == 0 && reinterpret_cast<size_t>(dY) % 16 == 0 && dy_rs % el == 0;
-        const dim3 grid(static_cast<unsigned>(cdiv(units, ET / 64)));
-        if (dtype == KDEC_F32)
-            hipLaunchKernelGGL(embed_sums_k<float>, grid, dim3(ET), 0, ctx->stream, s, static_cast<const float*>(dY), dy_rs, vec);
-        else
-            hipLaunchKernelGGL(embed_sums_k<bf16>, grid, dim3(ET), 0, ctx->stream, s, static_cast<const bf16*>(dY), dy_rs, vec);
-        if (s.pieces > 1)
-            hipLaunchKernelGGL(embed_join_k, dim3(static_cast<unsigned>(s.pieces - 1), static_cast<unsigned>(cdiv(cols, 256))), dim3(ET), 0,
-                               ctx->stream, s);
-    }
+    const bool vec = cols % el == 0 && reinterpret_cast<size_t>(dY) % 16 == 0 && dy_rs % el == 0;
+    const dim3 grid(static_cast<unsigned>(cdiv(units, ET / 64)));
+    if (dtype == KDEC_F32)
+        hipLaunchKernelGGL(embed_sums_k<float>, grid, dim3(ET), 0, ctx->stream, s, static_cast<const float*>(dY), dy_rs, vec);
+    else
+        hipLaunchKernelGGL(embed_sums_k<bf16>, grid, dim3(ET), 0, ctx->stream, s, static_cast<const bf16*>(dY), dy_rs, vec);
+    if (s.pieces > 1)
+        hipLaunchKernelGGL(embed_join_k, dim3(static_cast<unsigned>(s.pieces - 1), static_cast<unsigned>(cdiv(cols, 256))), dim3(ET), 0,
+                           ctx->stream, s);
     return launch_check(ctx, "kdec_embed_bwd");
 }
 

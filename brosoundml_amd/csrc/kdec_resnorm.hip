@@ -21,6 +21,8 @@
 #include "kdec_internal.hpp"
 
 #include <climits>
+#include <cmath>
+#include <type_traits>
 
 namespace kdec {
 namespace {
@@ -43,75 +45,114 @@ struct Norm {
     long r_rs, y_rs;
 };
 
-// W waves hold a row, R rows are in a block.
+// A row's waves and a block's rows: W is 1 or 2, with 4 or 2 rows a block, or 0
+// for one row in as many waves as the block has.
 template <int W>
 struct Block {
-    static constexpr int R = W >= 4 ? 1 : 4 / W, NT = 64 * W * R;
+    static constexpr int R = W ? 4 / W : 1, MAX = W ? 256 : 512;
+    __device__ static inline int waves() { return W ? W : blockDim.x >> 6; }
 };
 
+// The sum over a wave's lanes, in all of them.
 __device__ inline float wave_sum(float x) {
-#pragma unroll
-    for (int o = 32; o; o >>= 1) x += __shfl_xor(x, o);
-    return x;
+    const auto add = [&](auto ctrl, auto rows) __attribute__((always_inline)) {
+        x += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), decltype(ctrl)::value, decltype(rows)::value, 15, false));
+    };
+    typedef std::integral_constant<int, 15> All;
+    add(std::integral_constant<int, 0x111>{}, All{});  // lanes of 16 to the right by 1, 2, 4, 8
+    add(std::integral_constant<int, 0x112>{}, All{});
+    add(std::integral_constant<int, 0x114>{}, All{});
+    add(std::integral_constant<int, 0x118>{}, All{});
+    add(std::integral_constant<int, 0x142>{}, std::integral_constant<int, 10>{});  // the 16's last lane to the next 16
+    add(std::integral_constant<int, 0x143>{}, std::integral_constant<int, 12>{});  // lane 31 to the upper half
+    return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), 63));
 }
 
 // Two sums over a row's lanes, the same in all of them. Waves of a row meet in
 // shared memory, in two buffers in turn so that one barrier a sum is enough.
+typedef float Meet[2][2][8];  // buffer, sum, wave of the row (or row and wave)
 template <int W>
-__device__ inline void row_sums(float& a, float& b, float (*red)[2][2 * W], int& turn) {
+__device__ inline void row_sums(float& a, float& b, Meet& red, int& turn) {
     a = wave_sum(a);
     b = wave_sum(b);
     if (W == 1) return;
-    const int wave = threadIdx.x >> 6, slot = wave / W, w = wave % W;
-    float* at = red[slot][turn];
+    const int wave = threadIdx.x >> 6, n = W ? W : blockDim.x >> 6, first = W ? wave / W * W : 0;
     if ((threadIdx.x & 63) == 0) {
-        at[2 * w] = a;
-        at[2 * w + 1] = b;
+        red[turn][0][wave] = a;
+        red[turn][1][wave] = b;
     }
     __syncthreads();
-    a = b = 0.0f;
+    a = red[turn][0][first];
+    b = red[turn][1][first];
+    if constexpr (W == 2) {
+        a += red[turn][0][first + 1];
+        b += red[turn][1][first + 1];
+    } else {
 #pragma unroll
-    for (int i = 0; i < W; ++i) {
-        a += at[2 * i];
-        b += at[2 * i + 1];
+        for (int i = 1; i < 8; ++i) {  // past the row's waves the sums stay as they are
+            a += i < n ? red[turn][0][i] : 0.0f;
+            b += i < n ? red[turn][1][i] : 0.0f;
+        }
     }
     turn ^= 1;
 }
 
+// Eight columns of a tensor's row, from byte offset `off` of it: zeros past the
+// row's end or where the tensor is absent, without a branch around the load, so
+// that a row's tensors are on their way together.
 template <class T>
-__device__ inline f32x8 floats8(const T* p, int n, bool vec) {
-    const Frag<T> f = load8(p, n, vec);
-    f32x8 r;
+struct Raw {
+    Frag<T> f;
+    __device__ inline f32x8 floats() const {
+        f32x8 r;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) r[i] = static_cast<float>(f[i]);
-    return r;
-}
-template <class T>
-__device__ inline f32x8 vector8(const void* p, int c, int n, bool vec, float none) {
-    if (p) return floats8(static_cast<const T*>(p) + c, n, vec);
-    f32x8 r;
+        for (int i = 0; i < 8; ++i) r[i] = static_cast<float>(f[i]);
+        return r;
+    }
+};
+template <class T, bool VEC>
+__device__ inline Raw<T> load_raw(const Rows& t, long row, int C, int c) {
+    const __amdgpu_buffer_rsrc_t r = uniform_rsrc(static_cast<const T*>(t.p) + row * t.rs, t.p ? C * static_cast<int>(sizeof(T)) : 0);
+    Raw<T> x;
+    if constexpr (VEC) {
+        x.f = buffer_load8(r, c * static_cast<int>(sizeof(T)), T{});
+    } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) r[i] = none;
-    return r;
+        for (int i = 0; i < 8; ++i) {
+            if constexpr (sizeof(T) == 2)
+                x.f[i] = __builtin_bit_cast(bf16, static_cast<unsigned short>(__builtin_amdgcn_raw_buffer_load_b16(r, 2 * (c + i), 0, 0)));
+            else
+                x.f[i] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(r, 4 * (c + i), 0, 0));
+        }
+    }
+    return x;
 }
-template <class T>
-__device__ inline void store8(T* p, int n, bool vec, const f32x8& v) {
+// The same of a vector of C, `none` where it is absent.
+template <class T, bool VEC>
+__device__ inline Raw<T> load_vector(const void* p, int C, int c, float none) {
+    if (p) return load_raw<T, VEC>(Rows{p, 0}, 0, C, c);
+    Raw<T> x;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x.f[i] = static_cast<T>(none);
+    return x;
+}
+template <class T, bool VEC>
+__device__ inline void store8(T* p, int n, const f32x8& v) {
     Frag<T> f;
 #pragma unroll
     for (int i = 0; i < 8; ++i) f[i] = static_cast<T>(v[i]);
-    if (vec) {
+    if constexpr (VEC) {
         if (n > 0) *reinterpret_cast<Frag<T>*>(p) = f;
-        return;
-    }
+    } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-        if (i < n) p[i] = f[i];
+        for (int i = 0; i < 8; ++i)
+            if (i < n) p[i] = f[i];
+    }
 }
 
 // A row's mean (0 for the RMS norm) and 1 / sqrt(mean square around it + eps).
 template <int V, int W>
-__device__ inline void moments(const Norm& p, const f32x8 (&u)[V], const int (&n)[V], float (*red)[2][2 * W], int& turn, float& mean,
-                               float& rstd) {
+__device__ inline void moments(const Norm& p, const f32x8 (&u)[V], const int (&n)[V], Meet& red, int& turn, float& mean, float& rstd) {
     float s = 0.0f, none = 0.0f;
     mean = 0.0f;
     if (p.layer) {
@@ -134,57 +175,68 @@ __device__ inline void moments(const Norm& p, const f32x8 (&u)[V], const int (&n
     rstd = 1.0f / sqrtf(s / static_cast<float>(p.C) + p.eps);
 }
 
-template <class T, int V, int W>
-__global__ __launch_bounds__(Block<W>::NT) void resnorm_k(Norm p) {
-    constexpr int R = Block<W>::R;
-    __shared__ float red[R][2][2 * W];
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-    const long row = static_cast<long>(blockIdx.x) * R + wave / W;
+template <class T, int V, int W, bool VEC>
+__global__ __launch_bounds__(Block<W>::MAX) void resnorm_k(Norm p) {
+    __shared__ Meet red;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, waves = Block<W>::waves();
+    const long row = static_cast<long>(blockIdx.x) * Block<W>::R + wave / waves;
     const bool live = row < p.T;
     const long at = live ? row : p.T - 1;
     int c[V], n[V], turn = 0;
+    f32x8 x[V], u[V], g[V];
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-        c[v] = 512 * (v * W + wave % W) + 8 * lane;
+        c[v] = 512 * (v * waves + wave % waves) + 8 * lane;
         n[v] = max(min(8, p.C - c[v]), 0);
+        x[v] = load_raw<T, VEC>(p.x, at, p.C, c[v]).floats();
+        u[v] = load_raw<T, VEC>(p.z, at, p.C, c[v]).floats();
+        g[v] = load_raw<T, VEC>(p.gate, at, p.C, c[v]).floats();
     }
-    f32x8 x[V], u[V];
-#pragma unroll
-    for (int v = 0; v < V; ++v) x[v] = floats8(static_cast<const T*>(p.x.p) + at * p.x.rs + c[v], n[v], p.vec);
     float m1 = 0.0f, s1 = 0.0f, m2 = 0.0f, s2 = 0.0f;
     if (p.z.p) {
-#pragma unroll
-        for (int v = 0; v < V; ++v) u[v] = floats8(static_cast<const T*>(p.z.p) + at * p.z.rs + c[v], n[v], p.vec);
         if (p.post) {
+            Raw<T> w[V], b[V];
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                w[v] = load_vector<T, VEC>(p.w1, p.C, c[v], 1.0f);
+                b[v] = load_vector<T, VEC>(p.b1, p.C, c[v], 0.0f);
+            }
             moments<V, W>(p, u, n, red, turn, m1, s1);
 #pragma unroll
             for (int v = 0; v < V; ++v) {
-                const f32x8 w = vector8<T>(p.w1, c[v], n[v], p.vec, 1.0f), b = vector8<T>(p.b1, c[v], n[v], p.vec, 0.0f);
+                const f32x8 wf = w[v].floats(), bf = b[v].floats();
 #pragma unroll
-                for (int i = 0; i < 8; ++i) u[v][i] = __builtin_fmaf((u[v][i] - m1) * s1, w[i], b[i]);
+                for (int i = 0; i < 8; ++i) u[v][i] = __builtin_fmaf((u[v][i] - m1) * s1, wf[i], bf[i]);
             }
         }
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-            const f32x8 g = p.gate.p ? vector8<T>(static_cast<const T*>(p.gate.p) + at * p.gate.rs, c[v], n[v], p.vec, 1.0f)
-                                     : vector8<T>(nullptr, 0, 0, false, 1.0f);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) x[v][i] = i < n[v] ? __builtin_fmaf(p.scale * g[i], u[v][i], p.x_scale * x[v][i]) : 0.0f;
-            if (live) store8(static_cast<T*>(p.r) + at * p.r_rs + c[v], n[v], p.vec, x[v]);
+            for (int i = 0; i < 8; ++i) {
+                const float a = p.gate.p ? p.scale * g[v][i] : p.scale;
+                x[v][i] = i < n[v] ? __builtin_fmaf(a, u[v][i], p.x_scale * x[v][i]) : 0.0f;
+            }
+            if (live) store8<T, VEC>(static_cast<T*>(p.r) + at * p.r_rs + c[v], n[v], x[v]);
         }
     }
     if (p.pre) {
+        Raw<T> w[V], b[V];
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            w[v] = load_vector<T, VEC>(p.w2, p.C, c[v], 1.0f);
+            b[v] = load_vector<T, VEC>(p.b2, p.C, c[v], 0.0f);
+        }
         moments<V, W>(p, x, n, red, turn, m2, s2);
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-            const f32x8 w = vector8<T>(p.w2, c[v], n[v], p.vec, 1.0f), b = vector8<T>(p.b2, c[v], n[v], p.vec, 0.0f);
+            const f32x8 wf = w[v].floats(), bf = b[v].floats();
             f32x8 y;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) y[i] = __builtin_fmaf((x[v][i] - m2) * s2, w[i], b[i]);
-            if (live) store8(static_cast<T*>(p.y) + at * p.y_rs + c[v], n[v], p.vec, y);
+            for (int i = 0; i < 8; ++i) y[i] = __builtin_fmaf((x[v][i] - m2) * s2, wf[i], bf[i]);
+            if (live) store8<T, VEC>(static_cast<T*>(p.y) + at * p.y_rs + c[v], n[v], y);
         }
     }
-    if (p.stats && live && lane == 0 && wave % W == 0) *reinterpret_cast<f32x4*>(p.stats + 4 * at) = f32x4{m1, s1, m2, s2};
+    if (p.stats && live && lane == 0 && wave % waves == 0) *reinterpret_cast<f32x4*>(p.stats + 4 * at) = f32x4{m1, s1, m2, s2};
 }
 
 struct Back {
@@ -195,54 +247,72 @@ struct Back {
     int sums, at[5];        // where dw1, db1, dw2, db2 and the columns' dgate are among them, -1: not in use
 };
 
-template <class T, int V, int W>
-__global__ __launch_bounds__(Block<W>::NT) void resnorm_bwd_k(Back b) {
+// A row's tensors, and its kept statistics, as they are loaded.
+template <class T, int V>
+struct Row {
+    Raw<T> x[V], z[V], g[V], dr[V], dy[V];
+    f32x4 st;
+};
+
+// Blocks take rows in turn, the next row's tensors on their way.
+template <class T, int V, int W, bool VEC>
+__global__ __launch_bounds__(Block<W>::MAX) void resnorm_bwd_k(Back b) {
     constexpr int R = Block<W>::R;
-    __shared__ float red[R][2][2 * W];
+    __shared__ Meet red;
     __shared__ float join[R > 1 ? R - 1 : 1][R > 1 ? 64 * W * 8 : 1];
     const Norm& p = b.n;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, waves = Block<W>::waves();
     int c[V], n[V], turn = 0;
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-        c[v] = 512 * (v * W + wave % W) + 8 * lane;
-        n[v] = max(min(8, p.C - c[v]), 0);
-    }
+    Raw<T> w1[V], b1[V], w2[V];
     f32x8 sum[5][V];
 #pragma unroll
-    for (int k = 0; k < 5; ++k)
+    for (int v = 0; v < V; ++v) {
+        c[v] = 512 * (v * waves + wave % waves) + 8 * lane;
+        n[v] = max(min(8, p.C - c[v]), 0);
+        if (V == 1) {
+            w1[v] = load_vector<T, VEC>(p.w1, p.C, c[v], 1.0f);
+            b1[v] = load_vector<T, VEC>(p.b1, p.C, c[v], 0.0f);
+            w2[v] = load_vector<T, VEC>(p.w2, p.C, c[v], 1.0f);
+        }
 #pragma unroll
-        for (int v = 0; v < V; ++v) sum[k][v] = f32x8{};
+        for (int k = 0; k < 5; ++k) sum[k][v] = f32x8{};
+    }
+    // A vector's columns: held over the rows, where the registers hold them.
+    const auto vec = [&](const Raw<T>& held, const void* from, int v, float none) __attribute__((always_inline)) {
+        return V == 1 ? held.floats() : load_vector<T, VEC>(from, p.C, c[v], none).floats();
+    };
     const float over = 1.0f / static_cast<float>(p.C);
-    for (long row0 = static_cast<long>(blockIdx.x) * R; row0 < p.T; row0 += static_cast<long>(gridDim.x) * R) {
-        const long row = row0 + wave / W;
-        const bool live = row < p.T;
-        const long at = live ? row : p.T - 1;
-        const auto load = [&](const Rows& t, int v) __attribute__((always_inline)) {
-            return floats8(static_cast<const T*>(t.p) + at * t.rs + c[v], live ? n[v] : 0, p.vec);
-        };
-        f32x8 rh[V], zh[V], d[V], dy[V];
-        const f32x4 st = *reinterpret_cast<const f32x4*>(p.stats + 4 * at);
+    const auto load = [&](long row0, Row<T, V>& o) __attribute__((always_inline)) {
+        const long at = min(row0 + wave / waves, p.T - 1L);
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-            rh[v] = load(p.x, v);
-            zh[v] = p.z.p ? load(p.z, v) : f32x8{};
-            d[v] = b.dr.p ? load(b.dr, v) : f32x8{};
-            dy[v] = p.pre ? load(b.dy, v) : f32x8{};
+            o.x[v] = load_raw<T, VEC>(p.x, at, p.C, c[v]);
+            o.z[v] = load_raw<T, VEC>(p.z, at, p.C, c[v]);
+            o.dr[v] = load_raw<T, VEC>(b.dr, at, p.C, c[v]);
+            o.dy[v] = load_raw<T, VEC>(b.dy, at, p.C, c[v]);
+            o.g[v] = load_raw<T, VEC>(p.gate, at, p.C, c[v]);
         }
+        o.st = *reinterpret_cast<const f32x4*>(p.stats + 4 * at);
+    };
+    const auto take = [&](long row0, const Row<T, V>& o) __attribute__((always_inline)) {
+        const long row = row0 + wave / waves;
+        const bool live = row < p.T;
+        const long at = live ? row : p.T - 1;
+        f32x8 rh[V], zh[V], d[V];
+        const f32x4 st = o.st;
         const auto gate = [&](int v) __attribute__((always_inline)) {
-            f32x8 g = p.gate.p ? load(p.gate, v) : vector8<T>(nullptr, 0, 0, false, 1.0f);
+            f32x8 g = o.g[v].floats();
 #pragma unroll
-            for (int i = 0; i < 8; ++i) g[i] *= p.scale;
+            for (int i = 0; i < 8; ++i) g[i] = p.gate.p ? p.scale * g[i] : p.scale;
             return g;
         };
         // the normalised rows
 #pragma unroll
         for (int v = 0; v < V; ++v) {
+            rh[v] = o.x[v].floats();
+            zh[v] = o.z[v].floats();
             if (p.z.p) {
-                const f32x8 w = p.post ? vector8<T>(p.w1, c[v], n[v], p.vec, 1.0f) : f32x8{};
-                const f32x8 bias = p.post ? vector8<T>(p.b1, c[v], n[v], p.vec, 0.0f) : f32x8{};
-                const f32x8 g = gate(v);
+                const f32x8 g = gate(v), w = vec(w1[v], p.w1, v, 1.0f), bias = vec(b1[v], p.b1, v, 0.0f);
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
                     float u = zh[v][i];
@@ -255,63 +325,65 @@ __global__ __launch_bounds__(Block<W>::NT) void resnorm_bwd_k(Back b) {
             }
 #pragma unroll
             for (int i = 0; i < 8; ++i) rh[v][i] = (rh[v][i] - st[2]) * st[3];
+            d[v] = o.dr[v].floats();
         }
         if (p.pre) {
             float e1 = 0.0f, e2 = 0.0f;
 #pragma unroll
             for (int v = 0; v < V; ++v) {
-                const f32x8 w = vector8<T>(p.w2, c[v], n[v], p.vec, 1.0f);
+                const f32x8 w = vec(w2[v], p.w2, v, 1.0f), dy = o.dy[v].floats();
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    if (i < n[v] && live) {
-                        sum[2][v][i] = __builtin_fmaf(dy[v][i], rh[v][i], sum[2][v][i]);
-                        sum[3][v][i] += dy[v][i];
+                    if (live) {
+                        sum[2][v][i] = __builtin_fmaf(dy[i], rh[v][i], sum[2][v][i]);
+                        sum[3][v][i] += dy[i];
                     }
-                    dy[v][i] = i < n[v] ? dy[v][i] * w[i] : 0.0f;
-                    e1 += dy[v][i];
-                    e2 = i < n[v] ? __builtin_fmaf(dy[v][i], rh[v][i], e2) : e2;
+                    const float e = dy[i] * w[i];  // zero past the row's end
+                    e1 += e;
+                    e2 = i < n[v] ? __builtin_fmaf(e, rh[v][i], e2) : e2;
                 }
             }
             row_sums<W>(e1, e2, red, turn);
             e1 = p.layer ? e1 * over : 0.0f;
             e2 *= over;
 #pragma unroll
-            for (int v = 0; v < V; ++v)
+            for (int v = 0; v < V; ++v) {
+                const f32x8 w = vec(w2[v], p.w2, v, 1.0f), dy = o.dy[v].floats();
 #pragma unroll
-                for (int i = 0; i < 8; ++i) d[v][i] += st[3] * (dy[v][i] - e1 - rh[v][i] * e2);
+                for (int i = 0; i < 8; ++i) d[v][i] += st[3] * (dy[i] * w[i] - e1 - rh[v][i] * e2);
+            }
         }
         if (live)
 #pragma unroll
             for (int v = 0; v < V; ++v) {
-                f32x8 o;
+                f32x8 x;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) o[i] = p.x_scale * d[v][i];
-                store8(static_cast<T*>(b.dx) + at * p.C + c[v], n[v], p.vec, o);
+                for (int i = 0; i < 8; ++i) x[i] = p.x_scale * d[v][i];
+                store8<T, VEC>(static_cast<T*>(b.dx) + at * p.C + c[v], n[v], x);
             }
-        if (!p.z.p) continue;
+        if (!p.z.p) return;
         float f1 = 0.0f, f2 = 0.0f;
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-            const f32x8 w = p.post ? vector8<T>(p.w1, c[v], n[v], p.vec, 1.0f) : f32x8{};
+            const f32x8 g = gate(v), w = vec(w1[v], p.w1, v, 1.0f);
             if (p.gate.p) {  // scale u d
-                const f32x8 bias = p.post ? vector8<T>(p.b1, c[v], n[v], p.vec, 0.0f) : f32x8{};
-                f32x8 o;
+                const f32x8 bias = vec(b1[v], p.b1, v, 0.0f);
+                f32x8 x;
 #pragma unroll
                 for (int i = 0; i < 8; ++i)
-                    o[i] = p.scale * (p.post ? __builtin_fmaf(zh[v][i], w[i], bias[i]) : zh[v][i]) * d[v][i];
+                    x[i] = p.scale * (p.post ? __builtin_fmaf(zh[v][i], w[i], bias[i]) : zh[v][i]) * d[v][i];
                 if (b.dgate) {
-                    if (live) store8(static_cast<T*>(b.dgate) + at * p.C + c[v], n[v], p.vec, o);
+                    if (live) store8<T, VEC>(static_cast<T*>(b.dgate) + at * p.C + c[v], n[v], x);
                 } else if (live) {
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) sum[4][v][i] += i < n[v] ? o[i] : 0.0f;
+                    for (int i = 0; i < 8; ++i) sum[4][v][i] += x[i];
                 }
             }
-            const f32x8 g = gate(v);
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                d[v][i] = i < n[v] ? d[v][i] * g[i] : 0.0f;  // du
+                d[v][i] *= g[i];  // du
                 if (p.post) {
-                    if (i < n[v] && live) {
+                    if (live) {
                         sum[0][v][i] = __builtin_fmaf(d[v][i], zh[v][i], sum[0][v][i]);
                         sum[1][v][i] += d[v][i];
                     }
@@ -332,7 +404,24 @@ __global__ __launch_bounds__(Block<W>::NT) void resnorm_bwd_k(Back b) {
         }
         if (live)
 #pragma unroll
-            for (int v = 0; v < V; ++v) store8(static_cast<T*>(b.dz) + at * p.C + c[v], n[v], p.vec, d[v]);
+            for (int v = 0; v < V; ++v) store8<T, VEC>(static_cast<T*>(b.dz) + at * p.C + c[v], n[v], d[v]);
+    };
+    const long step = static_cast<long>(gridDim.x) * R;
+    long row0 = static_cast<long>(blockIdx.x) * R;
+    Row<T, V> cur;
+    if constexpr (V == 1) {
+        Row<T, V> next;
+        load(row0, cur);
+        for (; row0 < p.T; row0 += step) {
+            load(row0 + step, next);
+            take(row0, cur);
+            cur = next;
+        }
+    } else {  // two rows at once do not fit the registers
+        for (; row0 < p.T; row0 += step) {
+            load(row0, cur);
+            take(row0, cur);
+        }
     }
     // the block's rows together, then its share of every sum
 #pragma unroll
@@ -340,7 +429,7 @@ __global__ __launch_bounds__(Block<W>::NT) void resnorm_bwd_k(Back b) {
         if (b.at[k] < 0) continue;
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-            if (R > 1) {
+            if constexpr (R > 1) {
                 const int slot = wave / W, place = 8 * (threadIdx.x % (64 * W));
                 __syncthreads();
                 if (slot > 0)
@@ -385,15 +474,27 @@ __global__ __launch_bounds__(64 * JW) void resnorm_join_k(const float* part, int
     out.p[k][c] = a;
 }
 
-// Waves and columns a lane of a row: as few waves as hold it in a register
-// block of 8 V columns a lane.
-template <class T, class F>
-int by_width(int C, F f) {
-    if (C <= 512) return f(std::integral_constant<int, 1>{}, std::integral_constant<int, 1>{});
-    if (C <= 1024) return f(std::integral_constant<int, 1>{}, std::integral_constant<int, 2>{});
-    if (C <= 2048) return f(std::integral_constant<int, 1>{}, std::integral_constant<int, 4>{});
-    if (C <= 4096) return f(std::integral_constant<int, 2>{}, std::integral_constant<int, 4>{});
-    return f(std::integral_constant<int, 2>{}, std::integral_constant<int, 8>{});
+// A row's registers and waves: 512 columns a wave and register block.
+struct Shape {
+    int V, W, rows, threads;
+};
+Shape shape(int C) {
+    const int V = C <= 4096 ? 1 : 2, W = static_cast<int>(cdiv(C, 512 * V)), rows = W <= 2 ? 4 / W : 1;
+    return Shape{V, W, rows, 64 * W * rows};
+}
+template <class F>
+void by_shape(const Shape& s, bool vec, F f) {
+    const auto go = [&](auto V, auto W) {
+        if (vec) f(V, W, std::true_type{});
+        else f(V, W, std::false_type{});
+    };
+    typedef std::integral_constant<int, 0> Any;
+    typedef std::integral_constant<int, 1> One;
+    typedef std::integral_constant<int, 2> Two;
+    if (s.V == 2) go(Two{}, Any{});
+    else if (s.W == 1) go(One{}, One{});
+    else if (s.W == 2) go(One{}, Two{});
+    else go(One{}, Any{});
 }
 
 bool wide(const void* p, long rs, int es) { return reinterpret_cast<size_t>(p) % 16 == 0 && rs * es % 16 == 0; }
@@ -457,13 +558,12 @@ int kdec_resnorm_fwd(kdec_ctx* ctx, int dtype, int layer, const void* X, long x_
     p.y_rs = y_rs;
     p.stats = stats;
     ProfScope ps(ctx, "resnorm", 0.0, static_cast<double>(es) * T * C * (1 + (Z ? 2 : 0) + (pre ? 1 : 0) + (gate && gate_rs ? 1 : 0)));
+    const Shape sh = shape(C);
     const auto run = [&](auto ty) {
         typedef decltype(ty) E;
-        return by_width<E>(C, [&](auto v, auto w) {
-            constexpr int V = decltype(v)::value, W = decltype(w)::value;
-            hipLaunchKernelGGL((resnorm_k<E, V, W>), dim3(static_cast<unsigned>(cdiv(T, Block<W>::R))), dim3(Block<W>::NT), 0, ctx->stream,
-                               p);
-            return KDEC_OK;
+        by_shape(sh, p.vec, [&](auto v, auto w, auto vec) {
+            hipLaunchKernelGGL((resnorm_k<E, decltype(v)::value, decltype(w)::value, decltype(vec)::value>),
+                               dim3(static_cast<unsigned>(cdiv(T, sh.rows))), dim3(sh.threads), 0, ctx->stream, p);
         });
     };
     if (dtype == KDEC_F32) run(0.0f);
@@ -501,24 +601,26 @@ int kdec_resnorm_bwd(kdec_ctx* ctx, int dtype, int layer, const void* X, long x_
         if (given[k]) outs.p[b.sums++] = given[k];
     }
     ProfScope ps(ctx, "resnorm", 0.0, static_cast<double>(es) * T * C * (3 + (Z ? 2 : 0) + (pre ? 1 : 0) + (by_row ? 2 : 0)));
+    const Shape sh = shape(C);
+    long blocks = cdiv(T, sh.rows);
+    if (blocks > 2L * ctx->num_cus) blocks = 2L * ctx->num_cus;
+    Workspace ws(ctx, static_cast<size_t>(blocks) * b.sums * C * sizeof(float));
+    if (!ws.p) return KDEC_ENOMEM;
+    b.part = ws.as<float>();
     const auto run = [&](auto ty) {
         typedef decltype(ty) E;
-        return by_width<E>(C, [&](auto v, auto w) {
-            constexpr int V = decltype(v)::value, W = decltype(w)::value, R = Block<W>::R;
-            long blocks = cdiv(T, R);
-            if (blocks > 2L * ctx->num_cus) blocks = 2L * ctx->num_cus;
-            Workspace ws(ctx, static_cast<size_t>(blocks) * b.sums * C * sizeof(float));
-            if (!ws.p) return KDEC_ENOMEM;
-            b.part = ws.as<float>();
-            if (T > 0)
-                hipLaunchKernelGGL((resnorm_bwd_k<E, V, W>), dim3(static_cast<unsigned>(blocks)), dim3(Block<W>::NT), 0, ctx->stream, b);
-            if (b.sums)
-                hipLaunchKernelGGL(resnorm_join_k, dim3(static_cast<unsigned>(cdiv(C, 64)), static_cast<unsigned>(b.sums)), dim3(64 * JW), 0,
-                                   ctx->stream, b.part, static_cast<int>(blocks), b.sums, C, outs);
-            return KDEC_OK;
+        by_shape(sh, b.n.vec, [&](auto v, auto w, auto vec) {
+            hipLaunchKernelGGL((resnorm_bwd_k<E, decltype(v)::value, decltype(w)::value, decltype(vec)::value>),
+                               dim3(static_cast<unsigned>(blocks)), dim3(sh.threads), 0, ctx->stream, b);
         });
     };
-    if (int rc = dtype == KDEC_F32 ? run(0.0f) : run(bf16{})) return rc;
+    if (T > 0) {
+        if (dtype == KDEC_F32) run(0.0f);
+        else run(bf16{});
+    }
+    if (b.sums)
+        hipLaunchKernelGGL(resnorm_join_k, dim3(static_cast<unsigned>(cdiv(C, 64)), static_cast<unsigned>(b.sums)), dim3(64 * JW), 0,
+                           ctx->stream, b.part, static_cast<int>(blocks), b.sums, C, outs);
     return launch_check(ctx, "kdec_resnorm_bwd");
 }
 
