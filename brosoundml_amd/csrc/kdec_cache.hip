@@ -2,10 +2,8 @@
 // back as floats. The attention over it is kdec_attn_cache.hip.
 //
 // A token's values in one head share a scale, s = max(max |x| / 127, 2^-126) in
-// float, and are held as the integers nearest to x / s. Nearest is decided
-// exactly (the product with 1 / s may be one off near a half, the remainder
-// x - q s is exact and says so; ties go to the even integer), so the codes are
-// those of the definition on every machine. A token with a value that is not
+// float, and are held as the integers nearest to x / s, ties to the even one,
+// decided exactly: the codes are those of the definition on every machine. A token with a value that is not
 // finite gets the scale NaN and codes of zero.
 //
 // 8 or 16 lanes take the values of a token in a head, eight each; bound by
@@ -37,12 +35,58 @@ __device__ inline long cache_row(const Docs& m, int i, int first) {
     return p < 0 ? -1 : static_cast<long>(c.k0) + p;
 }
 
-__device__ inline int nearest(float x, float s, float inv) {
-    float q = rintf(x * inv);
-    const float r = __builtin_fmaf(-q, s, x), r2 = 2.0f * __builtin_fabsf(r);
-    const bool odd = static_cast<int>(q) & 1;
-    if (r2 > s || (r2 == s && odd)) q += r > 0.0f ? 1.0f : -1.0f;
-    return static_cast<int>(q);
+// The largest magnitude of eight values as the bits of a float; more than
+// infinity's where one of them is NaN.
+__device__ inline unsigned top8(bf16x8 f) {
+    typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+    typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+    const u32x4 b = __builtin_bit_cast(u32x4, f) & 0x7FFF7FFFu;
+    u16x2 m = __builtin_bit_cast(u16x2, static_cast<unsigned>(b[0]));
+#pragma unroll
+    for (int i = 1; i < 4; ++i) m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, static_cast<unsigned>(b[i])));
+    return static_cast<unsigned>(max(m[0], m[1])) << 16;
+}
+__device__ inline unsigned top8(f32x8 f) {
+    unsigned m = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(f[i]) & 0x7FFFFFFFu);
+    return m;
+}
+// The largest over L neighbouring lanes, in all of them.
+template <int L>
+__device__ inline unsigned top_lanes(unsigned x) {
+    const auto with = [&](auto ctrl) __attribute__((always_inline)) {
+        x = max(x, static_cast<unsigned>(__builtin_amdgcn_update_dpp(0, static_cast<int>(x), decltype(ctrl)::value, 15, 15, true)));
+    };
+    with(std::integral_constant<int, 0xB1>{});   // the lane beside
+    with(std::integral_constant<int, 0x4E>{});   // the pair beside
+    with(std::integral_constant<int, 0x141>{});  // the four of eight opposite
+    if (L == 16) with(std::integral_constant<int, 0x140>{});  // the eight of sixteen opposite
+    return x;
+}
+
+// Eight values' codes under scale s. x / s by the reciprocal is off by 2^-22 of
+// it, so that its nearest integer q is the quotient's own, but next to a half:
+// the remainder x - q s is exact, and tells by being half of s or more.
+__device__ inline i8x8 nearest8(const f32x8& x, float s) {
+    const float inv = __builtin_amdgcn_rcpf(s);
+    float q[8], most = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        q[i] = __builtin_rintf(x[i] * inv);
+        most = fmaxf(most, __builtin_fabsf(__builtin_fmaf(-q[i], s, x[i])));
+    }
+    if (__builtin_amdgcn_ballot_w64(2.0f * most >= s)) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float r = __builtin_fmaf(-q[i], s, x[i]), r2 = 2.0f * __builtin_fabsf(r);
+            if (r2 > s || (r2 == s && (static_cast<int>(q[i]) & 1))) q[i] += r > 0.0f ? 1.0f : -1.0f;
+        }
+    }
+    i8x8 c;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) c[i] = static_cast<signed char>(static_cast<int>(q[i]));
+    return c;
 }
 
 // L lanes take UNITS heads' keys or values of a row (unit u: head u / 2, keys or
@@ -64,24 +108,14 @@ __global__ __launch_bounds__(CT) void cache_write_k(Docs m, Heads K, Heads V, Co
     for (int j = 0; j < UNITS; ++j) {
         const bool keys = !((u0 + j) & 1);
         const int head = (u0 + j) >> 1;
-        float x[8], top = 0.0f, zero = 0.0f;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            x[i] = static_cast<float>(f[j][i]);
-            top = fmaxf(top, __builtin_fabsf(x[i]));
-            zero = __builtin_fmaf(x[i], 0.0f, zero);
-        }
-#pragma unroll
-        for (int s = 1; s < L; s *= 2) {
-            top = fmaxf(top, __shfl_xor(top, s));
-            zero += __shfl_xor(zero, s);
-        }
+        const unsigned top = top_lanes<L>(top8(f[j]));
         if (at < 0 || head >= H) continue;
-        const bool bad = !(zero == 0.0f);
-        const float s = bad ? __builtin_nanf("") : fmaxf(top / 127.0f, 0x1p-126f), inv = 1.0f / s;
-        i8x8 q;
+        const bool bad = top >= 0x7F800000u;
+        const float s = bad ? __builtin_nanf("") : fmaxf(__uint_as_float(top) / 127.0f, 0x1p-126f);
+        f32x8 x;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) q[i] = static_cast<signed char>(bad ? 0 : nearest(x[i], s, inv));
+        for (int i = 0; i < 8; ++i) x[i] = bad ? 0.0f : static_cast<float>(f[j][i]);
+        const i8x8 q = nearest8(x, bad ? 1.0f : s);
         signed char* to = (keys ? o.k + at * o.k_rs + head * o.k_hs : o.v + at * o.v_rs + head * o.v_hs) + c;
         if (c < W) *reinterpret_cast<i8x8*>(to) = q;
         if (lane == 0) (keys ? o.ks : o.vs)[static_cast<long>(head) * m.Tk + at] = s;

@@ -13,8 +13,8 @@
 //
 // The sort is one launch: block b owns a range of ids, looks at all tokens,
 // counts those of lower ids and ranks its own (within 64 tokens by ballots over
-// the id's bits, then by wave and id with one scan). It also clears the table's
-// rows that no token has, which the sums leave alone. More tokens than a block
+// the id's bits, then by wave and id with one scan). It also begins its ids' rows of the table (cleared, or scaled by beta),
+// before anything else: these stores go their way while the block sorts. More tokens than a block
 // holds take a radix sort over several blocks.
 #include "kdec_frag.hpp"
 #include "kdec_internal.hpp"
@@ -237,6 +237,22 @@ __global__ __launch_bounds__(ST) void sort_range_k(Sort s, int per, Tokens out, 
         const int i = first + 64 * g;
         id[g] = g < r.n && i < s.T ? key_of(s.ids[i], s.vocab) : INT_MAX;
     }
+    // the table's rows, a wave 64 places of a row at a time
+    const int n = min(per, s.vocab - lo);
+    const bool vec = cols % 4 == 0 && reinterpret_cast<size_t>(s.table) % 16 == 0;
+    const int width = vec ? cols / 4 : cols, each = (width + 63) / 64;
+    if (s.beta != 1.0f)
+        for (int u = __builtin_amdgcn_readfirstlane(wave); u < n * each; u += WAVES) {
+            const int row = u / each, c = 64 * (u - row * each) + (tid & 63);
+            if (c >= width) continue;
+            float* to = s.table + static_cast<long>(lo + row) * cols;
+            if (vec) {
+                f32x4* q = reinterpret_cast<f32x4*>(to) + c;
+                *q = s.beta == 0.0f ? f32x4{} : *q * s.beta;
+            } else {
+                to[c] = s.beta == 0.0f ? 0.0f : to[c] * s.beta;
+            }
+        }
 #pragma unroll
     for (int g = 0; g < SI; ++g) {
         less += id[g] < lo;
@@ -264,22 +280,6 @@ __global__ __launch_bounds__(ST) void sort_range_k(Sort s, int per, Tokens out, 
         }
     });
     __syncthreads();
-    // rows that no token has, a wave 64 places of a row at a time
-    const int n = min(per, s.vocab - lo);
-    const bool vec = cols % 4 == 0 && reinterpret_cast<size_t>(s.table) % 16 == 0;
-    const int width = vec ? cols / 4 : cols, each = (width + 63) / 64;
-    if (s.beta != 1.0f)
-        for (int u = __builtin_amdgcn_readfirstlane(wave); u < n * each; u += WAVES) {
-            const int row = u / each, c = 64 * (u - row * each) + (tid & 63);
-            if ((s.beta == 0.0f && start[row] != start[row + 1]) || c >= width) continue;
-            float* to = s.table + static_cast<long>(lo + row) * cols;
-            if (vec) {
-                f32x4* q = reinterpret_cast<f32x4*>(to) + c;
-                *q = s.beta == 0.0f ? f32x4{} : *q * s.beta;
-            } else {
-                to[c] = s.beta == 0.0f ? 0.0f : to[c] * s.beta;
-            }
-        }
     if (!SUM) return;
     __syncthreads();
     for (int row = 0; row < n; ++row) {
@@ -545,8 +545,8 @@ int kdec_embed_bwd(kdec_ctx* ctx, int dtype, const void* dY, long dy_rs, const i
     const auto bits_of = [](unsigned last) { return last ? 32 - __builtin_clz(last) : 0; };  // of the numbers 0 .. last
     const int chunks = static_cast<int>(cdiv(T, CHUNK));
     Sort so{ids, T, vocab, 0, dtable, n, beta};
-    // Ids of a block of the one-launch sort: two blocks a CU, up to a digit's.
-    long per = cdiv(static_cast<long>(vocab) + 1, 2L * ctx->num_cus);
+    // Ids of a block of the one-launch sort: a block a CU, up to a digit's.
+    long per = cdiv(static_cast<long>(vocab) + 1, static_cast<long>(ctx->num_cus));
     if (per > DIGITS) per = DIGITS;
     const dim3 ranges(static_cast<unsigned>(cdiv(static_cast<long>(vocab) + 1, per)));
     if (T <= FEW) {
