@@ -46,17 +46,17 @@ def _no_graph(x):
 
 def _dtype(ctx, x, *others):
     """The C ABI's type of x, which the others must share, all on the context's device."""
-    ty, dev = x.dtype, x.device
+    ty, dev = x.dtype, ctx.device
     if ty not in _TYPES:
         _fail("tensors must be float32 or bfloat16")
-    if dev.type != "cuda" or dev.index != ctx.device:
+    if x.get_device() != dev:
         _fail("tensors must be on the context's HIP device")
     if x.requires_grad:
         _no_graph(x)
     for t in others:
         if t.requires_grad:
             _no_graph(t)
-        if t.dtype != ty or t.device != dev:
+        if t.dtype != ty or t.get_device() != dev:
             _fail("tensors must share one type and device")
     return _TYPES[ty]
 
@@ -109,7 +109,7 @@ def _whole(x, shape, what):
 def _empty(ctx, x, shape, dtype=None):
     """A new tensor of x's type (or dtype) and device that belongs to the context's stream."""
     if _raw_stream(ctx.device) == ctx.stream.cuda_stream:
-        return x.new_empty(shape, dtype=dtype)
+        return x.new_empty(shape) if dtype is None else x.new_empty(shape, dtype=dtype)
     with torch.cuda.stream(ctx.stream):
         return x.new_empty(shape, dtype=dtype)
 
@@ -265,16 +265,15 @@ def embedding(ctx: Context, table, ids, *, scale=1.0, out=None):
     dt = _dtype(ctx, table)
     W = _rows(table, "table")
     vocab, cols = table.shape
+    t = ids.numel()
     if ids.dim() != 1:
         _fail("ids must be (T)")
-    t = ids.shape[0]
-    I = _ints(ctx, ids, t, "ids")
-    y = _empty(ctx, table, (t, cols)) if out is None else out
-    if out is not None:
-        _dtype(ctx, table, y)
-        if y.shape != (t, cols):
-            _fail("out must be (T, columns)")
-    ctx.call("kdec_embed_fwd", dt, *W, I, t, vocab, cols, float(scale), *_rows(y, "out"))
+    if out is None:
+        y = _empty(ctx, table, (t, cols))
+        Y = y.data_ptr(), cols
+    else:
+        y, Y = out, _as(ctx, out, table.dtype, (t, cols), "out must be (T, columns)")
+    ctx.call("kdec_embed_fwd", dt, *W, _ints(ctx, ids, t, "ids"), t, vocab, cols, float(scale), *Y)
     return y
 
 
@@ -295,48 +294,64 @@ def embedding_bwd(ctx: Context, ids, dy, vocab, *, scale=1.0, dtable=None, beta=
     return g
 
 
+def _as(ctx, t, ty, shape, what):
+    """Address and row stride of a (rows, columns) tensor that must have this type and shape."""
+    if t.dtype != ty or t.get_device() != ctx.device:
+        _fail("tensors must share one type and device")
+    if t.requires_grad:
+        _no_graph(t)
+    if t.shape != shape:
+        _fail(what)
+    return _rows(t, what)
+
+
+def _norm_vectors(ctx, wb, ty, c, what):
+    """A norm's flag and the addresses of its weight and bias."""
+    if wb is None:
+        return 0, None, None
+    if not isinstance(wb, (tuple, list)):
+        wb = (wb, None)
+    if len(wb) != 2:
+        _fail(f"{what} must be a weight or (weight, bias)")
+    return 1, _vector(ctx, wb[0], ty, c, what), _vector(ctx, wb[1], ty, c, what)
+
+
+def _vector(ctx, v, ty, c, what):
+    if v is None:
+        return None
+    if v.dtype != ty or v.get_device() != ctx.device:
+        _fail("tensors must share one type and device")
+    if v.requires_grad:
+        _no_graph(v)
+    if v.shape != (c,) or not v.is_contiguous():
+        _fail(f"{what} must be contiguous, of shape {(c,)}")
+    return v.data_ptr()
+
+
 def _norm_args(ctx, x, z, gate, post, pre, kind, eps, scale, x_scale):
-    dt = _dtype(ctx, x)
-    X = _rows(x, "x")
-    t, c = x.shape
-    if kind not in ("rms", "layer"):
+    """The arguments that both directions share, and x's type and shape."""
+    dt, X, ty, shape = _dtype(ctx, x), _rows(x, "x"), x.dtype, x.shape
+    t, c = shape
+    if kind != "rms" and kind != "layer":
         _fail("kind must be 'rms' or 'layer'")
-
-    def rows(v, what):
-        if v is None:
-            return None, 0
-        _dtype(ctx, x, v)
-        if v.shape != x.shape:
-            _fail(f"{what} must be as x")
-        return _rows(v, what)
-
-    def norm(wb, what):
-        if wb is None:
-            return 0, None, None
-        if not isinstance(wb, (tuple, list)):
-            wb = (wb, None)
-        if len(wb) != 2:
-            _fail(f"{what} must be a weight or (weight, bias)")
-        for v in wb:
-            if v is not None:
-                _dtype(ctx, x, v)
-                _whole(v, (c,), what)
-        return (1, *(None if v is None else v.data_ptr() for v in wb))
-
-    if gate is not None and gate.dim() == 1:
-        _dtype(ctx, x, gate)
-        G = _whole(gate, (c,), "gate"), 0
+    G = None, 0
+    if z is None:
+        Z = None, 0
+        if post is not None or gate is not None or x_scale != 1.0 or pre is None:
+            _fail("without z there is the norm of x alone")
     else:
-        G = rows(gate, "gate")
-        if gate is not None and G[1] == 0:  # which the C ABI takes for one gate for all rows
-            if t > 1:
-                _fail("one gate for all rows must be (columns)")
-            G = G[0], c
-    if z is None and (post is not None or gate is not None or x_scale != 1.0 or pre is None):
-        _fail("without z there is the norm of x alone")
-    args = (dt, int(kind == "layer"), *X, *rows(z, "z"), *G, *norm(post, "post"), *norm(pre, "pre"), float(eps), float(scale), float(x_scale),
-            t, c)
-    return args, rows
+        Z = _as(ctx, z, ty, shape, "z must be as x")
+        if gate is not None:
+            if gate.dim() == 1:
+                G = _vector(ctx, gate, ty, c, "gate"), 0
+            else:
+                G = _as(ctx, gate, ty, shape, "gate must be (columns) or as x")
+                if G[1] == 0:  # which the C ABI takes for one gate for all rows
+                    if t > 1:
+                        _fail("one gate for all rows must be (columns)")
+                    G = G[0], c
+    return (dt, int(kind == "layer"), *X, *Z, *G, *_norm_vectors(ctx, post, ty, c, "post"), *_norm_vectors(ctx, pre, ty, c, "pre"), float(eps),
+            float(scale), float(x_scale), t, c), ty, (t, c)
 
 
 def residual_norm(ctx: Context, x, z=None, *, gate=None, post=None, pre=None, kind="rms", eps=1e-5, scale=1.0, x_scale=1.0, keep=False,
@@ -353,20 +368,25 @@ def residual_norm(ctx: Context, x, z=None, *, gate=None, post=None, pre=None, ki
     N_pre(x), and r is x. ``out`` may give r and y, (r, y). Returns (r, y), y
     None without ``pre``, and with ``keep`` also the statistics that the
     backward takes."""
-    args, rows = _norm_args(ctx, x, z, gate, post, pre, kind, eps, scale, x_scale)
-    t, c = x.shape
+    args, ty, shape = _norm_args(ctx, x, z, gate, post, pre, kind, eps, scale, x_scale)
     r, y = out if out is not None else (None, None)
+    R = Y = None, 0
     if z is None:
         r = x
     elif r is None:
-        r = _empty(ctx, x, (t, c))
+        r = _empty(ctx, x, shape)
+        R = r.data_ptr(), shape[1]
+    else:
+        R = _as(ctx, r, ty, shape, "r must be as x")
     if pre is None:
         y = None
     elif y is None:
-        y = _empty(ctx, x, (t, c))
-    stats = _empty(ctx, x, (t, 4), torch.float32) if keep else None
-    R = (None, 0) if z is None else rows(r, "r")
-    ctx.call("kdec_resnorm_fwd", *args, *R, *rows(y, "y"), None if stats is None else stats.data_ptr())
+        y = _empty(ctx, x, shape)
+        Y = y.data_ptr(), shape[1]
+    else:
+        Y = _as(ctx, y, ty, shape, "y must be as x")
+    stats = _empty(ctx, x, (shape[0], 4), torch.float32) if keep else None
+    ctx.call("kdec_resnorm_fwd", *args, *R, *Y, None if stats is None else stats.data_ptr())
     return (r, y, stats) if keep else (r, y)
 
 
@@ -376,26 +396,27 @@ def residual_norm_bwd(ctx: Context, x, z, dr, dy, stats, *, gate=None, post=None
     (kdec_resnorm_bwd). dx, dz and the gate's of each row are of x's type; the
     gradients of (C) vectors are float, dpost and dpre (weight's, bias's) with
     None where there is none."""
-    args, rows = _norm_args(ctx, x, z, gate, post, pre, kind, eps, scale, x_scale)
-    t, c = x.shape
+    args, ty, shape = _norm_args(ctx, x, z, gate, post, pre, kind, eps, scale, x_scale)
+    t, c = shape
     if (dy is None) != (pre is None):
         _fail("dy comes with pre")
     st = _floats(ctx, stats, (t, 4), "stats")
-    DR, DY = rows(dr, "dr"), rows(dy, "dy")
-    new = lambda *s: _empty(ctx, x, s)  # noqa: E731
-    floats = lambda: _empty(ctx, x, (c,), torch.float32)  # noqa: E731
-    dx, dz = new(t, c), None if z is None else new(t, c)
-    dgate = None if gate is None else floats() if gate.dim() == 1 else new(t, c)
+    DR = (None, 0) if dr is None else _as(ctx, dr, ty, shape, "dr must be as x")
+    DY = (None, 0) if dy is None else _as(ctx, dy, ty, shape, "dy must be as x")
+    dx, dz = _empty(ctx, x, shape), None if z is None else _empty(ctx, x, shape)
+    floats = lambda v: None if v is None else _empty(ctx, x, (c,), torch.float32)  # noqa: E731
+    dgate = None if gate is None else floats(gate) if gate.dim() == 1 else _empty(ctx, x, shape)
 
     def grads(wb):
         if wb is None:
             return None
         wb = wb if isinstance(wb, (tuple, list)) else (wb, None)
-        return tuple(None if v is None else floats() for v in wb)
+        return floats(wb[0]), floats(wb[1])
 
     dpost, dpre = grads(post), grads(pre)
     at = lambda v: None if v is None else v.data_ptr()  # noqa: E731
-    ctx.call("kdec_resnorm_bwd", *args, st, *DR, *DY, at(dx), at(dz), at(dgate), *map(at, dpost or (None, None)), *map(at, dpre or (None, None)))
+    ctx.call("kdec_resnorm_bwd", *args, st, *DR, *DY, dx.data_ptr(), at(dz), at(dgate), *map(at, dpost or (None, None)),
+             *map(at, dpre or (None, None)))
     return dx, dz, dgate, dpost, dpre
 
 
@@ -417,16 +438,16 @@ def new_cache(ctx: Context, rows, heads, width):
 
 
 def _cache_args(ctx, cache, width):
-    """Addresses and strides of a cache for the C ABI (codes, scales), its rows and heads."""
-    k, v = cache.k, cache.v
-    for t, what in ((k, "the cache's k"), (v, "the cache's v")):
-        if t.dtype != torch.int8 or t.get_device() != ctx.device:
-            _fail(f"{what} must be int8 on the device")
-    K, V = _heads(k, "the cache's k"), _heads(v, "the cache's v")
-    rows, heads, wide = k.shape
-    if v.shape != k.shape or wide != (width + 15) // 16 * 16:
-        _fail(f"the cache's k and v must be (rows, heads, {(width + 15) // 16 * 16})")
-    return K, V, (_floats(ctx, cache.k_scale, (heads, rows), "k_scale"), _floats(ctx, cache.v_scale, (heads, rows), "v_scale")), rows, heads
+    """A cache's codes and scales as the C ABI takes them, its rows and heads."""
+    k, v, ks, vs = cache
+    dev, shape, wide = ctx.device, k.shape, (width + 15) // 16 * 16
+    if k.dtype != torch.int8 or v.dtype != torch.int8 or k.get_device() != dev or v.get_device() != dev:
+        _fail("the cache's k and v must be int8 on the device")
+    if len(shape) != 3 or v.shape != shape or shape[2] != wide:
+        _fail(f"the cache's k and v must be (rows, heads, {wide})")
+    heads = shape[1], shape[0]
+    return (*_heads(k, "the cache's k"), *_heads(v, "the cache's v"), _floats(ctx, ks, heads, "k_scale"), _floats(ctx, vs, heads, "v_scale")), \
+        shape[0], shape[1]
 
 
 def _places(ctx, q_off, k_off, k_len):
@@ -445,26 +466,29 @@ def cache_write(ctx: Context, k, v, cache, q_off, k_off, k_len=None):
     dt = _dtype(ctx, k, v)
     K, V = _heads(k, "k"), _heads(v, "v")
     t, h, d = k.shape
-    Kc, Vc, scales, rows, heads = _cache_args(ctx, cache, d)
+    C, rows, heads = _cache_args(ctx, cache, d)
     if v.shape != k.shape or heads != h:
         _fail("k and v must share their shape, and the cache's heads")
-    ctx.call("kdec_cache_write", dt, *K, *V, *_places(ctx, q_off, k_off, k_len), t, rows, h, d, *Kc, *Vc, *scales)
+    ctx.call("kdec_cache_write", dt, *K, *V, *_places(ctx, q_off, k_off, k_len), t, rows, h, d, *C)
 
 
 def cache_read(ctx: Context, cache, q_off, k_off, k_len=None, *, rows, width, dtype=torch.bfloat16, out=None):
     """The tokens that ``cache_write`` with the same arguments wrote, as (k, v)
     of `rows` rows: (rows, heads, width) of ``dtype`` (kdec_cache_read). Rows
     that it would not have written are zeros."""
-    Kc, Vc, scales, tk, heads = _cache_args(ctx, cache, width)
+    C, tk, heads = _cache_args(ctx, cache, width)
     if out is None:
-        k, v = (_empty(ctx, cache.k, (rows, heads, width), dtype) for _ in range(2))
+        if dtype not in _TYPES:
+            _fail("tensors must be float32 or bfloat16")
+        shape = rows, heads, width
+        k, v = _empty(ctx, cache.k, shape, dtype), _empty(ctx, cache.k, shape, dtype)
+        dt, K, V = _TYPES[dtype], (k.data_ptr(), heads * width, width), (v.data_ptr(), heads * width, width)
     else:
         k, v = out
-    dt = _dtype(ctx, k, v)
-    if k.shape != (rows, heads, width) or v.shape != k.shape:
-        _fail("out must be two tensors (rows, heads, width)")
-    ctx.call("kdec_cache_read", dt, *Kc, *Vc, *scales, *_places(ctx, q_off, k_off, k_len), rows, tk, heads, width, *_heads(k, "k"),
-             *_heads(v, "v"))
+        dt, K, V = _dtype(ctx, k, v), _heads(k, "k"), _heads(v, "v")
+        if k.shape != (rows, heads, width) or v.shape != k.shape:
+            _fail("out must be two tensors (rows, heads, width)")
+    ctx.call("kdec_cache_read", dt, *C, *_places(ctx, q_off, k_off, k_len), rows, tk, heads, width, *K, *V)
     return k, v
 
 
@@ -476,15 +500,17 @@ def cache_attention(ctx: Context, q, cache, q_off, k_off, k_len=None, *, causal=
     dt = _dtype(ctx, q)
     Q = _heads(q, "q")
     tq, hq, d = q.shape
-    Kc, Vc, scales, tk, hkv = _cache_args(ctx, cache, d)
+    C, tk, hkv = _cache_args(ctx, cache, d)
     qo, ko, kl, docs = _places(ctx, q_off, k_off, k_len)
-    o = _empty(ctx, q, q.shape) if out is None else out
-    if out is not None:
-        _dtype(ctx, q, o)
-        if o.shape != q.shape:
+    if out is None:
+        o = _empty(ctx, q, (tq, hq, d))
+        O = o.data_ptr(), hq * d, d  # noqa: E741
+    else:
+        _dtype(ctx, q, out)
+        if out.shape != q.shape:
             _fail("out must be as q")
+        o, O = out, _heads(out, "out")  # noqa: E741
     lse = _empty(ctx, q, (hq, tq), torch.float32)
-    ctx.call("kdec_attn_cache_fwd", dt, *Q, *Kc, *Vc, *scales, qo, ko, kl, _ints(ctx, prefix, docs, "prefix"), docs, int(causal),
-             _floats(ctx, slopes, (hq,), "slopes"), float(d ** -0.5 if scale is None else scale), float(cap), tq, tk, hq, hkv, d,
-             *_heads(o, "out"), lse.data_ptr())
+    ctx.call("kdec_attn_cache_fwd", dt, *Q, *C, qo, ko, kl, _ints(ctx, prefix, docs, "prefix"), docs, int(causal),
+             _floats(ctx, slopes, (hq,), "slopes"), float(d ** -0.5 if scale is None else scale), float(cap), tq, tk, hq, hkv, d, *O, lse.data_ptr())
     return o, lse
