@@ -63,9 +63,57 @@ __device__ inline int doc_holding(const Docs& m, int row) {
     return __builtin_amdgcn_readfirstlane(d >= 0 && d < m.docs && row < m.q_off[d + 1] ? d : -1);
 }
 
+// A stretch of a block's rows that one document holds (or none), from row0 on.
+struct Segment {
+    Doc doc;
+    int causal, stop;  // the row behind it
+    __device__ inline int position(int row) const { return row - doc.q0 + doc.lk - doc.lq; }
+    // Keys that a row sees, from the slot's first: more of them from row to row.
+    __device__ inline int sees(int row) const {
+        return causal ? min(max(max(position(row) + 1, doc.prefix), 0), doc.lk) : doc.lk;
+    }
+};
+// The rows of a block: `rows` from a multiple of it, or as many of one document.
+__device__ inline bool block_rows(const Cached& p, int b, int& row0, int& end) {
+    row0 = b * p.rows;
+    end = min(row0 + p.rows, p.a.m.Tq);
+    if (!p.a.by_doc) return true;
+    Piece c;
+    if (!piece_at(p.a.m.q_off, p.a.m.docs, p.a.m.Tq, 1, p.rows, b, c)) return false;
+    row0 = c.lo + c.place * p.rows;
+    end = min(row0 + p.rows, c.hi);
+    return true;
+}
+// A part's tiles: of every document an equal share. (Parts of a fixed length, the
+// same work for short and long documents, were slower: one token for 48 requests
+// over 90 to 4096 keys 31 us for 26, since fewer of them run at once.)
+__device__ inline void part_tiles(const Cached& p, int tiles, int& t0, int& t1) {
+    t0 = static_cast<int>(static_cast<long>(tiles) * blockIdx.y / p.splits);
+    t1 = static_cast<int>(static_cast<long>(tiles) * (blockIdx.y + 1) / p.splits);
+}
+__device__ inline Segment segment_at(const Docs& m, int row0, int end) {
+    Segment s{Doc{0, 0, 0, 0, 0}, m.causal, end};
+    const int d = doc_holding(m, row0);
+    if (d >= 0) {
+        s.doc = doc_at(m, d);
+        s.stop = min(m.q_off[d + 1], end);
+    } else if (m.docs > 0 && row0 < m.q_off[0]) {
+        s.stop = min(m.q_off[0], end);
+    }
+    s.stop = __builtin_amdgcn_readfirstlane(max(s.stop, row0 + 1));
+    return s;
+}
+
+__device__ inline void empty_part(const Cached& p, int kvh, int e) {
+    const long to = (static_cast<long>(blockIdx.y) * p.a.Hkv + kvh) * p.a.E + e;
+    p.part_ml[2 * to] = -INF;
+    p.part_ml[2 * to + 1] = 0.0f;
+}
+
 // One step of the running softmax of a lane's column over the scores of 32 keys
 // from j0, `at` the lane's first: s become probabilities, acc is rescaled when
-// the wave's maxima move far enough. As soft_step of the float keys.
+// the wave's maxima move far enough: m in the units of raw products without cap
+// and bias, in log2 units with either.
 struct Soft {
     float m = -INF, l = 0.0f;
 };
@@ -117,8 +165,8 @@ __global__ __launch_bounds__(AT, sizeof(T) == 2 ? (CB == 1 ? 3 : 2) : 1) void at
     const int kvh = b % a.Hkv;
     b /= a.Hkv;
     const int piece = b % p.pieces, split = blockIdx.y, W = code_width(a.D);
-    int row0 = b / p.pieces * p.rows;
-    const int end = min(row0 + p.rows, a.m.Tq);
+    int row0, end;
+    if (!block_rows(p, b / p.pieces, row0, end)) return;
     const signed char* kb = static_cast<const signed char*>(a.K.p) + kvh * a.K.hs;
     const signed char* vb = static_cast<const signed char*>(a.V.p) + kvh * a.V.hs;
     const float* ks = p.ks + static_cast<long>(kvh) * a.m.Tk;
@@ -131,32 +179,25 @@ __global__ __launch_bounds__(AT, sizeof(T) == 2 ? (CB == 1 ? 3 : 2) : 1) void at
 
     // the documents that the block's rows belong to, one after the other
     while (row0 < end) {
-        const int d = doc_holding(a.m, row0);
-        int stop = end;  // of this document's rows, or of rows that belong to none
-        Doc doc{0, 0, 0, 0, 0};
-        if (d >= 0) {
-            doc = doc_at(a.m, d);
-            stop = min(a.m.q_off[d + 1], end);
-        } else if (a.m.docs > 0 && row0 < a.m.q_off[0]) {
-            stop = min(a.m.q_off[0], end);
-        }
-        stop = __builtin_amdgcn_readfirstlane(max(stop, row0 + 1));
-        const int e0 = row0 * a.G + COLS * piece, e1 = min(stop * a.G, p.pieces > 1 ? min(e0 + COLS, (row0 + 1) * a.G) : INT_MAX);
-        // keys that a row sees, of its document's: more of them from row to row
-        const auto position = [&](int row) { return row - doc.q0 + doc.lk - doc.lq; };
-        const auto sees = [&](int row) { return a.m.causal ? min(max(max(position(row) + 1, doc.prefix), 0), doc.lk) : doc.lk; };
-        const int k0 = doc.k0, all = sees(row0), keys = sees((e1 - 1) / a.G);
+        const Segment sg = segment_at(a.m, row0, end);
+        const int e0 = row0 * a.G + COLS * piece, e1 = min(sg.stop * a.G, p.pieces > 1 ? min(e0 + COLS, (row0 + 1) * a.G) : INT_MAX);
+        const int k0 = sg.doc.k0, all = sg.sees(row0), keys = sg.sees((e1 - 1) / a.G);
         const int tiles = (keys + CN - 1) / CN;
-        const int t0 = static_cast<int>(static_cast<long>(tiles) * split / p.splits);
-        const int t1 = static_cast<int>(static_cast<long>(tiles) * (split + 1) / p.splits);
+        int t0, t1;
+        part_tiles(p, tiles, t0, t1);
+        if (split > 0 && t0 == t1) {  // nothing of this document's
+            if (tid < min(e1 - e0, COLS)) empty_part(p, kvh, e0 + tid);
+            row0 = sg.stop;
+            continue;
+        }
         int pos[CB];
         unsigned seen[CB];
         float slope[CB];
 #pragma unroll
         for (int x = 0; x < CB; ++x) {
             const int e = e0 + 16 * x + col, row = e < e1 ? e / a.G : row0;
-            pos[x] = position(row);
-            seen[x] = e < e1 ? static_cast<unsigned>(sees(row)) : 0u;
+            pos[x] = sg.position(row);
+            seen[x] = e < e1 ? static_cast<unsigned>(sg.sees(row)) : 0u;
             slope[x] = BIAS && e < e1 ? a.slopes[kvh * a.G + e - row * a.G] : 0.0f;
         }
         Score<T, CAP, BIAS> rule(a);
@@ -356,7 +397,7 @@ __global__ __launch_bounds__(AT, sizeof(T) == 2 ? (CB == 1 ? 3 : 2) : 1) void at
             }
         }
         __syncthreads();
-        row0 = stop;
+        row0 = sg.stop;
     }
 }
 
@@ -388,10 +429,11 @@ __global__ __launch_bounds__(64) void attn_cache_join_k(Cached p) {
 #pragma unroll
         for (int x = 0; x < 8; ++x)
 #pragma unroll
-            for (int i = 0; i < DP / 64; ++i) v[x][i] = s + x < p.splits ? p.part_o[((s + x) * n + w) * DP + lane + 64 * i] : 0.0f;
+            for (int i = 0; i < DP / 64; ++i)  // parts of no weight hold nothing
+                v[x][i] = __builtin_amdgcn_readlane(__float_as_int(f), s + x) ? p.part_o[((s + x) * n + w) * DP + lane + 64 * i] : 0.0f;
 #pragma unroll
         for (int x = 0; x < 8; ++x) {
-            const float g = __shfl(f, s + x);
+            const float g = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(f), s + x));
 #pragma unroll
             for (int i = 0; i < DP / 64; ++i) o[i] = __builtin_fmaf(g, v[x][i], o[i]);
         }
@@ -451,17 +493,21 @@ extern "C" int kdec_attn_cache_fwd(kdec_ctx* ctx, int dtype, const void* Q, long
     p.vec_o = D % 4 == 0 && aligned(Heads{O, o_rs, o_hs}, size, 4 * size);
     p.vec_q = D % 8 == 0 && aligned(p.a.Q, size, 16);
     p.lse = lse;
-    // Entries of a block: 16 where a document's rows have no more, else 32. Rows:
-    // what these hold, fewer where documents have fewer.
+    // Entries of a block: 16 where a document's rows have no more, else 32 that
+    // share a code's way to a float. Rows: what these hold, fewer where documents
+    // have fewer.
     const long mean = docs > 0 ? cdiv(Tq, docs) : Tq;
     const int cols = mean * G <= 16 ? 16 : 32;
     p.pieces = static_cast<int>(cdiv(G, cols));
     p.rows = static_cast<int>(G >= cols ? 1 : mean < cols / G ? mean : cols / G);
-    const long blocks = cdiv(Tq, p.rows) * p.pieces * Hkv;
+    // Blocks that end with their document, as far as finding them is quick.
+    p.a.by_doc = p.rows > 1 && docs < 127;
+    const long units = cdiv(Tq, p.rows) * p.pieces * Hkv, blocks = doc_blocks(p.a.by_doc, docs, Tq, p.rows) * p.pieces * Hkv;
     KDEC_CHECK(ctx, blocks < INT_MAX && static_cast<long>(Hkv) * p.a.E < INT_MAX, "kdec_attn_cache_fwd: too many rows");
-    // Split the keys where the rows alone do not fill the device.
-    const long each = docs > 0 ? Tk / docs : 0;
-    long splits = cdiv(4L * ctx->num_cus, blocks);
+    // Split the keys where the rows alone do not fill the device, as far as all
+    // parts' blocks are on it at once.
+    const long each = docs > 0 ? Tk / docs : 0, held = (dtype == KDEC_F32 ? (cols == 16 ? 2L : 1L) : cols == 16 ? 3L : 2L) * ctx->num_cus;
+    long splits = held / units;
     if (splits > each / 256) splits = each / 256;
     if (splits > 64) splits = 64;  // what the join holds
     if (splits < 1) splits = 1;
