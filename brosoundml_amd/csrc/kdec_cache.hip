@@ -18,6 +18,7 @@ using attn::Heads;
 
 constexpr int CT = 256;
 typedef signed char i8x8 __attribute__((ext_vector_type(8)));
+typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
 
 struct Codes {
     signed char *k, *v;
@@ -65,32 +66,48 @@ __device__ inline unsigned top_lanes(unsigned x) {
     return x;
 }
 
-// Eight values' codes under scale s. x / s by the reciprocal is off by 2^-22 of
-// it, so that its nearest integer q is the quotient's own, but next to a half:
-// the remainder x - q s is exact, and tells by being half of s or more.
-__device__ inline i8x8 nearest8(const f32x8& x, float s) {
-    const float inv = __builtin_amdgcn_rcpf(s);
-    float q[8], most = 0.0f;
+// max |x| / 127 to the nearest float: the product with 1 / 127 and one correction
+// by its exact remainder (127 and the rounded 1 / 127 meet the conditions under
+// which that is the quotient; no step leaves the normal numbers above 2^-119,
+// below which the scale is 2^-126 whatever the quotient's last bit).
+__device__ inline float scale_of(float top) {
+    const float c = 1.0f / 127.0f, q = top * c;
+    return fmaxf(__builtin_fmaf(__builtin_fmaf(-q, 127.0f, top), c, q), 0x1p-126f);
+}
+
+// Eight values' codes under scale s, as bytes. x / s by the reciprocal is off by
+// 2^-22 of it, so that its nearest integer q (the low bits of 1.5 2^23 + q) is
+// the quotient's own, but next to a half: the remainder x - q s is exact, and
+// tells by being half of s or more.
+__device__ inline u32x2 nearest8(const f32x8& x, float s) {
+    const float inv = __builtin_amdgcn_rcpf(s), magic = 0x1.8p23f;
+    float t[8], most = 0.0f;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-        q[i] = __builtin_rintf(x[i] * inv);
-        most = fmaxf(most, __builtin_fabsf(__builtin_fmaf(-q[i], s, x[i])));
+        t[i] = __builtin_fmaf(x[i], inv, magic);
+        most = fmaxf(most, __builtin_fabsf(__builtin_fmaf(magic - t[i], s, x[i])));
     }
     if (__builtin_amdgcn_ballot_w64(2.0f * most >= s)) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            const float r = __builtin_fmaf(-q[i], s, x[i]), r2 = 2.0f * __builtin_fabsf(r);
-            if (r2 > s || (r2 == s && (static_cast<int>(q[i]) & 1))) q[i] += r > 0.0f ? 1.0f : -1.0f;
+            const float r = __builtin_fmaf(magic - t[i], s, x[i]), r2 = 2.0f * __builtin_fabsf(r);
+            if (r2 > s || (r2 == s && (__float_as_uint(t[i]) & 1))) t[i] += r > 0.0f ? 1.0f : -1.0f;
         }
     }
-    i8x8 c;
+    u32x2 c;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) c[i] = static_cast<signed char>(static_cast<int>(q[i]));
+    for (int i = 0; i < 2; ++i)
+        c[i] = __builtin_amdgcn_perm(__float_as_uint(t[4 * i + 1]), __float_as_uint(t[4 * i]), 0x0c0c0400) |
+               __builtin_amdgcn_perm(__float_as_uint(t[4 * i + 3]), __float_as_uint(t[4 * i + 2]), 0x04000c0c);
     return c;
 }
 
 // L lanes take UNITS heads' keys or values of a row (unit u: head u / 2, keys or
-// values), their loads together behind one search for the row's place.
+// values), their loads together, on their way during the search for the row's
+// place. More units a thread leave fewer waves, fewer a search for each (17000
+// rows of 12 heads of width 64, bf16, written and read back: 2 units 25.8 and 20.7
+// us, 4 24.2 and 16.9, 8 23.5 and 17.7; 48 rows of 4 heads of width 128: 4.4 and
+// 3.6, 5.0 and 3.9, 6.6 and 4.6).
 constexpr int UNITS = 4;
 template <class T, int L>
 __global__ __launch_bounds__(CT) void cache_write_k(Docs m, Heads K, Heads V, Codes o, int H, int D, int W, bool vec) {
@@ -104,6 +121,8 @@ __global__ __launch_bounds__(CT) void cache_write_k(Docs m, Heads K, Heads V, Co
         f[j] = load8(p, n, vec);
     }
     const long at = cache_row(m, row, __builtin_amdgcn_readfirstlane(row));
+    signed char* to[2] = {o.k + at * o.k_rs + c, o.v + at * o.v_rs + c};
+    float* scales[2] = {o.ks + at, o.vs + at};
 #pragma unroll
     for (int j = 0; j < UNITS; ++j) {
         const bool keys = !((u0 + j) & 1);
@@ -111,14 +130,14 @@ __global__ __launch_bounds__(CT) void cache_write_k(Docs m, Heads K, Heads V, Co
         const unsigned top = top_lanes<L>(top8(f[j]));
         if (at < 0 || head >= H) continue;
         const bool bad = top >= 0x7F800000u;
-        const float s = bad ? __builtin_nanf("") : fmaxf(__uint_as_float(top) / 127.0f, 0x1p-126f);
+        const float s = bad ? __builtin_nanf("") : scale_of(__uint_as_float(top));
         f32x8 x;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = bad ? 0.0f : static_cast<float>(f[j][i]);
-        const i8x8 q = nearest8(x, bad ? 1.0f : s);
-        signed char* to = (keys ? o.k + at * o.k_rs + head * o.k_hs : o.v + at * o.v_rs + head * o.v_hs) + c;
-        if (c < W) *reinterpret_cast<i8x8*>(to) = q;
-        if (lane == 0) (keys ? o.ks : o.vs)[static_cast<long>(head) * m.Tk + at] = s;
+        for (int i = 0; i < 8; ++i) x[i] = static_cast<float>(f[j][i]);
+        u32x2 q = nearest8(x, s);
+        if (bad) q = u32x2{};
+        if (c < W) *reinterpret_cast<u32x2*>((keys ? to[0] : to[1]) + head * (keys ? o.k_hs : o.v_hs)) = q;
+        if (lane == 0) (keys ? scales[0] : scales[1])[static_cast<long>(head) * m.Tk] = s;
     }
 }
 

@@ -404,20 +404,17 @@ def residual_norm_bwd(ctx: Context, x, z, dr, dy, stats, *, gate=None, post=None
     DR = (None, 0) if dr is None else _as(ctx, dr, ty, shape, "dr must be as x")
     DY = (None, 0) if dy is None else _as(ctx, dy, ty, shape, "dy must be as x")
     dx, dz = _empty(ctx, x, shape), None if z is None else _empty(ctx, x, shape)
-    floats = lambda v: None if v is None else _empty(ctx, x, (c,), torch.float32)  # noqa: E731
-    dgate = None if gate is None else floats(gate) if gate.dim() == 1 else _empty(ctx, x, shape)
-
-    def grads(wb):
-        if wb is None:
-            return None
-        wb = wb if isinstance(wb, (tuple, list)) else (wb, None)
-        return floats(wb[0]), floats(wb[1])
-
-    dpost, dpre = grads(post), grads(pre)
-    at = lambda v: None if v is None else v.data_ptr()  # noqa: E731
-    ctx.call("kdec_resnorm_bwd", *args, st, *DR, *DY, dx.data_ptr(), at(dz), at(dgate), *map(at, dpost or (None, None)),
-             *map(at, dpre or (None, None)))
-    return dx, dz, dgate, dpost, dpre
+    wide = gate is not None and gate.dim() == 2
+    wb = [v if isinstance(v, (tuple, list)) else (v, None) for v in (post, pre)]
+    want = (wb[0][0], wb[0][1], wb[1][0], wb[1][1], None if wide else gate)
+    n = sum(v is not None for v in want)
+    parts = iter(_empty(ctx, x, (n, c), torch.float32).unbind(0) if n else ())  # one allocation for the vectors' gradients
+    got = [None if v is None else next(parts) for v in want]
+    if wide:
+        got[4] = _empty(ctx, x, shape)
+    at = [None if v is None else v.data_ptr() for v in got]
+    ctx.call("kdec_resnorm_bwd", *args, st, *DR, *DY, dx.data_ptr(), None if dz is None else dz.data_ptr(), at[4], *at[:4])
+    return dx, dz, got[4], None if post is None else (got[0], got[1]), None if pre is None else (got[2], got[3])
 
 
 class Cache(NamedTuple):
