@@ -115,17 +115,20 @@ struct Sort {
 // Ids outside the table sort behind it.
 __device__ inline int key_of(int id, int vocab) { return static_cast<unsigned>(id) < static_cast<unsigned>(vocab) ? id : vocab; }
 
-__device__ inline void begin_table(const Sort& s, long block, long blocks) {
-    if (s.beta == 1.0f) return;
-    const bool vec = reinterpret_cast<size_t>(s.table) % 16 == 0;
-    const long quads = vec ? s.n / 4 : 0, step = blocks * blockDim.x, first = block * blockDim.x + threadIdx.x;
-    f32x4* q = reinterpret_cast<f32x4*>(s.table);
-    if (s.beta == 0.0f) {
+// Clears n floats or scales them by beta, from place `first` on in steps of `step`
+// threads.
+__device__ inline void begin_rows(float* to, long n, float beta, long first, long step) {
+    if (beta == 1.0f) return;
+    const long quads = reinterpret_cast<size_t>(to) % 16 == 0 ? n / 4 : 0;
+    f32x4* q = reinterpret_cast<f32x4*>(to);
+    if (beta == 0.0f) {
+#pragma unroll 4
         for (long i = first; i < quads; i += step) q[i] = f32x4{};
-        for (long i = 4 * quads + first; i < s.n; i += step) s.table[i] = 0.0f;
+        for (long i = 4 * quads + first; i < n; i += step) to[i] = 0.0f;
     } else {
-        for (long i = first; i < quads; i += step) q[i] *= s.beta;
-        for (long i = 4 * quads + first; i < s.n; i += step) s.table[i] *= s.beta;
+#pragma unroll 4
+        for (long i = first; i < quads; i += step) q[i] *= beta;
+        for (long i = 4 * quads + first; i < n; i += step) to[i] *= beta;
     }
 }
 
@@ -221,65 +224,83 @@ __device__ inline void place_all(const Ranks& r, int (*cnt)[DIGITS], F f) {
 }
 
 // Block b's ids, `per` of them from b * per (those outside the table count as
-// one more, vocab), of up to CHUNK tokens. FEW tokens are summed right here, a
-// thread's columns over every run in order.
+// one more, vocab), of up to CHUNK tokens: the block lists its own tokens in
+// order, most of what it looks at is not, and sorts the list (16381 tokens of
+// 32000 ids with the table's 131 MB, which take 21 us by themselves: 28 us, and 32
+// with ranks of all tokens in place; 8190 tokens of 181 ids 6.6 and 8.5). FEW
+// tokens are summed right here, a thread's columns over every run in order.
 constexpr int FEW = 256;
 template <class T, bool SUM>
 __global__ __launch_bounds__(ST) void sort_range_k(Sort s, int per, Tokens out, const T* __restrict__ dY, long rs, int cols, float scale) {
-    __shared__ int cnt[WAVES][DIGITS], sums[WAVES], start[DIGITS + 1], lower[WAVES], owned[WAVES], list[SUM ? FEW : 1];
-    const int tid = threadIdx.x, wave = tid >> 6, lo = blockIdx.x * per;
-    Ranks r;
-    r.n = (s.T + ST - 1) / ST;
-    const int first = wave * 64 * r.n + (tid & 63);
-    int id[SI], less = 0, mine = 0;
+    __shared__ int cnt[WAVES][DIGITS], sums[WAVES], start[DIGITS + 1], lower[WAVES], owned[WAVES];
+    __shared__ int list[SUM ? FEW : CHUNK];  // token, digit above it
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, lo = blockIdx.x * per;
+    const int places = (s.T + ST - 1) / ST, first = wave * 64 * places + lane;
+    int id[SI];
 #pragma unroll
     for (int g = 0; g < SI; ++g) {
         const int i = first + 64 * g;
-        id[g] = g < r.n && i < s.T ? key_of(s.ids[i], s.vocab) : INT_MAX;
+        id[g] = g < places && i < s.T ? key_of(s.ids[i], s.vocab) : INT_MAX;
     }
-    // the table's rows, a wave 64 places of a row at a time
     const int n = min(per, s.vocab - lo);
-    const bool vec = cols % 4 == 0 && reinterpret_cast<size_t>(s.table) % 16 == 0;
-    const int width = vec ? cols / 4 : cols, each = (width + 63) / 64;
-    if (s.beta != 1.0f)
-        for (int u = __builtin_amdgcn_readfirstlane(wave); u < n * each; u += WAVES) {
-            const int row = u / each, c = 64 * (u - row * each) + (tid & 63);
-            if (c >= width) continue;
-            float* to = s.table + static_cast<long>(lo + row) * cols;
-            if (vec) {
-                f32x4* q = reinterpret_cast<f32x4*>(to) + c;
-                *q = s.beta == 0.0f ? f32x4{} : *q * s.beta;
-            } else {
-                to[c] = s.beta == 0.0f ? 0.0f : to[c] * s.beta;
-            }
-        }
+    begin_rows(s.table + static_cast<long>(lo) * cols, static_cast<long>(n) * cols, s.beta, tid, ST);
+    const auto mine = [&](int g) __attribute__((always_inline)) { return static_cast<unsigned>(id[g] - lo) < static_cast<unsigned>(per); };
+    int less = 0, own = 0;
 #pragma unroll
     for (int g = 0; g < SI; ++g) {
-        less += id[g] < lo;
-        const bool in = id[g] >= lo && id[g] - lo < per;
-        r.digit[g] = in ? id[g] - lo : -1;
-        mine += in;
+        less += __builtin_popcountll(__builtin_amdgcn_ballot_w64(id[g] < lo));
+        own += __builtin_popcountll(__builtin_amdgcn_ballot_w64(mine(g)));
     }
-    block_offsets(r, s.bits, cnt, sums);
-    if (tid < DIGITS) start[tid] = cnt[0][tid];
-    less = wave_scan(less);
-    mine = wave_scan(mine);
-    if ((tid & 63) == 63) {
+    if (lane == 0) {
         lower[wave] = less;
-        owned[wave] = mine;
+        owned[wave] = own;
     }
     __syncthreads();
-    const int base = first_waves(lower, WAVES);
-    if (wave == 0) start[DIGITS] = first_waves(owned, WAVES);
-    place_all(r, cnt, [&](int g, int to) {
-        if (SUM) {
-            list[to] = first + 64 * g;
-        } else {
-            out.id[base + to] = id[g];
-            out.at[base + to] = first + 64 * g;
+    const int base = first_waves(lower, WAVES), total = first_waves(owned, WAVES);
+    int at = first_waves(owned, wave);
+#pragma unroll
+    for (int g = 0; g < SI; ++g) {
+        const unsigned long long m = __builtin_amdgcn_ballot_w64(mine(g));
+        if (m) {
+            if (mine(g)) list[at + __builtin_popcountll(m & ((1ull << lane) - 1))] = (first + 64 * g) | (id[g] - lo) << 16;
+            at += __builtin_popcountll(m);
         }
-    });
+    }
     __syncthreads();
+    if (per > 1) {
+        Ranks r;
+        r.n = (total + ST - 1) / ST;
+        const int from = wave * 64 * r.n + lane;
+        int token[SI];
+#pragma unroll
+        for (int g = 0; g < SI; ++g) {
+            const int i = from + 64 * g;
+            token[g] = g < r.n && i < total ? list[i] : 0;
+            r.digit[g] = g < r.n && i < total ? token[g] >> 16 : -1;
+        }
+        block_offsets(r, s.bits, cnt, sums);  // behind the list's last reads
+        if (tid < DIGITS) start[tid] = cnt[0][tid];
+        if (tid == 0) start[DIGITS] = total;
+        __syncthreads();
+        place_all(r, cnt, [&](int g, int to) {
+            if (SUM) {
+                list[to] = token[g] & 0xFFFF;
+            } else {
+                out.id[base + to] = lo + r.digit[g];
+                out.at[base + to] = token[g] & 0xFFFF;
+            }
+        });
+    } else {
+        if (tid == 0) {
+            start[0] = 0;
+            start[1] = total;
+        }
+        if (!SUM)
+            for (int i = tid; i < total; i += ST) {
+                out.id[base + i] = lo;
+                out.at[base + i] = list[i];
+            }
+    }
     if (!SUM) return;
     __syncthreads();
     for (int row = 0; row < n; ++row) {
@@ -307,7 +328,7 @@ __global__ __launch_bounds__(ST) void sort_range_k(Sort s, int per, Tokens out, 
 __global__ __launch_bounds__(ST) void sort_count_k(Sort s, int pass, int chunks, const int* src, int* counts) {
     __shared__ int cnt[DIGITS];
     if (static_cast<int>(blockIdx.x) >= chunks) {
-        begin_table(s, blockIdx.x - chunks, gridDim.x - chunks);
+        begin_rows(s.table, s.n, s.beta, static_cast<long>(blockIdx.x - chunks) * ST + threadIdx.x, static_cast<long>(gridDim.x - chunks) * ST);
         return;
     }
     const int tid = threadIdx.x, base = blockIdx.x * CHUNK;
@@ -534,7 +555,7 @@ int kdec_embed_bwd(kdec_ctx* ctx, int dtype, const void* dY, long dy_rs, const i
                    float* dtable, float beta) {
     if (!ctx) return KDEC_EINVAL;
     KDEC_CHECK(ctx, dtype == KDEC_F32 || dtype == KDEC_BF16, "kdec_embed_bwd: unknown type");
-    KDEC_CHECK(ctx, T >= 0 && T <= INT_MAX - CHUNK && vocab >= 0 && vocab < INT_MAX && cols >= 0 && cols <= 0x7FFFFF00,
+    KDEC_CHECK(ctx, T >= 0 && T <= INT_MAX - CHUNK && vocab >= 0 && vocab <= INT_MAX - 2 * DIGITS && cols >= 0 && cols <= 0x7FFFFF00,
                "kdec_embed_bwd: bad sizes");
     if (vocab == 0 || cols == 0) return KDEC_OK;
     KDEC_CHECK(ctx, dtable && (T == 0 || (dY && ids)), "kdec_embed_bwd: null tensor");
