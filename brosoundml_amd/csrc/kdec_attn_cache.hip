@@ -73,16 +73,31 @@ struct Segment {
         return causal ? min(max(max(position(row) + 1, doc.prefix), 0), doc.lk) : doc.lk;
     }
 };
-// The rows of a block: `rows` from a multiple of it, or as many of one document.
-__device__ inline bool block_rows(const Cached& p, int b, int& row0, int& end) {
+// The rows of a block: `rows` from a multiple of it (doc: -2), or as many of one
+// document (or of the rows before the first or past the last, -1 and docs), found
+// by a scan over the documents' numbers of blocks.
+__device__ inline bool block_rows(const Cached& p, int b, int& row0, int& end, int& doc) {
+    const Docs& m = p.a.m;
+    doc = -2;
     row0 = b * p.rows;
-    end = min(row0 + p.rows, p.a.m.Tq);
+    end = min(row0 + p.rows, m.Tq);
     if (!p.a.by_doc) return true;
-    Piece c;
-    if (!piece_at(p.a.m.q_off, p.a.m.docs, p.a.m.Tq, 1, p.rows, b, c)) return false;
-    row0 = c.lo + c.place * p.rows;
-    end = min(row0 + p.rows, c.hi);
-    return true;
+    const int lane = threadIdx.x & 63;
+    const auto at = [&](int d) { return d < 0 ? 0 : d <= m.docs ? min(max(m.q_off[d], 0), m.Tq) : m.Tq; };
+    int before = 0;
+    for (int base = -1; base <= m.docs; base += 64) {
+        const int lo = at(base + lane), hi = at(base + lane + 1), n = hi > lo ? (hi - lo + p.rows - 1) / p.rows : 0;
+        const int upto = wave_scan(n), all = __builtin_amdgcn_readlane(upto, 63);
+        if (b - before < all) {
+            const int l = __builtin_popcountll(__builtin_amdgcn_ballot_w64(before + upto <= b));
+            doc = base + l;
+            row0 = __builtin_amdgcn_readlane(lo, l) + (b - before - __builtin_amdgcn_readlane(upto - n, l)) * p.rows;
+            end = min(row0 + p.rows, __builtin_amdgcn_readlane(hi, l));
+            return true;
+        }
+        before += all;
+    }
+    return false;
 }
 // A part's tiles: of every document an equal share. (Parts of a fixed length, the
 // same work for short and long documents, were slower: one token for 48 requests
@@ -91,13 +106,13 @@ __device__ inline void part_tiles(const Cached& p, int tiles, int& t0, int& t1) 
     t0 = static_cast<int>(static_cast<long>(tiles) * blockIdx.y / p.splits);
     t1 = static_cast<int>(static_cast<long>(tiles) * (blockIdx.y + 1) / p.splits);
 }
-__device__ inline Segment segment_at(const Docs& m, int row0, int end) {
+__device__ inline Segment segment_at(const Docs& m, int row0, int end, int doc) {
     Segment s{Doc{0, 0, 0, 0, 0}, m.causal, end};
-    const int d = doc_holding(m, row0);
-    if (d >= 0) {
+    const int d = doc == -2 ? doc_holding(m, row0) : doc;
+    if (d >= 0 && d < m.docs) {
         s.doc = doc_at(m, d);
-        s.stop = min(m.q_off[d + 1], end);
-    } else if (m.docs > 0 && row0 < m.q_off[0]) {
+        if (doc == -2) s.stop = min(m.q_off[d + 1], end);
+    } else if (doc == -2 && m.docs > 0 && row0 < m.q_off[0]) {
         s.stop = min(m.q_off[0], end);
     }
     s.stop = __builtin_amdgcn_readfirstlane(max(s.stop, row0 + 1));
@@ -165,8 +180,8 @@ __global__ __launch_bounds__(AT, sizeof(T) == 2 ? (CB == 1 ? 3 : 2) : 1) void at
     const int kvh = b % a.Hkv;
     b /= a.Hkv;
     const int piece = b % p.pieces, split = blockIdx.y, W = code_width(a.D);
-    int row0, end;
-    if (!block_rows(p, b / p.pieces, row0, end)) return;
+    int row0, end, doc;
+    if (!block_rows(p, b / p.pieces, row0, end, doc)) return;
     const signed char* kb = static_cast<const signed char*>(a.K.p) + kvh * a.K.hs;
     const signed char* vb = static_cast<const signed char*>(a.V.p) + kvh * a.V.hs;
     const float* ks = p.ks + static_cast<long>(kvh) * a.m.Tk;
@@ -179,7 +194,7 @@ __global__ __launch_bounds__(AT, sizeof(T) == 2 ? (CB == 1 ? 3 : 2) : 1) void at
 
     // the documents that the block's rows belong to, one after the other
     while (row0 < end) {
-        const Segment sg = segment_at(a.m, row0, end);
+        const Segment sg = segment_at(a.m, row0, end, doc);
         const int e0 = row0 * a.G + COLS * piece, e1 = min(sg.stop * a.G, p.pieces > 1 ? min(e0 + COLS, (row0 + 1) * a.G) : INT_MAX);
         const int k0 = sg.doc.k0, all = sg.sees(row0), keys = sg.sees((e1 - 1) / a.G);
         const int tiles = (keys + CN - 1) / CN;
@@ -473,6 +488,7 @@ extern "C" int kdec_attn_cache_fwd(kdec_ctx* ctx, int dtype, const void* Q, long
                                    float scale, float cap, int Tq, int Tk, int Hq, int Hkv, int D, void* O, long o_rs, long o_hs,
                                    float* lse) {
     if (!ctx) return KDEC_EINVAL;
+    const DeviceScope device(ctx);
     const char* who = "kdec_attn_cache_fwd";
     if (int rc = check(ctx, who, dtype, q_off, k_off, docs, scale, cap, Tq, Tk, Hq, Hkv, D)) return rc;
     const Heads k{Kc, kc_rs, kc_hs}, v{Vc, vc_rs, vc_hs};
@@ -494,18 +510,26 @@ extern "C" int kdec_attn_cache_fwd(kdec_ctx* ctx, int dtype, const void* Q, long
     p.vec_q = D % 8 == 0 && aligned(p.a.Q, size, 16);
     p.lse = lse;
     // Entries of a block: 16 where a document's rows have no more, else 32 that
-    // share a code's way to a float. Rows: what these hold, fewer where documents
-    // have fewer.
+    // share a code's way to a float (bf16, 16 heads on 4 of width 128, blocks of 16
+    // and 32: 48 documents of 90 to 4096 keys and 1 row 31 us and 42, 16 of 2000 to
+    // 4096 and 8 rows 30 and 28, 5 of them and 200 rows 82 and 62). Rows: what these
+    // hold, fewer where documents have fewer.
     const long mean = docs > 0 ? cdiv(Tq, docs) : Tq;
     const int cols = mean * G <= 16 ? 16 : 32;
     p.pieces = static_cast<int>(cdiv(G, cols));
     p.rows = static_cast<int>(G >= cols ? 1 : mean < cols / G ? mean : cols / G);
-    // Blocks that end with their document, as far as finding them is quick.
-    p.a.by_doc = p.rows > 1 && docs < 127;
+    // Blocks that end with their document where rows may not be even, as far as
+    // finding them is quick: one that holds rows of two walks twice (48 documents of
+    // up to 4096 keys, 1 to 4 rows 50 us for 62, 2 to 9 rows 59 for 74, 5 of 100 to
+    // 300 rows 80 for 89; even ones of 4 rows 24.6 for 22.5).
+    p.a.by_doc = p.rows > 1 && docs > 0 && docs < 127 && (Tq % docs != 0 || mean % p.rows != 0);
     const long units = cdiv(Tq, p.rows) * p.pieces * Hkv, blocks = doc_blocks(p.a.by_doc, docs, Tq, p.rows) * p.pieces * Hkv;
     KDEC_CHECK(ctx, blocks < INT_MAX && static_cast<long>(Hkv) * p.a.E < INT_MAX, "kdec_attn_cache_fwd: too many rows");
     // Split the keys where the rows alone do not fill the device, as far as all
-    // parts' blocks are on it at once.
+    // parts' blocks are on it at once (48 documents of 90 to 4096 keys and 1 row: 4
+    // parts, which fill it, 26 us, 3 and 6 parts 31 and 32), to no fewer than 256
+    // keys a part (one float row over 6000 keys, 12 heads of width 64: 15.9 us with
+    // the join, of 128 keys 16.8).
     const long each = docs > 0 ? Tk / docs : 0, held = (dtype == KDEC_F32 ? (cols == 16 ? 2L : 1L) : cols == 16 ? 3L : 2L) * ctx->num_cus;
     long splits = held / units;
     if (splits > each / 256) splits = each / 256;

@@ -199,6 +199,7 @@ int kdec_cache_write(kdec_ctx* ctx, int dtype, const void* K, long k_rs, long k_
                      const int* q_off, const int* k_off, const int* k_len, int docs, int Tq, int Tk, int H, int D, void* Kc, long kc_rs,
                      long kc_hs, void* Vc, long vc_rs, long vc_hs, float* k_scale, float* v_scale) {
     if (!ctx) return KDEC_EINVAL;
+    const DeviceScope device(ctx);
     const Codes o{static_cast<signed char*>(Kc), static_cast<signed char*>(Vc), kc_rs, kc_hs, vc_rs, vc_hs, k_scale, v_scale};
     if (int rc = check(ctx, "kdec_cache_write", dtype, q_off, k_off, docs, Tq, Tk, H, D, o)) return rc;
     const int W = attn::code_width(D);
@@ -223,6 +224,7 @@ int kdec_cache_read(kdec_ctx* ctx, int dtype, const void* Kc, long kc_rs, long k
                     const float* k_scale, const float* v_scale, const int* q_off, const int* k_off, const int* k_len, int docs, int Tq,
                     int Tk, int H, int D, void* K, long k_rs, long k_hs, void* V, long v_rs, long v_hs) {
     if (!ctx) return KDEC_EINVAL;
+    const DeviceScope device(ctx);
     const auto bytes = [](const void* p) { return static_cast<signed char*>(const_cast<void*>(p)); };
     const Codes o{bytes(Kc), bytes(Vc), kc_rs, kc_hs, vc_rs, vc_hs, const_cast<float*>(k_scale), const_cast<float*>(v_scale)};
     if (int rc = check(ctx, "kdec_cache_read", dtype, q_off, k_off, docs, Tq, Tk, H, D, o)) return rc;

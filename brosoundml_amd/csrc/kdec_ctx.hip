@@ -94,6 +94,13 @@ void* ws_alloc(kdec_ctx* ctx, size_t bytes) {
         ctx->pool.erase(it);
     } else {
         hipError_t e = hipMalloc(&base, need);
+        hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
+        if (e != hipSuccess && hipStreamIsCapturing(ctx->stream, &capture) == hipSuccess && capture != hipStreamCaptureStatusNone) {
+            // The pool's blocks may be an earlier graph's: none is given back here.
+            (void)hipGetLastError();
+            fail(ctx, KDEC_ENOMEM, "no workspace while a graph is captured: make the call once before");
+            return nullptr;
+        }
         if (e != hipSuccess) {
             // Return every pooled block to the driver and try once more.
             hipStreamSynchronize(ctx->stream);

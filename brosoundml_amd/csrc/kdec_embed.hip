@@ -51,9 +51,11 @@ __device__ inline Part<T> load_part(const T* p, int n, bool vec) {
     return f;
 }
 
-// J parts a thread, a block's width apart: their ids, then their rows are on
-// their way together.
-template <class T, int J>
+// Four parts a thread, a block's width apart: their ids, then their rows are on
+// their way together (16381 rows of 1024 bf16 from a table of 32000: 12.2 us, one
+// part a thread 13.2; rows that one round of blocks holds take the same).
+constexpr int J = 4;
+template <class T>
 __global__ __launch_bounds__(ET) void embed_k(const T* __restrict__ table, long t_rs, const int* __restrict__ ids, T* __restrict__ Y,
                                               long y_rs, int rows, int vocab, int cols, unsigned groups, bool vec, float scale) {
     constexpr int E = PART<T>;
@@ -152,20 +154,6 @@ __device__ inline void rank64(int digit, int bits, int& place) {
     place = before | __builtin_popcountll(same) << 8;
 }
 
-// The sum over a wave's lanes up to each lane's own.
-__device__ inline int wave_scan(int x) {
-    const auto add = [&](auto ctrl, auto rows) __attribute__((always_inline)) {
-        x += __builtin_amdgcn_update_dpp(0, x, decltype(ctrl)::value, decltype(rows)::value, 15, false);
-    };
-    typedef std::integral_constant<int, 15> All;
-    add(std::integral_constant<int, 0x111>{}, All{});  // lanes of 16 to the right by 1, 2, 4, 8
-    add(std::integral_constant<int, 0x112>{}, All{});
-    add(std::integral_constant<int, 0x114>{}, All{});
-    add(std::integral_constant<int, 0x118>{}, All{});
-    add(std::integral_constant<int, 0x142>{}, std::integral_constant<int, 10>{});  // the 16's last lane to the next 16
-    add(std::integral_constant<int, 0x143>{}, std::integral_constant<int, 12>{});  // lane 31 to the upper half
-    return x;
-}
 // The sum of the first n of the block's waves' values.
 __device__ inline int first_waves(const int* sums, int n) {
     const int lane = threadIdx.x & 63;
@@ -229,7 +217,7 @@ __device__ inline void place_all(const Ranks& r, int (*cnt)[DIGITS], F f) {
 // 32000 ids with the table's 131 MB, which take 21 us by themselves: 28 us, and 32
 // with ranks of all tokens in place; 8190 tokens of 181 ids 6.6 and 8.5). FEW
 // tokens are summed right here, a thread's columns over every run in order.
-constexpr int FEW = 256;
+constexpr int FEW = 512;
 template <class T, bool SUM>
 __global__ __launch_bounds__(ST) void sort_range_k(Sort s, int per, Tokens out, const T* __restrict__ dY, long rs, int cols, float scale) {
     __shared__ int cnt[WAVES][DIGITS], sums[WAVES], start[DIGITS + 1], lower[WAVES], owned[WAVES];
@@ -284,7 +272,7 @@ __global__ __launch_bounds__(ST) void sort_range_k(Sort s, int per, Tokens out, 
         __syncthreads();
         place_all(r, cnt, [&](int g, int to) {
             if (SUM) {
-                list[to] = token[g] & 0xFFFF;
+                list[to] = token[g];
             } else {
                 out.id[base + to] = lo + r.digit[g];
                 out.at[base + to] = token[g] & 0xFFFF;
@@ -303,21 +291,23 @@ __global__ __launch_bounds__(ST) void sort_range_k(Sort s, int per, Tokens out, 
     }
     if (!SUM) return;
     __syncthreads();
-    for (int row = 0; row < n; ++row) {
-        const int i0 = start[row], i1 = start[row + 1];
-        if (i0 == i1) continue;
+    for (int i0 = 0, i1; i0 < total; i0 = i1) {
+        const int digit = per > 1 ? list[i0] >> 16 : 0;
+        i1 = start[digit + 1];
+        if (digit >= n) break;  // outside the table
+        const auto row = [&](int i) __attribute__((always_inline)) { return dY + (list[i] & 0xFFFF) * rs; };
         for (int c = tid; c < cols; c += ST) {
             float acc = 0.0f;
             int i = i0;
             for (; i + 8 <= i1; i += 8) {
                 float f[8];
 #pragma unroll
-                for (int j = 0; j < 8; ++j) f[j] = static_cast<float>(dY[list[i + j] * rs + c]);
+                for (int j = 0; j < 8; ++j) f[j] = static_cast<float>(row(i + j)[c]);
 #pragma unroll
                 for (int j = 0; j < 8; ++j) acc += f[j];
             }
-            for (; i < i1; ++i) acc += static_cast<float>(dY[list[i] * rs + c]);
-            float* to = s.table + static_cast<long>(lo + row) * cols + c;
+            for (; i < i1; ++i) acc += static_cast<float>(row(i)[c]);
+            float* to = s.table + static_cast<long>(lo + digit) * cols + c;
             *to = s.beta == 0.0f ? scale * acc : *to + scale * acc;
         }
     }
@@ -521,11 +511,9 @@ void lookup(kdec_ctx* ctx, const void* table, long t_rs, const int* ids, void* Y
     const bool vec = cols % E == 0 && ok(table, t_rs) && ok(Y, y_rs);
     const unsigned groups = static_cast<unsigned>(cdiv(cols, E));
     const long threads = static_cast<long>(rows) * groups;
-    const bool many = threads >= 4L * ET * 4 * ctx->num_cus;  // four parts a thread where that leaves four blocks a CU
-    long blocks = cdiv(threads, ET * (many ? 4 : 1));
+    long blocks = cdiv(threads, ET * J);
     if (blocks > 64L * ctx->num_cus) blocks = 64L * ctx->num_cus;
-    const auto k = many ? embed_k<T, 4> : embed_k<T, 1>;
-    hipLaunchKernelGGL(k, dim3(static_cast<unsigned>(blocks)), dim3(ET), 0, ctx->stream, static_cast<const T*>(table), t_rs, ids,
+    hipLaunchKernelGGL(embed_k<T>, dim3(static_cast<unsigned>(blocks)), dim3(ET), 0, ctx->stream, static_cast<const T*>(table), t_rs, ids,
                        static_cast<T*>(Y), y_rs, rows, vocab, cols, groups, vec, scale);
 }
 
@@ -539,6 +527,7 @@ extern "C" {
 int kdec_embed_fwd(kdec_ctx* ctx, int dtype, const void* table, long t_rs, const int* ids, int T, int vocab, int cols, float scale,
                    void* Y, long y_rs) {
     if (!ctx) return KDEC_EINVAL;
+    const DeviceScope device(ctx);
     KDEC_CHECK(ctx, dtype == KDEC_F32 || dtype == KDEC_BF16, "kdec_embed_fwd: unknown type");
     KDEC_CHECK(ctx, T >= 0 && vocab >= 0 && cols >= 0 && cols <= 0x7FFFFFF0, "kdec_embed_fwd: bad sizes");
     if (T == 0 || cols == 0) return KDEC_OK;
@@ -554,6 +543,7 @@ int kdec_embed_fwd(kdec_ctx* ctx, int dtype, const void* table, long t_rs, const
 int kdec_embed_bwd(kdec_ctx* ctx, int dtype, const void* dY, long dy_rs, const int* ids, int T, int vocab, int cols, float scale,
                    float* dtable, float beta) {
     if (!ctx) return KDEC_EINVAL;
+    const DeviceScope device(ctx);
     KDEC_CHECK(ctx, dtype == KDEC_F32 || dtype == KDEC_BF16, "kdec_embed_bwd: unknown type");
     KDEC_CHECK(ctx, T >= 0 && T <= INT_MAX - CHUNK && vocab >= 0 && vocab <= INT_MAX - 2 * DIGITS && cols >= 0 && cols <= 0x7FFFFF00,
                "kdec_embed_bwd: bad sizes");
@@ -566,11 +556,18 @@ int kdec_embed_bwd(kdec_ctx* ctx, int dtype, const void* dY, long dy_rs, const i
     const auto bits_of = [](unsigned last) { return last ? 32 - __builtin_clz(last) : 0; };  // of the numbers 0 .. last
     const int chunks = static_cast<int>(cdiv(T, CHUNK));
     Sort so{ids, T, vocab, 0, dtable, n, beta};
-    // Ids of a block of the one-launch sort: a block a CU, up to a digit's.
+    // Ids of a block of the one-launch sort: a block a CU, up to a digit's. Past
+    // eight blocks a CU, each of which looks at all tokens, the radix sort is
+    // quicker (8192 tokens of 64 columns, ids of 500000: 77 us for 90, of a million
+    // 131 for 106), as past what a block holds.
     long per = cdiv(static_cast<long>(vocab) + 1, static_cast<long>(ctx->num_cus));
     if (per > DIGITS) per = DIGITS;
     const dim3 ranges(static_cast<unsigned>(cdiv(static_cast<long>(vocab) + 1, per)));
-    if (T <= FEW) {
+    const bool one = chunks <= 1 && ranges.x <= 8u * static_cast<unsigned>(ctx->num_cus);
+    // Few tokens: the sums in the sort's launch (512 tokens as texts have them, 181
+    // ids, 512 columns, forward and backward 16.5 us, in launches of their own 21.8;
+    // all of one id, 1024 columns, 36 and 22).
+    if (one && T <= FEW) {
         so.bits = bits_of(static_cast<unsigned>(per - 1));
         if (dtype == KDEC_F32)
             hipLaunchKernelGGL((sort_range_k<float, true>), ranges, dim3(ST), 0, ctx->stream, so, static_cast<int>(per), Tokens{},
@@ -597,7 +594,7 @@ int kdec_embed_bwd(kdec_ctx* ctx, int dtype, const void* dY, long dy_rs, const i
     KDEC_CHECK(ctx, cdiv(units, ET / 64) < INT_MAX && cdiv(cols, 256) <= 65535, "kdec_embed_bwd: bad sizes");
     int bits = bits_of(static_cast<unsigned>(vocab));
     const int passes = (bits + 7) / 8;
-    const bool two = chunks > 1 && passes > 1;  // passes that read what the last one wrote
+    const bool two = !one && passes > 1;  // passes that read what the last one wrote
     const size_t part = cdiv(static_cast<long>(s.pieces) * 2 * cols, 4) * 4, ints = cdiv(T, 4) * 4;
     Workspace ws(ctx, (part + (two ? 4 : 2) * ints + static_cast<size_t>(DIGITS) * chunks) * 4);
     if (!ws.p) return KDEC_ENOMEM;
@@ -606,7 +603,7 @@ int kdec_embed_bwd(kdec_ctx* ctx, int dtype, const void* dY, long dy_rs, const i
     const Tokens to[2] = {{room, room + ints}, {room + 2 * ints, room + 3 * ints}};
     int* counts = room + (two ? 4 : 2) * ints;
     Tokens from{const_cast<int*>(ids), nullptr};
-    if (chunks == 1) {
+    if (one) {
         so.bits = bits_of(static_cast<unsigned>(per - 1));
         from = to[0];
         hipLaunchKernelGGL((sort_range_k<float, false>), ranges, dim3(ST), 0, ctx->stream, so, static_cast<int>(per), from, nullptr, 0, cols,

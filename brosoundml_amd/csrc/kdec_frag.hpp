@@ -15,6 +15,8 @@
 
 #include <hip/hip_runtime.h>
 
+#include <type_traits>
+
 #include "kdec_buffer.hpp"
 
 namespace kdec {
@@ -312,6 +314,21 @@ template <int N, bool WILD> struct Terms<float, N, WILD> {
     f32x8 t[1];
     __device__ explicit Terms(f32x8 f) { t[0] = f; }
 };
+
+// The sum over a wave's lanes up to each lane's own.
+__device__ inline int wave_scan(int x) {
+    const auto add = [&](auto ctrl, auto rows) __attribute__((always_inline)) {
+        x += __builtin_amdgcn_update_dpp(0, x, decltype(ctrl)::value, decltype(rows)::value, 15, false);
+    };
+    typedef std::integral_constant<int, 15> All;
+    add(std::integral_constant<int, 0x111>{}, All{});  // lanes of 16 to the right by 1, 2, 4, 8
+    add(std::integral_constant<int, 0x112>{}, All{});
+    add(std::integral_constant<int, 0x114>{}, All{});
+    add(std::integral_constant<int, 0x118>{}, All{});
+    add(std::integral_constant<int, 0x142>{}, std::integral_constant<int, 10>{});  // the 16's last lane to the next 16
+    add(std::integral_constant<int, 0x143>{}, std::integral_constant<int, 12>{});  // lane 31 to the upper half
+    return x;
+}
 
 // Four values rounded to T at p, of which the first n are the tensor's.
 // vec: p is aligned to the four and n is 0 or 4 (or less).

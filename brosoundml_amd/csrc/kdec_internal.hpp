@@ -85,6 +85,19 @@ struct Workspace {
     template <class T> T* as() const { return static_cast<T*>(p); }
 };
 
+// Makes a context's device the current one for a call (its workspaces are
+// allocated there, its kernels launched there), and the caller's again after it.
+struct DeviceScope {
+    int before = -1;
+    explicit DeviceScope(const kdec_ctx* ctx) {
+        if (hipGetDevice(&before) == hipSuccess && before != ctx->device) (void)hipSetDevice(ctx->device);
+        else before = -1;
+    }
+    ~DeviceScope() { if (before >= 0) (void)hipSetDevice(before); }
+    DeviceScope(const DeviceScope&) = delete;
+    DeviceScope& operator=(const DeviceScope&) = delete;
+};
+
 // Profiling bracket around the launches of one kernel family (a null
 // context records nothing).
 struct ProfScope {

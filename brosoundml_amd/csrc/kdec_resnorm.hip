@@ -542,6 +542,7 @@ int kdec_resnorm_fwd(kdec_ctx* ctx, int dtype, int layer, const void* X, long x_
                      long gate_rs, int post, const void* w1, const void* b1, int pre, const void* w2, const void* b2, float eps,
                      float scale, float x_scale, int T, int C, void* R, long r_rs, void* Y, long y_rs, float* stats) {
     if (!ctx) return KDEC_EINVAL;
+    const DeviceScope device(ctx);
     Norm p;
     if (int rc = fill(ctx, "kdec_resnorm_fwd", dtype, layer, X, x_rs, Z, z_rs, gate, gate_rs, post, w1, b1, pre, w2, b2, eps, scale, x_scale,
                       T, C, p))
@@ -576,6 +577,7 @@ int kdec_resnorm_bwd(kdec_ctx* ctx, int dtype, int layer, const void* X, long x_
                      float scale, float x_scale, int T, int C, const float* stats, const void* dR, long dr_rs, const void* dY, long dy_rs,
                      void* dX, void* dZ, void* dgate, float* dw1, float* db1, float* dw2, float* db2) {
     if (!ctx) return KDEC_EINVAL;
+    const DeviceScope device(ctx);
     Back b{};
     if (int rc = fill(ctx, "kdec_resnorm_bwd", dtype, layer, X, x_rs, Z, z_rs, gate, gate_rs, post, w1, b1, pre, w2, b2, eps, scale, x_scale,
                       T, C, b.n))
@@ -602,8 +604,14 @@ int kdec_resnorm_bwd(kdec_ctx* ctx, int dtype, int layer, const void* X, long x_
     }
     ProfScope ps(ctx, "resnorm", 0.0, static_cast<double>(es) * T * C * (3 + (Z ? 2 : 0) + (pre ? 1 : 0) + (by_row ? 2 : 0)));
     const Shape sh = shape(C);
-    long blocks = cdiv(T, sh.rows);
+    // A block's rows: at least eight, since its sums cost as much to write and read
+    // as two or three rows, unless that leaves CUs without a block; two blocks a CU
+    // at most (bf16, forward and backward, one block a CU, two, four: 8192 x 2048
+    // 112 us, 98, 102; 8192 x 1024 57, 51, 57; 2048 x 5120 90, 100, 117).
+    long blocks = cdiv(T, 8L * sh.rows);
+    if (blocks < ctx->num_cus) blocks = ctx->num_cus;
     if (blocks > 2L * ctx->num_cus) blocks = 2L * ctx->num_cus;
+    if (blocks > cdiv(T, sh.rows)) blocks = cdiv(T, sh.rows);
     Workspace ws(ctx, static_cast<size_t>(blocks) * b.sums * C * sizeof(float));
     if (!ws.p) return KDEC_ENOMEM;
     b.part = ws.as<float>();
