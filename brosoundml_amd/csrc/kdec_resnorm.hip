@@ -17,6 +17,12 @@
 // and sums dw1 = du z^, db1 = du, dw2 = dy r^, db2 = dy, and dg of a column's
 // gate over the rows: every block over its rows in registers, a second kernel
 // over the blocks in their order.
+//
+// Bound by memory where rows are many: 8192 x 2048, bf16, a gate for each row,
+// forward 35 us for 168 MB (4.8 TB/s; a large copy reaches 5.1), backward 53 and 5
+// for 268; 2050 x 5120 forward 18.6 for 84 MB; 4093 x 768, float, layer norms,
+// 12 for 50 MB, then 21 and 4 for 75. 16 rows of 1024 take 3.6 us, a launch and
+// three reductions.
 #include "kdec_frag.hpp"
 #include "kdec_internal.hpp"
 
@@ -604,13 +610,11 @@ int kdec_resnorm_bwd(kdec_ctx* ctx, int dtype, int layer, const void* X, long x_
     }
     ProfScope ps(ctx, "resnorm", 0.0, static_cast<double>(es) * T * C * (3 + (Z ? 2 : 0) + (pre ? 1 : 0) + (by_row ? 2 : 0)));
     const Shape sh = shape(C);
-    // A block's rows: at least eight, since its sums cost as much to write and read
-    // as two or three rows, unless that leaves CUs without a block; two blocks a CU
-    // at most (bf16, forward and backward, one block a CU, two, four: 8192 x 2048
-    // 112 us, 98, 102; 8192 x 1024 57, 51, 57; 2048 x 5120 90, 100, 117).
-    long blocks = cdiv(T, 8L * sh.rows);
-    if (blocks < ctx->num_cus) blocks = ctx->num_cus;
-    if (blocks > 2L * ctx->num_cus) blocks = 2L * ctx->num_cus;
+    // Two blocks a CU, one of more than four waves: their sums are so much more to
+    // write and read (bf16, forward and backward, one block a CU, two, four: 8192 x
+    // 2048 112 us, 98, 102; 16000 x 1024 98, 85; 4096 x 4096 94, 102; 2048 x 5120 91,
+    // 101, 117).
+    long blocks = (sh.threads > 256 ? 1L : 2L) * ctx->num_cus;
     if (blocks > cdiv(T, sh.rows)) blocks = cdiv(T, sh.rows);
     Workspace ws(ctx, static_cast<size_t>(blocks) * b.sums * C * sizeof(float));
     if (!ws.p) return KDEC_ENOMEM;
