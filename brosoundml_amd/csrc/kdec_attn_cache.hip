@@ -17,6 +17,11 @@
 // whatever bytes a lane has: of a key 16 bytes in each 64, the query's fragments
 // following, and of a value ND neighbouring columns, so that row m of the
 // output's block dt is column ND m + dt and no byte moves between lanes.
+//
+// Steps are bound by memory: one token for 48 requests over up to 4096 keys, 16
+// heads on 4 of width 128, 27 us for 106 MB (3.9 TB/s) and 4 for the join. Pieces of
+// 90 to 301 rows with a cap (73 us; the products alone would take 18.5) are
+// bound by the vector unit: codes to floats, exponentials of cap and softmax.
 #include "kdec_attn.hpp"
 
 namespace kdec {

@@ -389,8 +389,8 @@ struct Sums {
 };
 
 // A wave walks a piece's tokens for 64 parts of a row, sixteen rows' loads at a
-// time: 16381 rows of 1024 bf16 take 14.1 us (34 MB read, 20 written), 8190 of 768
-// floats 9.0 (25 and 13), of which the ids' and the first rows' way is about five.
+// time: 16381 rows of 1024 bf16 take 14.1 us (34 MB read), 8190 of 768
+// floats 9.2 (25 read).
 template <class T>
 __global__ __launch_bounds__(ET) void embed_sums_k(Sums s, const T* __restrict__ dY, long rs, bool vec) {
     constexpr int E = PART<T>, N = 16;
@@ -586,7 +586,7 @@ int kdec_embed_bwd(kdec_ctx* ctx, int dtype, const void* dY, long dy_rs, const i
     s.chunks = static_cast<int>(cdiv(cols, 64 * el));
     // Tokens of a piece: a piece leaves up to two partial rows, eight waves a CU are
     // what the loads need (the two cases above with pieces of 8, 16 and 32, sums and
-    // join: 23.5 us, 20.0, 20.9 and 14.3, 13.9, 18.3).
+    // join: 23.5 us, 20.0, 20.9 and 14.3, 14.1, 18.3).
     s.piece = 64;
     while (s.piece > 16 && cdiv(T, s.piece) * s.chunks < 8L * ctx->num_cus) s.piece /= 2;
     s.pieces = static_cast<int>(cdiv(T, s.piece));

@@ -19,9 +19,9 @@
 // over the blocks in their order.
 //
 // Bound by memory where rows are many: 8192 x 2048, bf16, a gate for each row,
-// forward 35 us for 168 MB (4.8 TB/s; a large copy reaches 5.1), backward 53 and 5
-// for 268; 2050 x 5120 forward 18.6 for 84 MB; 4093 x 768, float, layer norms,
-// 12 for 50 MB, then 21 and 4 for 75. 16 rows of 1024 take 3.6 us, a launch and
+// forward 37 us for 168 MB (4.5 TB/s; a large copy reaches 5.1), backward 53 and 5
+// for 268; 2050 x 5120 forward 18.4 for 84 MB; 4093 x 768, float, layer norms,
+// 12.4 for 50 MB, then 21 and 4 for 75. 16 rows of 1024 take 3.6 us, a launch and
 // three reductions.
 #include "kdec_frag.hpp"
 #include "kdec_internal.hpp"
