@@ -579,6 +579,14 @@ int kdec_embed_bwd(kdec_ctx* ctx, int dtype, const void* dY, long dy_rs, const i
                                static_cast<const bf16*>(dY), dy_rs, cols, scale);
         return launch_check(ctx, "kdec_embed_bwd");
     }
+    // Blocks that clear or scale the table beside the first count's, or alone.
+    long fill = beta == 1.0f ? 0 : cdiv(n, 16L * ST);
+    if (fill > 2L * ctx->num_cus) fill = 2L * ctx->num_cus;
+    if (T == 0) {
+        if (fill)
+            hipLaunchKernelGGL(sort_count_k, dim3(static_cast<unsigned>(fill)), dim3(ST), 0, ctx->stream, so, 0, 0, ids, nullptr);
+        return launch_check(ctx, "kdec_embed_bwd");
+    }
     Sums s{};
     s.T = T;
     s.vocab = vocab;
@@ -613,8 +621,6 @@ int kdec_embed_bwd(kdec_ctx* ctx, int dtype, const void* dY, long dy_rs, const i
                            scale);
     } else {
         so.bits = (bits + passes - 1) / passes;
-        long fill = beta == 1.0f ? 0 : cdiv(n, 16L * ST);  // blocks beside the first count's
-        if (fill > 2L * ctx->num_cus) fill = 2L * ctx->num_cus;
         for (int p = 0; p < passes; ++p) {
             hipLaunchKernelGGL(sort_count_k, dim3(static_cast<unsigned>(chunks + (p == 0 ? fill : 0))), dim3(ST), 0, ctx->stream, so, p,
                                chunks, from.id, counts);

@@ -181,3 +181,14 @@ def test_refusals(ctx):
     assert tokens.embedding(ctx, table[:0], ids).abs().sum() == 0
     with torch.no_grad():
         assert torch.equal(tokens.embedding(ctx, table.clone().requires_grad_(), ids), table[:3])
+
+
+@pytest.mark.parametrize("vocab", [9, 600001])
+def test_gradient_of_no_tokens(ctx, vocab):
+    """The table is cleared, scaled or left as it was, however many ids it has."""
+    from brosoundml_amd import tokens
+    ids, dy = ints([]), torch.empty(0, 3, device="cuda")
+    assert (tokens.embedding_bwd(ctx, ids, dy, vocab) == 0).all()
+    for beta, want in ((1.0, 7.0), (0.5, 3.5), (0.0, 0.0)):
+        held = torch.full((vocab, 3), 7.0, device="cuda")
+        assert (tokens.embedding_bwd(ctx, ids, dy, vocab, dtable=held, beta=beta) == want).all(), beta
