@@ -79,9 +79,20 @@ int guard_check_all(kdec_ctx* ctx, const char* where) {
     return hits;
 }
 
+// Whether the context's stream is being captured into a graph.
+static bool capturing(const kdec_ctx* ctx) {
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    if (hipStreamIsCapturing(ctx->stream, &status) != hipSuccess) {
+        (void)hipGetLastError();
+        return false;
+    }
+    return status != hipStreamCaptureStatusNone;
+}
+
 void* ws_alloc(kdec_ctx* ctx, size_t bytes) {
     if (bytes == 0) bytes = 256;
     bytes = (bytes + 255) & ~size_t(255);
+    const bool captures = capturing(ctx);
     const size_t need = guard_mode() ? bytes + 2 * kGuard : bytes;
     void* base = nullptr;
     size_t size = need;
@@ -94,26 +105,33 @@ void* ws_alloc(kdec_ctx* ctx, size_t bytes) {
         ctx->pool.erase(it);
     } else {
         hipError_t e = hipMalloc(&base, need);
-        hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
-        if (e != hipSuccess && hipStreamIsCapturing(ctx->stream, &capture) == hipSuccess && capture != hipStreamCaptureStatusNone) {
-            // The pool's blocks may be an earlier graph's: none is given back here.
+        if (e != hipSuccess && captures) {
             (void)hipGetLastError();
             fail(ctx, KDEC_ENOMEM, "no workspace while a graph is captured: make the call once before");
             return nullptr;
         }
         if (e != hipSuccess) {
-            // Return every pooled block to the driver and try once more.
+            // Return every pooled block that no graph uses to the driver and try once more.
+            (void)hipGetLastError();
             hipStreamSynchronize(ctx->stream);
-            for (auto& kv : ctx->pool) hipFree(kv.second);
-            ctx->pool.clear();
-            ctx->pooled_bytes = 0;
+            for (auto b = ctx->pool.begin(); b != ctx->pool.end();) {
+                if (ctx->captured.count(b->second)) {
+                    ++b;
+                    continue;
+                }
+                hipFree(b->second);
+                ctx->pooled_bytes -= b->first;
+                b = ctx->pool.erase(b);
+            }
             e = hipMalloc(&base, need);
             if (e != hipSuccess) {
+                (void)hipGetLastError();  // not the next launch's
                 hip_fail(ctx, e, "hipMalloc");
                 return nullptr;
             }
         }
     }
+    if (captures) ctx->captured.insert(base);
     const kdec_ctx::Block blk{base, size, bytes};
     void* user = guard_mode() ? static_cast<char*>(base) + kGuard : base;
     if (guard_mode()) guard_fill(ctx, blk);

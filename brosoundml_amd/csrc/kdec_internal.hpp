@@ -7,6 +7,7 @@
 #include <map>
 #include <string>
 #include <unordered_map>
+#include <unordered_set>
 #include <utility>
 #include <vector>
 
@@ -29,6 +30,9 @@ struct kdec_ctx {
         size_t bytes;  // bytes handed out (after the front guard in guard mode)
     };
     std::unordered_map<void*, Block> live;  // handed-out pointer -> its block
+    // Blocks that a captured graph uses: pooled like the others, but given back
+    // to the driver only with the context, which outlives the graph.
+    std::unordered_set<void*> captured;
     size_t pooled_bytes = 0;
     // Set by kdec_ctx_destroy while blocks are still live (tensors that
     // outlive their context): the last ws_free then releases the context.

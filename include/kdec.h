@@ -546,9 +546,10 @@ int kdec_adapter_bwd(kdec_ctx* ctx, int dtype, const void* X, long x_rs,
                      long dx_rs, float* dA, float* dB, float beta);
 
 /* The calls from here on can be captured into a graph once they were made with
- * the same sizes before (their workspaces are then the context's). Graphs of one
- * context share these with each other and with its other calls, so they are
- * replayed on its stream, and the context outlives them. */
+ * the same sizes before (their workspaces are then the context's, which keeps
+ * them until it is destroyed). Graphs of one context share these with each other
+ * and with its other calls, so they are replayed on its stream, and the context
+ * outlives them. */
 
 /* Embedding: Y[t] = scale * table[ids[t]] (table (vocab, cols) at row stride
  * t_rs, Y (T, cols) at y_rs); an id outside [0, vocab) gives a row of zeros. */

@@ -81,3 +81,33 @@ def test_two_graphs_of_one_context():
                 want = work(ctx, fresh)
             side.synchronize()
             assert same(o, want), turn
+
+
+def test_a_graph_keeps_its_workspaces():
+    """A later call whose workspace the device cannot hold makes the context give back its pooled blocks: not those that a
+    graph uses. What the blocks' memory could become meanwhile is written over between the replays."""
+    from brosoundml_amd import native, tokens
+    side = torch.cuda.Stream()
+    ctx = native.Context(0, stream=side)
+    s = state(4)
+    want = [t.clone() for t in work(native.Context(0), state(4))]
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        work(ctx, s)
+    side.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=side):
+        out = work(ctx, s)
+    ids = torch.zeros(1 << 24, dtype=torch.int32, device="cuda")
+    dy = torch.zeros(1, 1 << 20, dtype=torch.bfloat16, device="cuda").expand(1 << 24, 1 << 20)
+    torch.cuda.synchronize()
+    for _ in range(3):
+        with torch.cuda.stream(side):
+            with pytest.raises(native.KdecError, match="memory|hipMalloc"):
+                tokens.embedding_bwd(ctx, ids, dy, 1)  # 2 TB of partial sums
+        other = torch.full((1 << 24,), float("nan"), device="cuda")
+        with torch.cuda.stream(side):
+            g.replay()
+        side.synchronize()
+        assert same(out, want)
+        del other
