@@ -532,7 +532,7 @@ extern "C" int kdec_attn_cache_fwd(kdec_ctx* ctx, int dtype, const void* Q, long
     // 300 rows 80 for 89; even ones of 4 rows 24.6 for 22.5).
     p.a.by_doc = p.rows > 1 && docs > 0 && docs < 127 && (Tq % docs != 0 || mean % p.rows != 0);
     const long units = cdiv(Tq, p.rows) * p.pieces * Hkv, blocks = doc_blocks(p.a.by_doc, docs, Tq, p.rows) * p.pieces * Hkv;
-    KDEC_CHECK(ctx, blocks < INT_MAX && static_cast<long>(Hkv) * p.a.E < INT_MAX, "kdec_attn_cache_fwd: too many rows");
+    KDEC_CHECK(ctx, grid_holds(blocks, AT) && static_cast<long>(Hkv) * p.a.E < INT_MAX, "kdec_attn_cache_fwd: too many rows");
     // Split the keys where the rows alone do not fill the device, as far as all
     // parts' blocks are on it at once (48 documents of 90 to 4096 keys and 1 row: 4
     // parts, which fill it, 26 us, 3 and 6 parts 31 and 32), to no fewer than 256

@@ -216,6 +216,7 @@ int kdec_cache_write(kdec_ctx* ctx, int dtype, const void* K, long k_rs, long k_
     const int L = W <= 64 ? 8 : 16;
     const dim3 grid(static_cast<unsigned>(cdiv(Tq, CT / L)), static_cast<unsigned>(cdiv(2L * H, UNITS)));
     KDEC_CHECK(ctx, cdiv(2L * H, UNITS) <= 65535, "kdec_cache_write: too many heads");
+    KDEC_CHECK(ctx, grid_holds(cdiv(Tq, CT / L), CT), "kdec_cache_write: too many rows");
     const auto run = [&](auto k_) { hipLaunchKernelGGL(k_, grid, dim3(CT), 0, ctx->stream, m, k, v, o, H, D, W, vec); };
     if (dtype == KDEC_F32) run(L == 8 ? cache_write_k<float, 8> : cache_write_k<float, 16>);
     else run(L == 8 ? cache_write_k<bf16, 8> : cache_write_k<bf16, 16>);
@@ -240,6 +241,7 @@ int kdec_cache_read(kdec_ctx* ctx, int dtype, const void* Kc, long kc_rs, long k
     const int L = W <= 64 ? 8 : 16;
     const dim3 grid(static_cast<unsigned>(cdiv(Tq, CT / L)), static_cast<unsigned>(cdiv(2L * H, UNITS)));
     KDEC_CHECK(ctx, cdiv(2L * H, UNITS) <= 65535, "kdec_cache_read: too many heads");
+    KDEC_CHECK(ctx, grid_holds(cdiv(Tq, CT / L), CT), "kdec_cache_read: too many rows");
     const auto run = [&](auto k_, auto ty) {
         typedef decltype(ty) E;
         hipLaunchKernelGGL(k_, grid, dim3(CT), 0, ctx->stream, m, o, H, D, W, static_cast<E*>(K), k_rs, k_hs, static_cast<E*>(V), v_rs, v_hs,

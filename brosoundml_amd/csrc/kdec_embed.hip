@@ -602,13 +602,14 @@ int kdec_embed_bwd(kdec_ctx* ctx, int dtype, const void* dY, long dy_rs, const i
     s.table = dtable;
     s.add = beta != 0.0f;
     const long units = static_cast<long>(s.pieces) * s.chunks;
-    KDEC_CHECK(ctx, cdiv(units, ET / 64) < INT_MAX && cdiv(cols, 256) <= 65535, "kdec_embed_bwd: bad sizes");
+    KDEC_CHECK(ctx, cdiv(cols, 256) <= 65535, "kdec_embed_bwd: too many columns");
     int bits = bits_of(static_cast<unsigned>(vocab));
     const int passes = (bits + 7) / 8;
     const bool two = !one && passes > 1;  // passes that read what the last one wrote
     const size_t part = cdiv(static_cast<long>(s.pieces) * 2 * cols, 4) * 4, ints = cdiv(T, 4) * 4;
     Workspace ws(ctx, (part + (two ? 4 : 2) * ints + static_cast<size_t>(DIGITS) * chunks) * 4);
     if (!ws.p) return KDEC_ENOMEM;
+    KDEC_CHECK(ctx, grid_holds(cdiv(units, ET / 64), ET) && grid_holds(s.pieces, ET), "kdec_embed_bwd: too many tokens");
     s.part = ws.as<float>();
     int* room = reinterpret_cast<int*>(s.part + part);
     const Tokens to[2] = {{room, room + ints}, {room + 2 * ints, room + 3 * ints}};

@@ -102,6 +102,10 @@ struct DeviceScope {
     DeviceScope& operator=(const DeviceScope&) = delete;
 };
 
+// Whether a launch of so many blocks stays below the 2^32 threads that a grid's
+// dimension holds.
+inline bool grid_holds(long blocks, long threads) { return blocks * threads < (1L << 32); }
+
 // Profiling bracket around the launches of one kernel family (a null
 // context records nothing).
 struct ProfScope {

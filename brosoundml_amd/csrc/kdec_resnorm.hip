@@ -566,6 +566,7 @@ int kdec_resnorm_fwd(kdec_ctx* ctx, int dtype, int layer, const void* X, long x_
     p.stats = stats;
     ProfScope ps(ctx, "resnorm", 0.0, static_cast<double>(es) * T * C * (1 + (Z ? 2 : 0) + (pre ? 1 : 0) + (gate && gate_rs ? 1 : 0)));
     const Shape sh = shape(C);
+    KDEC_CHECK(ctx, grid_holds(cdiv(T, sh.rows), sh.threads), "kdec_resnorm_fwd: too many rows");
     const auto run = [&](auto ty) {
         typedef decltype(ty) E;
         by_shape(sh, p.vec, [&](auto v, auto w, auto vec) {

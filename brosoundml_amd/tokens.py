@@ -28,6 +28,7 @@ except ImportError:
     def _raw_stream(device):
         return torch.cuda.current_stream(device).cuda_stream
 
+_INT_MAX = 0x7FFFFFFF
 _TYPES = {torch.float32: 0, torch.bfloat16: 1}
 
 
@@ -265,6 +266,8 @@ def embedding(ctx: Context, table, ids, *, scale=1.0, out=None):
     dt = _dtype(ctx, table)
     W = _rows(table, "table")
     vocab, cols = table.shape
+    if vocab > _INT_MAX:
+        _fail("a table has from 0 to 2^31 - 1 rows")
     t = ids.numel()
     if ids.dim() != 1:
         _fail("ids must be (T)")
@@ -287,6 +290,8 @@ def embedding_bwd(ctx: Context, ids, dy, vocab, *, scale=1.0, dtable=None, beta=
     if ids.dim() != 1:
         _fail("ids must be (T)")
     I = _ints(ctx, ids, t, "ids")
+    if not 0 <= vocab <= _INT_MAX:
+        _fail("a table has from 0 to 2^31 - 1 rows")
     if not (beta == 0.0 or dtable is not None):
         _fail("beta without dtable to add to")
     g = _empty(ctx, dy, (vocab, cols), torch.float32) if dtable is None else dtable

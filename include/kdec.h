@@ -573,7 +573,8 @@ int kdec_embed_bwd(kdec_ctx* ctx, int dtype, const void* dY, long dy_rs,
  * Y = N_pre(X) alone, without post, gate and R. stats (T, 4 floats, aligned to
  * 16 bytes) is written when not NULL, for the backward. R enters N_pre before
  * its rounding. R may be X or Z, and Y either of them. Sums are floats: squares
- * past 2^127 overflow. C <= 8192, eps > 0. */
+ * past 2^127 overflow. C <= 8192, eps > 0; up to 2^26 - 4 rows of up
+ * to 512 columns, fewer of more. */
 int kdec_resnorm_fwd(kdec_ctx* ctx, int dtype, int layer, const void* X,
                      long x_rs, const void* Z, long z_rs, const void* gate,
                      long gate_rs, int post, const void* w1, const void* b1,

@@ -192,3 +192,16 @@ def test_gradient_of_no_tokens(ctx, vocab):
     for beta, want in ((1.0, 7.0), (0.5, 3.5), (0.0, 0.0)):
         held = torch.full((vocab, 3), 7.0, device="cuda")
         assert (tokens.embedding_bwd(ctx, ids, dy, vocab, dtable=held, beta=beta) == want).all(), beta
+
+
+def test_tables_past_what_a_call_takes(ctx):
+    """Sizes that do not fit the C ABI's int are refused, not cut to it."""
+    from brosoundml_amd import tokens
+    ids = ints([1, 2, 3])
+    for vocab in (2 ** 31, 2 ** 32 + 5):
+        with pytest.raises(ValueError, match="rows"):
+            tokens.embedding(ctx, torch.ones(1, 8, device="cuda").expand(vocab, 8), ids)
+        with pytest.raises(ValueError, match="rows"):
+            tokens.embedding_bwd(ctx, ids, torch.ones(3, 8, device="cuda"), vocab)
+    with pytest.raises(ValueError, match="rows"):
+        tokens.embedding_bwd(ctx, ids, torch.ones(3, 8, device="cuda"), -1)

@@ -335,3 +335,18 @@ def test_refusals(ctx):
     assert r.shape == y.shape == (0, 32)
     dx, dz, dg, (dw, _), _ = tokens.residual_norm_bwd(ctx, none, none, none, none, s, gate=w, **fine)
     assert dx.shape == (0, 32) and not dg.any() and not dw.any()
+
+
+def test_more_rows_than_a_launch_holds(ctx):
+    """2^26 rows in blocks of four would be 2^32 threads: refused, with nothing written."""
+    from brosoundml_amd import native, tokens
+    t = 1 << 26
+    y = torch.full((t, 1), 7.0, device="cuda")
+    x = torch.ones(1, 1, device="cuda").expand(t, 1)
+    with pytest.raises(native.KdecError, match="too many rows"):
+        tokens.residual_norm(ctx, x, pre=torch.ones(1, device="cuda"), out=(None, y))
+    assert (y == 7).all()
+    n = t - 4
+    tokens.residual_norm(ctx, x[:n], pre=torch.ones(1, device="cuda"), out=(None, y[:n]), eps=3.0)
+    # 1 / sqrt(1 + 3), the root and its reciprocal within a few steps of a float's half rounding
+    assert ((y[:n] - 0.5).abs() <= 4 * 2.0 ** -24).all() and (y[n:] == 7).all()
