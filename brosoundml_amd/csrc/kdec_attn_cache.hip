@@ -3,11 +3,13 @@
 // A key's score is its scale times q . codes, a value enters the output with
 // its scale in its probability: o = sum_j (p_j vs_j) codes_j / sum_j p_j. The
 // codes themselves are exact in bf16, so the products are bf16 ones. Float tensors
-// enter them as three bf16 terms, which hold their 24 bits. For bf16 tensors p vs
-// enters as two where few rows leave the matrix units time (one token for 48
-// requests 26.8 us, with one term 26.6; relative error of o 0.0017, that of its
-// rounding, for 0.0024), rounded to one where a block holds 32 entries (pieces of
-// 90 to 301 rows 72 us for 81), as the attention over float keys rounds it.
+// enter them as three bf16 terms, which hold their 24 bits, and p vs as three as
+// well. For bf16 tensors p vs enters as two, which leave 2^-16 of it at most: o is
+// off by its own rounding alone (relative error 0.0017, as the formula's in float
+// sums rounded once; one term made it 0.0023), whatever else a call holds. Where
+// memory bounds a call the second term costs nothing (one token for 48 requests 26.8
+// us, with one 26.6), where the vector unit does a seventh (5 documents of 200 rows
+// 70 us for 62).
 //
 // A block holds 16 or 32 entries (rows of one document times the heads that share
 // a key head) and its four waves take tiles of 32 keys in turn, each with a
@@ -178,7 +180,7 @@ __device__ inline void cache_soft(const Score<T, CAP, BIAS>& rule, int pos, unsi
 // CB: blocks of 16 entries that a wave holds.
 template <class T, int DP, int CAP, bool BIAS, int CB>
 __global__ __launch_bounds__(AT, sizeof(T) == 2 ? (CB == 1 ? 3 : 2) : 1) void attn_cache_k(Cached p) {
-    constexpr int NC = DP / 32, NK = DP / 64, ND = DP / 16, TERMS = sizeof(T) == 2 ? 1 : 3, WTERMS = sizeof(T) == 4 ? 3 : CB == 1 ? 2 : 1, PITCH = DP + 4, COLS = 16 * CB;
+    constexpr int NC = DP / 32, NK = DP / 64, ND = DP / 16, TERMS = sizeof(T) == 2 ? 1 : 3, WTERMS = sizeof(T) == 2 ? 2 : 3, PITCH = DP + 4, COLS = 16 * CB;
     __shared__ __align__(16) float so[4][COLS][PITCH];
     __shared__ __align__(16) float scales[4][2][CN];
     __shared__ float sml[4][2][COLS];
@@ -519,17 +521,19 @@ extern "C" int kdec_attn_cache_fwd(kdec_ctx* ctx, int dtype, const void* Q, long
     p.lse = lse;
     // Entries of a block: 16 where a document's rows have no more, else 32 that
     // share a code's way to a float (bf16, 16 heads on 4 of width 128, blocks of 16
-    // and 32: 48 documents of 90 to 4096 keys and 1 row 31 us and 42, 16 of 2000 to
-    // 4096 and 8 rows 30 and 28, 5 of them and 200 rows 82 and 62). Rows: what these
-    // hold, fewer where documents have fewer.
+    // and 32: 48 documents of 90 to 4096 keys and 1 row 32 us and 45, 16 of 2000 to
+    // 4096 and 4 rows 22.8 and 23.6, 8 rows 30 and 27, 5 of them and 200 rows 83 and
+    // 70; rows that leave blocks of 32 part empty cost that again, 20 of 1000 to 2000
+    // keys and 10 to 40 rows 36 and 43). Rows: what these hold, fewer where documents
+    // have fewer.
     const long mean = docs > 0 ? cdiv(Tq, docs) : Tq;
     const int cols = mean * G <= 16 ? 16 : 32;
     p.pieces = static_cast<int>(cdiv(G, cols));
     p.rows = static_cast<int>(G >= cols ? 1 : mean < cols / G ? mean : cols / G);
     // Blocks that end with their document where rows may not be even, as far as
     // finding them is quick: one that holds rows of two walks twice (48 documents of
-    // up to 4096 keys, 1 to 4 rows 50 us for 62, 2 to 9 rows 59 for 74, 5 of 100 to
-    // 300 rows 80 for 89; even ones of 4 rows 24.6 for 22.5).
+    // up to 4096 keys, 1 to 4 rows 51 us for 63, 2 to 9 rows 62 for 79, 5 of 100 to
+    // 300 rows 91 for 102; even ones of 4 rows 24.6 for 22.5).
     p.a.by_doc = p.rows > 1 && docs > 0 && docs < 127 && (Tq % docs != 0 || mean % p.rows != 0);
     const long units = cdiv(Tq, p.rows) * p.pieces * Hkv, blocks = doc_blocks(p.a.by_doc, docs, Tq, p.rows) * p.pieces * Hkv;
     KDEC_CHECK(ctx, grid_holds(blocks, AT) && static_cast<long>(Hkv) * p.a.E < INT_MAX, "kdec_attn_cache_fwd: too many rows");
