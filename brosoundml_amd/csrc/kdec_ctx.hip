@@ -89,7 +89,7 @@ static bool capturing(const kdec_ctx* ctx) {
     return status != hipStreamCaptureStatusNone;
 }
 
-void* ws_alloc(kdec_ctx* ctx, size_t bytes) {
+void* ws_alloc(kdec_ctx* ctx, size_t bytes, bool scoped) {
     if (bytes == 0) bytes = 256;
     bytes = (bytes + 255) & ~size_t(255);
     const bool captures = capturing(ctx);
@@ -97,7 +97,12 @@ void* ws_alloc(kdec_ctx* ctx, size_t bytes) {
     void* base = nullptr;
     size_t size = need;
     // Reuse a pooled block of at least `need` bytes but not absurdly larger.
+    const auto usable = [&](void* block) {
+        const auto graph = ctx->captured.find(block);
+        return graph == ctx->captured.end() || (scoped && graph->second == ctx->stream);
+    };
     auto it = ctx->pool.lower_bound(need);
+    while (it != ctx->pool.end() && !usable(it->second)) ++it;
     if (it != ctx->pool.end() && it->first <= need * 2 + (1 << 20)) {
         base = it->second;
         size = it->first;
@@ -131,7 +136,7 @@ void* ws_alloc(kdec_ctx* ctx, size_t bytes) {
             }
         }
     }
-    if (captures) ctx->captured.insert(base);
+    if (captures) ctx->captured[base] = ctx->stream;
     const kdec_ctx::Block blk{base, size, bytes};
     void* user = guard_mode() ? static_cast<char*>(base) + kGuard : base;
     if (guard_mode()) guard_fill(ctx, blk);
@@ -280,7 +285,7 @@ int kdec_synchronize(kdec_ctx* ctx) {
 
 int kdec_malloc(kdec_ctx* ctx, size_t bytes, void** out) {
     if (!ctx || !out) return KDEC_EINVAL;
-    *out = ws_alloc(ctx, bytes);
+    *out = ws_alloc(ctx, bytes, false);
     return *out ? KDEC_OK : KDEC_ENOMEM;
 }
 

@@ -7,7 +7,6 @@
 #include <map>
 #include <string>
 #include <unordered_map>
-#include <unordered_set>
 #include <utility>
 #include <vector>
 
@@ -30,9 +29,13 @@ struct kdec_ctx {
         size_t bytes;  // bytes handed out (after the front guard in guard mode)
     };
     std::unordered_map<void*, Block> live;  // handed-out pointer -> its block
-    // Blocks that a captured graph uses: pooled like the others, but given back
-    // to the driver only with the context, which outlives the graph.
-    std::unordered_set<void*> captured;
+    // Blocks that a captured graph uses, with the stream it was captured on. A
+    // replay writes them whenever it comes, so they are given back to the driver
+    // only with the context, which outlives the graph, and the pool hands them out
+    // again only to a call's own workspace on that stream: its kernels and a
+    // replay's come one after the other, while memory that outlives a call, or work
+    // on another stream, would meet a replay in between.
+    std::unordered_map<void*, hipStream_t> captured;
     size_t pooled_bytes = 0;
     // Set by kdec_ctx_destroy while blocks are still live (tensors that
     // outlive their context): the last ws_free then releases the context.
@@ -75,14 +78,15 @@ int hip_fail(kdec_ctx* ctx, hipError_t e, const char* where);
 
 // Workspace from the context allocator (returns nullptr and sets the error on
 // failure); release with ws_free once the kernels that use it are enqueued.
-void* ws_alloc(kdec_ctx* ctx, size_t bytes);
+// `scoped`: it is released before the call that asks for it ends.
+void* ws_alloc(kdec_ctx* ctx, size_t bytes, bool scoped);
 void ws_free(kdec_ctx* ctx, void* p);
 
 // RAII workspace block.
 struct Workspace {
     kdec_ctx* ctx;
     void* p = nullptr;
-    Workspace(kdec_ctx* c, size_t bytes) : ctx(c) { p = ws_alloc(c, bytes); }
+    Workspace(kdec_ctx* c, size_t bytes) : ctx(c) { p = ws_alloc(c, bytes, true); }
     ~Workspace() { if (p) ws_free(ctx, p); }
     Workspace(const Workspace&) = delete;
     Workspace& operator=(const Workspace&) = delete;

@@ -547,9 +547,10 @@ int kdec_adapter_bwd(kdec_ctx* ctx, int dtype, const void* X, long x_rs,
 
 /* The calls from here on can be captured into a graph once they were made with
  * the same sizes before (their workspaces are then the context's, which keeps
- * them until it is destroyed). Graphs of one context share these with each other
- * and with its other calls, so they are replayed on its stream, and the context
- * outlives them. */
+ * them until it is destroyed). Graphs that were captured on one stream share these
+ * with each other and with the context's calls on it, so they are replayed on that
+ * stream, and the context outlives them. Memory from kdec_malloc (the drop-in
+ * layer's tensors among it) and calls on another stream get none of them. */
 
 /* Embedding: Y[t] = scale * table[ids[t]] (table (vocab, cols) at row stride
  * t_rs, Y (T, cols) at y_rs); an id outside [0, vocab) gives a row of zeros. */
