@@ -34,10 +34,15 @@ _TYPES = {torch.float32: 0, torch.bfloat16: 1}
 
 # A single token's kernels take a few microseconds, about what these checks
 # do: each reads what it needs of a tensor once, and forms no message that it
-# does not raise.
+# does not raise. Sizes that become ints of the C ABI are checked together, by
+# their bits: where one is past 2^31 - 1, so is (a | b).
 
 def _fail(what):
     raise ValueError("brosoundml: " + what)
+
+
+def _large():
+    _fail("sizes past 2^31 - 1: more than the C ABI's ints hold")
 
 
 def _no_graph(x):
@@ -125,6 +130,8 @@ def _attn_args(ctx, q, k, v, q_off, k_off, k_len, causal, prefix, scale, cap, sl
     docs = q_off.numel() - 1
     if not (docs >= 0):
         _fail("q_off must hold one offset more than there are documents")
+    if (tq | tk | hq | hkv | d | docs) > _INT_MAX:
+        _large()
     if k_off is None:
         if not (tq == tk):
             _fail("without k_off the keys are the query rows' own")
@@ -184,6 +191,8 @@ def _adapter_args(ctx, x, w, a, b, scale, idx, unit_off):
     if not (b.dim() == 3 and units >= 1):
         _fail("b must be (adapters, out, rank), unit_off units + 1 offsets")
     rank = b.shape[2]
+    if (t | cin | out | n | units | rank) > _INT_MAX:
+        _large()
     return (_whole(w, (out, cin), "w"), _whole(a, (n, units * rank, cin), "a"), _whole(b, (n, out, rank), "b"),
             _floats(ctx, scale, (n,), "scale"), _ints(ctx, idx, t, "idx"), _ints(ctx, unit_off, units + 1, "unit_off"), t, cin, out,
             n, units, rank)
@@ -246,6 +255,8 @@ def dropout(ctx: Context, x, p, seed, offset=0, *, residual=None, out=None):
     offsets of their own. ``out`` may be x."""
     dt = _dtype(ctx, x)
     X = _rows(x, "x")
+    if x.shape[1] > _INT_MAX:  # the rows are a long
+        _large()
     y = _empty(ctx, x, x.shape) if out is None else out
     _dtype(ctx, x, y)
     if not (y.shape == x.shape):
@@ -266,9 +277,9 @@ def embedding(ctx: Context, table, ids, *, scale=1.0, out=None):
     dt = _dtype(ctx, table)
     W = _rows(table, "table")
     vocab, cols = table.shape
-    if vocab > _INT_MAX:
-        _fail("a table has from 0 to 2^31 - 1 rows")
     t = ids.numel()
+    if (vocab | cols | t) > _INT_MAX:
+        _fail("a table has from 0 to 2^31 - 1 rows and columns, and as many ids")
     if ids.dim() != 1:
         _fail("ids must be (T)")
     if out is None:
@@ -289,9 +300,9 @@ def embedding_bwd(ctx: Context, ids, dy, vocab, *, scale=1.0, dtable=None, beta=
     t, cols = dy.shape
     if ids.dim() != 1:
         _fail("ids must be (T)")
-    I = _ints(ctx, ids, t, "ids")
-    if not 0 <= vocab <= _INT_MAX:
-        _fail("a table has from 0 to 2^31 - 1 rows")
+    if vocab < 0 or (vocab | cols | t) > _INT_MAX:
+        _fail("a table has from 0 to 2^31 - 1 rows and columns, and as many ids")
+    I = _ints(ctx, ids, t, "ids")  # noqa: E741
     if not (beta == 0.0 or dtable is not None):
         _fail("beta without dtable to add to")
     g = _empty(ctx, dy, (vocab, cols), torch.float32) if dtable is None else dtable
@@ -337,6 +348,8 @@ def _norm_args(ctx, x, z, gate, post, pre, kind, eps, scale, x_scale):
     """The arguments that both directions share, and x's type and shape."""
     dt, X, ty, shape = _dtype(ctx, x), _rows(x, "x"), x.dtype, x.shape
     t, c = shape
+    if (t | c) > _INT_MAX:
+        _large()
     if kind != "rms" and kind != "layer":
         _fail("kind must be 'rms' or 'layer'")
     G = None, 0
@@ -448,6 +461,8 @@ def _cache_args(ctx, cache, width):
     if len(shape) != 3 or v.shape != shape or shape[2] != wide:
         _fail(f"the cache's k and v must be (rows, heads, {wide})")
     heads = shape[1], shape[0]
+    if (shape[0] | shape[1] | wide) > _INT_MAX:
+        _large()
     return (*_heads(k, "the cache's k"), *_heads(v, "the cache's v"), _floats(ctx, ks, heads, "k_scale"), _floats(ctx, vs, heads, "v_scale")), \
         shape[0], shape[1]
 
@@ -456,6 +471,8 @@ def _places(ctx, q_off, k_off, k_len):
     docs = q_off.numel() - 1
     if docs < 0:
         _fail("q_off must hold one offset more than there are documents")
+    if docs > _INT_MAX:
+        _large()
     return _ints(ctx, q_off, docs + 1, "q_off"), _ints(ctx, k_off, docs + 1, "k_off"), _ints(ctx, k_len, docs, "k_len"), docs
 
 
@@ -471,6 +488,8 @@ def cache_write(ctx: Context, k, v, cache, q_off, k_off, k_len=None):
     C, rows, heads = _cache_args(ctx, cache, d)
     if v.shape != k.shape or heads != h:
         _fail("k and v must share their shape, and the cache's heads")
+    if t > _INT_MAX:
+        _large()
     ctx.call("kdec_cache_write", dt, *K, *V, *_places(ctx, q_off, k_off, k_len), t, rows, h, d, *C)
 
 
@@ -479,6 +498,8 @@ def cache_read(ctx: Context, cache, q_off, k_off, k_len=None, *, rows, width, dt
     of `rows` rows: (rows, heads, width) of ``dtype`` (kdec_cache_read). Rows
     that it would not have written are zeros."""
     C, tk, heads = _cache_args(ctx, cache, width)
+    if not 0 <= rows <= _INT_MAX:
+        _fail("rows must be from 0 to 2^31 - 1")
     if out is None:
         if dtype not in _TYPES:
             _fail("tensors must be float32 or bfloat16")
@@ -503,6 +524,8 @@ def cache_attention(ctx: Context, q, cache, q_off, k_off, k_len=None, *, causal=
     Q = _heads(q, "q")
     tq, hq, d = q.shape
     C, tk, hkv = _cache_args(ctx, cache, d)
+    if (tq | hq) > _INT_MAX:
+        _large()
     qo, ko, kl, docs = _places(ctx, q_off, k_off, k_len)
     if out is None:
         o = _empty(ctx, q, (tq, hq, d))
