@@ -395,7 +395,8 @@ template <class T>
 __global__ __launch_bounds__(ET) void embed_sums_k(Sums s, const T* __restrict__ dY, long rs, bool vec) {
     constexpr int E = PART<T>, N = 16;
     const int lane = threadIdx.x & 63;
-    const long unit = static_cast<long>(blockIdx.x) * (ET / 64) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const long block = static_cast<long>(blockIdx.y) * gridDim.x + blockIdx.x;
+    const long unit = block * (ET / 64) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int piece = static_cast<int>(unit / s.chunks), chunk = static_cast<int>(unit - static_cast<long>(piece) * s.chunks);
     if (piece >= s.pieces) return;
     const int s0 = piece * s.piece, n = min(s.piece, s.T - s0);
@@ -602,14 +603,19 @@ int kdec_embed_bwd(kdec_ctx* ctx, int dtype, const void* dY, long dy_rs, const i
     s.table = dtable;
     s.add = beta != 0.0f;
     const long units = static_cast<long>(s.pieces) * s.chunks;
+    // Blocks of the sums: past GX in rows of them, so that what a call takes is a
+    // matter of memory, and what no launch takes is refused before any is asked for.
+    constexpr long GX = 1 << 16;
+    const long blocks = cdiv(units, ET / 64);
+    const dim3 grid(static_cast<unsigned>(blocks < GX ? blocks : GX), static_cast<unsigned>(cdiv(blocks, GX)));
     KDEC_CHECK(ctx, cdiv(cols, 256) <= 65535, "kdec_embed_bwd: too many columns");
+    KDEC_CHECK(ctx, cdiv(blocks, GX) <= 65535 && grid_holds(s.pieces, ET), "kdec_embed_bwd: too many tokens");
     int bits = bits_of(static_cast<unsigned>(vocab));
     const int passes = (bits + 7) / 8;
     const bool two = !one && passes > 1;  // passes that read what the last one wrote
     const size_t part = cdiv(static_cast<long>(s.pieces) * 2 * cols, 4) * 4, ints = cdiv(T, 4) * 4;
     Workspace ws(ctx, (part + (two ? 4 : 2) * ints + static_cast<size_t>(DIGITS) * chunks) * 4);
     if (!ws.p) return KDEC_ENOMEM;
-    KDEC_CHECK(ctx, grid_holds(cdiv(units, ET / 64), ET) && grid_holds(s.pieces, ET), "kdec_embed_bwd: too many tokens");
     s.part = ws.as<float>();
     int* room = reinterpret_cast<int*>(s.part + part);
     const Tokens to[2] = {{room, room + ints}, {room + 2 * ints, room + 3 * ints}};
@@ -633,7 +639,6 @@ int kdec_embed_bwd(kdec_ctx* ctx, int dtype, const void* dY, long dy_rs, const i
     s.id = from.id;
     s.at = from.at;
     const bool vec = cols % el == 0 && reinterpret_cast<size_t>(dY) % 16 == 0 && dy_rs % el == 0;
-    const dim3 grid(static_cast<unsigned>(cdiv(units, ET / 64)));
     if (dtype == KDEC_F32)
         hipLaunchKernelGGL(embed_sums_k<float>, grid, dim3(ET), 0, ctx->stream, s, static_cast<const float*>(dY), dy_rs, vec);
     else
