@@ -71,14 +71,6 @@ int guard_mode() {
     return mode;
 }
 
-int guard_check_all(kdec_ctx* ctx, const char* where) {
-    if (!guard_mode()) return 0;
-    hipStreamSynchronize(ctx->stream);
-    int hits = 0;
-    for (const auto& kv : ctx->live) hits += guard_check(ctx, kv.first, kv.second, where);
-    return hits;
-}
-
 // Whether the context's stream is being captured into a graph.
 static bool capturing(const kdec_ctx* ctx) {
     hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
@@ -87,6 +79,17 @@ static bool capturing(const kdec_ctx* ctx) {
         return false;
     }
     return status != hipStreamCaptureStatusNone;
+}
+
+// A capture takes neither the bands' fills nor the waits and copies of a check: a
+// block that is handed out during one has no bands, and checks wait for its end.
+int guard_check_all(kdec_ctx* ctx, const char* where) {
+    if (!guard_mode() || capturing(ctx)) return 0;
+    hipStreamSynchronize(ctx->stream);
+    int hits = 0;
+    for (const auto& kv : ctx->live)
+        if (kv.second.bands) hits += guard_check(ctx, kv.first, kv.second, where);
+    return hits;
 }
 
 void* ws_alloc(kdec_ctx* ctx, size_t bytes, bool scoped) {
@@ -137,9 +140,9 @@ void* ws_alloc(kdec_ctx* ctx, size_t bytes, bool scoped) {
         }
     }
     if (captures) ctx->captured[base] = ctx->stream;
-    const kdec_ctx::Block blk{base, size, bytes};
+    const kdec_ctx::Block blk{base, size, bytes, guard_mode() && !captures};
     void* user = guard_mode() ? static_cast<char*>(base) + kGuard : base;
-    if (guard_mode()) guard_fill(ctx, blk);
+    if (blk.bands) guard_fill(ctx, blk);
     ctx->live[user] = blk;
     return user;
 }
@@ -149,7 +152,7 @@ void ws_free(kdec_ctx* ctx, void* p) {
     auto it = ctx->live.find(p);
     if (it == ctx->live.end()) return;
     const kdec_ctx::Block blk = it->second;
-    if (guard_mode()) {
+    if (blk.bands && !capturing(ctx)) {
         hipStreamSynchronize(ctx->stream);
         guard_check(ctx, p, blk, "free");
     }

@@ -27,6 +27,7 @@ struct kdec_ctx {
         void* base;    // start of the device block
         size_t size;   // bytes of the device block
         size_t bytes;  // bytes handed out (after the front guard in guard mode)
+        bool bands;    // whether its guard bands were filled
     };
     std::unordered_map<void*, Block> live;  // handed-out pointer -> its block
     // Blocks that a captured graph uses, with the stream it was captured on. A
@@ -140,7 +141,8 @@ int launch_check(kdec_ctx* ctx, const char* where);
 // of a block lands in a band and is reported (stderr and the context error)
 // when the block is freed, at kdec_synchronize, and with KDEC_GUARD=2 after
 // every launch, naming that launch. A debugging aid: it costs a device sync
-// per check. Returns the number of overwritten bands found.
+// per check. Blocks that are handed out while a graph is captured have none.
+// Returns the number of overwritten bands found.
 int guard_mode();
 int guard_check_all(kdec_ctx* ctx, const char* where);
 
