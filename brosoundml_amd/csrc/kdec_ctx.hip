@@ -179,7 +179,8 @@ static hipEvent_t get_event(kdec_ctx* ctx) {
 
 ProfScope::ProfScope(kdec_ctx* c, const char* n, double f, double b)
     : ctx(c), name(n), flops(f), bytes(b) {
-    if (ctx && ctx->prof) {
+    // a captured event never holds a time: reading one would fail
+    if (ctx && ctx->prof && !capturing(ctx)) {
         start = get_event(ctx);
         hipEventRecord(start, ctx->stream);
     }

@@ -64,7 +64,8 @@ int kdec_synchronize(kdec_ctx* ctx);
 /* Device memory from the context's stream-ordered caching allocator. */
 int kdec_malloc(kdec_ctx* ctx, size_t bytes, void** out);
 int kdec_free(kdec_ctx* ctx, void* ptr);
-/* Per-kernel-family timing with HIP events on the context stream (0 = off). */
+/* Per-kernel-family timing with HIP events on the context stream (0 = off).
+ * Calls that are captured into a graph are not timed. */
 int kdec_profile_enable(kdec_ctx* ctx, int on);
 /* Fills names / ms / launches / algorithmic FLOP / algorithmic HBM bytes
  * (any may be NULL) for up to `cap` families; returns the count. */

@@ -118,3 +118,28 @@ def test_calls_on_another_stream_stay_apart():
             got.append(work(ctx, s2))
     torch.cuda.synchronize()
     assert same(out, want) and all(same(o, want2) for o in got)
+
+
+def test_a_capture_while_calls_are_timed():
+    """With the context's timing on, captured calls are not timed (their events would never be read), and later calls work."""
+    from brosoundml_amd import native
+    side = torch.cuda.Stream()
+    ctx = native.Context(0, stream=side)
+    s = state(8)
+    want = [t.clone() for t in work(native.Context(0), state(8))]
+    torch.cuda.synchronize()
+    ctx.profile(True)
+    g, out = capture(ctx, side, s)
+    with torch.cuda.stream(side):
+        g.replay()
+    side.synchronize()
+    times = ctx.profile_read()
+    with torch.cuda.stream(side):
+        got = work(ctx, s)
+        g.replay()
+    side.synchronize()
+    assert same(got, want) and same(out, want)
+    again = ctx.profile_read()
+    ctx.profile(False)
+    for name in ("embed", "resnorm", "cache", "attn"):
+        assert times[name]["ms"] > 0 and again[name]["launches"] == 2 * times[name]["launches"]
