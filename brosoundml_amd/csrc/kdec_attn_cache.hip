@@ -273,7 +273,9 @@ __global__ __launch_bounds__(AT, sizeof(T) == 2 ? (CB == 1 ? 3 : 2) : 1) void at
         bf16x8 q[CB][NC][TERMS];
         const auto step = [&](auto masked, int t) __attribute__((always_inline)) {
             constexpr bool MASKED = decltype(masked)::value;
-            scales[wave][lane >> 5][lane & 31] = lane >> 5 ? vscale : kscale;
+            // an infinite scale as NaN: its scores could be minus infinity, or a cap's end
+            const float scale = lane >> 5 ? vscale : kscale;
+            scales[wave][lane >> 5][lane & 31] = __builtin_fmaf(scale, 0.0f, scale);
             f32x4 s[CB][2];
 #pragma unroll
             for (int g = 0; g < 2; ++g) {
