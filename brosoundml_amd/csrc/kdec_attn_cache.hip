@@ -137,7 +137,7 @@ __device__ inline void empty_part(const Cached& p, int kvh, int e) {
 
 // One step of the running softmax of a lane's column over the scores of 32 keys
 // from j0, `at` the lane's first: s become probabilities, acc is rescaled when
-// the wave's maxima move far enough: m in the units of raw products without cap
+// the column's maximum moves far enough: m in the units of raw products without cap
 // and bias, in log2 units with either.
 struct Soft {
     float m = -INF, l = 0.0f;
@@ -158,8 +158,10 @@ __device__ inline void cache_soft(const Score<T, CAP, BIAS>& rule, int pos, unsi
             mx = fmaxf(mx, t);
         }
     mx = max_column(mx);
-    if (__builtin_amdgcn_ballot_w64((mx - st.m) * unit > 8.0f || (st.m == -INF && mx > -INF))) {
-        const float m = fmaxf(st.m, mx), f = __builtin_amdgcn_exp2f((st.m - (m == -INF ? 0.0f : m)) * unit);
+    // each column by its own maximum: its sums do not depend on its neighbours'
+    const bool moves = (mx - st.m) * unit > 8.0f || (st.m == -INF && mx > -INF);
+    if (__builtin_amdgcn_ballot_w64(moves)) {
+        const float m = moves ? mx : st.m, f = __builtin_amdgcn_exp2f((st.m - (m == -INF ? 0.0f : m)) * unit);
         st.l *= f;
 #pragma unroll
         for (int d = 0; d < ND; ++d) acc[d] *= f;
