@@ -53,7 +53,7 @@ struct Soft {
 
 // One step of the running softmax of a lane's column over N score blocks of
 // 32 keys from j0 (whole: all of the wave's rows see all of them). Scores
-// become probabilities; acc is rescaled when the wave's maxima move far enough.
+// become probabilities; acc is rescaled when the column's maximum moves far enough.
 template <bool MASKED, class T, int CAP, bool BIAS, int N, int ND>
 __device__ inline void soft_step(const Score<T, CAP, BIAS>& rule, const Row& row, bool whole, int j0, int half,
                                  f32x16 (&s)[N], f32x16 (&acc)[ND], Soft& st) {
@@ -84,8 +84,10 @@ __device__ inline void soft_step(const Score<T, CAP, BIAS>& rule, const Row& row
 #pragma unroll
         for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[n][r]);
     mx = max32(mx);
-    if (__builtin_amdgcn_ballot_w64((mx - st.m) * unit > 8.0f || (st.m == -INF && mx > -INF))) {
-        const float m = fmaxf(st.m, mx);
+    // each row by its own maximum: its sums do not depend on its neighbours'
+    const bool moves = (mx - st.m) * unit > 8.0f || (st.m == -INF && mx > -INF);
+    if (__builtin_amdgcn_ballot_w64(moves)) {
+        const float m = moves ? mx : st.m;
         const float f = __builtin_amdgcn_exp2f((st.m - (m == -INF ? 0.0f : m)) * unit);
         st.l *= f;
 #pragma unroll

@@ -30,6 +30,17 @@ OFF = dict(dtype=torch.int32, device="cuda")
 @pytest.mark.parametrize("ty", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
 @pytest.mark.parametrize("rows", [2, 5, 16, 40, 200])
 @pytest.mark.parametrize("cap", [0.0, 30.0])
+def test_over_keys(ctx, ty, rows, cap):
+    from brosoundml_amd import tokens
+    q, k, far, v = inputs(2, rows, 400, 64, ty)
+    where = torch.tensor([0, rows], **OFF), torch.tensor([0, 400], **OFF)
+    a, b = (tokens.attention(ctx, q, x, v, *where, causal=True, cap=cap) for x in (k, far))
+    assert torch.equal(a[0][:-1], b[0][:-1]) and torch.equal(a[1][:, :-1], b[1][:, :-1]) and not torch.equal(a[0][-1], b[0][-1])
+
+
+@pytest.mark.parametrize("ty", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("rows", [2, 5, 16, 40, 200])
+@pytest.mark.parametrize("cap", [0.0, 30.0])
 def test_over_the_cache(ctx, ty, rows, cap):
     from brosoundml_amd import tokens
     q, k, far, v = inputs(2, rows, 400, 64, ty)
