@@ -128,12 +128,7 @@ __device__ inline bool piece_at(const int* off, int docs, int rows, int each, in
     for (int base = -1; base <= docs; base += 64) {
         const int lo = at(base + lane), hi = at(base + lane + 1);
         const int n = hi > lo ? ((hi - lo) * each + size - 1) / size : 0;
-        int sum = n;
-#pragma unroll
-        for (int o = 1; o < 64; o *= 2) {
-            const int s = __shfl_up(sum, o);
-            sum += lane >= o ? s : 0;
-        }
+        const int sum = wave_scan(n);
         const int all = __builtin_amdgcn_readlane(sum, 63);
         if (b - before < all) {
             const int l = __builtin_popcountll(__builtin_amdgcn_ballot_w64(before + sum <= b));

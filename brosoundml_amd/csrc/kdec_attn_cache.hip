@@ -92,22 +92,12 @@ __device__ inline bool block_rows(const Cached& p, int b, int& row0, int& end, i
     row0 = b * p.rows;
     end = min(row0 + p.rows, m.Tq);
     if (!p.a.by_doc) return true;
-    const int lane = threadIdx.x & 63;
-    const auto at = [&](int d) { return d < 0 ? 0 : d <= m.docs ? min(max(m.q_off[d], 0), m.Tq) : m.Tq; };
-    int before = 0;
-    for (int base = -1; base <= m.docs; base += 64) {
-        const int lo = at(base + lane), hi = at(base + lane + 1), n = hi > lo ? (hi - lo + p.rows - 1) / p.rows : 0;
-        const int upto = wave_scan(n), all = __builtin_amdgcn_readlane(upto, 63);
-        if (b - before < all) {
-            const int l = __builtin_popcountll(__builtin_amdgcn_ballot_w64(before + upto <= b));
-            doc = base + l;
-            row0 = __builtin_amdgcn_readlane(lo, l) + (b - before - __builtin_amdgcn_readlane(upto - n, l)) * p.rows;
-            end = min(row0 + p.rows, __builtin_amdgcn_readlane(hi, l));
-            return true;
-        }
-        before += all;
-    }
-    return false;
+    Piece piece;
+    if (!piece_at(m.q_off, m.docs, m.Tq, 1, p.rows, b, piece)) return false;
+    doc = piece.doc;
+    row0 = piece.lo + piece.place * p.rows;
+    end = min(row0 + p.rows, piece.hi);
+    return true;
 }
 // A part's tiles: of every document an equal share. (Parts of a fixed length, the
 // same work for short and long documents, were slower: one token for 48 requests
