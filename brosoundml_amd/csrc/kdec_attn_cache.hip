@@ -21,9 +21,10 @@
 // output's block dt is column ND m + dt and no byte moves between lanes.
 //
 // Steps are bound by memory: one token for 48 requests over up to 4096 keys, 16
-// heads on 4 of width 128, 27 us for 106 MB (3.9 TB/s) and 4 for the join. Pieces of
-// 90 to 301 rows with a cap (73 us; the products alone would take 18.5) are
-// bound by the vector unit: codes to floats, exponentials of cap and softmax.
+// heads on 4 of width 128, 28 us for 106 MB (3.9 TB/s) and 4 for the join. Pieces of
+// 90 to 301 rows with a cap (80 to 95 us by their lengths; the products, the values'
+// twice, would take 28) are bound by the vector unit: codes to floats, exponentials
+// of cap and softmax, the probabilities' terms.
 #include "kdec_attn.hpp"
 
 namespace kdec {
@@ -535,7 +536,11 @@ extern "C" int kdec_attn_cache_fwd(kdec_ctx* ctx, int dtype, const void* Q, long
     // parts' blocks are on it at once (48 documents of 90 to 4096 keys and 1 row: 4
     // parts, which fill it, 26 us, 3 and 6 parts 31 and 32), to no fewer than 256
     // keys a part (one float row over 6000 keys, 12 heads of width 64: 15.9 us with
-    // the join, of 128 keys 16.8).
+    // the join, of 128 keys 16.8). The device is not filled evenly where the parts do
+    // not divide it (32 heads on 8, 90 to 4096 keys, 1, 2 and 3 parts: 24 requests 41
+    // us, 44 and 39 and by the rule, of 4, 35; 32 46, 51 and 51 by the rule; 48 73, 64
+    // by the rule and 63), and past half of it one part is the rule's (50 requests 73,
+    // 68, 64; 64 83, 78, 77; 96 116, 112, 112).
     const long each = docs > 0 ? Tk / docs : 0, held = (dtype == KDEC_F32 ? (cols == 16 ? 2L : 1L) : cols == 16 ? 3L : 2L) * ctx->num_cus;
     long splits = held / units;
     if (splits > each / 256) splits = each / 256;

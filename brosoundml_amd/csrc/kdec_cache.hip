@@ -8,8 +8,9 @@
 //
 // 8 or 16 lanes take the values of a token in a head, eight each; bound by
 // memory, or for single tokens by the launch and three dependent loads. 32 texts
-// of 77 to 1000 tokens, 12 heads of width 64, bf16: written in 24 us (2.8 TB/s),
-// read back in 17 (4.0); 48 single tokens of 4 heads of width 128 in 5.1 and 3.9.
+// of 77 to 1000 tokens, 12 heads of width 64, bf16: written in 23 us for 87 MB (3.7
+// TB/s), read back in 17 (5.1), float 39 and 27 for 144 MB; 48 single tokens of 4
+// heads of width 128, bf16, in 5.1 and 3.9.
 #include "kdec_attn.hpp"
 
 namespace kdec {
@@ -70,8 +71,9 @@ __device__ inline unsigned top_lanes(unsigned x) {
 
 // max |x| / 127 to the nearest float: the product with 1 / 127 and one correction
 // by its exact remainder (127 and the rounded 1 / 127 meet the conditions under
-// which that is the quotient; no step leaves the normal numbers above 2^-119,
-// below which the scale is 2^-126 whatever the quotient's last bit).
+// which that is the quotient). Quotients below 2^-126, of a top below 2^-119, make
+// the scale 2^-126 whatever their last bit; just above, the remainder is subnormal (a
+// top near 2^-119 leaves about 2^-143), which these kernels' floats keep.
 __device__ inline float scale_of(float top) {
     const float c = 1.0f / 127.0f, q = top * c;
     return fmaxf(__builtin_fmaf(__builtin_fmaf(-q, 127.0f, top), c, q), 0x1p-126f);

@@ -32,7 +32,9 @@ constexpr int CHUNK = ST * SI;  // tokens a sorting block holds
 constexpr int WAVES = ST / 64;
 constexpr int DIGITS = 256;
 
-// A lane's part of a row: 16 bytes.
+// A lane's part of a row: 16 bytes, a value at a time where rows do not start on
+// them (16381 rows of 1021 bf16: lookup 35 us and sums 42 where 1024 columns take 12
+// and 14; 8190 rows of 765 floats 16 and 12 for 8 and 9).
 template <class T> constexpr int PART = 16 / sizeof(T);
 template <class T> struct PartOf;
 template <> struct PartOf<float> { typedef f32x4 type; };

@@ -19,10 +19,12 @@
 // over the blocks in their order.
 //
 // Bound by memory where rows are many: 8192 x 2048, bf16, a gate for each row,
-// forward 37 us for 168 MB (4.5 TB/s; a large copy reaches 5.1), backward 53 and 5
-// for 268; 2050 x 5120 forward 18.4 for 84 MB; 4093 x 768, float, layer norms,
-// 12.4 for 50 MB, then 21 and 4 for 75. 16 rows of 1024 take 3.6 us, a launch and
-// three reductions.
+// forward 38 us for 168 MB (4.5 TB/s; a large copy reaches 5.1), backward 54 and 5
+// for 268; 2050 x 5120 forward 18.6 for 84 MB; 4093 x 768, float, layer norms,
+// 12.7 for 50 MB, then 21 and 4 for 75. Past 4096 columns the backward waits for its
+// rows, one at a time: 2048 x 5120 with a gate for each row 61 and 5 us for 168 MB,
+// 1024 x 8192 47 and 5 for 134. 16 rows of 1024 take 3.6 us, a launch and three
+// reductions.
 #include "kdec_frag.hpp"
 #include "kdec_internal.hpp"
 
@@ -105,7 +107,10 @@ __device__ inline void row_sums(float& a, float& b, Meet& red, int& turn) {
 
 // Eight columns of a tensor's row, from byte offset `off` of it: zeros past the
 // row's end or where the tensor is absent, without a branch around the load, so
-// that a row's tensors are on their way together.
+// that a row's tensors are on their way together. Rows of other widths than
+// multiples of 8 (or that start elsewhere) take eight loads: 4093 x 1021, bf16,
+// forward 27 us and backward 37 where 1024 columns take 10.8 and 15, float 43 and 63
+// for 14 and 22.
 template <class T>
 struct Raw {
     Frag<T> f;

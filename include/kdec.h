@@ -627,7 +627,9 @@ int kdec_cache_read(kdec_ctx* ctx, int dtype, const void* Kc, long kc_rs,
                     long k_hs, void* V, long v_rs, long v_hs);
 /* kdec_attn_fwd over such a cache: the same documents, masks, scores and
  * outputs, keys and values scale times code (Q, O of `dtype`). A row that sees
- * a token whose key or value scale is not finite becomes NaN. */
+ * a token whose key or value scale is not finite becomes NaN. Weights up to 2^8
+ * are summed before the division: values past 2^119 over the number of keys may
+ * overflow, and make their row NaN. */
 int kdec_attn_cache_fwd(kdec_ctx* ctx, int dtype, const void* Q, long q_rs,
                         long q_hs, const void* Kc, long kc_rs, long kc_hs,
                         const void* Vc, long vc_rs, long vc_hs,
