@@ -71,10 +71,10 @@ int guard_mode() {
     return mode;
 }
 
-// Whether the context's stream is being captured into a graph.
-static bool capturing(const kdec_ctx* ctx) {
+// Whether the context's stream is being captured into a graph, and which capture it is.
+static bool capturing(const kdec_ctx* ctx, unsigned long long* id = nullptr) {
     hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
-    if (hipStreamIsCapturing(ctx->stream, &status) != hipSuccess) {
+    if (hipStreamGetCaptureInfo(ctx->stream, &status, id) != hipSuccess) {
         (void)hipGetLastError();
         return false;
     }
@@ -95,14 +95,17 @@ int guard_check_all(kdec_ctx* ctx, const char* where) {
 void* ws_alloc(kdec_ctx* ctx, size_t bytes, bool scoped) {
     if (bytes == 0) bytes = 256;
     bytes = (bytes + 255) & ~size_t(255);
-    const bool captures = capturing(ctx);
+    unsigned long long capture = 0;
+    const bool captures = capturing(ctx, &capture);
     const size_t need = guard_mode() ? bytes + 2 * kGuard : bytes;
     void* base = nullptr;
     size_t size = need;
     // Reuse a pooled block of at least `need` bytes but not absurdly larger.
     const auto usable = [&](void* block) {
         const auto graph = ctx->captured.find(block);
-        return graph == ctx->captured.end() || (scoped && graph->second == ctx->stream);
+        if (graph == ctx->captured.end()) return true;
+        const kdec_ctx::Captured& c = graph->second;
+        return scoped ? c.stream == ctx->stream : captures && !c.shared && c.capture == capture;
     };
     auto it = ctx->pool.lower_bound(need);
     while (it != ctx->pool.end() && !usable(it->second)) ++it;
@@ -139,7 +142,10 @@ void* ws_alloc(kdec_ctx* ctx, size_t bytes, bool scoped) {
             }
         }
     }
-    if (captures) ctx->captured[base] = ctx->stream;
+    if (captures) {
+        const auto graph = ctx->captured.emplace(base, kdec_ctx::Captured{ctx->stream, capture, false}).first;
+        if (graph->second.capture != capture) graph->second.shared = true;
+    }
     const kdec_ctx::Block blk{base, size, bytes, guard_mode() && !captures};
     void* user = guard_mode() ? static_cast<char*>(base) + kGuard : base;
     if (blk.bands) guard_fill(ctx, blk);

@@ -30,13 +30,19 @@ struct kdec_ctx {
         bool bands;    // whether its guard bands were filled
     };
     std::unordered_map<void*, Block> live;  // handed-out pointer -> its block
-    // Blocks that a captured graph uses, with the stream it was captured on. A
-    // replay writes them whenever it comes, so they are given back to the driver
-    // only with the context, which outlives the graph, and the pool hands them out
-    // again only to a call's own workspace on that stream: its kernels and a
-    // replay's come one after the other, while memory that outlives a call, or work
-    // on another stream, would meet a replay in between.
-    std::unordered_map<void*, hipStream_t> captured;
+    // Blocks that a captured graph uses. A replay writes them whenever it comes, so
+    // they are given back to the driver only with the context, which outlives the
+    // graph, and the pool hands them out again only to a call's own workspace on the
+    // stream of the capture: its kernels and a replay's come one after the other,
+    // while memory that outlives a call, or work on another stream, would meet a
+    // replay in between. Memory that a capture itself asks for may be what the same
+    // capture gave back, as long as no other graph uses it.
+    struct Captured {
+        hipStream_t stream;
+        unsigned long long capture;  // the first that used it
+        bool shared;                 // whether others do
+    };
+    std::unordered_map<void*, Captured> captured;
     size_t pooled_bytes = 0;
     // Set by kdec_ctx_destroy while blocks are still live (tensors that
     // outlive their context): the last ws_free then releases the context.

@@ -99,6 +99,38 @@ def test_memory_held_before_a_capture_stays_apart():
     assert same(out, want)
 
 
+def test_a_capture_reuses_what_it_gave_back():
+    """Memory that is asked for and given back within a capture serves its next request, as outside of one, but no later
+    capture's, whose memory outlives the first graph's replays."""
+    from brosoundml_amd import native
+    n = 1 << 22  # more than any of this context's other blocks
+    side = torch.cuda.Stream()
+    ctx = native.Context(0, stream=side)
+    Held(ctx, n).free()  # one block for them all
+    held, graphs = [], []
+    torch.cuda.synchronize()
+    for i in range(2):
+        if i:
+            Held(ctx, n).free()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=side):
+            for _ in range(3):
+                h = Held(ctx, n)
+                h.tensor().fill_(float(i))
+                h.free()
+            held.append(Held(ctx, n))
+            held[i].tensor().fill_(float(i + 5))
+        graphs.append(g)
+    assert held[0].p.value != held[1].p.value
+    with torch.cuda.stream(side):
+        for g in graphs + graphs:
+            g.replay()
+    side.synchronize()
+    for i, h in enumerate(held):
+        assert (h.tensor() == i + 5).all()
+        h.free()
+
+
 def test_calls_on_another_stream_stay_apart():
     """A context that moved to another stream makes its calls there while the graph is replayed on its own."""
     from brosoundml_amd import native
